@@ -15,7 +15,7 @@ from typing import Optional
 from . import abi
 
 __all__ = ["HelixError", "Context", "desc_from_tensors", "scan", "shard_state", "scan_shard", "carry_combine",
-           "abi"]
+           "rms_norm", "rms_norm_grad", "quantize8", "abi"]
 
 
 class HelixError(RuntimeError):
@@ -258,3 +258,15 @@ def carry_combine(s0, states, log_decays, ids=None, *, ctx: Optional[Context] = 
     if st != abi.HELIX_OK:
         raise HelixError(st, ctx.last_error())
     return carry
+
+
+# block.py needs torch at import; the rest of the package does not.
+_BLOCK = ("rms_norm", "rms_norm_grad", "quantize8")
+
+
+def __getattr__(name):
+    if name in _BLOCK:
+        from . import block
+        globals().update({n: getattr(block, n) for n in _BLOCK})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -23,11 +23,14 @@ STATUS_NAMES = {0: "OK", 1: "UNSUPPORTED_SHAPE", 2: "NO_DEVICE", 3: "SCRATCH_TOO
                 4: "INVALID_ARG", 5: "PIPELINE"}
 
 # helix_dtype
-HELIX_F32, HELIX_F16, HELIX_BF16 = 0, 1, 2
+HELIX_F32, HELIX_F16, HELIX_BF16, HELIX_E4M3 = 0, 1, 2, 3
 # helix_a_form
 HELIX_A_SCALAR_PER_HEAD, HELIX_A_DIAG_PER_CHANNEL = 0, 1
 # helix_backend
 HELIX_BACKEND_AUTO, HELIX_BACKEND_SGMMA, HELIX_BACKEND_MPP, HELIX_BACKEND_REF = 0, 1, 2, 3
+# include/helix/helix_block.h: values that share a scale; helix_scale_form
+HELIX_GROUP = 128
+HELIX_SCALE_ROWS, HELIX_SCALE_BLOCKS = 0, 1
 
 I32, I64 = C.c_int32, C.c_int64
 
@@ -68,7 +71,24 @@ EXPORTS = (
     "helix_device_fault", "helix_scan_encode_static",
     "helix_scan_shard_state_scratch_size", "helix_scan_shard_state", "helix_scan_carry_combine",
     "helix_scan_plan_info", "helix_scan_encode_shard",
+    # include/helix/helix_block.h
+    "helix_rms_norm_desc_init", "helix_rms_norm_encode", "helix_rms_norm_grad_scratch_size",
+    "helix_rms_norm_grad_encode", "helix_quant8_desc_init", "helix_quant8_encode",
 )
+
+
+class RmsNormDesc(C.Structure):
+    """helix_rms_norm_desc (include/helix/helix_block.h)."""
+    _fields_ = [("n_row", I64), ("n_col", I32), ("eps", C.c_float), ("x_dtype", C.c_int), ("sum_dtype", C.c_int),
+                ("out_dtype", C.c_int), ("w_dtype", C.c_int), ("ld_x", I64), ("ld_res", I64), ("ld_sum", I64),
+                ("ld_out", I64), ("ld_scale", I64), ("ld_dout", I64), ("ld_dsum", I64), ("ld_dx", I64),
+                ("ld_dres", I64)]
+
+
+class Quant8Desc(C.Structure):
+    """helix_quant8_desc (include/helix/helix_block.h)."""
+    _fields_ = [("n_row", I64), ("n_col", I64), ("x_dtype", C.c_int), ("form", C.c_int), ("transpose", C.c_bool),
+                ("ld_x", I64), ("ld_q", I64), ("ld_scale", I64)]
 
 
 class PlanInfo(C.Structure):
@@ -126,6 +146,18 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.helix_scan_encode_shard.restype = C.c_int
     lib.helix_scan_plan_info.argtypes = [C.c_void_p, P(ScanDesc), P(PlanInfo)]
     lib.helix_scan_plan_info.restype = C.c_int
+    lib.helix_rms_norm_desc_init.argtypes = [P(RmsNormDesc), I64, I32]
+    lib.helix_rms_norm_desc_init.restype = None
+    lib.helix_rms_norm_encode.argtypes = [C.c_void_p, C.c_void_p, P(RmsNormDesc)] + [Tensor] * 7
+    lib.helix_rms_norm_encode.restype = C.c_int
+    lib.helix_rms_norm_grad_scratch_size.argtypes = [C.c_void_p, P(RmsNormDesc)]
+    lib.helix_rms_norm_grad_scratch_size.restype = C.c_size_t
+    lib.helix_rms_norm_grad_encode.argtypes = [C.c_void_p, C.c_void_p, P(RmsNormDesc)] + [Tensor] * 9
+    lib.helix_rms_norm_grad_encode.restype = C.c_int
+    lib.helix_quant8_desc_init.argtypes = [P(Quant8Desc), I64, I64, C.c_int, C.c_bool]
+    lib.helix_quant8_desc_init.restype = None
+    lib.helix_quant8_encode.argtypes = [C.c_void_p, C.c_void_p, P(Quant8Desc)] + [Tensor] * 3
+    lib.helix_quant8_encode.restype = C.c_int
     if path is None:
         _lib = lib
     return lib

@@ -35,7 +35,7 @@ def sources() -> list[Path]:
 
 def headers() -> list[Path]:
     return (sorted(CSRC.rglob("*.h")) + sorted(CSRC.rglob("*.cuh"))
-            + [ROOT / "include" / "helix" / "helix.h"])
+            + sorted((ROOT / "include" / "helix").glob("*.h")))
 
 
 def _obj(src: Path) -> Path:

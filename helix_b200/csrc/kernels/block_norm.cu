@@ -1,0 +1,328 @@
+// block_norm.cu -- root-mean-square norm with the residual's addition, its
+// output in 8 bits or not, and its gradient.
+//
+//     s = x + r,  rstd = 1 / sqrt(mean(s^2) + eps),  n = s rstd w
+//     ds = dsum + rstd (dn w - s rstd^2 mean(dn w s)),  dw = sum_rows dn s rstd
+//
+// Both are bound by memory: one pass, the row kept in registers between its
+// statistic and its output.  A row belongs to wpr warps; a warp holds V
+// segments of 256 columns (segment j * wpr + warp), a lane 8 values of each.
+// With vector accesses a lane's 8 values are consecutive, so 16 lanes hold a
+// group of 128; without (odd widths or strides) lane l holds columns l + 32 e
+// of the segment, so every access is still a run of 32 values, and the whole
+// warp holds each of the segment's two groups.
+//
+// Sums, statistics and the products are fp32; the only roundings are those
+// of the stored sum, the output and (8 bits) 1 / scale.
+#include "block_common.cuh"
+
+namespace hx {
+namespace {
+
+constexpr int kSeg = 256;        // columns of a warp's segment
+constexpr int kMaxWarps = 16;    // 16 warps x 4 segments x 256 = 16384 columns
+
+template <bool VEC>
+__device__ __forceinline__ int col_of(int c0, int lane, int e) {
+    return VEC ? c0 + 8 * lane + e : c0 + 32 * e + lane;
+}
+
+// The lane's 8 values of the segment at c0; 0 past the row's end.
+template <bool VEC, typename T>
+__device__ __forceinline__ void ld_seg(const T* row, int c0, int lane, int n_col, float (&v)[8]) {
+    if (VEC && c0 + 8 * lane + 8 <= n_col) {
+        ld8(row + c0 + 8 * lane, v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = col_of<VEC>(c0, lane, e);
+        v[e] = c < n_col ? to_f32(row[c]) : 0.0f;
+    }
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void st_seg(T* row, int c0, int lane, int n_col, const float (&v)[8]) {
+    if (VEC && c0 + 8 * lane + 8 <= n_col) {
+        st8(row + c0 + 8 * lane, v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = col_of<VEC>(c0, lane, e);
+        if (c < n_col) row[c] = from_f32<T>(v[e]);
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void ld_weight(const NormParams& p, int c0, int lane, float (&v)[8]) {
+    if (p.w_bf16)
+        ld_seg<VEC>(static_cast<const __nv_bfloat16*>(p.w), c0, lane, p.n_col, v);
+    else
+        ld_seg<VEC>(static_cast<const float*>(p.w), c0, lane, p.n_col, v);
+}
+
+// Sum over the wpr warps of a row (every warp of the block calls it).
+// `part` holds one float per warp; buffers alternate between calls so that
+// one barrier a call is enough.
+__device__ __forceinline__ float row_sum(float v, int wpr, int warp, int lane, float* part) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (wpr == 1) return v;
+    if (lane == 0) part[warp] = v;
+    __syncthreads();
+    const int first = warp / wpr * wpr;
+    float s = 0.0f;
+    for (int w = 0; w < wpr; ++w) s += part[first + w];
+    return s;
+}
+
+// The segment's 8 values a lane holds, as e4m3 with its group's scale.
+template <bool VEC>
+__device__ __forceinline__ void st_seg_e4m3(const NormParams& p, int64_t row, int c0, int lane,
+                                            const float (&n)[8]) {
+    uint8_t* q = static_cast<uint8_t*>(p.out) + row * p.ld_out;
+    float* sc = p.scale + row * p.ld_scale;
+    if constexpr (VEC) {
+        float a = fabsf(n[0]);
+#pragma unroll
+        for (int e = 1; e < 8; ++e) a = max_nan(a, fabsf(n[e]));
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const float scale = group_scale(a), inv = 1.0f / scale;
+        const int c = c0 + 8 * lane;
+        if ((lane & 15) == 0 && c < p.n_col) sc[c / HELIX_GROUP] = scale;
+        if (c + 8 <= p.n_col) {
+            *reinterpret_cast<uint2*>(q + c) =
+                make_uint2(e4m3x2(n[0] * inv, n[1] * inv) | e4m3x2(n[2] * inv, n[3] * inv) << 16,
+                           e4m3x2(n[4] * inv, n[5] * inv) | e4m3x2(n[6] * inv, n[7] * inv) << 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < p.n_col) q[c + e] = (uint8_t)e4m3x2(n[e] * inv, 0.0f);
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {  // the segment's groups: e = 0..3 and 4..7
+            float a = 0.0f;
+#pragma unroll
+            for (int e = 4 * g; e < 4 * g + 4; ++e) a = max_nan(a, fabsf(n[e]));
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+            const float scale = group_scale(a), inv = 1.0f / scale;
+            const int first = c0 + HELIX_GROUP * g;
+            if (lane == 0 && first < p.n_col) sc[first / HELIX_GROUP] = scale;
+#pragma unroll
+            for (int e = 4 * g; e < 4 * g + 4; ++e) {
+                const int c = c0 + 32 * e + lane;
+                if (c < p.n_col) q[c] = (uint8_t)e4m3x2(n[e] * inv, 0.0f);
+            }
+        }
+    }
+}
+
+template <typename TX, typename TR, int V, bool VEC>
+__global__ void __launch_bounds__(32 * kMaxWarps) norm_kernel(const NormParams p) {
+    __shared__ float part[kMaxWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * p.rpb + warp / p.wpr;
+    const int wr = warp % p.wpr;
+    const bool live = row < p.n_row;
+
+    float s[V][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c0 = (j * p.wpr + wr) * kSeg;
+        const int n = live ? p.n_col : 0;
+        ld_seg<VEC>(static_cast<const TX*>(p.x) + (live ? row : 0) * p.ld_x, c0, lane, n, s[j]);
+    }
+    if (p.res) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c0 = (j * p.wpr + wr) * kSeg;
+            float r[8];
+            ld_seg<VEC>(static_cast<const TR*>(p.res) + (live ? row : 0) * p.ld_res, c0, lane, live ? p.n_col : 0,
+                        r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[j][e] += r[e];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += s[j][e] * s[j][e];
+    ss = row_sum(ss, p.wpr, warp, lane, part);
+    if (!live) return;
+    const float rstd = 1.0f / sqrtf(ss / (float)p.n_col + p.eps);
+    if (p.rstd && wr == 0 && lane == 0) p.rstd[row] = rstd;
+
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c0 = (j * p.wpr + wr) * kSeg;
+        if (p.sum) st_seg<VEC>(static_cast<TR*>(p.sum) + row * p.ld_sum, c0, lane, p.n_col, s[j]);
+        float w[8];
+        ld_weight<VEC>(p, c0, lane, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] *= s[j][e] * rstd;
+        if (p.out_dtype == HELIX_E4M3)
+            st_seg_e4m3<VEC>(p, row, c0, lane, w);
+        else if (p.out_dtype == HELIX_BF16)
+            st_seg<VEC>(static_cast<__nv_bfloat16*>(p.out) + row * p.ld_out, c0, lane, p.n_col, w);
+        else
+            st_seg<VEC>(static_cast<float*>(p.out) + row * p.ld_out, c0, lane, p.n_col, w);
+    }
+}
+
+// Persistent: a row slot takes every slots-th row and keeps its share of
+// dweight in registers, written to partial[slot] at the end.
+template <typename TX, typename TR, int V, bool VEC>
+__global__ void __launch_bounds__(32 * kMaxWarps) norm_grad_kernel(const NormParams p) {
+    __shared__ float part[2][kMaxWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rg = warp / p.wpr, wr = warp % p.wpr;
+    float dw[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[j][e] = 0.0f;
+
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * p.rpb; base < p.n_row; base += (int64_t)gridDim.x * p.rpb) {
+        const bool live = base + rg < p.n_row;
+        const int64_t row = live ? base + rg : 0;
+        const int n = live ? p.n_col : 0;
+        const float rstd = live ? p.rstd[row] : 0.0f;
+        float d[V][8], s[V][8];
+        float along = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c0 = (j * p.wpr + wr) * kSeg;
+            ld_seg<VEC>(static_cast<const TX*>(p.dout) + row * p.ld_dout, c0, lane, n, d[j]);
+            ld_seg<VEC>(static_cast<const TR*>(p.sum) + row * p.ld_sum, c0, lane, n, s[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float w[8];
+            ld_weight<VEC>(p, (j * p.wpr + wr) * kSeg, lane, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s[j][e] *= rstd;              // s rstd
+                dw[j][e] += d[j][e] * s[j][e];
+                d[j][e] *= w[e];              // dn w
+                along += d[j][e] * s[j][e];
+            }
+        }
+        along = row_sum(along, p.wpr, warp, lane, part[turn]) / (float)p.n_col;
+        turn ^= 1;
+        if (!live) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c0 = (j * p.wpr + wr) * kSeg;
+            float o[8];
+            if (p.dsum)
+                ld_seg<VEC>(static_cast<const TR*>(p.dsum) + row * p.ld_dsum, c0, lane, n, o);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] += rstd * (d[j][e] - s[j][e] * along);
+            st_seg<VEC>(static_cast<TX*>(p.dx) + row * p.ld_dx, c0, lane, n, o);
+            if (p.dres) st_seg<VEC>(static_cast<TR*>(p.dres) + row * p.ld_dres, c0, lane, n, o);
+        }
+    }
+    float* mine = p.partial + ((int64_t)blockIdx.x * p.rpb + rg) * p.n_col;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c0 = (j * p.wpr + wr) * kSeg;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = col_of<VEC>(c0, lane, e);
+            if (c < p.n_col) mine[c] = dw[j][e];
+        }
+    }
+}
+
+// dweight[c] = the partials' sum in the order of the slots.
+constexpr int kDwRows = 16;
+__global__ void __launch_bounds__(32 * kDwRows) norm_dw_kernel(const float* partial, int slots, int n_col,
+                                                              float* dweight) {
+    __shared__ float part[kDwRows][33];
+    const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;
+    float v = 0.0f;
+    if (c < n_col)
+        for (int s = r; s < slots; s += kDwRows) v += partial[(int64_t)s * n_col + c];
+    part[r][lane] = v;
+    __syncthreads();
+    if (r == 0 && c < n_col) {
+#pragma unroll
+        for (int i = 1; i < kDwRows; ++i) v += part[i][lane];
+        dweight[c] = v;
+    }
+}
+
+template <typename TX, typename TR, bool VEC>
+int launch_norm_v(const NormParams& p, int v, dim3 grid, dim3 block, bool grad, void* stream) {
+    if (grad)
+        return v == 1   ? block_launch(norm_grad_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
+               : v == 2 ? block_launch(norm_grad_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p)
+                        : block_launch(norm_grad_kernel<TX, TR, 4, VEC>, grid, block, 0, stream, p);
+    return v == 1   ? block_launch(norm_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
+           : v == 2 ? block_launch(norm_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p)
+                    : block_launch(norm_kernel<TX, TR, 4, VEC>, grid, block, 0, stream, p);
+}
+
+int launch_norm_any(const helix_rms_norm_desc& d, const NormParams& p, int v, dim3 grid, dim3 block, bool vec,
+                    bool grad, void* stream) {
+    using bf = __nv_bfloat16;
+    if (d.x_dtype == HELIX_F32)
+        return vec ? launch_norm_v<float, float, true>(p, v, grid, block, grad, stream)
+                   : launch_norm_v<float, float, false>(p, v, grid, block, grad, stream);
+    if (d.sum_dtype == HELIX_F32)
+        return vec ? launch_norm_v<bf, float, true>(p, v, grid, block, grad, stream)
+                   : launch_norm_v<bf, float, false>(p, v, grid, block, grad, stream);
+    return vec ? launch_norm_v<bf, bf, true>(p, v, grid, block, grad, stream)
+               : launch_norm_v<bf, bf, false>(p, v, grid, block, grad, stream);
+}
+
+}  // namespace
+
+NormShape norm_shape(const helix_rms_norm_desc& d) {
+    const int segs = (d.n_col + kSeg - 1) / kSeg;
+    NormShape s{};
+    s.v = segs <= 1 ? 1 : segs <= 2 * kMaxWarps ? 2 : 4;
+    s.wpr = (segs + s.v - 1) / s.v;
+    s.rpb = s.wpr >= 8 ? 1 : 8 / s.wpr;
+    return s;
+}
+
+NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d) {
+    NormGradPlan pl{};
+    pl.shape = norm_shape(d);
+    const int n_sm = ctx && ctx->n_sm > 0 ? ctx->n_sm : 148;
+    const int64_t per_sm = 32 / (pl.shape.wpr * pl.shape.rpb);  // about 1024 threads per SM
+    const int64_t need = (d.n_row + pl.shape.rpb - 1) / pl.shape.rpb;
+    const int64_t most = (int64_t)n_sm * (per_sm > 0 ? per_sm : 1);
+    pl.blocks = (int)(need < most ? need : most);
+    pl.slots = pl.blocks * pl.shape.rpb;
+    pl.total = ((size_t)pl.slots * (size_t)d.n_col * sizeof(float) + 255) & ~(size_t)255;
+    return pl;
+}
+
+int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream) {
+    const NormShape s = norm_shape(d);
+    const dim3 grid((unsigned)((d.n_row + s.rpb - 1) / s.rpb)), block(32 * s.wpr * s.rpb);
+    return launch_norm_any(d, p, s.v, grid, block, vec, false, stream);
+}
+
+int launch_norm_grad(const helix_rms_norm_desc& d, const NormGradPlan& pl, const NormParams& p, bool vec,
+                     float* dweight, void* stream) {
+    if (pl.blocks > 0) {
+        const dim3 grid((unsigned)pl.blocks), block(32 * pl.shape.wpr * pl.shape.rpb);
+        const int e = launch_norm_any(d, p, pl.shape.v, grid, block, vec, true, stream);
+        if (e != cudaSuccess) return e;
+    }
+    return block_launch(norm_dw_kernel, dim3((unsigned)((d.n_col + 31) / 32)), dim3(32 * kDwRows), 0, stream,
+                        (const float*)p.partial, pl.slots, d.n_col, dweight);
+}
+
+}  // namespace hx

@@ -66,6 +66,9 @@ typedef enum {
     HELIX_F32  = 0,
     HELIX_F16  = 1,
     HELIX_BF16 = 2,
+    HELIX_E4M3 = 3,  /* not in the reference: 8-bit floats (4 exponent, 3
+                        mantissa bits, no infinity, largest 448) of the
+                        operators in helix_block.h; the scan rejects it     */
 } helix_dtype;
 
 typedef enum {

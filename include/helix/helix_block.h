@@ -1,0 +1,117 @@
+/* helix_block.h -- the operators of a recurrent block around its scan.
+ *
+ * No counterpart in the reference, which holds the scan alone.  Everything
+ * here follows the scan's contract (helix.h): a call is enqueued on `stream`
+ * (a cudaStream_t; NULL = legacy default stream), never synchronises, never
+ * allocates, and enqueues nothing when it returns an error; the message is in
+ * helix_ctx_last_error().  Tensors are device memory on ctx's device, aligned
+ * to their element size.  Strides are in elements; the innermost stride is 1.
+ * An output may not overlap an input or another output, except where a
+ * comment says "in place": then it is the same address, type and strides.
+ *
+ * 8-bit tensors are e4m3 floats (HELIX_E4M3) with one fp32 scale for each
+ * group of HELIX_GROUP: a value is (float)q * scale, and
+ *     scale = max(largest magnitude of the group, 2^-100) / 448,
+ *     q     = value / scale rounded to nearest even.
+ * A group that holds a NaN or an infinity has that as its scale, and NaN (or
+ * zero, for the finite values beside an infinity) as its q.
+ */
+#ifndef HELIX_BLOCK_H
+#define HELIX_BLOCK_H
+
+#include "helix/helix.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define HELIX_GROUP 128
+
+/* ------------------------------------------------------------------------ */
+/* Root-mean-square norm with the residual's addition                       */
+/* ------------------------------------------------------------------------ */
+
+/* Per row, with s = x + residual in fp32:
+ *     rstd = 1 / sqrt(mean(s^2) + eps),   n = s rstd weight
+ * sum receives s rounded to sum_dtype; n is taken from the unrounded s. */
+typedef struct {
+    int64_t     n_row;
+    int32_t     n_col;      /* 1 .. 16384                                      */
+    float       eps;        /* >= 0                                            */
+    helix_dtype x_dtype;    /* F32 or BF16: x; dout and dx of the gradient      */
+    helix_dtype sum_dtype;  /* residual and sum, dsum and dres: F32, or x_dtype */
+    helix_dtype out_dtype;  /* out: F32, BF16 or E4M3                           */
+    helix_dtype w_dtype;    /* weight: F32 or BF16                              */
+    int64_t     ld_x;       /* row strides: x                                   */
+    int64_t     ld_res;     /* residual                                         */
+    int64_t     ld_sum;     /* sum                                              */
+    int64_t     ld_out;     /* out                                              */
+    int64_t     ld_scale;   /* scale [n_row][ceil(n_col / 128)] f32             */
+    int64_t     ld_dout;    /* gradient: dout, dsum, dx, dres                   */
+    int64_t     ld_dsum;
+    int64_t     ld_dx;
+    int64_t     ld_dres;
+} helix_rms_norm_desc;
+
+/* Dense strides, every type F32, eps 1e-6. */
+void helix_rms_norm_desc_init(helix_rms_norm_desc* d, int64_t n_row, int32_t n_col);
+
+/* residual may be null (s = x).  sum may be null; in place of residual or of
+ * x it is allowed.  scale is written when out_dtype is E4M3 (and required
+ * then), rstd [n_row] f32 when not null. */
+helix_status helix_rms_norm_encode(helix_ctx* ctx, void* stream, const helix_rms_norm_desc* d,
+                                   helix_tensor x, helix_tensor residual, helix_tensor weight,
+                                   helix_tensor out, helix_tensor scale, helix_tensor sum,
+                                   helix_tensor rstd);
+
+/* The gradient.  dout (x_dtype) is the gradient of n; rounding to 8 bits is
+ * passed through.  dsum (sum_dtype, may be null) is the gradient that reaches
+ * sum by another way.  With s = the stored sum (sum_dtype) and rstd as the
+ * forward pass left them:
+ *     ds = dsum + rstd (dout w - s rstd^2 mean(dout w s))
+ *     dweight = sum over rows of dout s rstd         (f32, [n_col])
+ * dx (x_dtype) and, when not null, dres (sum_dtype) both receive ds.  dx may
+ * be in place of dout, dres in place of dsum.  The sum over rows is taken in
+ * an order that depends on the sizes and the device alone.  Needs
+ * helix_rms_norm_grad_scratch_size() bytes of 256-byte-aligned scratch. */
+size_t       helix_rms_norm_grad_scratch_size(helix_ctx* ctx, const helix_rms_norm_desc* d);
+helix_status helix_rms_norm_grad_encode(helix_ctx* ctx, void* stream, const helix_rms_norm_desc* d,
+                                        helix_tensor dout, helix_tensor sum, helix_tensor rstd,
+                                        helix_tensor weight, helix_tensor dsum, helix_tensor dx,
+                                        helix_tensor dres, helix_tensor dweight,
+                                        helix_tensor scratch);
+
+/* ------------------------------------------------------------------------ */
+/* Quantiser                                                                */
+/* ------------------------------------------------------------------------ */
+
+typedef enum {
+    HELIX_SCALE_ROWS   = 0, /* one scale per row and 128 columns               */
+    HELIX_SCALE_BLOCKS = 1, /* one scale per 128 rows and 128 columns          */
+} helix_scale_form;
+
+/* q = x, or x transposed, in 8 bits.  The groups are those of q: transposed,
+ * HELIX_SCALE_ROWS puts 128 consecutive rows of x under one scale. */
+typedef struct {
+    int64_t          n_row;     /* of x                                        */
+    int64_t          n_col;
+    helix_dtype      x_dtype;   /* F32 or BF16                                 */
+    helix_scale_form form;
+    bool             transpose; /* q is [n_col][n_row], else [n_row][n_col]    */
+    int64_t          ld_x;
+    int64_t          ld_q;
+    int64_t          ld_scale;  /* scale: [q rows, or their blocks][ceil(q columns / 128)] f32 */
+} helix_quant8_desc;
+
+/* Dense strides except ld_q, which is rounded up to 16 (what the product
+ * needs of its operands). */
+void         helix_quant8_desc_init(helix_quant8_desc* d, int64_t n_row, int64_t n_col,
+                                    helix_scale_form form, bool transpose);
+helix_status helix_quant8_encode(helix_ctx* ctx, void* stream, const helix_quant8_desc* d,
+                                 helix_tensor x, helix_tensor q, helix_tensor scale);
+
+#ifdef __cplusplus
+}  /* extern "C" */
+#endif
+
+#endif  /* HELIX_BLOCK_H */
