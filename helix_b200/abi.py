@@ -74,6 +74,7 @@ EXPORTS = (
     # include/helix/helix_block.h
     "helix_rms_norm_desc_init", "helix_rms_norm_encode", "helix_rms_norm_grad_scratch_size",
     "helix_rms_norm_grad_encode", "helix_quant8_desc_init", "helix_quant8_encode",
+    "helix_matmul8_desc_init", "helix_matmul8_encode",
 )
 
 
@@ -89,6 +90,12 @@ class Quant8Desc(C.Structure):
     """helix_quant8_desc (include/helix/helix_block.h)."""
     _fields_ = [("n_row", I64), ("n_col", I64), ("x_dtype", C.c_int), ("form", C.c_int), ("transpose", C.c_bool),
                 ("ld_x", I64), ("ld_q", I64), ("ld_scale", I64)]
+
+
+class Matmul8Desc(C.Structure):
+    """helix_matmul8_desc (include/helix/helix_block.h)."""
+    _fields_ = [("m", I32), ("n", I32), ("k", I32), ("b_form", C.c_int), ("out_dtype", C.c_int), ("ld_a", I64),
+                ("ld_b", I64), ("ld_out", I64), ("ld_a_scale", I64), ("ld_b_scale", I64)]
 
 
 class PlanInfo(C.Structure):
@@ -158,6 +165,10 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.helix_quant8_desc_init.restype = None
     lib.helix_quant8_encode.argtypes = [C.c_void_p, C.c_void_p, P(Quant8Desc)] + [Tensor] * 3
     lib.helix_quant8_encode.restype = C.c_int
+    lib.helix_matmul8_desc_init.argtypes = [P(Matmul8Desc), I32, I32, I32, C.c_int]
+    lib.helix_matmul8_desc_init.restype = None
+    lib.helix_matmul8_encode.argtypes = [C.c_void_p, C.c_void_p, P(Matmul8Desc)] + [Tensor] * 5
+    lib.helix_matmul8_encode.restype = C.c_int
     if path is None:
         _lib = lib
     return lib

@@ -221,3 +221,37 @@ def quantize8(x: torch.Tensor, *, blocks: bool = False, transpose: bool = False,
     d.ld_scale = _groups(cols)
     call.done(call.ctx.lib.helix_quant8_encode(call.ctx.handle, call.handle, C.byref(d), _t(x), _t(q), _t(scale)))
     return q, scale
+
+
+def matmul8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *,
+            out_dtype: torch.dtype = torch.bfloat16, ctx: Optional[Context] = None, stream=None) -> torch.Tensor:
+    """a b^T of 8-bit matrices a (..., k) and b (n, k): (..., n) in out_dtype.
+
+    a_scale (..., ceil(k / 128)); b_scale (ceil(n / 128), ceil(k / 128)) by
+    blocks or (n, ceil(k / 128)) by rows.  Rows of a and b must start at
+    multiples of 16 bytes, as rms_norm and quantize8 leave them."""
+    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
+        raise TypeError("a and b must be torch.float8_e4m3fn")
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        raise TypeError("scales must be torch.float32")
+    if b.dim() != 2 or a.shape[-1] != b.shape[1]:
+        raise ValueError("b must be a matrix with as many columns as a")
+    n, k = b.shape
+    groups = _groups(k)
+    d = abi.Matmul8Desc()
+    d.m, d.n, d.k = (a.numel() // k if k else 0), n, k
+    d.ld_a, d.ld_b = _matrix("a", a), _matrix("b", b)
+    d.ld_a_scale = _matrix("a_scale", a_scale, (*a.shape[:-1], groups))
+    d.b_form = abi.HELIX_SCALE_ROWS if tuple(b_scale.shape) == (n, groups) else abi.HELIX_SCALE_BLOCKS
+    d.ld_b_scale = _matrix("b_scale", b_scale, (n if d.b_form == abi.HELIX_SCALE_ROWS else _groups(n), groups))
+    try:
+        d.out_dtype = _IO[out_dtype]
+    except KeyError:
+        raise TypeError(f"out_dtype {out_dtype} is not supported") from None
+    d.ld_out = n
+    call = _Call(a, ctx, stream, a_scale, b, b_scale)
+    with call.alloc():
+        out = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
+    call.done(call.ctx.lib.helix_matmul8_encode(call.ctx.handle, call.handle, C.byref(d), _t(a), _t(a_scale), _t(b),
+                                                _t(b_scale), _t(out)))
+    return out

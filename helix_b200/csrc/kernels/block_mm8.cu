@@ -1,0 +1,355 @@
+// block_mm8.cu -- product of e4m3 matrices with an fp32 scale for each block
+// of 128 along k, on tcgen05.
+//
+//     out[i][j] = sum_b sa[i][b] sb[j][b] D_b[i][j],  D_b = sum_{k in b} a[i][k] b[j][k]
+//
+// The scales differ from block to block of k, so the sum over blocks cannot
+// stay in the tensor core's accumulator: each block's D_b is four MMAs of
+// K = 32 into one of several TMEM buffers, and the epilogue warps add
+// (sa sb) D_b to fp32 registers while the next blocks' MMAs run.
+//
+// A CTA has a tile of 128 rows of P x BN rows of Q: warp 0 issues the TMA
+// loads (128-byte rows, one block of k per stage), warp 1 the MMAs, warps
+// 2-9 are the epilogue, each with a quarter of the rows (the TMEM lanes it
+// can reach) and half of the columns.  P is a and Q is b, or the other way
+// round where a has few rows: the MMA is always 128 rows tall, so the weight
+// takes those and the tokens become a narrow N.
+//
+// With few tiles the blocks of k are shared by a cluster of CTAs; their
+// partial sums meet in distributed shared memory and every CTA adds up and
+// writes a share of the columns, in the order of the ranks.
+//
+// Every wait is bounded: one that runs out records kFaultProduct, the CTA
+// lets its copies and MMAs land, frees its TMEM and returns.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "block_common.cuh"
+#include "common.cuh"
+#include "tc_shared.cuh"
+
+namespace hx {
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace umma;
+
+constexpr int kRows = 128;                 // of P in a tile
+constexpr int kBk = HELIX_GROUP;           // bytes of k in a stage: one scale block
+constexpr int kEpiWarps = 8;
+constexpr int kMmThreads = 32 * (2 + kEpiWarps);
+
+template <int BN>
+struct Mm8Cfg {
+    static constexpr int kStageBytes = (kRows + BN) * kBk;
+    static constexpr int kStages = BN == 128 ? 3 : BN == 64 ? 4 : BN == 32 ? 5 : 6;  // two CTAs per SM
+    static constexpr int kBufs = BN >= 128 ? 2 : 4;          // TMEM accumulators
+    static constexpr int kCols = kBufs * BN < 32 ? 32 : kBufs * BN;
+    static constexpr int kRun = BN / 2;                      // columns of an epilogue thread
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
+};
+
+struct Mm8Maps {
+    CUtensorMap p, q;
+};
+
+// The first n of v: consecutive columns qc.. of row pr of P.
+template <typename T>
+__device__ __forceinline__ void st_out(const Mm8Params& a, int pr, int qc, int n, const float (&v)[8]) {
+    if (pr >= a.p.rows) return;
+    if (a.swap) {  // out[q][p]: lanes hold consecutive p
+        T* o = static_cast<T*>(a.out) + (int64_t)qc * a.ld_out + pr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n && qc + i < a.q.rows) o[(int64_t)i * a.ld_out] = from_f32<T>(v[i]);
+        return;
+    }
+    T* o = static_cast<T*>(a.out) + (int64_t)pr * a.ld_out + qc;
+    if (n == 8 && a.vec_out && qc + 8 <= a.q.rows) {
+        st8(o, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n && qc + i < a.q.rows) o[i] = from_f32<T>(v[i]);
+}
+
+template <int BN, bool QROWS, typename T>
+__global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constant__ Mm8Maps maps, const Mm8Params a) {
+    using Cfg = Mm8Cfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = tc::align1024(smem_raw);
+    __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ float col_scale[2][QROWS ? BN : 1];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x % (unsigned)a.splits), tile = (int)(blockIdx.x / (unsigned)a.splits);
+    const int p0 = tile / a.tiles_q * kRows, q0 = tile % a.tiles_q * BN;
+    const int kb0 = (int)((int64_t)a.k_blocks * rank / a.splits);
+    const int nkb = (int)((int64_t)a.k_blocks * (rank + 1) / a.splits) - kb0;
+
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&maps.p);
+        prefetch_tmap(&maps.q);
+#pragma unroll
+        for (int i = 0; i < Cfg::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+#pragma unroll
+        for (int i = 0; i < Cfg::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps);
+        mbar_init(&drain, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(&tmem_slot, Cfg::kCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    auto wait = [&](uint64_t* bar, int phase) {
+        if (mbar_wait(bar, (uint32_t)(phase & 1), tc::kWaitBudget)) return true;
+        if (a.fault) atomicCAS(a.fault, 0u, (unsigned)kFaultProduct);
+        return false;
+    };
+
+    float acc[Cfg::kRun];
+#pragma unroll
+    for (int i = 0; i < Cfg::kRun; ++i) acc[i] = 0.0f;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int i = 0;
+            for (; i < nkb; ++i) {
+                const int s = i % Cfg::kStages, turn = i / Cfg::kStages;
+                if (turn > 0 && !wait(&empty[s], turn - 1)) break;
+                uint8_t* st = smem + s * Cfg::kStageBytes;
+                mbar_expect_tx(&full[s], Cfg::kStageBytes);
+                tma_load_2d(st, &maps.p, &full[s], (kb0 + i) * kBk, p0);
+                tma_load_2d(st + kRows * kBk, &maps.q, &full[s], (kb0 + i) * kBk, q0);
+            }
+            // whatever the other warps do, the loads issued land before the CTA ends
+            for (int j = i > Cfg::kStages ? i - Cfg::kStages : 0; j < i; ++j)
+                mbar_wait(&full[j % Cfg::kStages], (uint32_t)((j / Cfg::kStages) & 1), tc::kWaitBudget);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(kRows, BN);
+            const uint32_t base = smem_u32(smem);
+            int i = 0;
+            for (; i < nkb; ++i) {
+                const int s = i % Cfg::kStages, b = i % Cfg::kBufs;
+                if (i >= Cfg::kBufs && !wait(&acc_empty[b], i / Cfg::kBufs - 1)) break;
+                if (!wait(&full[s], i / Cfg::kStages)) break;
+                tc_fence_after();
+                const uint64_t dp = sdesc_sw128(base + s * Cfg::kStageBytes, 16, 1024);
+                const uint64_t dq = sdesc_sw128(base + s * Cfg::kStageBytes + kRows * kBk, 16, 1024);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    mma_e4m3(tmem + b * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
+                mma_commit(&empty[s]);
+                mma_commit(&acc_full[b]);
+            }
+            if (i < nkb) {
+                mma_commit(&drain);
+                mbar_wait(&drain, 0, tc::kWaitBudget);
+            }
+        }
+    } else {
+        const int half = (warp - 2) / 4;
+        const int row = 32 * (warp & 3) + lane;                   // the TMEM lane
+        const int c0 = half * Cfg::kRun;                          // the thread's first column
+        const int tid = threadIdx.x - 64;                         // 0 .. 255
+        const int pr = min(p0 + row, a.p.rows - 1);
+        const float* ps = a.p.scale + (int64_t)(pr / a.p.per) * a.p.ld_scale + kb0;
+        // QROWS: thread tid < BN stages column tid's scale; else one scale for the tile
+        const int qr = min(q0 + (QROWS ? tid : 0), a.q.rows - 1);
+        const float* qs = a.q.scale + (int64_t)(qr / a.q.per) * a.q.ld_scale + kb0;
+        const bool stage = QROWS && tid < BN;
+        float ps_next = nkb > 0 ? __ldg(ps) : 0.0f;
+        float qs_next = nkb > 0 && (stage || !QROWS) ? __ldg(qs) : 0.0f;
+        if constexpr (QROWS) {
+            if (stage) col_scale[0][tid] = qs_next;
+            named_sync(1, 32 * kEpiWarps);
+        }
+        bool alive = true;  // once a wait has run out the warp only keeps its turns at the barrier
+        for (int i = 0; i < nkb; ++i) {
+            const int b = i % Cfg::kBufs;
+            const float r = QROWS ? ps_next : ps_next * qs_next;
+            if (i + 1 < nkb) {
+                ps_next = __ldg(ps + i + 1);
+                if (stage || !QROWS) qs_next = __ldg(qs + i + 1);
+            }
+            if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[b], i / Cfg::kBufs));
+            if (alive) {
+                tc_fence_after();
+                const uint32_t t = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(b * BN + c0);
+                constexpr int kStep = Cfg::kRun < 16 ? 8 : 16;
+#pragma unroll
+                for (int c = 0; c < Cfg::kRun; c += kStep) {
+                    float v[kStep];
+                    if constexpr (kStep == 8)
+                        tmem_ld8(t + c, v);
+                    else
+                        tmem_ld16(t + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < kStep; ++e)
+                        acc[c + e] += v[e] * (QROWS ? r * col_scale[i & 1][c0 + c + e] : r);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[b]);
+            }
+            if constexpr (QROWS) {
+                if (stage) col_scale[(i + 1) & 1][tid] = qs_next;
+                named_sync(1, 32 * kEpiWarps);
+            }
+        }
+        if (a.splits == 1) {
+#pragma unroll
+            for (int c = 0; c < Cfg::kRun; c += 8) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = acc[c + e];
+                st_out<T>(a, p0 + row, q0 + c0 + c, 8, v);
+            }
+        }
+    }
+
+    if (a.splits > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        // every MMA of this CTA has retired, so the stages are free
+        __syncthreads();
+        float* part = reinterpret_cast<float*>(smem);  // [BN][128]
+        if (warp >= 2) {
+            const int row = 32 * (warp & 3) + lane, c0 = (warp - 2) / 4 * Cfg::kRun;
+#pragma unroll
+            for (int c = 0; c < Cfg::kRun; ++c) part[(c0 + c) * kRows + row] = acc[c];
+        }
+        cluster.sync();
+        if (warp >= 2) {
+            const int row = 32 * (warp & 3) + lane;
+            const int run = Cfg::kRun / a.splits;  // columns of this thread's share
+            const int c0 = rank * (BN / a.splits) + (warp - 2) / 4 * run;
+            for (int c = 0; c < run; c += 8) {
+                const int n = min(8, run - c);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+                for (int k = 0; k < a.splits; ++k) {
+                    const float* other = cluster.map_shared_rank(part, k);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < n) v[e] += other[(c0 + c + e) * kRows + row];
+                }
+                st_out<T>(a, p0 + row, q0 + c0 + c, n, v);
+            }
+        }
+        cluster.sync();  // a peer may still be reading this CTA's share
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_relinquish();
+        tmem_dealloc(tmem, Cfg::kCols);
+    }
+}
+
+template <int BN, bool QROWS, typename T>
+int launch_mm8_t(const Mm8Maps& maps, const Mm8Params& p, int tiles, void* stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles * p.splits));
+    cfg.blockDim = dim3(kMmThreads);
+    cfg.dynamicSmemBytes = Mm8Cfg<BN>::kSmem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)p.splits;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, mm8_kernel<BN, QROWS, T>, maps, p);
+}
+
+template <int BN>
+int launch_mm8_n(bool qrows, helix_dtype out, const Mm8Maps& maps, const Mm8Params& p, int tiles, void* stream) {
+    if (out == HELIX_F32)
+        return qrows ? launch_mm8_t<BN, true, float>(maps, p, tiles, stream)
+                     : launch_mm8_t<BN, false, float>(maps, p, tiles, stream);
+    return qrows ? launch_mm8_t<BN, true, __nv_bfloat16>(maps, p, tiles, stream)
+                 : launch_mm8_t<BN, false, __nv_bfloat16>(maps, p, tiles, stream);
+}
+
+template <int BN>
+int configure_mm8_n() {
+    const void* k[] = {(const void*)mm8_kernel<BN, true, float>, (const void*)mm8_kernel<BN, false, float>,
+                       (const void*)mm8_kernel<BN, true, __nv_bfloat16>,
+                       (const void*)mm8_kernel<BN, false, __nv_bfloat16>};
+    for (const void* f : k) {
+        const int e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Mm8Cfg<BN>::kSmem);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+// rows x k bytes in boxes of box_rows x 128, swizzled; zeros past the ends.
+bool make_map_u8(const helix_ctx* ctx, CUtensorMap* m, const void* base, int64_t rows, int64_t k, int64_t ld,
+                 int box_rows) {
+    const auto fn = reinterpret_cast<tc::EncodeFn>(ctx->encode_tiled);
+    if (rows == 1) ld = (k + 15) / 16 * 16;  // unused, but it has to be valid
+    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {(cuuint32_t)kBk, (cuuint32_t)box_rows};
+    cuuint32_t es[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int tiles_of(int rows, int per) { return (rows + per - 1) / per; }
+
+}  // namespace
+
+int configure_mm8() {
+    int e;
+    if ((e = configure_mm8_n<16>()) != cudaSuccess) return e;
+    if ((e = configure_mm8_n<32>()) != cudaSuccess) return e;
+    if ((e = configure_mm8_n<64>()) != cudaSuccess) return e;
+    return configure_mm8_n<128>();
+}
+
+Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
+    Mm8Plan pl{};
+    pl.swap = d.m <= 64;
+    pl.bn = !pl.swap ? 128 : d.m <= 16 ? 16 : d.m <= 32 ? 32 : 64;
+    const int64_t tiles = (int64_t)tiles_of(pl.swap ? d.n : d.m, kRows) * tiles_of(pl.swap ? d.m : d.n, pl.bn);
+    const int kb = tiles_of(d.k, kBk);
+    pl.splits = 1;
+    while (pl.splits < 8 && tiles * pl.splits * 2 <= 2 * ctx->n_sm && kb >= 4 * pl.splits) pl.splits *= 2;
+    return pl;
+}
+
+int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan& pl, Mm8Params p, const void* a,
+               const void* b, void* stream) {
+    Mm8Maps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    const bool ok = pl.swap ? make_map_u8(ctx, &maps.p, b, d.n, d.k, d.ld_b, kRows) &&
+                                  make_map_u8(ctx, &maps.q, a, d.m, d.k, d.ld_a, pl.bn)
+                            : make_map_u8(ctx, &maps.p, a, d.m, d.k, d.ld_a, kRows) &&
+                                  make_map_u8(ctx, &maps.q, b, d.n, d.k, d.ld_b, pl.bn);
+    if (!ok) return cudaErrorInvalidValue;
+    p.tiles_q = tiles_of(p.q.rows, pl.bn);
+    const int64_t tiles = (int64_t)tiles_of(p.p.rows, kRows) * p.tiles_q;
+    if (tiles * p.splits > INT32_MAX) return cudaErrorInvalidValue;
+    const bool qrows = p.q.per == 1;
+    switch (pl.bn) {
+        case 16: return launch_mm8_n<16>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
+        case 32: return launch_mm8_n<32>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
+        case 64: return launch_mm8_n<64>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
+        default: return launch_mm8_n<128>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
+    }
+}
+
+}  // namespace hx

@@ -304,3 +304,64 @@ extern "C" helix_status helix_quant8_encode(helix_ctx* ctx, void* stream, const 
         return hx::launch_quant(*d, p, whole(m[0], 16) && whole(m[1], 8), stream);
     });
 }
+
+// ---------------------------------------------------------------------------
+// Product
+// ---------------------------------------------------------------------------
+extern "C" void helix_matmul8_desc_init(helix_matmul8_desc* d, int32_t m, int32_t n, int32_t k,
+                                        helix_scale_form b_form) {
+    if (!d) return;
+    *d = helix_matmul8_desc{};
+    d->m = m, d->n = n, d->k = k;
+    d->b_form = b_form;
+    d->out_dtype = HELIX_BF16;
+    d->ld_a = d->ld_b = ((int64_t)k + 15) / 16 * 16;
+    d->ld_out = n;
+    d->ld_a_scale = d->ld_b_scale = ((int64_t)k + HELIX_GROUP - 1) / HELIX_GROUP;
+}
+
+extern "C" helix_status helix_matmul8_encode(helix_ctx* ctx, void* stream, const helix_matmul8_desc* d,
+                                             helix_tensor a, helix_tensor a_scale, helix_tensor b,
+                                             helix_tensor b_scale, helix_tensor out) {
+    return entry(ctx, d, [&]() -> int {
+        if (d->m < 0 || d->n < 0 || d->k < 1) unsupported("m and n must be >= 0 and k >= 1");
+        if (d->b_form != HELIX_SCALE_ROWS && d->b_form != HELIX_SCALE_BLOCKS) unsupported("unknown scale form");
+        if (!io(d->out_dtype)) unsupported("out_dtype must be F32 or BF16");
+        // the kernel's coordinates are 32-bit, and reach a tile past the end
+        if (d->m > INT_MAX - 512 || d->n > INT_MAX - 512 || d->k > INT_MAX - 512)
+            unsupported("m, n and k must be at most 2^31 - 513");
+        if (d->m == 0 || d->n == 0) return cudaSuccess;
+        if (!ctx->encode_tiled) unsupported("tensor maps are unavailable on this device");
+        need(a, "a");
+        need(a_scale, "a_scale");
+        need(b, "b");
+        need(b_scale, "b_scale");
+        need(out, "out");
+        const int64_t kb = ((int64_t)d->k + HELIX_GROUP - 1) / HELIX_GROUP;
+        const bool blocks = d->b_form == HELIX_SCALE_BLOCKS;
+        const int64_t nb = blocks ? ((int64_t)d->n + HELIX_GROUP - 1) / HELIX_GROUP : d->n;
+        const Mat m[] = {{"a", a, d->m, d->k, d->ld_a, 1, false},
+                         {"a_scale", a_scale, d->m, kb, d->ld_a_scale, 4, false},
+                         {"b", b, d->n, d->k, d->ld_b, 1, false},
+                         {"b_scale", b_scale, nb, kb, d->ld_b_scale, 4, false},
+                         {"out", out, d->m, d->n, d->ld_out, elem(d->out_dtype), true}};
+        check_mats(m, kNoneInPlace);
+        if (!whole(m[0], 16) || !whole(m[2], 16)) unsupported("a and b need 16-byte aligned rows");
+        if (d->m > 1 && d->ld_a < d->k) invalid("a: row stride too small");
+        if (d->n > 1 && d->ld_b < d->k) invalid("b: row stride too small");
+        const hx::Mm8Plan pl = hx::mm8_plan(ctx, *d);
+        hx::Mm8Params p{};
+        const hx::Mm8Operand oa{ptr<float>(a_scale), d->ld_a_scale, d->m, 1};
+        const hx::Mm8Operand ob{ptr<float>(b_scale), d->ld_b_scale, d->n, blocks ? HELIX_GROUP : 1};
+        p.p = pl.swap ? ob : oa;
+        p.q = pl.swap ? oa : ob;
+        p.k_blocks = (int32_t)kb;
+        p.splits = pl.splits;
+        p.swap = pl.swap;
+        p.ld_out = d->ld_out;
+        p.out = ptr(out);
+        p.vec_out = whole(m[4], 16);
+        p.fault = ctx->fault_word;
+        return hx::launch_mm8(ctx, *d, pl, p, ptr(a), ptr(b), stream);
+    });
+}

@@ -51,6 +51,35 @@ struct QuantParams {
     float*      scale;
 };
 
+// One operand of the product as the kernel sees it.  P gives the rows of a
+// tile (the MMA's M, 128 of them), Q its columns.
+struct Mm8Operand {
+    const float* scale;
+    int64_t      ld_scale;
+    int32_t      rows;
+    int32_t      per;      // rows under one scale: 1 or 128
+};
+// How one product runs.
+struct Mm8Plan {
+    bool swap;             // P is b (few rows of a: they become the columns)
+    int  bn;               // columns of a tile
+    int  splits;           // CTAs of a cluster that share a tile's blocks of k
+};
+struct Mm8Params {
+    Mm8Operand p, q;
+    int32_t    k_blocks, splits, tiles_q;
+    int32_t    vec_out;    // rows of out can be written in 16-byte pieces
+    int32_t    swap;
+    int64_t    ld_out;
+    void*      out;
+    unsigned*  fault;
+};
+Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d);
+int configure_mm8();
+// a, b: operands as the caller laid them out.
+int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan& pl, Mm8Params p, const void* a,
+               const void* b, void* stream);
+
 // Kernel launchers (kernels/block_*.cu): cudaSuccess or the launch error.
 // `vec`: every tensor allows whole 16-byte accesses at 8-column boundaries.
 int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream);

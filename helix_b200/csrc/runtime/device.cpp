@@ -9,6 +9,7 @@
 #include <mutex>
 #include <string>
 
+#include "block_internal.h"
 #include "helix/helix_ext.h"
 #include "internal.h"
 
@@ -98,8 +99,9 @@ extern "C" helix_status helix_ctx_create(helix_ctx** out, void* device, const ch
 
     {
         DeviceGuard g(dev);
-        if (hx::configure_simt(ctx) != cudaSuccess || hx::configure_diag(ctx) != cudaSuccess) {
-            hx::set_error(nullptr, std::string("configuring fp32 kernels failed: ") +
+        if (hx::configure_simt(ctx) != cudaSuccess || hx::configure_diag(ctx) != cudaSuccess ||
+            hx::configure_mm8() != cudaSuccess) {
+            hx::set_error(nullptr, std::string("configuring kernels failed: ") +
                                        cudaGetErrorString(cudaGetLastError()));
             delete ctx;
             return HELIX_ERR_PIPELINE;

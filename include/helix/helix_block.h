@@ -110,6 +110,39 @@ void         helix_quant8_desc_init(helix_quant8_desc* d, int64_t n_row, int64_t
 helix_status helix_quant8_encode(helix_ctx* ctx, void* stream, const helix_quant8_desc* d,
                                  helix_tensor x, helix_tensor q, helix_tensor scale);
 
+/* ------------------------------------------------------------------------ */
+/* Product of 8-bit matrices                                                */
+/* ------------------------------------------------------------------------ */
+
+/* out[i][j] = sum over blocks of 128 columns b of
+ *     a_scale[i][b] b_scale[j or j / 128][b] sum_{k in b} a[i][k] b[j][k]
+ * a [m][k] has its scales by rows (what the norm and the quantiser write),
+ * b [n][k] by blocks (a weight) or by rows.  Products and their sum over a
+ * block are exact to fp32 on the tensor cores, blocks are scaled and summed
+ * in fp32 in an order that depends on the sizes and the device alone, and
+ * out is rounded once.
+ *
+ * The gradients are two more such products: of a, the gradient of out (by
+ * rows) with b transposed (blocks); of b, the gradient of out and a, both
+ * transposed, by rows.  helix_quant8_encode lays all of them out.
+ *
+ * a and b are read in tiles: their bases must be 16-byte aligned and their
+ * row strides multiples of 16 (HELIX_ERR_UNSUPPORTED_SHAPE otherwise). */
+typedef struct {
+    int32_t          m, n, k;
+    helix_scale_form b_form;
+    helix_dtype      out_dtype;  /* F32 or BF16                                 */
+    int64_t          ld_a, ld_b, ld_out;
+    int64_t          ld_a_scale, ld_b_scale;
+} helix_matmul8_desc;
+
+/* Dense strides except ld_a and ld_b, which are rounded up to 16; BF16 out. */
+void         helix_matmul8_desc_init(helix_matmul8_desc* d, int32_t m, int32_t n, int32_t k,
+                                     helix_scale_form b_form);
+helix_status helix_matmul8_encode(helix_ctx* ctx, void* stream, const helix_matmul8_desc* d,
+                                  helix_tensor a, helix_tensor a_scale, helix_tensor b,
+                                  helix_tensor b_scale, helix_tensor out);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
