@@ -15,7 +15,8 @@ from typing import Optional
 from . import abi
 
 __all__ = ["HelixError", "Context", "desc_from_tensors", "scan", "shard_state", "scan_shard", "carry_combine",
-           "rms_norm", "rms_norm_grad", "quantize8", "matmul8", "abi"]
+           "rms_norm", "rms_norm_grad", "quantize8", "matmul8",
+           "gated_scan", "gated_scan_grad", "abi"]
 
 
 class HelixError(RuntimeError):
@@ -261,7 +262,7 @@ def carry_combine(s0, states, log_decays, ids=None, *, ctx: Optional[Context] = 
 
 
 # block.py needs torch at import; the rest of the package does not.
-_BLOCK = ("rms_norm", "rms_norm_grad", "quantize8", "matmul8")
+_BLOCK = ("rms_norm", "rms_norm_grad", "quantize8", "matmul8", "gated_scan", "gated_scan_grad")
 
 
 def __getattr__(name):

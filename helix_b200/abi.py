@@ -31,6 +31,7 @@ HELIX_BACKEND_AUTO, HELIX_BACKEND_SGMMA, HELIX_BACKEND_MPP, HELIX_BACKEND_REF = 
 # include/helix/helix_block.h: values that share a scale; helix_scale_form
 HELIX_GROUP = 128
 HELIX_SCALE_ROWS, HELIX_SCALE_BLOCKS = 0, 1
+HELIX_GATED_CHUNK = 128
 
 I32, I64 = C.c_int32, C.c_int64
 
@@ -75,6 +76,8 @@ EXPORTS = (
     "helix_rms_norm_desc_init", "helix_rms_norm_encode", "helix_rms_norm_grad_scratch_size",
     "helix_rms_norm_grad_encode", "helix_quant8_desc_init", "helix_quant8_encode",
     "helix_matmul8_desc_init", "helix_matmul8_encode",
+    "helix_gated_scan_desc_init", "helix_gated_scan_states_size", "helix_gated_scan_encode",
+    "helix_gated_scan_grad_encode",
 )
 
 
@@ -96,6 +99,13 @@ class Matmul8Desc(C.Structure):
     """helix_matmul8_desc (include/helix/helix_block.h)."""
     _fields_ = [("m", I32), ("n", I32), ("k", I32), ("b_form", C.c_int), ("out_dtype", C.c_int), ("ld_a", I64),
                 ("ld_b", I64), ("ld_out", I64), ("ld_a_scale", I64), ("ld_b_scale", I64)]
+
+
+class GatedScanDesc(C.Structure):
+    """helix_gated_scan_desc (include/helix/helix_block.h)."""
+    _fields_ = [("n_tok", I32), ("n_seq", I32), ("n_chan", I32), ("io_dtype", C.c_int)] + [
+        (n, I64) for n in ("s_v", "s_g", "s_y", "s_dy", "s_dv", "s_dg", "seq_v", "seq_g", "seq_y", "seq_dy",
+                           "seq_dv", "seq_dg", "seq_h0", "seq_h1", "seq_dh1", "seq_dh0")]
 
 
 class PlanInfo(C.Structure):
@@ -169,6 +179,14 @@ def load(path: Path | str | None = None) -> C.CDLL:
     lib.helix_matmul8_desc_init.restype = None
     lib.helix_matmul8_encode.argtypes = [C.c_void_p, C.c_void_p, P(Matmul8Desc)] + [Tensor] * 5
     lib.helix_matmul8_encode.restype = C.c_int
+    lib.helix_gated_scan_desc_init.argtypes = [P(GatedScanDesc), I32, I32, I32]
+    lib.helix_gated_scan_desc_init.restype = None
+    lib.helix_gated_scan_states_size.argtypes = [P(GatedScanDesc)]
+    lib.helix_gated_scan_states_size.restype = C.c_size_t
+    lib.helix_gated_scan_encode.argtypes = [C.c_void_p, C.c_void_p, P(GatedScanDesc)] + [Tensor] * 7
+    lib.helix_gated_scan_encode.restype = C.c_int
+    lib.helix_gated_scan_grad_encode.argtypes = [C.c_void_p, C.c_void_p, P(GatedScanDesc)] + [Tensor] * 9
+    lib.helix_gated_scan_grad_encode.restype = C.c_int
     if path is None:
         _lib = lib
     return lib

@@ -255,3 +255,97 @@ def matmul8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     call.done(call.ctx.lib.helix_matmul8_encode(call.ctx.handle, call.handle, C.byref(d), _t(a), _t(a_scale), _t(b),
                                                 _t(b_scale), _t(out)))
     return out
+
+
+def _tokens(name: str, t: torch.Tensor, shape, dtype) -> tuple[int, int]:
+    """(token stride, sequence stride) of a (sequences, tokens, channels) tensor."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}")
+    s, k, c = t.stride()
+    if shape[2] > 1 and c != 1:
+        raise ValueError(f"{name} needs unit stride along the channels")
+    return k, s
+
+
+def _state(name: str, t: torch.Tensor, shape) -> int:
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be torch.float32")
+    return _matrix(name, t, shape)
+
+
+def _lengths(t: Optional[torch.Tensor], seqs: int) -> None:
+    if t is not None:
+        _vector("lengths", t, seqs, torch.int32)
+
+
+def gated_scan(v: torch.Tensor, g: torch.Tensor, h0: Optional[torch.Tensor] = None, *,
+               lengths: Optional[torch.Tensor] = None, h1: Optional[torch.Tensor] = None, keep_states: bool = False,
+               ctx: Optional[Context] = None, stream=None):
+    """h_t = f_t h_{t-1} + (1 - f_t) v_t with f = sigmoid(g), per channel:
+    (y, h1), or (y, h1, states) with keep_states (for gated_scan_grad).
+
+    v and g are (sequences, tokens, channels) and may be slices of one wider
+    tensor; h0 (sequences, channels) f32 is the state before the first token
+    (zeros without), h1 the one after the last, written into the tensor given
+    (h0 itself for a step in place) or a new one.  lengths (int32, one per
+    sequence) ends sequences early: later tokens keep the state and have y 0."""
+    if v.dim() != 3:
+        raise ValueError("v must be (sequences, tokens, channels)")
+    d = abi.GatedScanDesc()
+    d.n_seq, d.n_tok, d.n_chan = seqs, toks, chans = v.shape
+    d.io_dtype = _dtype("v", v)
+    d.s_v, d.seq_v = _tokens("v", v, v.shape, v.dtype)
+    d.s_g, d.seq_g = _tokens("g", g, v.shape, v.dtype)
+    _lengths(lengths, seqs)
+    if h0 is not None:
+        d.seq_h0 = _state("h0", h0, (seqs, chans))
+    call = _Call(v, ctx, stream, g, h0, lengths, h1)
+    with call.alloc():
+        y = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        if h1 is None:
+            h1 = torch.empty((seqs, chans), dtype=torch.float32, device=v.device)
+        states = None
+        if keep_states:
+            states = torch.empty((seqs, -(-toks // abi.HELIX_GATED_CHUNK), chans), dtype=torch.float32, device=v.device)
+    d.s_y, d.seq_y = chans, toks * chans
+    d.seq_h1 = _state("h1", h1, (seqs, chans))
+    call.done(call.ctx.lib.helix_gated_scan_encode(call.ctx.handle, call.handle, C.byref(d), _t(v), _t(g), _t(h0),
+                                                   _t(lengths), _t(y), _t(h1), _t(states)))
+    return (y, h1, states) if keep_states else (y, h1)
+
+
+def gated_scan_grad(dy: torch.Tensor, v: torch.Tensor, g: torch.Tensor, states: torch.Tensor,
+                    dh1: Optional[torch.Tensor] = None, *, lengths: Optional[torch.Tensor] = None,
+                    dv: Optional[torch.Tensor] = None, dg: Optional[torch.Tensor] = None,
+                    ctx: Optional[Context] = None, stream=None):
+    """Gradient of gated_scan: (dv, dg, dh0) from the gradients of y and of h1
+    (zeros without), with the states the forward pass kept.  dv and dg are
+    written into the tensors given (slices of one wider tensor, say) or new ones."""
+    if v.dim() != 3:
+        raise ValueError("v must be (sequences, tokens, channels)")
+    d = abi.GatedScanDesc()
+    d.n_seq, d.n_tok, d.n_chan = seqs, toks, chans = v.shape
+    d.io_dtype = _dtype("v", v)
+    d.s_v, d.seq_v = _tokens("v", v, v.shape, v.dtype)
+    d.s_g, d.seq_g = _tokens("g", g, v.shape, v.dtype)
+    d.s_dy, d.seq_dy = _tokens("dy", dy, v.shape, v.dtype)
+    if (states.dtype != torch.float32 or not states.is_contiguous()
+            or tuple(states.shape) != (seqs, -(-toks // abi.HELIX_GATED_CHUNK), chans)):
+        raise ValueError("states must be what gated_scan(keep_states=True) gave")
+    _lengths(lengths, seqs)
+    if dh1 is not None:
+        d.seq_dh1 = _state("dh1", dh1, (seqs, chans))
+    call = _Call(dy, ctx, stream, v, g, states, dh1, lengths, dv, dg)
+    with call.alloc():
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
+        dg = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dg is None else dg
+        dh0 = torch.empty((seqs, chans), dtype=torch.float32, device=v.device)
+    d.s_dv, d.seq_dv = _tokens("dv", dv, v.shape, v.dtype)
+    d.s_dg, d.seq_dg = _tokens("dg", dg, v.shape, v.dtype)
+    d.seq_dh0 = chans
+    call.done(call.ctx.lib.helix_gated_scan_grad_encode(
+        call.ctx.handle, call.handle, C.byref(d), _t(dy), _t(v), _t(g), _t(states), _t(dh1), _t(lengths), _t(dv),
+        _t(dg), _t(dh0)))
+    return dv, dg, dh0

@@ -365,3 +365,174 @@ extern "C" helix_status helix_matmul8_encode(helix_ctx* ctx, void* stream, const
         return hx::launch_mm8(ctx, *d, pl, p, ptr(a), ptr(b), stream);
     });
 }
+
+// ---------------------------------------------------------------------------
+// Gated linear recurrence
+// ---------------------------------------------------------------------------
+namespace {
+
+// A token tensor [n_seq][n_tok][n_chan].
+struct Tok {
+    const char*  name;
+    helix_tensor t;
+    int64_t      s_tok, s_seq;
+    bool         written;
+};
+
+void check_tok(const helix_gated_scan_desc& d, const Tok& x) {
+    const std::string n = x.name;
+    if (addr(x.t) % (uintptr_t)elem(d.io_dtype)) invalid(n + " is not aligned to its elements");
+    if (x.s_tok < 0 || x.s_seq < 0) invalid(n + ": negative stride");
+    if (x.written) {
+        // distinct elements have distinct addresses: the token rows do not
+        // overlap within a sequence, nor the sequences (or they interleave)
+        const bool rows = d.n_tok <= 1 || x.s_tok >= d.n_chan;
+        const int64_t span = (int64_t)(d.n_tok - 1) * x.s_tok + d.n_chan;
+        const bool seqs = d.n_seq <= 1 || x.s_seq >= span ||
+                          (x.s_seq >= d.n_chan && (int64_t)(d.n_seq - 1) * x.s_seq + d.n_chan <= x.s_tok);
+        if (!rows || !seqs) invalid(n + ": strides make its elements overlap");
+    }
+    const int64_t most = INT64_MAX / 64;
+    if ((d.n_tok > 1 && x.s_tok > most / d.n_tok) || (d.n_seq > 1 && x.s_seq > most / d.n_seq))
+        invalid(n + ": reaches past 64-bit offsets");
+}
+
+// One address range per token tensor; where tokens follow one another at one
+// pitch through all sequences, a matrix with that pitch (slices of one wider
+// tensor may then lie side by side).
+Mat mat_of(const helix_gated_scan_desc& d, const Tok& x) {
+    const int64_t size = elem(d.io_dtype);
+    if (d.n_seq <= 1 || x.s_seq == (int64_t)d.n_tok * x.s_tok)
+        return {x.name, x.t, (int64_t)d.n_tok * d.n_seq, d.n_chan, x.s_tok, size, x.written};
+    if (d.n_tok <= 1) return {x.name, x.t, d.n_seq, d.n_chan, x.s_seq, size, x.written};
+    const int64_t last = (int64_t)(d.n_tok - 1) * x.s_tok + (int64_t)(d.n_seq - 1) * x.s_seq + d.n_chan;
+    return {x.name, x.t, 1, last, last, size, x.written};
+}
+bool same_tok(const helix_gated_scan_desc& d, const Tok& a, const Tok& b) {
+    return addr(a.t) == addr(b.t) && (d.n_tok <= 1 || a.s_tok == b.s_tok) && (d.n_seq <= 1 || a.s_seq == b.s_seq);
+}
+
+void check_gated_desc(const helix_gated_scan_desc& d) {
+    if (d.n_tok < 0 || d.n_seq < 0 || d.n_chan < 0) unsupported("n_tok, n_seq and n_chan must be >= 0");
+    if (!io(d.io_dtype)) unsupported("io_dtype must be F32 or BF16");
+    // chunk indexes and the grid are 32-bit
+    if (d.n_tok > INT_MAX - 4096) unsupported("n_tok must be at most 2^31 - 4097");
+    const int64_t slabs = ((int64_t)d.n_chan + 31) / 32;
+    if ((int64_t)d.n_seq * slabs > INT_MAX / 16) unsupported("problem too large for one launch");
+}
+
+// Two channels at once: 4-byte aligned rows.
+bool pairs(const helix_gated_scan_desc& d, const Tok& x) {
+    return !x.t.buf || (addr(x.t) % 4 == 0 && (d.n_tok <= 1 || x.s_tok % 2 == 0) && (d.n_seq <= 1 || x.s_seq % 2 == 0));
+}
+
+int64_t gated_chunks(const helix_gated_scan_desc& d) {
+    return ((int64_t)d.n_tok + HELIX_GATED_CHUNK - 1) / HELIX_GATED_CHUNK;
+}
+
+}  // namespace
+
+extern "C" void helix_gated_scan_desc_init(helix_gated_scan_desc* d, int32_t n_tok, int32_t n_seq, int32_t n_chan) {
+    if (!d) return;
+    *d = helix_gated_scan_desc{};
+    d->n_tok = n_tok, d->n_seq = n_seq, d->n_chan = n_chan;
+    d->io_dtype = HELIX_F32;
+    d->s_v = d->s_g = d->s_y = d->s_dy = d->s_dv = d->s_dg = n_chan;
+    d->seq_v = d->seq_g = d->seq_y = d->seq_dy = d->seq_dv = d->seq_dg = (int64_t)n_tok * n_chan;
+    d->seq_h0 = d->seq_h1 = d->seq_dh1 = d->seq_dh0 = n_chan;
+}
+
+extern "C" size_t helix_gated_scan_states_size(const helix_gated_scan_desc* d) {
+    if (!d || d->n_tok < 0 || d->n_seq < 0 || d->n_chan < 0) return 0;
+    return (size_t)d->n_seq * (size_t)gated_chunks(*d) * (size_t)d->n_chan * sizeof(float);
+}
+
+extern "C" helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, const helix_gated_scan_desc* d,
+                                                helix_tensor v, helix_tensor g, helix_tensor h0,
+                                                helix_tensor lengths, helix_tensor y, helix_tensor h1,
+                                                helix_tensor states) {
+    return entry(ctx, d, [&]() -> int {
+        check_gated_desc(*d);
+        if (d->n_seq == 0 || d->n_chan == 0) return cudaSuccess;
+        need(h1, "h1");
+        const Tok tv{"v", v, d->s_v, d->seq_v, false}, tg{"g", g, d->s_g, d->seq_g, false},
+            ty{"y", y, d->s_y, d->seq_y, true};
+        if (d->n_tok > 0) {
+            need(v, "v");
+            need(g, "g");
+            need(y, "y");
+            for (const Tok* t : {&tv, &tg, &ty}) check_tok(*d, *t);
+        }
+        const bool any = d->n_tok > 0;
+        const int64_t ns = d->n_seq, nc = d->n_chan;
+        Mat none{"", HELIX_TENSOR_NULL, 0, 0, 0, 1, false};
+        const Mat m[] = {any ? mat_of(*d, tv) : none,
+                         any ? mat_of(*d, tg) : none,
+                         {"h0", h0, ns, nc, d->seq_h0, 4, false},
+                         {"lengths", lengths, 1, ns, ns, 4, false},
+                         any ? mat_of(*d, ty) : none,
+                         {"h1", h1, ns, nc, d->seq_h1, 4, true},
+                         {"states", states, 1, ns * gated_chunks(*d) * nc, ns * gated_chunks(*d) * nc, 4, true}};
+        const int in_place[][2] = {{5, 2}};
+        check_mats(m, in_place);
+        hx::GatedParams p{};
+        p.n_tok = d->n_tok, p.n_seq = d->n_seq, p.n_chan = d->n_chan;
+        p.n_chunk = (int32_t)gated_chunks(*d);
+        p.s_v = d->s_v, p.s_g = d->s_g, p.s_y = d->s_y;
+        p.seq_v = d->seq_v, p.seq_g = d->seq_g, p.seq_y = d->seq_y;
+        p.seq_h0 = d->seq_h0, p.seq_h1 = d->seq_h1;
+        p.v = ptr(v), p.g = ptr(g), p.y = ptr(y);
+        p.h0 = ptr<float>(h0), p.h1 = ptr<float>(h1), p.states = ptr<float>(states);
+        p.lengths = ptr<int32_t>(lengths);
+        return hx::launch_gated(ctx, *d, p, pairs(*d, tv) && pairs(*d, tg) && pairs(*d, ty), stream);
+    });
+}
+
+extern "C" helix_status helix_gated_scan_grad_encode(helix_ctx* ctx, void* stream, const helix_gated_scan_desc* d,
+                                                     helix_tensor dy, helix_tensor v, helix_tensor g,
+                                                     helix_tensor states, helix_tensor dh1, helix_tensor lengths,
+                                                     helix_tensor dv, helix_tensor dg, helix_tensor dh0) {
+    return entry(ctx, d, [&]() -> int {
+        check_gated_desc(*d);
+        if (d->n_seq == 0 || d->n_chan == 0) return cudaSuccess;
+        const Tok tdy{"dy", dy, d->s_dy, d->seq_dy, false}, tv{"v", v, d->s_v, d->seq_v, false},
+            tg{"g", g, d->s_g, d->seq_g, false}, tdv{"dv", dv, d->s_dv, d->seq_dv, true},
+            tdg{"dg", dg, d->s_dg, d->seq_dg, true};
+        const bool any = d->n_tok > 0;
+        if (any) {
+            need(dy, "dy");
+            need(v, "v");
+            need(g, "g");
+            need(states, "states");
+            need(dv, "dv");
+            need(dg, "dg");
+            for (const Tok* t : {&tdy, &tv, &tg, &tdv, &tdg}) check_tok(*d, *t);
+        }
+        const int64_t ns = d->n_seq, nc = d->n_chan;
+        Mat none{"", HELIX_TENSOR_NULL, 0, 0, 0, 1, false};
+        const Mat m[] = {any ? mat_of(*d, tdy) : none,
+                         any ? mat_of(*d, tv) : none,
+                         any ? mat_of(*d, tg) : none,
+                         {"states", states, 1, ns * gated_chunks(*d) * nc, ns * gated_chunks(*d) * nc, 4, false},
+                         {"dh1", dh1, ns, nc, d->seq_dh1, 4, false},
+                         {"lengths", lengths, 1, ns, ns, 4, false},
+                         any ? mat_of(*d, tdv) : none,
+                         any ? mat_of(*d, tdg) : none,
+                         {"dh0", dh0, ns, nc, d->seq_dh0, 4, true}};
+        const int dv_on_dy = any && same_tok(*d, tdv, tdy) ? 6 : -1;
+        const int in_place[][2] = {{dv_on_dy, 0}, {8, 4}};
+        check_mats(m, in_place);
+        hx::GatedParams p{};
+        p.n_tok = d->n_tok, p.n_seq = d->n_seq, p.n_chan = d->n_chan;
+        p.n_chunk = (int32_t)gated_chunks(*d);
+        p.s_v = d->s_v, p.s_g = d->s_g, p.s_dy = d->s_dy, p.s_dv = d->s_dv, p.s_dg = d->s_dg;
+        p.seq_v = d->seq_v, p.seq_g = d->seq_g, p.seq_dy = d->seq_dy, p.seq_dv = d->seq_dv, p.seq_dg = d->seq_dg;
+        p.seq_dh1 = d->seq_dh1, p.seq_dh0 = d->seq_dh0;
+        p.v = ptr(v), p.g = ptr(g), p.dy = ptr(dy), p.dv = ptr(dv), p.dg = ptr(dg);
+        p.dh1 = ptr<float>(dh1), p.dh0 = ptr<float>(dh0), p.states = ptr<float>(states);
+        p.lengths = ptr<int32_t>(lengths);
+        if (!any && !dh0.buf) return cudaSuccess;
+        const bool vec = pairs(*d, tdy) && pairs(*d, tv) && pairs(*d, tg) && pairs(*d, tdv) && pairs(*d, tdg);
+        return hx::launch_gated_grad(ctx, *d, p, vec, stream);
+    });
+}

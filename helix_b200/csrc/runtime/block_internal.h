@@ -80,6 +80,23 @@ int configure_mm8();
 int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan& pl, Mm8Params p, const void* a,
                const void* b, void* stream);
 
+struct GatedParams {
+    int32_t        n_tok, n_seq, n_chan;
+    int32_t        n_chunk;    // ceil(n_tok / HELIX_GATED_CHUNK)
+    int32_t        cluster;    // CTAs that share a sequence's chunks
+    int64_t        s_v, s_g, s_y, s_dy, s_dv, s_dg;
+    int64_t        seq_v, seq_g, seq_y, seq_dy, seq_dv, seq_dg;
+    int64_t        seq_h0, seq_h1, seq_dh1, seq_dh0;
+    const void    *v, *g, *dy;
+    void          *y, *dv, *dg;
+    const float   *h0, *dh1;
+    float         *h1, *dh0, *states;
+    const int32_t* lengths;
+};
+// vec (bf16): two channels of every token tensor can be accessed at once.
+int launch_gated(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedParams p, bool vec, void* stream);
+int launch_gated_grad(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedParams p, bool vec, void* stream);
+
 // Kernel launchers (kernels/block_*.cu): cudaSuccess or the launch error.
 // `vec`: every tensor allows whole 16-byte accesses at 8-column boundaries.
 int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream);

@@ -143,6 +143,60 @@ helix_status helix_matmul8_encode(helix_ctx* ctx, void* stream, const helix_matm
                                   helix_tensor a, helix_tensor a_scale, helix_tensor b,
                                   helix_tensor b_scale, helix_tensor out);
 
+/* ------------------------------------------------------------------------ */
+/* Gated linear recurrence                                                  */
+/* ------------------------------------------------------------------------ */
+
+#define HELIX_GATED_CHUNK 128
+
+/* Per sequence and channel, with the gate f = 1 / (1 + exp(-g)) of every
+ * token and a state of its own:
+ *     h_t = f_t h_{t-1} + (1 - f_t) v_t,   y_t = h_t
+ * from h0 (zeros when null) to h1, the state after the last token.  The
+ * states are f32, the arithmetic fp32; v, g, y, dy, dv and dg are io_dtype.
+ * Token tensors are [n_seq][n_tok][n_chan] with strides of their own for the
+ * token and the sequence; states are [n_seq][n_chan].
+ *
+ * lengths (int32, [n_seq], may be null) ends sequences early: tokens at or
+ * past lengths[seq] (taken as 0 .. n_tok) leave the state as it is, whatever
+ * v, g and dy hold there, and have y = dv = dg = 0.
+ *
+ * n_tok = 1 is the step of a decoder, h1 in place of h0. */
+typedef struct {
+    int32_t     n_tok, n_seq, n_chan;
+    helix_dtype io_dtype;                    /* F32 or BF16                     */
+    int64_t     s_v, s_g, s_y;               /* token strides                   */
+    int64_t     s_dy, s_dv, s_dg;
+    int64_t     seq_v, seq_g, seq_y;         /* sequence strides                */
+    int64_t     seq_dy, seq_dv, seq_dg;
+    int64_t     seq_h0, seq_h1;
+    int64_t     seq_dh1, seq_dh0;
+} helix_gated_scan_desc;
+
+/* Dense strides, F32. */
+void helix_gated_scan_desc_init(helix_gated_scan_desc* d, int32_t n_tok, int32_t n_seq, int32_t n_chan);
+
+/* Bytes of `states`: f32 [n_seq][ceil(n_tok / HELIX_GATED_CHUNK)][n_chan],
+ * the state entering every chunk of tokens, which the gradient starts from. */
+size_t helix_gated_scan_states_size(const helix_gated_scan_desc* d);
+
+/* states may be null when no gradient follows.  h1 may be in place of h0. */
+helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, const helix_gated_scan_desc* d,
+                                     helix_tensor v, helix_tensor g, helix_tensor h0,
+                                     helix_tensor lengths, helix_tensor y, helix_tensor h1,
+                                     helix_tensor states);
+
+/* The gradient, from the forward pass's states.  dy is the gradient of y, dh1
+ * (null: zeros) of h1; dh0 may be null.  With lam_t the gradient of h_t:
+ *     lam_t = dy_t + f_{t+1} lam_{t+1},  lam_last = dy_last + dh1
+ *     dv_t = (1 - f_t) lam_t,  dg_t = lam_t (h_{t-1} - v_t) f_t (1 - f_t)
+ *     dh0 = f_0 lam_0
+ * dv may be in place of dy, dh0 in place of dh1. */
+helix_status helix_gated_scan_grad_encode(helix_ctx* ctx, void* stream, const helix_gated_scan_desc* d,
+                                          helix_tensor dy, helix_tensor v, helix_tensor g,
+                                          helix_tensor states, helix_tensor dh1, helix_tensor lengths,
+                                          helix_tensor dv, helix_tensor dg, helix_tensor dh0);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -75,3 +75,56 @@ def norm_grad(dout, s, rstd, w, dsum):
     if dsum is not None:
         ds, mag = ds + dsum, mag + dsum.abs()
     return ds, (dout * u).sum(0), mag, (dout * u).abs().sum(0)
+
+
+def gated(v, g, h0, lengths):
+    """The recurrence in fp64: (y, h1, hs with h_{-1} first, z, live, err).
+
+    err bounds what fp32 makes of h.  1 - f is off by 12 u (exponential 4,
+    sum, quotient 4, product, with slack) and 2 u |g| (the exponent's
+    rounding); a step adds that times z |v - h| and 4 roundings of magnitudes
+    up to M, M_t = f M_{t-1} + z |v| being the recurrence of the magnitudes;
+    twice, because a run's fold rounds as a step does."""
+    S, T, C = v.shape
+    live = torch.ones(S, T, 1, dtype=torch.bool)
+    if lengths is not None:
+        live = (torch.arange(T)[None] < lengths[:, None].clamp(0, T))[:, :, None]
+    z = torch.where(live, 1.0 / (1.0 + torch.exp(g)), torch.zeros(()).double())
+    v = torch.where(live, v, torch.zeros(()).double())
+    eg = torch.where(live, 12 + 2 * g.abs(), torch.zeros(()).double())
+    h = h0 if h0 is not None else torch.zeros(S, C).double()
+    m, e = h.abs(), torch.zeros(S, C).double()
+    hs, ms, es = [h], [m], [e]
+    for t in range(T):
+        e = (1 - z[:, t]) * e + 2 * U32 * (4 * m + eg[:, t] * z[:, t] * (v[:, t].abs() + m))
+        h = h + z[:, t] * (v[:, t] - h)
+        m = (1 - z[:, t]) * m + z[:, t] * v[:, t].abs()
+        hs.append(h), ms.append(m), es.append(e)
+    hs, ms, es = (torch.stack(x, 1) for x in (hs, ms, es))
+    return hs[:, 1:] * live, hs[:, -1], hs, ms, es, z, live
+
+
+def gated_grad(dy, v, g, h0, dh1, lengths):
+    """(dv, dg, dh0) in fp64 and bounds of their fp32 errors, as above."""
+    S, T, C = v.shape
+    _, _, hs, ms, es, z, live = gated(v, g, h0, lengths)
+    zero = torch.zeros(()).double()
+    dy, v = torch.where(live, dy, zero), torch.where(live, v, zero)
+    f = torch.where(live, 1.0 / (1.0 + torch.exp(-g)), torch.ones(()).double())
+    ga = torch.where(live, g.abs(), zero)
+    c = dh1 if dh1 is not None else torch.zeros(S, C).double()
+    mc, ec = c.abs(), torch.zeros(S, C).double()
+    dv, dg, bv, bg = (torch.zeros(S, T, C).double() for _ in range(4))
+    for t in range(T - 1, -1, -1):
+        lam, ml = dy[:, t] + c, dy[:, t].abs() + mc
+        el = ec + 2 * U32 * ml
+        zt, s = z[:, t], z[:, t] * f[:, t]
+        off, moff = hs[:, t] - v[:, t], ms[:, t] + v[:, t].abs()
+        dv[:, t] = zt * lam
+        bv[:, t] = zt * (el + ml * (14 + 2 * ga[:, t]) * U32)
+        dg[:, t] = lam * off * s
+        bg[:, t] = s * (el * moff + ml * es[:, t] + ml * moff * (24 + 2 * ga[:, t]) * U32)
+        c = lam * (1 - zt)
+        mc = ml * (1 - zt)
+        ec = (1 - zt) * el + 2 * U32 * ml * (2 + (12 + 2 * ga[:, t]) * zt)
+    return dv * live, dg * live, c, bv, bg, ec
