@@ -18,6 +18,7 @@ enum : unsigned {
     kFaultIdsOverlap = 5,  // an s0 row selected by ids overlaps the s1 rows written
     kFaultTestStall = 6,   // test hook HELIX_TEST_STALL_CYCLES: a wait nothing ends ran out
     kFaultProduct = 7,     // 8-bit product: a copy, MMA or hand-off wait ran out
+    kFaultGated = 8,       // gated recurrence: a copy's arrival wait ran out
 };
 
 constexpr float kNaN = __builtin_nanf("");

@@ -484,6 +484,7 @@ extern "C" helix_status helix_gated_scan_encode(helix_ctx* ctx, void* stream, co
         p.v = ptr(v), p.g = ptr(g), p.y = ptr(y);
         p.h0 = ptr<float>(h0), p.h1 = ptr<float>(h1), p.states = ptr<float>(states);
         p.lengths = ptr<int32_t>(lengths);
+        p.fault = ctx->fault_word;
         return hx::launch_gated(ctx, *d, p, pairs(*d, tv) && pairs(*d, tg) && pairs(*d, ty), stream);
     });
 }
@@ -531,6 +532,7 @@ extern "C" helix_status helix_gated_scan_grad_encode(helix_ctx* ctx, void* strea
         p.v = ptr(v), p.g = ptr(g), p.dy = ptr(dy), p.dv = ptr(dv), p.dg = ptr(dg);
         p.dh1 = ptr<float>(dh1), p.dh0 = ptr<float>(dh0), p.states = ptr<float>(states);
         p.lengths = ptr<int32_t>(lengths);
+        p.fault = ctx->fault_word;
         if (!any && !dh0.buf) return cudaSuccess;
         const bool vec = pairs(*d, tdy) && pairs(*d, tv) && pairs(*d, tg) && pairs(*d, tdv) && pairs(*d, tdg);
         return hx::launch_gated_grad(ctx, *d, p, vec, stream);

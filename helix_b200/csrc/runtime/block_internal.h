@@ -92,10 +92,12 @@ struct GatedParams {
     const float   *h0, *dh1;
     float         *h1, *dh0, *states;
     const int32_t* lengths;
+    unsigned*      fault;
 };
-// vec (bf16): two channels of every token tensor can be accessed at once.
-int launch_gated(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedParams p, bool vec, void* stream);
-int launch_gated_grad(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedParams p, bool vec, void* stream);
+int configure_gated(helix_ctx* ctx);  // fills ctx->gated_clusters
+// word (bf16): two channels of every token tensor can be accessed at once.
+int launch_gated(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedParams p, bool word, void* stream);
+int launch_gated_grad(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedParams p, bool word, void* stream);
 
 // Kernel launchers (kernels/block_*.cu): cudaSuccess or the launch error.
 // `vec`: every tensor allows whole 16-byte accesses at 8-column boundaries.

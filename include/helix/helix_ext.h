@@ -20,7 +20,7 @@ extern "C" {
  * output kernels (copy arrival; MMA or hand-off), 3, 4 the same in the state
  * kernel, 5 an s0 row selected by ids overlapped the s1 rows being written
  * (that sequence's outputs are NaN), 6 the test hook HELIX_TEST_STALL_CYCLES,
- * 7 a wait of the 8-bit product (helix_block.h).
+ * 7 a wait of the 8-bit product, 8 of the gated recurrence (helix_block.h).
  * Synchronous (it copies one word). */
 helix_status helix_device_fault(helix_ctx* ctx, uint32_t* code);
 
