@@ -12,28 +12,26 @@
 //
 // Bound by memory: every token is read once.  A CTA has 128 bytes of channels
 // (4 per lane: 2 bf16 channels, worked on as a pair, or 1 f32) of one chunk of
-// 128 tokens, a warp 8 consecutive tokens of it.  (D, B) of the warps meet in
-// shared memory, those of the CTAs of a cluster (as many consecutive chunks of
-// the same channels) in distributed shared memory; each CTA folds them onto
-// the running state and the warps walk their tokens again.  Then the cluster
-// moves on by its chunks.  The steps overlap: tiles arrive by TMA several
-// steps ahead, and the gates and (D, B) of the next step are formed between
-// arriving at the cluster's barrier and waiting for it.  Outputs overwrite
-// their inputs' tile and leave by TMA.  Tensors that TMA cannot describe take
-// the same kernel with plain loads, a lane's words one step ahead in its own
-// slots of the tile, and plain stores.  Folds go in the order of the tokens:
-// results do not depend on timing.
+// 128 tokens, a warp 16 consecutive tokens of it: one walk over them forms the
+// gates, which stay in registers, and (D, B); the warps' (D, B) meet in shared
+// memory, a CTA's totals go to the other CTAs of its cluster (as many
+// consecutive chunks of the same channels) by asynchronous stores that arrive
+// on an mbarrier, every CTA folds them onto the running state, and a second
+// walk writes the outputs.  Then the cluster moves on by its chunks.  Tiles
+// arrive by TMA, steps ahead; two CTAs per SM fill each other's waits.  Tensors
+// that TMA cannot describe take the same kernel with plain loads, a lane's
+// words one step ahead.  Folds go in the order of the tokens: results do not
+// depend on timing.
 //
 // The gradient walks the chunks from the end with c_t = f_t lam_t, the
 // gradient that leaves token t for h_{t-1}: lam_t = dy_t + c_{t+1}, c_t =
 // lam_t - z_t lam_t, so a run takes c to c - D c + E with the same D; h_{t-1}
 // is walked forward again from the chunk's stored state.
 //
-// Sequences of up to 8 tokens (a decoder's step) need none of this: a warp
+// Sequences of up to 16 tokens (a decoder's step) need none of this: a warp
 // walks its lanes' channels from global memory.
-#include <cooperative_groups.h>
-
 #include <cstring>
+#include <type_traits>
 
 #include "block_common.cuh"
 #include "common.cuh"
@@ -42,11 +40,10 @@
 namespace hx {
 namespace {
 
-namespace cg = cooperative_groups;
 using namespace umma;
 
 constexpr int kChunk = HELIX_GATED_CHUNK;
-constexpr int kTok = 8;                   // tokens of a warp
+constexpr int kTok = 16;                  // tokens of a warp
 constexpr int kWarps = kChunk / kTok;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
@@ -68,10 +65,10 @@ struct Lane<float> {
     static __device__ __forceinline__ void to(V v, float (&a)[1]) { a[0] = v; }
     static __device__ __forceinline__ V fma(V a, V b, V c) { return fmaf(a, b, c); }
     static __device__ __forceinline__ V add(V a, V b) { return a + b; }
-    static __device__ __forceinline__ V sub(V a, V b) { return a - b; }
     static __device__ __forceinline__ V mul(V a, V b) { return a * b; }
     static __device__ __forceinline__ V unpack(uint32_t w) { return __uint_as_float(w); }
     static __device__ __forceinline__ uint32_t pack(V v) { return __float_as_uint(v); }
+    static __device__ __forceinline__ uint32_t pack_neg(V v) { return __float_as_uint(-v); }
     static constexpr uint32_t kInf = 0x7f800000u;
 };
 template <>
@@ -83,7 +80,6 @@ struct Lane<__nv_bfloat16> {
     static __device__ __forceinline__ void to(V v, float (&a)[2]) { f2_to(v, a[0], a[1]); }
     static __device__ __forceinline__ V fma(V a, V b, V c) { return f2_fma(a, b, c); }
     static __device__ __forceinline__ V add(V a, V b) { return f2_add(a, b); }
-    static __device__ __forceinline__ V sub(V a, V b) { return f2_sub(a, b); }
     static __device__ __forceinline__ V mul(V a, V b) { return f2_mul(a, b); }
     static __device__ __forceinline__ V unpack(uint32_t w) { return f2_of_bf16x2(w); }
     static __device__ __forceinline__ uint32_t pack(V v) {
@@ -91,13 +87,18 @@ struct Lane<__nv_bfloat16> {
         to(v, a);
         return bf16x2(a[0], a[1]);
     }
+    static __device__ __forceinline__ uint32_t pack_neg(V v) {
+        float a[2];
+        to(v, a);
+        return bf16x2(-a[0], -a[1]);
+    }
     static constexpr uint32_t kInf = 0x7f807f80u;
 };
 
 // z = 1 - sigmoid(g), accurate relative to z for every g down to subnormal z,
 // and +infinity gives exactly 0 (what tokens past the end are given).
 //
-// z alone: with t = 2^-8 e^g, z = 2^-8 / (2^-8 + t).  The 2^-8 keeps the
+// gate gives -z: with t = 2^-8 e^g, z = 2^-8 / (2^-8 + t).  The 2^-8 keeps the
 // reciprocal's result normal until z is below 2^-134, so that small z come
 // out as subnormals and not as zero.
 template <typename T>
@@ -110,9 +111,9 @@ __device__ __forceinline__ typename Lane<T>::V gate(typename Lane<T>::V g) {
     L::to(L::add(L::of(a), L::splat(0x1p-8f)), r);
 #pragma unroll
     for (int e = 0; e < L::kN; ++e) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r[e]));
-    return L::mul(L::of(r), L::splat(0x1p-8f));
+    return L::mul(L::of(r), L::splat(-0x1p-8f));
 }
-// With s = z (1 - z), which needs 1 - z just as accurate: t = e^-|g| (formed
+// -z with s = z (1 - z), which needs 1 - z just as accurate: t = e^-|g| (formed
 // as 2^8 t, for the same reason), r = 1 / (1 + t), sigmoid(|g|) = r,
 // sigmoid(-|g|) = t r.
 template <typename T>
@@ -132,20 +133,26 @@ __device__ __forceinline__ void gate_slope(typename Lane<T>::V g, typename Lane<
     const typename L::V tr = L::mul(tv, L::of(r));
     L::to(tr, t);
 #pragma unroll
-    for (int e = 0; e < L::kN; ++e) zz[e] = x[e] >= 0.0f ? t[e] : r[e];
+    for (int e = 0; e < L::kN; ++e) zz[e] = x[e] >= 0.0f ? -t[e] : -r[e];
     z = L::of(zz);
     s = L::mul(tr, L::of(r));
 }
 
-// h - d h + b
+// Packed arithmetic has no negation, so z and D are carried as -z and -D.
+// h - D h + B
 template <typename L>
-__device__ __forceinline__ typename L::V fold(typename L::V h, typename L::V d, typename L::V b) {
-    return L::add(L::sub(h, L::mul(d, h)), b);
+__device__ __forceinline__ typename L::V fold(typename L::V h, typename L::V nd, typename L::V b) {
+    return L::add(L::fma(nd, h, h), b);
 }
-// a + z (v - a): a step of the recurrence, and (v = 1) of D
+// a + z (v - a): a step of the recurrence
 template <typename L>
-__device__ __forceinline__ typename L::V step(typename L::V a, typename L::V z, typename L::V v) {
-    return L::fma(z, L::sub(v, a), a);
+__device__ __forceinline__ typename L::V step(typename L::V a, typename L::V nz, typename L::V v) {
+    return L::fma(nz, L::fma(v, L::splat(-1.0f), a), a);
+}
+// -D after a step (or run) with -z: the step towards v = 1, negated
+template <typename L>
+__device__ __forceinline__ typename L::V grow(typename L::V nd, typename L::V nz) {
+    return L::fma(nz, L::add(nd, L::splat(1.0f)), nd);
 }
 
 // A lane's 4 bytes of a row; n: its channels that exist.
@@ -186,6 +193,17 @@ __device__ __forceinline__ int length_of(const GatedParams& p, int seq) {
     return p.lengths ? min(max(p.lengths[seq], 0), p.n_tok) : p.n_tok;
 }
 
+__device__ __forceinline__ uint32_t align128(const uint8_t* p) { return (smem_u32(p) + 127u) & ~127u; }
+// Shared memory by its 32-bit address: 64-bit generic addresses cost two more
+// instructions an access.
+__device__ __forceinline__ uint32_t lds(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void sts(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v)); }
+__host__ __device__ constexpr uint32_t word_of(int k, int i) { return (uint32_t)(k * kTileBytes + i * 128); }
+
 // Where a thread is: its group of channels, and its tokens of a chunk.
 template <typename T>
 struct Place {
@@ -205,403 +223,380 @@ struct Place {
     __device__ __forceinline__ int slab0() const { return c0 - Lane<T>::kN * lane; }
 };
 
-// The warps' (D, B) of a step, and the totals of the cluster's CTAs; two
-// steps' worth each, since a warp may be a step ahead of another.
+// The warps' (D, B) of a step, and the totals of the cluster's CTAs with the
+// mbarrier they arrive on; two steps' worth each, since a warp may be a step
+// ahead of another.
 template <typename V, int K>
 struct Meet {
-    V warp[2][K][kWarps][32];
-    V total[2][2][kMaxCluster][32];
+    V        warp[2][K][kWarps][32];
+    V        total[2][2][kMaxCluster][32];
+    uint64_t arrived[2];
 };
 
-__device__ __forceinline__ void cluster_arrive() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() {
-    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ uint32_t in_rank(const void* p, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+// Store to another CTA's shared memory; its mbarrier counts the bytes.
+__device__ __forceinline__ void st_async(uint32_t at, uint64_t v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(at), "l"(v),
+                 "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void st_async(uint32_t at, float v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(at),
+                 "r"(__float_as_uint(v)), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 struct GatedMaps {
-    CUtensorMap in[3], out[2];  // g, v, dy; y, or dg and dv
+    CUtensorMap in[3];  // g, v, dy
 };
 
-// The tiles of the steps to come: K input tensors per stage.
+// What the threads of a CTA share in the walk over its chunks: the tiles of
+// the K input tensors, kStages steps of them, and the meetings of a step.
 template <typename T, Access A, int K, int kStages>
-struct Tiles {
-    uint8_t*  base;
-    uint64_t* full;
-    bool      alive = true;
+struct Walk {
+    using L = Lane<T>;
+    using V = typename L::V;
+    const GatedMaps&   maps;
+    const GatedParams& p;
+    const Place<T>&    at;
+    uint32_t           base;  // shared-memory address of the tiles
+    uint64_t*          full;
+    Meet<V, K>*        meet;
+    int                steps;
+    bool               alive = true;
 
-    __device__ __forceinline__ uint8_t* tile(int turn, int k) const {
-        return base + ((turn % kStages) * K + k) * kTileBytes;
+    // The lane's words of step s; word i of tensor k is 128 i + kTileBytes k further on.
+    __device__ __forceinline__ uint32_t mine(int s) const {
+        return base + (uint32_t)((s % kStages) * K * kTileBytes + at.warp * kTok * 128 + at.lane * 4);
     }
-    __device__ __forceinline__ uint32_t* word(int turn, int k, int row, int lane) const {
-        return reinterpret_cast<uint32_t*>(tile(turn, k) + row * 128 + lane * 4);
-    }
-    // One thread: turn's tiles start to arrive.
-    __device__ __forceinline__ void load(const GatedMaps& m, int turn, int c0, int t0, int seq) const {
-        uint64_t* bar = &full[turn % kStages];
+    __device__ __forceinline__ bool issuer() const { return A == kTma && threadIdx.x == kThreads - 1; }
+    // One thread: step s's tiles (chunk `chunk`) start to arrive.
+    __device__ __forceinline__ void load(int s, int chunk) const {
+        uint64_t* bar = &full[s % kStages];
         mbar_expect_tx(bar, K * kTileBytes);
 #pragma unroll
-        for (int k = 0; k < K; ++k) tma_load_3d(tile(turn, k), &m.in[k], bar, c0, t0, seq);
+        for (int k = 0; k < K; ++k)
+            tma_load_3d(base + (uint32_t)(((s % kStages) * K + k) * kTileBytes), &maps.in[k], bar, at.slab0(),
+                        chunk * kChunk, at.seq);
     }
-    __device__ __forceinline__ void wait(int turn, unsigned* fault) {
-        if (A != kTma || !alive) return;
-        alive = mbar_wait(&full[turn % kStages], (uint32_t)((turn / kStages) & 1), tc::kWaitBudget);
-        if (!alive && fault) atomicCAS(fault, 0u, (unsigned)kFaultGated);
+    __device__ __forceinline__ void gave_up() {
+        alive = false;
+        if (p.fault) atomicCAS(p.fault, 0u, (unsigned)kFaultGated);
+    }
+    __device__ __forceinline__ void wait_tiles(int s) {
+        if (A != kTma) return;
+        if (alive && !mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget)) gave_up();
         __syncwarp();
+    }
+    __device__ __forceinline__ void begin() {
+        if (threadIdx.x == kThreads - 1) {
+#pragma unroll
+            for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
+            mbar_init(&meet->arrived[0], 1);
+            mbar_init(&meet->arrived[1], 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+        if (p.cluster > 1) cluster_sync();  // no CTA writes to another before that one's barriers stand
+    }
+    // Hands the totals of step s to every CTA of the cluster.
+    __device__ __forceinline__ void send(int s, V d, V t) {
+        const int b = s & 1;
+        if (at.warp == 0 && at.lane == 0)
+            mbar_expect_tx(&meet->arrived[b], (uint32_t)(p.cluster * 2 * 32 * sizeof(V)));
+        if (at.warp < p.cluster) {
+            const uint32_t bar = in_rank(&meet->arrived[b], at.warp);
+            st_async(in_rank(&meet->total[b][0][at.rank][at.lane], at.warp), d, bar);
+            st_async(in_rank(&meet->total[b][1][at.rank][at.lane], at.warp), t, bar);
+        }
+    }
+    __device__ __forceinline__ void receive(int s) {
+        if (alive) {
+            uint64_t*      bar = &meet->arrived[s & 1];
+            const uint32_t parity = (uint32_t)((s >> 1) & 1);
+            if (!try_wait_cluster(bar, parity)) {
+                const long long t0 = clock64();
+                while (!try_wait_cluster(bar, parity))
+                    if (clock64() - t0 > tc::kWaitBudget) {
+                        gave_up();
+                        break;
+                    }
+            }
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void end() {
+        if (issuer())  // whatever the other threads made of their waits, the loads land
+            for (int s = max(0, steps - kStages); s < steps; ++s)
+                mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget);
+        __syncwarp();
+        if (p.cluster > 1) cluster_sync();  // no CTA leaves while another may store to it
     }
 };
 
 template <typename T, Access A, int kStages>
-__global__ void __launch_bounds__(kThreads, 1)
-    gated_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
+__global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
+    gated_kernel(const __grid_constant__ GatedMaps maps, const __grid_constant__ GatedParams p) {
     using L = Lane<T>;
     using V = typename L::V;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Meet<V, 2> meet;
     __shared__ uint64_t full[kStages];
-    cg::cluster_group cluster = cg::this_cluster();
 
     const Place<T> at(p);
-    const int R = p.cluster, steps = (p.n_chunk + R - 1) / R;
-    const int warp = at.warp, lane = at.lane, n = at.n;
-    const bool issuer = threadIdx.x == kThreads - 1;
-    Tiles<T, A, 2, kStages> tiles{reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127)),
-                                  full};
-
-    const T* src[2] = {static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0,
-                       static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0};
-    const int64_t pitch[2] = {p.s_g, p.s_v};
-    T* y = static_cast<T*>(p.y) + (int64_t)at.seq * p.seq_y + at.c0;
-
+    const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
+    Walk<T, A, 2, kStages> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
+    const int steps = walk.steps;
     auto chunk_of = [&](int s) { return s * R + at.rank; };
+    walk.begin();
+    if (walk.issuer())
+        for (int s = 0; s < kStages && s < steps; ++s) walk.load(s, chunk_of(s));
+    __syncwarp();
+
     uint32_t ahead[A == kTma ? 1 : 2][A == kTma ? 1 : kTok];
     auto fetch = [&](int s) {  // plain access: the lane's words of step s
         if constexpr (A != kTma) {
+            const T* g = static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0;
+            const T* v = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0;
             const int t0 = chunk_of(s) * kChunk + warp * kTok;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int i = 0; i < kTok; ++i)
-                    ahead[k][i] = n > 0 && t0 + i < at.len ? ld_raw<T, A>(src[k] + (t0 + i) * pitch[k], n) : 0u;
+            for (int i = 0; i < kTok; ++i) {
+                const bool live = n > 0 && t0 + i < at.len;
+                ahead[0][i] = live ? ld_raw<T, A>(g + (int64_t)(t0 + i) * p.s_g, n) : 0u;
+                ahead[1][i] = live ? ld_raw<T, A>(v + (int64_t)(t0 + i) * p.s_v, n) : 0u;
+            }
         }
     };
-    auto keep = [&](int s) {
-        if constexpr (A != kTma) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int i = 0; i < kTok; ++i) *tiles.word(s, k, warp * kTok + i, lane) = ahead[k][i];
-        }
-    };
-
-    if (A == kTma) {
-        if (issuer) {
-#pragma unroll
-            for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
-            fence_mbar_init();
-            for (int s = 0; s < kStages && s < steps; ++s)
-                tiles.load(maps, s, at.slab0(), chunk_of(s) * kChunk, at.seq);
-        }
-        __syncthreads();
-    }
-
     V h = ld_state<L>(p.h0 ? p.h0 + (int64_t)at.seq * p.seq_h0 + at.c0 : nullptr, n);
-    V z[kTok], zn[kTok], D, B;
-    // gates and the warp's (D, B) of step s
-    auto first = [&](int s, V(&zs)[kTok]) {
-        tiles.wait(s, p.fault);
-        const int t0 = chunk_of(s) * kChunk + warp * kTok;
-        const bool whole = t0 + kTok <= at.len;
-        D = B = L::splat(0.0f);
+    if (steps > 0) fetch(0);
+    for (int s = 0; s < steps; ++s) {
+        const int chunk = chunk_of(s), t0 = chunk * kChunk + warp * kTok, b = s & 1;
+        const uint32_t my = walk.mine(s);
+        // every token and channel of the warp counts
+        const bool whole = t0 + kTok <= at.len && at.slab0() + 32 * L::kN <= p.n_chan;
+        V z[kTok], D = L::splat(0.0f), B = D;
+        walk.wait_tiles(s);
+        auto first = [&](auto all) {
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-            uint32_t gw = *tiles.word(s, 0, warp * kTok + i, lane), vw = *tiles.word(s, 1, warp * kTok + i, lane);
-            if (!whole && t0 + i >= at.len) gw = L::kInf, vw = 0u;
-            zs[i] = gate<T>(L::unpack(gw));
-            D = step<L>(D, zs[i], L::splat(1.0f));
-            B = step<L>(B, zs[i], L::unpack(vw));
-        }
-    };
-    // shares them: within the CTA, then its totals with the cluster
-    auto publish = [&](int s) {
-        const int b = s & 1;
+            for (int i = 0; i < kTok; ++i) {
+                uint32_t gw, vw;
+                if constexpr (A == kTma) {
+                    gw = lds(my + word_of(0, i)), vw = lds(my + word_of(1, i));
+                } else {
+                    gw = ahead[0][i], vw = ahead[1][i];
+                    sts(my + word_of(1, i), vw);
+                }
+                if (!decltype(all)::value && t0 + i >= at.len) gw = L::kInf, vw = 0u;
+                z[i] = gate<T>(L::unpack(gw));
+                D = grow<L>(D, z[i]);
+                B = step<L>(B, z[i], L::unpack(vw));
+            }
+        };
+        if (whole)
+            first(std::true_type{});
+        else
+            first(std::false_type{});
+        if (s + 1 < steps) fetch(s + 1);
         meet.warp[b][0][warp][lane] = D;
         meet.warp[b][1][warp][lane] = B;
         __syncthreads();
-        if (warp < R) {
-            V d = L::splat(0.0f), t = d;
+        // what the CTA's earlier warps, and all of them, make of a state
+        V dp = L::splat(0.0f), bp = dp, d = dp, t = dp;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const V dw = meet.warp[b][0][w][lane];
-                d = step<L>(d, dw, L::splat(1.0f));
-                t = fold<L>(t, dw, meet.warp[b][1][w][lane]);
-            }
-            Meet<V, 2>* to = cluster.map_shared_rank(&meet, warp);
-            to->total[b][0][at.rank][lane] = d;
-            to->total[b][1][at.rank][lane] = t;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) dp = d, bp = t;
+            const V dw = meet.warp[b][0][w][lane];
+            t = fold<L>(t, dw, meet.warp[b][1][w][lane]);
+            d = grow<L>(d, dw);
         }
-        cluster_arrive();
-    };
-
-    // no CTA writes to another's shared memory before that one runs
-    cluster_arrive();
-    cluster_wait();
-    if (steps > 0) {
-        fetch(0);
-        keep(0);
-        if (steps > 1) {
-            fetch(1);
-            keep(1);
-        }
-        first(0, z);
-        publish(0);
-    }
-    for (int s = 0; s < steps; ++s) {
-        const int chunk = chunk_of(s), b = s & 1, t0 = chunk * kChunk + warp * kTok;
-        if (s + 2 < steps) fetch(s + 2);
-        if (s + 1 < steps) first(s + 1, zn);
-        cluster_wait();
         V hw = h;
-        for (int k = 0; k < R; ++k) {
-            if (k == at.rank) hw = h;
-            h = fold<L>(h, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
+        if (R > 1) {
+            walk.send(s, d, t);
+            walk.receive(s);
+            for (int k = 0; k < R; ++k) {
+                if (k == at.rank) hw = h;
+                h = fold<L>(h, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
+            }
+        } else {
+            h = fold<L>(h, d, t);
         }
         if (p.states && warp == 0 && chunk < p.n_chunk)
             st_state<L>(p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0, n, hw);
-        for (int w = 0; w < warp; ++w)
-            hw = fold<L>(hw, meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
-        const bool whole = t0 + kTok <= at.len;
+        hw = fold<L>(hw, dp, bp);
+        T* y = static_cast<T*>(p.y) + (int64_t)at.seq * p.seq_y + at.c0 + (int64_t)t0 * p.s_y;
+        auto second = [&](auto all) {
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-            uint32_t* slot = tiles.word(s, 1, warp * kTok + i, lane);
-            const bool past = !whole && t0 + i >= at.len;
-            hw = step<L>(hw, z[i], past ? L::splat(0.0f) : L::unpack(*slot));
-            const uint32_t o = past ? 0u : L::pack(hw);
-            if (A == kTma)
-                *slot = o;
-            else if (t0 + i < p.n_tok && n > 0)
-                st_raw<T, A>(y + (t0 + i) * p.s_y, n, o);
-        }
-        if (s + 2 < steps) keep(s + 2);
-        if (A == kTma) fence_async_smem();
-        if (s + 1 < steps)
-            publish(s + 1);
-        else
-            __syncthreads();
-        if (A == kTma && issuer) {
-            if (chunk < p.n_chunk) tma_store_3d(&maps.out[0], tiles.tile(s, 1), at.slab0(), chunk * kChunk, at.seq);
-            bulk_commit();
-            // the stage of the step before is free once its output has been read
-            if (s >= 1 && s - 1 + kStages < steps) {
-                bulk_wait_read<1>();
-                tiles.load(maps, s - 1 + kStages, at.slab0(), chunk_of(s - 1 + kStages) * kChunk, at.seq);
+            for (int i = 0; i < kTok; ++i) {
+                const bool past = !decltype(all)::value && t0 + i >= at.len;
+                hw = step<L>(hw, z[i], past ? L::splat(0.0f) : L::unpack(lds(my + word_of(1, i))));
+                if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok))
+                    st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(hw));
+                y += p.s_y;
             }
+        };
+        if (whole)
+            second(std::true_type{});
+        else
+            second(std::false_type{});
+        if (s + kStages < steps) {
+            __syncthreads();  // every warp is done with the tiles
+            if (walk.issuer()) walk.load(s + kStages, chunk_of(s + kStages));
+            __syncwarp();
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kTok; ++i) z[i] = zn[i];
     }
-    if (A == kTma && issuer) {
-        // whatever the other threads made of their waits, the loads land
-        for (int s = max(0, steps - kStages); s < steps; ++s)
-            mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget);
-        bulk_wait0();
-    }
+    walk.end();
     // Every CTA holds the last state.  In place of h0 is safe: each has read
-    // h0 before the cluster's first barrier.
+    // h0 before the cluster's last barrier.
     if (at.rank == 0 && warp == 0) st_state<L>(p.h1 + (int64_t)at.seq * p.seq_h1 + at.c0, n, h);
 }
 
 template <typename T, Access A, int kStages>
-__global__ void __launch_bounds__(kThreads, 1)
-    gated_grad_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
+__global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
+    gated_grad_kernel(const __grid_constant__ GatedMaps maps, const __grid_constant__ GatedParams p) {
     using L = Lane<T>;
     using V = typename L::V;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Meet<V, 3> meet;
     __shared__ uint64_t full[kStages];
-    cg::cluster_group cluster = cg::this_cluster();
 
     const Place<T> at(p);
-    const int R = p.cluster, steps = (p.n_chunk + R - 1) / R;
-    const int warp = at.warp, lane = at.lane, n = at.n;
-    const bool issuer = threadIdx.x == kThreads - 1;
-    Tiles<T, A, 3, kStages> tiles{reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127)),
-                                  full};
-
-    const T* src[3] = {static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0,
-                       static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0,
-                       static_cast<const T*>(p.dy) + (int64_t)at.seq * p.seq_dy + at.c0};
-    const int64_t pitch[3] = {p.s_g, p.s_v, p.s_dy};
-    T* dg = static_cast<T*>(p.dg) + (int64_t)at.seq * p.seq_dg + at.c0;
-    T* dv = static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0;
-
-    // turns count from the end
-    auto chunk_of = [&](int s) { return (steps - 1 - s) * R + at.rank; };
-    uint32_t ahead[A == kTma ? 1 : 3][A == kTma ? 1 : kTok];
-    auto fetch = [&](int s) {
-        if constexpr (A != kTma) {
-            const int t0 = chunk_of(s) * kChunk + warp * kTok;
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-#pragma unroll
-                for (int i = 0; i < kTok; ++i)
-                    ahead[k][i] = n > 0 && t0 + i < at.len ? ld_raw<T, A>(src[k] + (t0 + i) * pitch[k], n) : 0u;
-        }
-    };
-    auto keep = [&](int s) {
-        if constexpr (A != kTma) {
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-#pragma unroll
-                for (int i = 0; i < kTok; ++i) *tiles.word(s, k, warp * kTok + i, lane) = ahead[k][i];
-        }
-    };
-
-    if (A == kTma) {
-        if (issuer) {
-#pragma unroll
-            for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
-            fence_mbar_init();
-            for (int s = 0; s < kStages && s < steps; ++s)
-                tiles.load(maps, s, at.slab0(), chunk_of(s) * kChunk, at.seq);
-        }
-        __syncthreads();
-    }
+    const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
+    Walk<T, A, 3, kStages> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
+    const int steps = walk.steps;
+    auto chunk_of = [&](int s) { return (steps - 1 - s) * R + at.rank; };  // from the end
+    walk.begin();
+    if (walk.issuer())
+        for (int s = 0; s < kStages && s < steps; ++s) walk.load(s, chunk_of(s));
+    __syncwarp();
 
     V c = ld_state<L>(p.dh1 ? p.dh1 + (int64_t)at.seq * p.seq_dh1 + at.c0 : nullptr, n);
-    V z[kTok], q[kTok], zn[kTok], qn[kTok], D, B, E, h, hn;
-    auto first = [&](int s, V(&zs)[kTok], V(&qs)[kTok], V& hs) {
-        const int chunk = chunk_of(s), t0 = chunk * kChunk + warp * kTok;
-        hs = ld_state<L>(chunk < p.n_chunk ? p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0 : nullptr,
-                         n);
-        tiles.wait(s, p.fault);
-        const bool whole = t0 + kTok <= at.len;
-        D = B = E = L::splat(0.0f);
+    for (int s = 0; s < steps; ++s) {
+        const int chunk = chunk_of(s), t0 = chunk * kChunk + warp * kTok, b = s & 1;
+        const uint32_t my = walk.mine(s);
+        // every token and channel of the warp counts
+        const bool whole = t0 + kTok <= at.len && at.slab0() + 32 * L::kN <= p.n_chan;
+        V h = ld_state<L>(chunk < p.n_chunk ? p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0 : nullptr,
+                          n);
+        if constexpr (A != kTma) {  // the lane's words, into its own slots
+            const T* g = static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0;
+            const T* v = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0;
+            const T* dy = static_cast<const T*>(p.dy) + (int64_t)at.seq * p.seq_dy + at.c0;
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-            uint32_t gw = *tiles.word(s, 0, warp * kTok + i, lane), vw = *tiles.word(s, 1, warp * kTok + i, lane);
-            if (!whole && t0 + i >= at.len) gw = L::kInf, vw = 0u;
-            gate_slope<T>(L::unpack(gw), zs[i], qs[i]);
-            D = step<L>(D, zs[i], L::splat(1.0f));
-            B = step<L>(B, zs[i], L::unpack(vw));
+            for (int i = 0; i < kTok; ++i) {
+                const bool live = n > 0 && t0 + i < at.len;
+                const uint32_t gw = live ? ld_raw<T, A>(g + (int64_t)(t0 + i) * p.s_g, n) : 0u;
+                const uint32_t vw = live ? ld_raw<T, A>(v + (int64_t)(t0 + i) * p.s_v, n) : 0u;
+                const uint32_t yw = live ? ld_raw<T, A>(dy + (int64_t)(t0 + i) * p.s_dy, n) : 0u;
+                sts(my + word_of(0, i), gw), sts(my + word_of(1, i), vw), sts(my + word_of(2, i), yw);
+            }
         }
+        V z[kTok], q[kTok], D = L::splat(0.0f), B = D, E = D;
+        walk.wait_tiles(s);
+        auto first = [&](auto all) {
+            auto past = [&](int i) { return !decltype(all)::value && t0 + i >= at.len; };
 #pragma unroll
-        for (int i = kTok - 1; i >= 0; --i) {
-            uint32_t yw = *tiles.word(s, 2, warp * kTok + i, lane);
-            if (!whole && t0 + i >= at.len) yw = 0u;
-            const V lam = L::add(L::unpack(yw), E);
-            E = L::sub(lam, L::mul(zs[i], lam));
-        }
-    };
-    auto publish = [&](int s) {
-        const int b = s & 1;
+            for (int i = 0; i < kTok; ++i) {
+                const uint32_t gw = past(i) ? L::kInf : lds(my + word_of(0, i)), vw = past(i) ? 0u : lds(my + word_of(1, i));
+                gate_slope<T>(L::unpack(gw), z[i], q[i]);
+                D = grow<L>(D, z[i]);
+                B = step<L>(B, z[i], L::unpack(vw));
+            }
+#pragma unroll
+            for (int i = kTok - 1; i >= 0; --i) {
+                const V lam = L::add(L::unpack(past(i) ? 0u : lds(my + word_of(2, i))), E);
+                E = L::fma(z[i], lam, lam);
+            }
+        };
+        if (whole)
+            first(std::true_type{});
+        else
+            first(std::false_type{});
         meet.warp[b][0][warp][lane] = D;
         meet.warp[b][1][warp][lane] = B;
         meet.warp[b][2][warp][lane] = E;
         __syncthreads();
-        if (warp < R) {
-            V d = L::splat(0.0f), t = d;
+        // what the CTA's later warps, and all of them, make of a gradient
+        V dp = L::splat(0.0f), ep = dp, d = dp, t = dp;
 #pragma unroll
-            for (int w = kWarps - 1; w >= 0; --w) {
-                const V dw = meet.warp[b][0][w][lane];
-                d = step<L>(d, dw, L::splat(1.0f));
-                t = fold<L>(t, dw, meet.warp[b][2][w][lane]);
-            }
-            Meet<V, 3>* to = cluster.map_shared_rank(&meet, warp);
-            to->total[b][0][at.rank][lane] = d;
-            to->total[b][1][at.rank][lane] = t;
+        for (int w = kWarps - 1; w >= 0; --w) {
+            if (w == warp) dp = d, ep = t;
+            const V dw = meet.warp[b][0][w][lane];
+            t = fold<L>(t, dw, meet.warp[b][2][w][lane]);
+            d = grow<L>(d, dw);
         }
-        cluster_arrive();
-    };
-
-    cluster_arrive();
-    cluster_wait();
-    if (steps > 0) {
-        fetch(0);
-        keep(0);
-        if (steps > 1) {
-            fetch(1);
-            keep(1);
-        }
-        first(0, z, q, h);
-        publish(0);
-    }
-    for (int s = 0; s < steps; ++s) {
-        const int chunk = chunk_of(s), b = s & 1, t0 = chunk * kChunk + warp * kTok;
-        const bool whole = t0 + kTok <= at.len;
-        if (s + 2 < steps) fetch(s + 2);
-        // h_{t-1} - v_t of the warp's tokens
-        for (int w = 0; w < warp; ++w)
-            h = fold<L>(h, meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
+        if (R > 1) walk.send(s, d, t);
+        // h_{t-1} - v_t of the warp's tokens, times the slopes
+#pragma unroll
+        for (int w = 0; w < kWarps - 1; ++w)
+            if (w < warp) h = fold<L>(h, meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
 #pragma unroll
         for (int i = 0; i < kTok; ++i) {
-            uint32_t vw = *tiles.word(s, 1, warp * kTok + i, lane);
-            if (!whole && t0 + i >= at.len) vw = 0u;
-            const V off = L::sub(h, L::unpack(vw));
+            const V off = L::fma(whole || t0 + i < at.len ? L::unpack(lds(my + word_of(1, i))) : L::splat(0.0f),
+                                 L::splat(-1.0f), h);
             q[i] = L::mul(q[i], off);
-            h = L::sub(h, L::mul(z[i], off));
+            h = L::fma(z[i], off, h);
         }
-        if (s + 1 < steps) first(s + 1, zn, qn, hn);
-        cluster_wait();
         V cw = c;
-        for (int k = R - 1; k >= 0; --k) {
-            if (k == at.rank) cw = c;
-            c = fold<L>(c, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
-        }
-        for (int w = kWarps - 1; w > warp; --w)
-            cw = fold<L>(cw, meet.warp[b][0][w][lane], meet.warp[b][2][w][lane]);
-#pragma unroll
-        for (int i = kTok - 1; i >= 0; --i) {
-            const int row = warp * kTok + i;
-            const bool past = !whole && t0 + i >= at.len;
-            const V lam = L::add(past ? L::splat(0.0f) : L::unpack(*tiles.word(s, 2, row, lane)), cw);
-            const V zl = L::mul(z[i], lam);
-            const uint32_t og = past ? 0u : L::pack(L::mul(lam, q[i])), ov = past ? 0u : L::pack(zl);
-            cw = L::sub(lam, zl);
-            if (A == kTma) {
-                *tiles.word(s, 0, row, lane) = og;
-                *tiles.word(s, 1, row, lane) = ov;
-            } else if (t0 + i < p.n_tok && n > 0) {
-                st_raw<T, A>(dg + (t0 + i) * p.s_dg, n, og);
-                st_raw<T, A>(dv + (t0 + i) * p.s_dv, n, ov);
+        if (R > 1) {
+            walk.receive(s);
+            for (int k = R - 1; k >= 0; --k) {
+                if (k == at.rank) cw = c;
+                c = fold<L>(c, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
             }
+        } else {
+            c = fold<L>(c, d, t);
         }
-        if (s + 2 < steps) keep(s + 2);
-        if (A == kTma) fence_async_smem();
-        if (s + 1 < steps)
-            publish(s + 1);
+        cw = fold<L>(cw, dp, ep);
+        T* dg = static_cast<T*>(p.dg) + (int64_t)at.seq * p.seq_dg + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dg;
+        T* dv = static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dv;
+        auto second = [&](auto all) {
+#pragma unroll
+            for (int i = kTok - 1; i >= 0; --i) {
+                const bool past = !decltype(all)::value && t0 + i >= at.len;
+                const V lam = L::add(past ? L::splat(0.0f) : L::unpack(lds(my + word_of(2, i))), cw);
+                if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok)) {
+                    const int k = decltype(all)::value ? L::kN : n;
+                    st_raw<T, A>(dg, k, past ? 0u : L::pack(L::mul(lam, q[i])));
+                    st_raw<T, A>(dv, k, past ? 0u : L::pack_neg(L::mul(z[i], lam)));
+                }
+                dg -= p.s_dg, dv -= p.s_dv;
+                cw = L::fma(z[i], lam, lam);
+            }
+        };
+        if (whole)
+            second(std::true_type{});
         else
+            second(std::false_type{});
+        if (s + kStages < steps) {
             __syncthreads();
-        if (A == kTma && issuer) {
-            if (chunk < p.n_chunk) {
-                tma_store_3d(&maps.out[0], tiles.tile(s, 0), at.slab0(), chunk * kChunk, at.seq);
-                tma_store_3d(&maps.out[1], tiles.tile(s, 1), at.slab0(), chunk * kChunk, at.seq);
-            }
-            bulk_commit();
-            if (s >= 1 && s - 1 + kStages < steps) {
-                bulk_wait_read<1>();
-                tiles.load(maps, s - 1 + kStages, at.slab0(), chunk_of(s - 1 + kStages) * kChunk, at.seq);
-            }
+            if (walk.issuer()) walk.load(s + kStages, chunk_of(s + kStages));
+            __syncwarp();
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kTok; ++i) z[i] = zn[i], q[i] = qn[i];
-        h = hn;
     }
-    if (A == kTma && issuer) {
-        for (int s = max(0, steps - kStages); s < steps; ++s)
-            mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget);
-        bulk_wait0();
-    }
+    walk.end();
     if (p.dh0 && at.rank == 0 && warp == 0) st_state<L>(p.dh0 + (int64_t)at.seq * p.seq_dh0 + at.c0, n, c);
 }
 
-// Up to kTok tokens: a warp has the channels of one slab of one sequence.
-template <typename T, Access A, bool GRAD>
+// Up to NT tokens: a warp has the channels of one slab of one sequence.
+template <typename T, Access A, bool GRAD, int NT>
 __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedParams p) {
     using L = Lane<T>;
     using V = typename L::V;
@@ -617,10 +612,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
     const T* v = static_cast<const T*>(p.v) + (int64_t)seq * p.seq_v + c0;
     const T* dy = static_cast<const T*>(p.dy) + (int64_t)seq * p.seq_dy + c0;
 
-    V z[kTok], q[GRAD ? kTok : 1];
-    uint32_t vw[kTok], yw[GRAD ? kTok : 1];
+    V z[NT], q[GRAD ? NT : 1];
+    uint32_t vw[NT], yw[GRAD ? NT : 1];
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
+    for (int i = 0; i < NT; ++i) {
         const bool live = i < len;
         const uint32_t gw = live ? ld_raw<T, A>(g + i * p.s_g, n) : L::kInf;
         vw[i] = live ? ld_raw<T, A>(v + i * p.s_v, n) : 0u;
@@ -635,7 +630,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
         V h = ld_state<L>(p.h0 ? p.h0 + (int64_t)seq * p.seq_h0 + c0 : nullptr, n);
         if (p.states && p.n_tok > 0) st_state<L>(p.states + (int64_t)seq * p.n_chan + c0, n, h);
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
+        for (int i = 0; i < NT; ++i) {
             if (i < len) h = step<L>(h, z[i], L::unpack(vw[i]));
             if (i < p.n_tok) st_raw<T, A>(y + i * p.s_y, n, i < len ? L::pack(h) : 0u);
         }
@@ -645,20 +640,20 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
         T* dv = static_cast<T*>(p.dv) + (int64_t)seq * p.seq_dv + c0;
         V h = ld_state<L>(p.n_tok > 0 ? p.states + (int64_t)seq * p.n_chan + c0 : nullptr, n);
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-            const V off = L::sub(h, L::unpack(vw[i]));
+        for (int i = 0; i < NT; ++i) {
+            const V off = L::fma(L::unpack(vw[i]), L::splat(-1.0f), h);
             q[i] = L::mul(q[i], off);
-            h = L::sub(h, L::mul(z[i], off));
+            h = L::fma(z[i], off, h);
         }
         V c = ld_state<L>(p.dh1 ? p.dh1 + (int64_t)seq * p.seq_dh1 + c0 : nullptr, n);
 #pragma unroll
-        for (int i = kTok - 1; i >= 0; --i) {
+        for (int i = NT - 1; i >= 0; --i) {
             if (i >= p.n_tok) continue;
             const bool live = i < len;
-            const V lam = L::add(L::unpack(yw[i]), c), zl = L::mul(z[i], lam);
+            const V lam = L::add(L::unpack(yw[i]), c);
             st_raw<T, A>(dg + i * p.s_dg, n, live ? L::pack(L::mul(lam, q[i])) : 0u);
-            st_raw<T, A>(dv + i * p.s_dv, n, live ? L::pack(zl) : 0u);
-            if (live) c = L::sub(lam, zl);
+            st_raw<T, A>(dv + i * p.s_dv, n, live ? L::pack_neg(L::mul(z[i], lam)) : 0u);
+            if (live) c = L::fma(z[i], lam, lam);
         }
         if (p.dh0) st_state<L>(p.dh0 + (int64_t)seq * p.seq_dh0 + c0, n, c);
     }
@@ -667,15 +662,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// One CTA per SM.  At the end of a step the tiles of that step and the next
-// are still held: the loads run kStages - 2 steps ahead of their use.
-constexpr int kFwdStages = 6, kGradStages = 4;
-constexpr size_t kFwdSmem = (size_t)kFwdStages * 2 * kTileBytes + 128;
-constexpr size_t kGradSmem = (size_t)kGradStages * 3 * kTileBytes + 128;
+// Stages of tiles: with two CTAs per SM, or (deep) with one, when the device
+// holds all clusters at once that way too.
+constexpr int kFwdStages = 3, kFwdDeep = 6, kGradStages = 2, kGradDeep = 4;
+constexpr size_t tiles_smem(int tensors, int stages) { return (size_t)stages * tensors * kTileBytes + 128; }
 
 // [n_seq][n_tok][n_chan] in boxes of 128 tokens x 128 bytes; false when TMA
-// cannot describe it.  Rows and channels past the ends read as zero and are
-// not written.
+// cannot describe it.  Rows and channels past the ends read as zero.
 bool make_map_tok(const helix_ctx* ctx, CUtensorMap* m, const GatedParams& p, const void* base, int64_t s_tok,
                   int64_t s_seq, int size) {
     if (reinterpret_cast<uintptr_t>(base) % 16) return false;
@@ -698,25 +691,45 @@ bool make_maps(const helix_ctx* ctx, GatedMaps* m, const GatedParams& p, bool gr
     if (!ctx->encode_tiled || p.n_tok <= 0) return false;
     if (!make_map_tok(ctx, &m->in[0], p, p.g, p.s_g, p.seq_g, size)) return false;
     if (!make_map_tok(ctx, &m->in[1], p, p.v, p.s_v, p.seq_v, size)) return false;
-    if (!grad) return make_map_tok(ctx, &m->out[0], p, p.y, p.s_y, p.seq_y, size);
-    return make_map_tok(ctx, &m->in[2], p, p.dy, p.s_dy, p.seq_dy, size) &&
-           make_map_tok(ctx, &m->out[0], p, p.dg, p.s_dg, p.seq_dg, size) &&
-           make_map_tok(ctx, &m->out[1], p, p.dv, p.s_dv, p.seq_dv, size);
+    return !grad || make_map_tok(ctx, &m->in[2], p, p.dy, p.s_dy, p.seq_dy, size);
 }
 
 // CTAs of a cluster: the size with the fewest steps, counting the waves that
-// its clusters take, one CTA per SM (large clusters leave SMs of a GPC idle),
+// its clusters take, two CTAs per SM (large clusters leave SMs of a GPC idle),
 // and two steps to fill and drain each.
-int cluster_of(const helix_ctx* ctx, int64_t groups, int chunks) {
+int cluster_of(const helix_ctx* ctx, int64_t groups, int chunks, bool* deep) {
     int best = 1;
     int64_t least = INT64_MAX;
     for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
         const int64_t at_once = ctx->gated_clusters[i];
         if (at_once <= 0 || (r > 1 && r >= 2 * chunks)) continue;
         const int64_t cost = (groups + at_once - 1) / at_once * ((chunks + r - 1) / r + 2);
-        if (cost < least) least = cost, best = r;
+        if (cost < least) least = cost, best = r, *deep = groups <= ctx->gated_deep[i];
     }
     return best;
+}
+
+struct ClusterLaunch {
+    cudaLaunchConfig_t  cfg{};
+    cudaLaunchAttribute at{};
+    ClusterLaunch(int64_t grid, int cluster, size_t smem, void* stream) {
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3((unsigned)kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = static_cast<cudaStream_t>(stream);
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = (unsigned)cluster;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+    }
+};
+
+template <typename T, Access A, int NT>
+int launch_few(const GatedParams& p, int64_t groups, bool grad, void* stream) {
+    const dim3 grid((unsigned)((groups + kFewWarps - 1) / kFewWarps)), block(32 * kFewWarps);
+    return grad ? block_launch(gated_few_kernel<T, A, true, NT>, grid, block, 0, stream, p)
+                : block_launch(gated_few_kernel<T, A, false, NT>, grid, block, 0, stream, p);
 }
 
 template <typename T, Access A>
@@ -724,25 +737,20 @@ int launch_gated_a(const helix_ctx* ctx, const GatedMaps& maps, GatedParams p, b
     constexpr int CB = 32 * Lane<T>::kN;
     constexpr Access few = A == kTma ? kWord : A;
     const int64_t groups = (int64_t)p.n_seq * ((p.n_chan + CB - 1) / CB);
-    if (p.n_tok <= kTok) {
-        const dim3 grid((unsigned)((groups + kFewWarps - 1) / kFewWarps)), block(32 * kFewWarps);
-        return grad ? block_launch(gated_few_kernel<T, few, true>, grid, block, 0, stream, p)
-                    : block_launch(gated_few_kernel<T, few, false>, grid, block, 0, stream, p);
+    if (p.n_tok <= 1) return launch_few<T, few, 1>(p, groups, grad, stream);
+    if (p.n_tok <= 4) return launch_few<T, few, 4>(p, groups, grad, stream);
+    if (p.n_tok <= kTok) return launch_few<T, few, kTok>(p, groups, grad, stream);
+    bool deep = false;
+    p.cluster = cluster_of(ctx, groups, p.n_chunk, &deep);
+    const int64_t grid = groups * p.cluster;
+    if (grad) {
+        ClusterLaunch l(grid, p.cluster, tiles_smem(3, deep ? kGradDeep : kGradStages), stream);
+        return deep ? cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep>, maps, p)
+                    : cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradStages>, maps, p);
     }
-    p.cluster = cluster_of(ctx, groups, p.n_chunk);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(groups * p.cluster));
-    cfg.blockDim = dim3((unsigned)kThreads);
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)p.cluster;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    cfg.dynamicSmemBytes = grad ? kGradSmem : kFwdSmem;
-    return grad ? cudaLaunchKernelEx(&cfg, gated_grad_kernel<T, A, kGradStages>, maps, p)
-                : cudaLaunchKernelEx(&cfg, gated_kernel<T, A, kFwdStages>, maps, p);
+    ClusterLaunch l(grid, p.cluster, tiles_smem(2, deep ? kFwdDeep : kFwdStages), stream);
+    return deep ? cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdDeep>, maps, p)
+                : cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdStages>, maps, p);
 }
 
 int launch_gated_any(const helix_ctx* ctx, const helix_gated_scan_desc& d, const GatedParams& p, bool word, bool grad,
@@ -752,18 +760,24 @@ int launch_gated_any(const helix_ctx* ctx, const helix_gated_scan_desc& d, const
     if (d.io_dtype == HELIX_F32)
         return tma ? launch_gated_a<float, kTma>(ctx, maps, p, grad, stream)
                    : launch_gated_a<float, kWord>(ctx, maps, p, grad, stream);
-    if (tma) return launch_gated_a<__nv_bfloat16, kTma>(ctx, maps, p, grad, stream);
+    // outputs are stored a word at a time in the TMA form too
+    if (tma && word) return launch_gated_a<__nv_bfloat16, kTma>(ctx, maps, p, grad, stream);
     return word ? launch_gated_a<__nv_bfloat16, kWord>(ctx, maps, p, grad, stream)
                 : launch_gated_a<__nv_bfloat16, kHalf>(ctx, maps, p, grad, stream);
 }
 
+template <typename K>
+int set_smem(K kernel, int tensors, int stages) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles_smem(tensors, stages));
+}
+
 template <typename T, Access A>
 int configure_gated_a() {
-    const int e = cudaFuncSetAttribute(gated_kernel<T, A, kFwdStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)kFwdSmem);
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(gated_grad_kernel<T, A, kGradStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)kGradSmem);
+    int e;
+    if ((e = set_smem(gated_kernel<T, A, kFwdStages>, 2, kFwdStages)) != cudaSuccess) return e;
+    if ((e = set_smem(gated_kernel<T, A, kFwdDeep>, 2, kFwdDeep)) != cudaSuccess) return e;
+    if ((e = set_smem(gated_grad_kernel<T, A, kGradStages>, 3, kGradStages)) != cudaSuccess) return e;
+    return set_smem(gated_grad_kernel<T, A, kGradDeep>, 3, kGradDeep);
 }
 
 }  // namespace
@@ -776,17 +790,12 @@ int configure_gated(helix_ctx* ctx) {
     if ((e = configure_gated_a<__nv_bfloat16, kWord>()) != cudaSuccess) return e;
     if ((e = configure_gated_a<__nv_bfloat16, kHalf>()) != cudaSuccess) return e;
     for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)r);
-        cfg.blockDim = dim3((unsigned)kThreads);
-        cfg.dynamicSmemBytes = kFwdSmem;
-        cudaLaunchAttribute at{};
-        at.id = cudaLaunchAttributeClusterDimension;
-        at.val.clusterDim.x = (unsigned)r;
-        at.val.clusterDim.y = at.val.clusterDim.z = 1;
-        cfg.attrs = &at;
-        cfg.numAttrs = 1;
-        e = cudaOccupancyMaxActiveClusters(&ctx->gated_clusters[i], gated_kernel<__nv_bfloat16, kTma, kFwdStages>, &cfg);
+        ClusterLaunch l(r, r, tiles_smem(2, kFwdStages), nullptr);
+        e = cudaOccupancyMaxActiveClusters(&ctx->gated_clusters[i], gated_kernel<__nv_bfloat16, kTma, kFwdStages>,
+                                           &l.cfg);
+        if (e != cudaSuccess) return e;
+        l.cfg.dynamicSmemBytes = tiles_smem(2, kFwdDeep);
+        e = cudaOccupancyMaxActiveClusters(&ctx->gated_deep[i], gated_kernel<__nv_bfloat16, kTma, kFwdDeep>, &l.cfg);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

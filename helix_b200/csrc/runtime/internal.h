@@ -160,7 +160,9 @@ struct helix_ctx {
     bool   tc_ready    = false;   // tensor-core kernels configured
     unsigned* fault_word = nullptr; // device address of the fault word
     void*  encode_tiled = nullptr; // cuTensorMapEncodeTiled entry point
-    int    gated_clusters[4] = {}; // gated recurrence: clusters of 1, 2, 4, 8 CTAs the device holds at once
+    // Gated recurrence: clusters of 1, 2, 4, 8 CTAs the device holds at once,
+    // two CTAs per SM and (deep) one.
+    int    gated_clusters[4] = {}, gated_deep[4] = {};
 };
 
 namespace hx {
