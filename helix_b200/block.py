@@ -17,85 +17,90 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import Context, HelixError, _ctx_for, _t, abi
+from . import Context, HelixError, _default_ctx, abi
 
-_IO = {torch.float32: abi.HELIX_F32, torch.bfloat16: abi.HELIX_BF16}
-_OUT = {**_IO, torch.float8_e4m3fn: abi.HELIX_E4M3}
+_F32, _BF16, _F8, _I32 = torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.int32
+_IO = {_F32: abi.HELIX_F32, _BF16: abi.HELIX_BF16}
+_OUT = {**_IO, _F8: abi.HELIX_E4M3}
+_HERE = nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(...).cuda_stream without the object
 
 
 def _groups(n: int) -> int:
-    return -(-n // abi.HELIX_GROUP)
+    return (n + abi.HELIX_GROUP - 1) // abi.HELIX_GROUP
 
 
-def _dtype(name: str, t: torch.Tensor, known=_IO) -> int:
-    try:
-        return known[t.dtype]
-    except KeyError:
-        raise TypeError(f"{name}: {t.dtype} is not supported") from None
+def _t(t: Optional[torch.Tensor]) -> abi.Tensor:
+    return abi.NULL_TENSOR if t is None else abi.Tensor(t.data_ptr(), 0)
 
 
-def _matrix(name: str, t: torch.Tensor, shape=None) -> int:
+def _dtype(name: str, dtype: torch.dtype, known=_IO) -> int:
+    code = known.get(dtype)
+    if code is None:
+        raise TypeError(f"{name}: {dtype} is not supported")
+    return code
+
+
+def _matrix(name: str, t: torch.Tensor, shape) -> int:
     """Row stride of t seen as rows of its last dimension; raises when it is
     not that, or not of `shape`."""
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.is_contiguous():
+        return shape[-1]
+    if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} needs unit stride along its last dimension")
-    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    lead = [(n, s) for n, s in zip(shape[:-1], t.stride()[:-1]) if n != 1]
     for (_, s0), (n1, s1) in zip(lead, lead[1:]):
         if s0 != n1 * s1:
             raise ValueError(f"{name}: rows must be equally far apart")
-    return lead[-1][1] if lead else t.shape[-1]
+    return lead[-1][1] if lead else shape[-1]
 
 
 def _vector(name: str, t: torch.Tensor, n: int, dtype=None) -> None:
-    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+    if t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a dense vector of {n}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}")
 
 
-class _Call:
-    """Where a call runs: the context, and the stream as a handle.  Outputs
-    are allocated under `with call.alloc():`, so that the allocator ties them
-    to the stream the call writes them on."""
-
-    __slots__ = ("ctx", "handle", "other")
-
-    def __init__(self, first: torch.Tensor, ctx: Optional[Context], stream, *tensors):
-        dev = first.device
-        if dev.type != "cuda":
-            raise ValueError("tensors must be on a CUDA device")
-        for t in tensors:
-            if t is not None and t.device != dev:
-                raise ValueError("tensors are on different devices")
-        self.ctx = _ctx_for(first, ctx)
-        self.other = None
-        if stream is None:
-            self.handle = torch.cuda.current_stream(dev).cuda_stream
-            return
-        if not hasattr(stream, "cuda_stream"):
-            stream = torch.cuda.ExternalStream(int(stream), device=dev)
-        self.handle = stream.cuda_stream
-        if self.handle != torch.cuda.current_stream(dev).cuda_stream:
-            self.other = stream
-            for t in (first, *tensors):  # they may be freed before the stream gets to the call
-                if t is not None:
-                    t.record_stream(stream)
-
-    def alloc(self):
-        return torch.cuda.stream(self.other) if self.other is not None else nullcontext()
-
-    def done(self, status: int) -> None:
-        if status != abi.HELIX_OK:
-            raise HelixError(status, self.ctx.last_error())
+def _begin(ctx: Optional[Context], stream, first: torch.Tensor, *rest):
+    """(context, stream handle, guard) of a call.  Outputs are allocated under
+    the guard, so that the allocator ties them to the stream that writes them."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError("tensors must be on a CUDA device")
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            raise ValueError("tensors are on different devices")
+    if ctx is None:
+        ctx = _default_ctx.get(index)
+        if ctx is None:
+            ctx = _default_ctx.setdefault(index, Context(index))
+    current = _raw_stream(index)
+    if stream is None:
+        return ctx, current, _HERE
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=first.device)
+    if stream.cuda_stream == current:
+        return ctx, current, _HERE
+    for t in (first, *rest):  # they may be freed before the stream gets to the call
+        if t is not None:
+            t.record_stream(stream)
+    return ctx, stream.cuda_stream, torch.cuda.stream(stream)
 
 
-def _empty8(shape, device) -> torch.Tensor:
+def _check(ctx: Context, status: int) -> None:
+    if status != abi.HELIX_OK:
+        raise HelixError(status, ctx.last_error())
+
+
+def _empty8(like: torch.Tensor, shape) -> torch.Tensor:
     """float8 tensor of `shape` whose rows start at multiples of 16 bytes."""
     cols = shape[-1]
-    held = torch.empty((*shape[:-1], -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)
-    return held if held.shape[-1] == cols else held[..., :cols]
+    if cols % 16 == 0:
+        return like.new_empty(shape, dtype=_F8)
+    return like.new_empty((*shape[:-1], (cols + 15) // 16 * 16), dtype=_F8)[..., :cols]
 
 
 class Norm(NamedTuple):
@@ -116,41 +121,35 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     torch.float8_e4m3fn gives 8 bits with a scale per 128 columns.  sum is s
     in the residual's type.  keep_rstd keeps 1 / sqrt(...) per row for
     rms_norm_grad."""
-    cols = x.shape[-1]
+    shape = x.shape
+    cols = shape[-1]
     rows = x.numel() // cols if cols else 0
-    d = abi.RmsNormDesc()
-    d.n_row, d.n_col, d.eps = rows, cols, eps
-    d.x_dtype = _dtype("x", x)
-    d.ld_x = _matrix("x", x)
-    d.sum_dtype = d.x_dtype
+    tx = _dtype("x", x.dtype)
+    ld_x = _matrix("x", x, shape)
+    tr, ld_res = tx, cols
     if residual is not None:
-        d.sum_dtype = _dtype("residual", residual)
-        d.ld_res = _matrix("residual", residual, x.shape)
+        tr, ld_res = _dtype("residual", residual.dtype), _matrix("residual", residual, shape)
     _vector("weight", weight, cols)
-    d.w_dtype = _dtype("weight", weight)
     out_dtype = x.dtype if out_dtype is None else out_dtype
-    try:
-        d.out_dtype = _OUT[out_dtype]
-    except KeyError:
-        raise TypeError(f"out_dtype {out_dtype} is not supported") from None
-    call = _Call(x, ctx, stream, residual, weight)
+    to = _dtype("out_dtype", out_dtype, _OUT)
+    ctx, handle, guard = _begin(ctx, stream, x, residual, weight)
     total = scale = rstd = None
-    with call.alloc():
-        if out_dtype == torch.float8_e4m3fn:
-            out = _empty8(x.shape, x.device)
-            scale = torch.empty((*x.shape[:-1], _groups(cols)), dtype=torch.float32, device=x.device)
-            d.ld_scale = scale.shape[-1]
-            d.ld_out = -(-cols // 16) * 16
+    with guard:
+        if out_dtype == _F8:
+            out = _empty8(x, shape)
+            scale = x.new_empty((*shape[:-1], _groups(cols)), dtype=_F32)
+            ld_out = (cols + 15) // 16 * 16
         else:
-            out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-            d.ld_out = cols
+            out = x.new_empty(shape, dtype=out_dtype)
+            ld_out = cols
         if residual is not None:
-            total = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-            d.ld_sum = cols
+            total = residual.new_empty(shape)
         if keep_rstd:
-            rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    call.done(call.ctx.lib.helix_rms_norm_encode(call.ctx.handle, call.handle, C.byref(d), _t(x), _t(residual),
-                                                 _t(weight), _t(out), _t(scale), _t(total), _t(rstd)))
+            rstd = x.new_empty(shape[:-1], dtype=_F32)
+    d = abi.RmsNormDesc(rows, cols, eps, tx, tr, to, _dtype("weight", weight.dtype), ld_x, ld_res, cols, ld_out,
+                        _groups(cols))
+    _check(ctx, ctx.lib.helix_rms_norm_encode(ctx.handle, handle, C.byref(d), _t(x), _t(residual), _t(weight),
+                                              _t(out), _t(scale), _t(total), _t(rstd)))
     return Norm(out, scale, x if total is None else total, rstd)
 
 
@@ -164,34 +163,31 @@ def rms_norm_grad(dout: torch.Tensor, sum: torch.Tensor, rstd: torch.Tensor, wei
     is passed through), dsum the one that reaches sum by another way; sum and
     rstd are what the forward pass gave.  dx has dout's type and dres, the
     same gradient for the residual, sum's; dweight is f32."""
-    cols = dout.shape[-1]
+    shape = dout.shape
+    cols = shape[-1]
     rows = dout.numel() // cols if cols else 0
-    d = abi.RmsNormDesc()
-    d.n_row, d.n_col = rows, cols
-    d.x_dtype, d.sum_dtype = _dtype("dout", dout), _dtype("sum", sum)
-    d.ld_dout, d.ld_sum = _matrix("dout", dout), _matrix("sum", sum, dout.shape)
+    tx, ts = _dtype("dout", dout.dtype), _dtype("sum", sum.dtype)
+    ld_dout, ld_sum, ld_dsum = _matrix("dout", dout, shape), _matrix("sum", sum, shape), cols
     if dsum is not None:
         if dsum.dtype != sum.dtype:
             raise TypeError("dsum must have sum's type")
-        d.ld_dsum = _matrix("dsum", dsum, dout.shape)
-    if rstd.dtype != torch.float32 or tuple(rstd.shape) != tuple(dout.shape[:-1]) or not rstd.is_contiguous():
+        ld_dsum = _matrix("dsum", dsum, shape)
+    if rstd.dtype != _F32 or rstd.shape != shape[:-1] or not rstd.is_contiguous():
         raise ValueError("rstd must be a dense float32 tensor with one value per row")
     _vector("weight", weight, cols)
-    d.w_dtype = _dtype("weight", weight)
-    call = _Call(dout, ctx, stream, sum, rstd, weight, dsum)
-    dres = None
-    with call.alloc():
-        dx = torch.empty(dout.shape, dtype=dout.dtype, device=dout.device)
-        dweight = torch.empty(cols, dtype=torch.float32, device=dout.device)
-        d.ld_dx = cols
-        if keep_dres and sum.dtype != dout.dtype:
-            dres = torch.empty(dout.shape, dtype=sum.dtype, device=dout.device)
-            d.ld_dres = cols
-        nbytes = call.ctx.lib.helix_rms_norm_grad_scratch_size(call.ctx.handle, C.byref(d))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dout.device) if nbytes else None
-    call.done(call.ctx.lib.helix_rms_norm_grad_encode(
-        call.ctx.handle, call.handle, C.byref(d), _t(dout), _t(sum), _t(rstd), _t(weight), _t(dsum), _t(dx),
-        _t(dres), _t(dweight), _t(scratch)))
+    ctx, handle, guard = _begin(ctx, stream, dout, sum, rstd, weight, dsum)
+    d = abi.RmsNormDesc(rows, cols, 0.0, tx, ts, tx, _dtype("weight", weight.dtype), 0, 0, ld_sum, 0, 0, ld_dout,
+                        ld_dsum, cols, cols)
+    lib, dres = ctx.lib, None
+    nbytes = lib.helix_rms_norm_grad_scratch_size(ctx.handle, C.byref(d))
+    with guard:
+        dx = dout.new_empty(shape)
+        dweight = dout.new_empty((cols,), dtype=_F32)
+        if keep_dres and ts != tx:
+            dres = sum.new_empty(shape)
+        scratch = dout.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    _check(ctx, lib.helix_rms_norm_grad_encode(ctx.handle, handle, C.byref(d), _t(dout), _t(sum), _t(rstd), _t(weight),
+                                               _t(dsum), _t(dx), _t(dres), _t(dweight), _t(scratch)))
     if keep_dres:
         return dx, dweight, dx if dres is None else dres
     return dx, dweight
@@ -206,20 +202,16 @@ def quantize8(x: torch.Tensor, *, blocks: bool = False, transpose: bool = False,
     of a weight, or (by rows) 128 tokens of a column under one scale."""
     if x.dim() != 2:
         raise ValueError("x must be a matrix")
-    d = abi.Quant8Desc()
-    d.n_row, d.n_col = x.shape
-    d.x_dtype = _dtype("x", x)
-    d.ld_x = _matrix("x", x)
-    d.form = abi.HELIX_SCALE_BLOCKS if blocks else abi.HELIX_SCALE_ROWS
-    d.transpose = transpose
-    rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape
-    call = _Call(x, ctx, stream)
-    with call.alloc():
-        q = _empty8((rows, cols), x.device)
-        scale = torch.empty((_groups(rows) if blocks else rows, _groups(cols)), dtype=torch.float32, device=x.device)
-    d.ld_q = -(-cols // 16) * 16
-    d.ld_scale = _groups(cols)
-    call.done(call.ctx.lib.helix_quant8_encode(call.ctx.handle, call.handle, C.byref(d), _t(x), _t(q), _t(scale)))
+    n_row, n_col = x.shape
+    tx, ld_x = _dtype("x", x.dtype), _matrix("x", x, x.shape)
+    rows, cols = (n_col, n_row) if transpose else (n_row, n_col)
+    ctx, handle, guard = _begin(ctx, stream, x)
+    with guard:
+        q = _empty8(x, (rows, cols))
+        scale = x.new_empty((_groups(rows) if blocks else rows, _groups(cols)), dtype=_F32)
+    d = abi.Quant8Desc(n_row, n_col, tx, abi.HELIX_SCALE_BLOCKS if blocks else abi.HELIX_SCALE_ROWS, transpose, ld_x,
+                       (cols + 15) // 16 * 16, _groups(cols))
+    _check(ctx, ctx.lib.helix_quant8_encode(ctx.handle, handle, C.byref(d), _t(x), _t(q), _t(scale)))
     return q, scale
 
 
@@ -230,54 +222,44 @@ def matmul8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
     a_scale (..., ceil(k / 128)); b_scale (ceil(n / 128), ceil(k / 128)) by
     blocks or (n, ceil(k / 128)) by rows.  Rows of a and b must start at
     multiples of 16 bytes, as rms_norm and quantize8 leave them."""
-    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
+    if a.dtype != _F8 or b.dtype != _F8:
         raise TypeError("a and b must be torch.float8_e4m3fn")
-    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+    if a_scale.dtype != _F32 or b_scale.dtype != _F32:
         raise TypeError("scales must be torch.float32")
     if b.dim() != 2 or a.shape[-1] != b.shape[1]:
         raise ValueError("b must be a matrix with as many columns as a")
     n, k = b.shape
-    groups = _groups(k)
-    d = abi.Matmul8Desc()
-    d.m, d.n, d.k = (a.numel() // k if k else 0), n, k
-    d.ld_a, d.ld_b = _matrix("a", a), _matrix("b", b)
-    d.ld_a_scale = _matrix("a_scale", a_scale, (*a.shape[:-1], groups))
-    d.b_form = abi.HELIX_SCALE_ROWS if tuple(b_scale.shape) == (n, groups) else abi.HELIX_SCALE_BLOCKS
-    d.ld_b_scale = _matrix("b_scale", b_scale, (n if d.b_form == abi.HELIX_SCALE_ROWS else _groups(n), groups))
-    try:
-        d.out_dtype = _IO[out_dtype]
-    except KeyError:
-        raise TypeError(f"out_dtype {out_dtype} is not supported") from None
-    d.ld_out = n
-    call = _Call(a, ctx, stream, a_scale, b, b_scale)
-    with call.alloc():
-        out = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
-    call.done(call.ctx.lib.helix_matmul8_encode(call.ctx.handle, call.handle, C.byref(d), _t(a), _t(a_scale), _t(b),
-                                                _t(b_scale), _t(out)))
+    groups, lead = _groups(k), a.shape[:-1]
+    rows = b_scale.shape == (n, groups)
+    to = _dtype("out_dtype", out_dtype)
+    strides = (_matrix("a", a, a.shape), _matrix("b", b, b.shape), n, _matrix("a_scale", a_scale, (*lead, groups)),
+               _matrix("b_scale", b_scale, (n if rows else _groups(n), groups)))
+    ctx, handle, guard = _begin(ctx, stream, a, a_scale, b, b_scale)
+    with guard:
+        out = a.new_empty((*lead, n), dtype=out_dtype)
+    d = abi.Matmul8Desc(a.numel() // k if k else 0, n, k, abi.HELIX_SCALE_ROWS if rows else abi.HELIX_SCALE_BLOCKS, to,
+                        *strides)
+    _check(ctx, ctx.lib.helix_matmul8_encode(ctx.handle, handle, C.byref(d), _t(a), _t(a_scale), _t(b), _t(b_scale),
+                                             _t(out)))
     return out
 
 
 def _tokens(name: str, t: torch.Tensor, shape, dtype) -> tuple[int, int]:
     """(token stride, sequence stride) of a (sequences, tokens, channels) tensor."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}")
     s, k, c = t.stride()
-    if shape[2] > 1 and c != 1:
+    if c != 1 and shape[2] > 1:
         raise ValueError(f"{name} needs unit stride along the channels")
     return k, s
 
 
 def _state(name: str, t: torch.Tensor, shape) -> int:
-    if t.dtype != torch.float32:
+    if t.dtype != _F32:
         raise TypeError(f"{name} must be torch.float32")
     return _matrix(name, t, shape)
-
-
-def _lengths(t: Optional[torch.Tensor], seqs: int) -> None:
-    if t is not None:
-        _vector("lengths", t, seqs, torch.int32)
 
 
 def gated_scan(v: torch.Tensor, g: torch.Tensor, h0: Optional[torch.Tensor] = None, *,
@@ -293,26 +275,29 @@ def gated_scan(v: torch.Tensor, g: torch.Tensor, h0: Optional[torch.Tensor] = No
     sequence) ends sequences early: later tokens keep the state and have y 0."""
     if v.dim() != 3:
         raise ValueError("v must be (sequences, tokens, channels)")
-    d = abi.GatedScanDesc()
-    d.n_seq, d.n_tok, d.n_chan = seqs, toks, chans = v.shape
-    d.io_dtype = _dtype("v", v)
-    d.s_v, d.seq_v = _tokens("v", v, v.shape, v.dtype)
-    d.s_g, d.seq_g = _tokens("g", g, v.shape, v.dtype)
-    _lengths(lengths, seqs)
+    shape, dtype = v.shape, v.dtype
+    seqs, toks, chans = shape
+    io = _dtype("v", dtype)
+    (s_v, seq_v), (s_g, seq_g) = _tokens("v", v, shape, dtype), _tokens("g", g, shape, dtype)
+    if lengths is not None:
+        _vector("lengths", lengths, seqs, _I32)
+    seq_h0 = seq_h1 = chans
     if h0 is not None:
-        d.seq_h0 = _state("h0", h0, (seqs, chans))
-    call = _Call(v, ctx, stream, g, h0, lengths, h1)
-    with call.alloc():
-        y = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        seq_h0 = _state("h0", h0, (seqs, chans))
+    if h1 is not None:
+        seq_h1 = _state("h1", h1, (seqs, chans))
+    ctx, handle, guard = _begin(ctx, stream, v, g, h0, lengths, h1)
+    states = None
+    with guard:
+        y = v.new_empty(shape)
         if h1 is None:
-            h1 = torch.empty((seqs, chans), dtype=torch.float32, device=v.device)
-        states = None
+            h1 = v.new_empty((seqs, chans), dtype=_F32)
         if keep_states:
-            states = torch.empty((seqs, -(-toks // abi.HELIX_GATED_CHUNK), chans), dtype=torch.float32, device=v.device)
-    d.s_y, d.seq_y = chans, toks * chans
-    d.seq_h1 = _state("h1", h1, (seqs, chans))
-    call.done(call.ctx.lib.helix_gated_scan_encode(call.ctx.handle, call.handle, C.byref(d), _t(v), _t(g), _t(h0),
-                                                   _t(lengths), _t(y), _t(h1), _t(states)))
+            states = v.new_empty((seqs, -(-toks // abi.HELIX_GATED_CHUNK), chans), dtype=_F32)
+    d = abi.GatedScanDesc(toks, seqs, chans, io, s_v, s_g, chans, 0, 0, 0, seq_v, seq_g, toks * chans, 0, 0, 0, seq_h0,
+                          seq_h1)
+    _check(ctx, ctx.lib.helix_gated_scan_encode(ctx.handle, handle, C.byref(d), _t(v), _t(g), _t(h0), _t(lengths),
+                                                _t(y), _t(h1), _t(states)))
     return (y, h1, states) if keep_states else (y, h1)
 
 
@@ -325,27 +310,25 @@ def gated_scan_grad(dy: torch.Tensor, v: torch.Tensor, g: torch.Tensor, states: 
     written into the tensors given (slices of one wider tensor, say) or new ones."""
     if v.dim() != 3:
         raise ValueError("v must be (sequences, tokens, channels)")
-    d = abi.GatedScanDesc()
-    d.n_seq, d.n_tok, d.n_chan = seqs, toks, chans = v.shape
-    d.io_dtype = _dtype("v", v)
-    d.s_v, d.seq_v = _tokens("v", v, v.shape, v.dtype)
-    d.s_g, d.seq_g = _tokens("g", g, v.shape, v.dtype)
-    d.s_dy, d.seq_dy = _tokens("dy", dy, v.shape, v.dtype)
-    if (states.dtype != torch.float32 or not states.is_contiguous()
-            or tuple(states.shape) != (seqs, -(-toks // abi.HELIX_GATED_CHUNK), chans)):
+    shape, dtype = v.shape, v.dtype
+    seqs, toks, chans = shape
+    io = _dtype("v", dtype)
+    (s_v, seq_v), (s_g, seq_g) = _tokens("v", v, shape, dtype), _tokens("g", g, shape, dtype)
+    s_dy, seq_dy = _tokens("dy", dy, shape, dtype)
+    if (states.dtype != _F32 or not states.is_contiguous()
+            or states.shape != (seqs, -(-toks // abi.HELIX_GATED_CHUNK), chans)):
         raise ValueError("states must be what gated_scan(keep_states=True) gave")
-    _lengths(lengths, seqs)
-    if dh1 is not None:
-        d.seq_dh1 = _state("dh1", dh1, (seqs, chans))
-    call = _Call(dy, ctx, stream, v, g, states, dh1, lengths, dv, dg)
-    with call.alloc():
-        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
-        dg = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dg is None else dg
-        dh0 = torch.empty((seqs, chans), dtype=torch.float32, device=v.device)
-    d.s_dv, d.seq_dv = _tokens("dv", dv, v.shape, v.dtype)
-    d.s_dg, d.seq_dg = _tokens("dg", dg, v.shape, v.dtype)
-    d.seq_dh0 = chans
-    call.done(call.ctx.lib.helix_gated_scan_grad_encode(
-        call.ctx.handle, call.handle, C.byref(d), _t(dy), _t(v), _t(g), _t(states), _t(dh1), _t(lengths), _t(dv),
-        _t(dg), _t(dh0)))
+    if lengths is not None:
+        _vector("lengths", lengths, seqs, _I32)
+    seq_dh1 = chans if dh1 is None else _state("dh1", dh1, (seqs, chans))
+    ctx, handle, guard = _begin(ctx, stream, dy, v, g, states, dh1, lengths, dv, dg)
+    with guard:
+        dv = v.new_empty(shape) if dv is None else dv
+        dg = v.new_empty(shape) if dg is None else dg
+        dh0 = v.new_empty((seqs, chans), dtype=_F32)
+    (s_dv, seq_dv), (s_dg, seq_dg) = _tokens("dv", dv, shape, dtype), _tokens("dg", dg, shape, dtype)
+    d = abi.GatedScanDesc(toks, seqs, chans, io, s_v, s_g, 0, s_dy, s_dv, s_dg, seq_v, seq_g, 0, seq_dy, seq_dv,
+                          seq_dg, 0, 0, seq_dh1, chans)
+    _check(ctx, ctx.lib.helix_gated_scan_grad_encode(ctx.handle, handle, C.byref(d), _t(dy), _t(v), _t(g), _t(states),
+                                                     _t(dh1), _t(lengths), _t(dv), _t(dg), _t(dh0)))
     return dv, dg, dh0

@@ -12,15 +12,16 @@
 
 namespace {
 
+// Makes ctx's device current for a call, and the caller's again after it.
 struct DeviceScope {
-    int prev = -1;
+    int restore = -1;
     explicit DeviceScope(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) cudaSetDevice(dev);
+        int cur = dev;
+        if (cudaGetDevice(&cur) == cudaSuccess && cur == dev) return;
+        if (cudaSetDevice(dev) == cudaSuccess) restore = cur;
     }
     ~DeviceScope() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+        if (restore >= 0) cudaSetDevice(restore);
     }
 };
 
