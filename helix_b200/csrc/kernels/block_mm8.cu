@@ -24,6 +24,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <cstring>
 
 #include "block_common.cuh"
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constan
     uint8_t* smem = tc::align1024(smem_raw);
     __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain;
     __shared__ uint32_t tmem_slot;
-    __shared__ float col_scale[2][QROWS ? BN : 1];
+    __shared__ __align__(16) float col_scale[2][QROWS ? BN : 4];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x % (unsigned)a.splits), tile = (int)(blockIdx.x / (unsigned)a.splits);
@@ -257,6 +258,301 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constan
     }
 }
 
+// ---------------------------------------------------------------------------
+// Large products: pairs of CTAs, tiles of 256 x BN.
+//
+// One CTA's MMA reads 128 + BN rows of shared memory per block; the pair's
+// MMA (cta_group::2) lets each CTA hold half of the columns' operand, so a
+// tile of 256 x 256 moves as many bytes per CTA as one of 128 x 128 for four
+// times the products, half of them each.  The grid is persistent, one CTA per
+// SM: the blocks of k of all of a pair's tiles run through one pipeline of
+// stages and TMEM buffers, and the next tile's MMAs run while the epilogue
+// writes.  An epilogue warp has 32 rows and half of the columns; it stages its
+// part in shared memory of its own and stores it by TMA.
+// ---------------------------------------------------------------------------
+// Warps 0 and 1 issue (2 and 3 fill up their warpgroup), 4-11 are the
+// epilogue.  The issuing warpgroup hands registers to the others, whose
+// accumulators take up to 128 each: 128 x 40 + 256 x 232 = 384 x 168, the
+// registers that the block is launched with.
+constexpr int kPairThreads = 32 * (4 + kEpiWarps);
+
+template <int BN>
+struct PairCfg {
+    static constexpr int kStageBytes = (kRows + BN / 2) * kBk;   // per CTA
+    static constexpr int kStages = BN == 256 ? 5 : 6;
+    static constexpr int kBufs = 512 / BN;
+    static constexpr int kRun = BN / 2;                          // columns of an epilogue warp
+    static constexpr int kOutBytes = BN == 256 ? 32 * 128 : 32 * 256;  // staging of an epilogue warp
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpiWarps * kOutBytes + 1024;
+};
+
+struct PairMaps {
+    CUtensorMap p, q, out;
+};
+
+// Tiles in strips of 8 tile rows, down the strip first: the tiles in flight
+// share rows of both operands in L2.
+__device__ __forceinline__ void pair_tile(int tile, int tiles_p, int tiles_q, int* tp, int* tq) {
+    constexpr int kStrip = 8;
+    const int strip = tile / (kStrip * tiles_q), first = strip * kStrip;
+    const int high = min(kStrip, tiles_p - first), in = tile - first * tiles_q;
+    *tp = first + in % high;
+    *tq = in / high;
+}
+
+template <int BN, bool QROWS, typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    mm8_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Mm8Params a) {
+    using Cfg = PairCfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = tc::align1024(smem_raw);
+    __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ __align__(16) float col_scale[2][QROWS ? BN : 4];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x & 1u), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+    const int tiles_p = (a.p.rows + 2 * kRows - 1) / (2 * kRows), n_tiles = tiles_p * a.tiles_q;
+    const int nkb = a.k_blocks;
+
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&maps.p);
+        prefetch_tmap(&maps.q);
+#pragma unroll
+        for (int i = 0; i < Cfg::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+#pragma unroll
+        for (int i = 0; i < Cfg::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 2 * kEpiWarps);
+        mbar_init(&drain, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc_pair(&tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // both CTAs' barriers and TMEM stand
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    auto wait = [&](uint64_t* bar, int phase) {
+        if (mbar_wait(bar, (uint32_t)(phase & 1), tc::kWaitBudget)) return true;
+        if (a.fault) atomicCAS(a.fault, 0u, (unsigned)kFaultProduct);
+        return false;
+    };
+
+    if (warp < 4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+      if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;  // blocks of k, over all tiles
+            bool ok = true;
+            for (int tile = pair; ok && tile < n_tiles; tile += pairs) {
+                int tp, tq;
+                pair_tile(tile, tiles_p, a.tiles_q, &tp, &tq);
+                const int row_p = (2 * tp + rank) * kRows, row_q = tq * BN + rank * (BN / 2);
+                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                    const int s = it % Cfg::kStages, turn = it / Cfg::kStages;
+                    if (turn > 0 && !(ok = wait(&empty[s], turn - 1))) break;
+                    uint8_t* st = smem + s * Cfg::kStageBytes;
+                    // the even CTA's barrier counts both CTAs' bytes
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * Cfg::kStageBytes);
+                    const uint32_t bar = cluster_addr(&full[s], 0);
+                    tma_load_2d_pair(st, &maps.p, bar, kb * kBk, row_p);
+                    tma_load_2d_pair(st + kRows * kBk, &maps.q, bar, kb * kBk, row_q);
+                }
+            }
+            // the loads issued land before the pair ends
+            if (rank == 0)
+                for (int j = it > Cfg::kStages ? it - Cfg::kStages : 0; j < it; ++j)
+                    mbar_wait(&full[j % Cfg::kStages], (uint32_t)((j / Cfg::kStages) & 1), tc::kWaitBudget);
+        }
+      } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(2 * kRows, BN);
+            const uint32_t base = smem_u32(smem);
+            const int mine = pair < n_tiles ? (n_tiles - pair + pairs - 1) / pairs : 0;
+            const int total = mine * nkb;
+            int it = 0;
+            for (; it < total; ++it) {
+                const int s = it % Cfg::kStages, b = it % Cfg::kBufs;
+                if (it >= Cfg::kBufs && !wait(&acc_empty[b], it / Cfg::kBufs - 1)) break;
+                if (!wait(&full[s], it / Cfg::kStages)) break;
+                tc_fence_after();
+                const uint64_t dp = sdesc_sw128(base + s * Cfg::kStageBytes, 16, 1024);
+                const uint64_t dq = sdesc_sw128(base + s * Cfg::kStageBytes + kRows * kBk, 16, 1024);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    mma_e4m3_pair(tmem + b * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
+                mma_commit_pair(&empty[s]);
+                mma_commit_pair(&acc_full[b]);
+            }
+            if (it < total) {
+                mma_commit_pair(&drain);
+                mbar_wait(&drain, 0, tc::kWaitBudget);
+            }
+        }
+      }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int half = (warp - 4) / 4;
+        const int row = 32 * (warp & 3) + lane;      // the TMEM lane
+        const int c0 = half * Cfg::kRun;
+        const int tid = threadIdx.x - 128;
+        uint8_t* mine = smem + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
+        const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)c0;
+        bool alive = true;
+        int it = 0;
+        for (int tile = pair; tile < n_tiles; tile += pairs) {
+            int tp, tq;
+            pair_tile(tile, tiles_p, a.tiles_q, &tp, &tq);
+            const int p0 = (2 * tp + rank) * kRows, q0 = tq * BN;
+            const int pr = min(p0 + row, a.p.rows - 1);
+            const float* ps = a.p.scale + (int64_t)(pr / a.p.per) * a.p.ld_scale;
+            const int qr = min(q0 + (QROWS ? tid : c0), a.q.rows - 1);
+            const float* qs = a.q.scale + (int64_t)(qr / a.q.per) * a.q.ld_scale;
+            const bool stage = QROWS && tid < BN;
+            float ps_next = __ldg(ps), qs_next = stage || !QROWS ? __ldg(qs) : 0.0f;
+            if constexpr (QROWS) {
+                named_sync(1, 32 * kEpiWarps);  // the last tile's scales are read
+                if (stage) col_scale[0][tid] = qs_next;
+                named_sync(1, 32 * kEpiWarps);
+            }
+            uint64_t acc[Cfg::kRun / 2];
+#pragma unroll
+            for (int i = 0; i < Cfg::kRun / 2; ++i) acc[i] = 0;
+            for (int kb = 0; kb < nkb; ++kb, ++it) {
+                const int b = it % Cfg::kBufs;
+                const float r = QROWS ? ps_next : ps_next * qs_next;
+                const uint64_t r2 = f2_of(r, r);
+                if (kb + 1 < nkb) {
+                    ps_next = __ldg(ps + kb + 1);
+                    if (stage || !QROWS) qs_next = __ldg(qs + kb + 1);
+                }
+                if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[b], it / Cfg::kBufs));
+                if (alive) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < Cfg::kRun; c += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(lane_addr + b * BN + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint64_t d = f2_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+                            uint64_t& o = acc[c / 2 + e];
+                            if constexpr (QROWS) {
+                                const float2 cs =
+                                    *reinterpret_cast<const float2*>(&col_scale[kb & 1][c0 + c + 2 * e]);
+                                o = f2_fma(d, f2_mul(r2, f2_of(cs.x, cs.y)), o);
+                            } else {
+                                o = f2_fma(d, r2, o);
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[b], 0));
+                }
+                if constexpr (QROWS) {
+                    if (stage) col_scale[(kb + 1) & 1][tid] = qs_next;
+                    named_sync(1, 32 * kEpiWarps);
+                }
+            }
+            // the warp's 32 rows x kRun columns
+            constexpr int kPer = 128 / (int)sizeof(T);      // columns of a 128-byte row
+            constexpr int kRound = Cfg::kOutBytes / 32 / 128 * kPer < Cfg::kRun ? Cfg::kOutBytes / 32 / 128 * kPer : Cfg::kRun;
+            if (a.vec_out) {
+#pragma unroll
+                for (int c = 0; c < Cfg::kRun; c += kRound) {
+                    bulk_wait_read0();  // (lane 0) the staging's last store has been read
+                    __syncwarp();
+#pragma unroll
+                    for (int x = 0; x < kRound; x += kPer) {
+                        uint8_t* box = mine + x / kPer * 32 * 128;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {  // 16-byte units of the lane's row
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float lo, up;
+                                if constexpr (sizeof(T) == 2) {
+                                    f2_to(acc[(c + x) / 2 + 4 * u + e], lo, up);
+                                    w[e] = bf16x2(lo, up);
+                                } else {
+                                    f2_to(acc[(c + x) / 2 + 2 * u + e / 2], lo, up);
+                                    w[e] = __float_as_uint(e & 1 ? up : lo);
+                                }
+                            }
+                            *reinterpret_cast<uint4*>(box + sw128_off(lane, u)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+#pragma unroll
+                        for (int x = 0; x < kRound; x += kPer)
+                            if (p0 + 32 * (warp & 3) < a.p.rows && q0 + c0 + c + x < a.q.rows)
+                                tma_store_2d(&maps.out, smem_u32(mine) + x / kPer * 32 * 128, q0 + c0 + c + x,
+                                             p0 + 32 * (warp & 3));
+                        bulk_commit();
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < Cfg::kRun; c += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f2_to(acc[c / 2 + e], v[2 * e], v[2 * e + 1]);
+                    st_out<T>(a, p0 + row, q0 + c0 + c, 8, v);
+                }
+            }
+        }
+        bulk_wait0();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // neither CTA leaves, or frees TMEM, under the other
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free_pair(tmem, 512);
+    }
+}
+
+template <int BN, bool QROWS, typename T>
+int launch_pair_t(const PairMaps& maps, const Mm8Params& p, int ctas, void* stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = PairCfg<BN>::kSmem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, mm8_pair_kernel<BN, QROWS, T>, maps, p);
+}
+
+template <int BN>
+int launch_pair_n(bool qrows, helix_dtype out, const PairMaps& maps, const Mm8Params& p, int ctas, void* stream) {
+    if (out == HELIX_F32)
+        return qrows ? launch_pair_t<BN, true, float>(maps, p, ctas, stream)
+                     : launch_pair_t<BN, false, float>(maps, p, ctas, stream);
+    return qrows ? launch_pair_t<BN, true, __nv_bfloat16>(maps, p, ctas, stream)
+                 : launch_pair_t<BN, false, __nv_bfloat16>(maps, p, ctas, stream);
+}
+
+template <int BN>
+int configure_pair_n() {
+    const void* k[] = {(const void*)mm8_pair_kernel<BN, true, float>, (const void*)mm8_pair_kernel<BN, false, float>,
+                       (const void*)mm8_pair_kernel<BN, true, __nv_bfloat16>,
+                       (const void*)mm8_pair_kernel<BN, false, __nv_bfloat16>};
+    for (const void* f : k) {
+        const int e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairCfg<BN>::kSmem);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
 template <int BN, bool QROWS, typename T>
 int launch_mm8_t(const Mm8Maps& maps, const Mm8Params& p, int tiles, void* stream) {
     cudaLaunchConfig_t cfg{};
@@ -308,7 +604,22 @@ bool make_map_u8(const helix_ctx* ctx, CUtensorMap* m, const void* base, int64_t
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int tiles_of(int rows, int per) { return (rows + per - 1) / per; }
+// out in boxes of 32 rows x 128 bytes, swizzled; what lies past the ends is not written.
+bool make_map_out(const helix_ctx* ctx, CUtensorMap* m, void* base, int64_t rows, int64_t cols, int64_t ld,
+                  helix_dtype type) {
+    const auto fn = reinterpret_cast<tc::EncodeFn>(ctx->encode_tiled);
+    const int size = type == HELIX_F32 ? 4 : 2;
+    if (rows == 1) ld = (cols + 7) / 8 * 8;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32};
+    cuuint32_t es[2] = {1, 1};
+    return fn(m, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides,
+              box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int tiles_of(int64_t rows, int64_t per) { return (int)((rows + per - 1) / per); }
 
 }  // namespace
 
@@ -317,7 +628,9 @@ int configure_mm8() {
     if ((e = configure_mm8_n<16>()) != cudaSuccess) return e;
     if ((e = configure_mm8_n<32>()) != cudaSuccess) return e;
     if ((e = configure_mm8_n<64>()) != cudaSuccess) return e;
-    return configure_mm8_n<128>();
+    if ((e = configure_mm8_n<128>()) != cudaSuccess) return e;
+    if ((e = configure_pair_n<128>()) != cudaSuccess) return e;
+    return configure_pair_n<256>();
 }
 
 Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
@@ -327,12 +640,28 @@ Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
     const int64_t tiles = (int64_t)tiles_of(pl.swap ? d.n : d.m, kRows) * tiles_of(pl.swap ? d.m : d.n, pl.bn);
     const int kb = tiles_of(d.k, kBk);
     pl.splits = 1;
+    if (const char* e = getenv("XP")) { if (!pl.swap) { pl.pair = atoi(e) > 0; if (pl.pair) { pl.bn = atoi(e); return pl; } } }
     while (pl.splits < 8 && tiles * pl.splits * 2 <= 2 * ctx->n_sm && kb >= 4 * pl.splits) pl.splits *= 2;
     return pl;
 }
 
 int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan& pl, Mm8Params p, const void* a,
                const void* b, void* stream) {
+    if (pl.pair) {
+        PairMaps maps;
+        std::memset(&maps, 0, sizeof(maps));
+        if (!make_map_u8(ctx, &maps.p, a, d.m, d.k, d.ld_a, kRows) ||
+            !make_map_u8(ctx, &maps.q, b, d.n, d.k, d.ld_b, pl.bn / 2) ||
+            (p.vec_out && !make_map_out(ctx, &maps.out, p.out, d.m, d.n, d.ld_out, d.out_dtype)))
+            return cudaErrorInvalidValue;
+        p.tiles_q = tiles_of(d.n, pl.bn);
+        const int64_t tiles = (int64_t)tiles_of(d.m, 2 * kRows) * p.tiles_q;
+        // a pair counts its blocks of k in 32 bits
+        if (tiles > INT32_MAX / 2 || (tiles / (ctx->n_sm / 2) + 1) * p.k_blocks > INT32_MAX) return cudaErrorInvalidValue;
+        const int ctas = 2 * (int)std::min<int64_t>(tiles, ctx->n_sm / 2);
+        return pl.bn == 256 ? launch_pair_n<256>(p.q.per == 1, d.out_dtype, maps, p, ctas, stream)
+                            : launch_pair_n<128>(p.q.per == 1, d.out_dtype, maps, p, ctas, stream);
+    }
     Mm8Maps maps;
     std::memset(&maps, 0, sizeof(maps));
     const bool ok = pl.swap ? make_map_u8(ctx, &maps.p, b, d.n, d.k, d.ld_b, kRows) &&

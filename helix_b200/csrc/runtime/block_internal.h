@@ -61,6 +61,7 @@ struct Mm8Operand {
 };
 // How one product runs.
 struct Mm8Plan {
+    bool pair;             // pairs of CTAs on tiles of 256 x bn (bn 128 or 256)
     bool swap;             // P is b (few rows of a: they become the columns)
     int  bn;               // columns of a tile
     int  splits;           // CTAs of a cluster that share a tile's blocks of k
