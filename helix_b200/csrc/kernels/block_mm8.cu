@@ -24,7 +24,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cstdlib>
 #include <cstring>
 
 #include "block_common.cuh"
@@ -45,15 +44,28 @@ constexpr int kMmThreads = 32 * (2 + kEpiWarps);
 template <int BN>
 struct Mm8Cfg {
     static constexpr int kStageBytes = (kRows + BN) * kBk;
-    static constexpr int kStages = BN == 128 ? 3 : BN == 64 ? 4 : BN == 32 ? 5 : 6;  // two CTAs per SM
+    static constexpr int kStages = BN == 64 ? 4 : BN == 32 ? 5 : 6;
+    static constexpr int kPerSm = BN == 128 ? 1 : 2;         // CTAs that fit
     static constexpr int kBufs = BN >= 128 ? 2 : 4;          // TMEM accumulators
     static constexpr int kCols = kBufs * BN < 32 ? 32 : kBufs * BN;
     static constexpr int kRun = BN / 2;                      // columns of an epilogue thread
+    static constexpr int kLoad = kRun < 32 ? kRun : 32;      // of them, read at once
+    static constexpr int kPiece = 16;                        // blocks of k whose column scales are staged at once
     static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
 };
 
 struct Mm8Maps {
     CUtensorMap p, q;
+};
+
+// A place in a ring of N barriers, and the parity of its turn.
+template <int N>
+struct Ring {
+    int      at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) at = 0, parity ^= 1u;
+    }
 };
 
 // The first n of v: consecutive columns qc.. of row pr of P.
@@ -78,13 +90,14 @@ __device__ __forceinline__ void st_out(const Mm8Params& a, int pr, int qc, int n
 }
 
 template <int BN, bool QROWS, typename T>
-__global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constant__ Mm8Maps maps, const Mm8Params a) {
+__global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(const __grid_constant__ Mm8Maps maps,
+                                                            const __grid_constant__ Mm8Params a) {
     using Cfg = Mm8Cfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = tc::align1024(smem_raw);
     __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain;
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float col_scale[2][QROWS ? BN : 4];
+    __shared__ __align__(16) float col_scale[QROWS ? Cfg::kPiece : 1][QROWS ? BN : 4];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x % (unsigned)a.splits), tile = (int)(blockIdx.x / (unsigned)a.splits);
@@ -92,24 +105,31 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constan
     const int kb0 = (int)((int64_t)a.k_blocks * rank / a.splits);
     const int nkb = (int)((int64_t)a.k_blocks * (rank + 1) / a.splits) - kb0;
 
+    auto load = [&](int i, int s) {
+        uint8_t* st = smem + s * Cfg::kStageBytes;
+        mbar_expect_tx(&full[s], Cfg::kStageBytes);
+        tma_load_2d(st, &maps.p, &full[s], (kb0 + i) * kBk, p0);
+        tma_load_2d(st + kRows * kBk, &maps.q, &full[s], (kb0 + i) * kBk, q0);
+    };
     if (threadIdx.x == 0) {
-        prefetch_tmap(&maps.p);
-        prefetch_tmap(&maps.q);
 #pragma unroll
         for (int i = 0; i < Cfg::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
 #pragma unroll
         for (int i = 0; i < Cfg::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps);
         mbar_init(&drain, 1);
         fence_mbar_init();
+        // the first loads wait for nobody
+        for (int i = 0; i < Cfg::kStages && i < nkb; ++i) load(i, i);
     }
+    __syncwarp();
     if (warp == 1) tmem_alloc(&tmem_slot, Cfg::kCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    auto wait = [&](uint64_t* bar, int phase) {
-        if (mbar_wait(bar, (uint32_t)(phase & 1), tc::kWaitBudget)) return true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_wait(bar, parity, tc::kWaitBudget)) return true;
         if (a.fault) atomicCAS(a.fault, 0u, (unsigned)kFaultProduct);
         return false;
     };
@@ -120,14 +140,12 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constan
 
     if (warp == 0) {
         if (lane == 0) {
-            int i = 0;
+            Ring<Cfg::kStages> st;
+            int i = min(Cfg::kStages, nkb);
             for (; i < nkb; ++i) {
-                const int s = i % Cfg::kStages, turn = i / Cfg::kStages;
-                if (turn > 0 && !wait(&empty[s], turn - 1)) break;
-                uint8_t* st = smem + s * Cfg::kStageBytes;
-                mbar_expect_tx(&full[s], Cfg::kStageBytes);
-                tma_load_2d(st, &maps.p, &full[s], (kb0 + i) * kBk, p0);
-                tma_load_2d(st + kRows * kBk, &maps.q, &full[s], (kb0 + i) * kBk, q0);
+                if (!wait(&empty[st.at], st.parity)) break;
+                load(i, st.at);
+                st.next();
             }
             // whatever the other warps do, the loads issued land before the CTA ends
             for (int j = i > Cfg::kStages ? i - Cfg::kStages : 0; j < i; ++j)
@@ -137,19 +155,28 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constan
         if (lane == 0) {
             constexpr uint32_t idesc = idesc_e4m3(kRows, BN);
             const uint32_t base = smem_u32(smem);
+            Ring<Cfg::kStages> st;
+            Ring<Cfg::kBufs> buf;
+            // A wait costs its latency even when nothing is left to wait for;
+            // the next block's two are polled between its issue and its commits.
+            bool ready = false, free = true;
             int i = 0;
             for (; i < nkb; ++i) {
-                const int s = i % Cfg::kStages, b = i % Cfg::kBufs;
-                if (i >= Cfg::kBufs && !wait(&acc_empty[b], i / Cfg::kBufs - 1)) break;
-                if (!wait(&full[s], i / Cfg::kStages)) break;
+                if (!free && !wait(&acc_empty[buf.at], buf.parity ^ 1u)) break;
+                if (!ready && !wait(&full[st.at], st.parity)) break;
                 tc_fence_after();
-                const uint64_t dp = sdesc_sw128(base + s * Cfg::kStageBytes, 16, 1024);
-                const uint64_t dq = sdesc_sw128(base + s * Cfg::kStageBytes + kRows * kBk, 16, 1024);
+                const uint32_t from = base + st.at * Cfg::kStageBytes;
+                const uint64_t dp = sdesc_sw128(from, 16, 1024), dq = sdesc_sw128(from + kRows * kBk, 16, 1024);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
-                    mma_e4m3(tmem + b * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
-                mma_commit(&empty[s]);
-                mma_commit(&acc_full[b]);
+                    mma_e4m3(tmem + buf.at * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
+                uint64_t *done = &acc_full[buf.at], *read = &empty[st.at];
+                st.next();
+                buf.next();
+                ready = i + 1 < nkb && mbar_try_wait(&full[st.at], st.parity);
+                free = i + 1 < Cfg::kBufs || mbar_try_wait(&acc_empty[buf.at], buf.parity ^ 1u);
+                mma_commit(done);
+                mma_commit(read);
             }
             if (i < nkb) {
                 mma_commit(&drain);
@@ -157,55 +184,67 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constan
             }
         }
     } else {
-        const int half = (warp - 2) / 4;
-        const int row = 32 * (warp & 3) + lane;                   // the TMEM lane
-        const int c0 = half * Cfg::kRun;                          // the thread's first column
-        const int tid = threadIdx.x - 64;                         // 0 .. 255
-        const int pr = min(p0 + row, a.p.rows - 1);
-        const float* ps = a.p.scale + (int64_t)(pr / a.p.per) * a.p.ld_scale + kb0;
-        // QROWS: thread tid < BN stages column tid's scale; else one scale for the tile
-        const int qr = min(q0 + (QROWS ? tid : 0), a.q.rows - 1);
-        const float* qs = a.q.scale + (int64_t)(qr / a.q.per) * a.q.ld_scale + kb0;
-        const bool stage = QROWS && tid < BN;
-        float ps_next = nkb > 0 ? __ldg(ps) : 0.0f;
-        float qs_next = nkb > 0 && (stage || !QROWS) ? __ldg(qs) : 0.0f;
-        if constexpr (QROWS) {
-            if (stage) col_scale[0][tid] = qs_next;
-            named_sync(1, 32 * kEpiWarps);
-        }
-        bool alive = true;  // once a wait has run out the warp only keeps its turns at the barrier
+        const int row = 32 * (warp & 3) + lane;       // the TMEM lane
+        const int c0 = (warp - 2) / 4 * Cfg::kRun;    // the thread's first column
+        const int tid = threadIdx.x - 64;             // 0 .. 255
+        const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)c0;
+        // the row's scale two blocks ahead; the columns', where they share
+        // one, too
+        const float* ps = a.p.scale + (int64_t)(min(p0 + row, a.p.rows - 1) / a.p.per) * a.p.ld_scale + kb0;
+        const float* qs = a.q.scale + (int64_t)(min(q0, a.q.rows - 1) / a.q.per) * a.q.ld_scale + kb0;
+        float ps_next = __ldg(ps), ps_then = __ldg(ps + min(1, nkb - 1));
+        float qs_next = QROWS ? 1.0f : __ldg(qs), qs_then = QROWS ? 1.0f : __ldg(qs + min(1, nkb - 1));
+        // column scales of kPiece blocks: value j of the piece at i is block
+        // i + j % kPiece of column j / kPiece
+        constexpr int kMine = (BN * Cfg::kPiece + 32 * kEpiWarps - 1) / (32 * kEpiWarps);
+        float piece[kMine];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) {
+                const int e = tid + 32 * kEpiWarps * j, q = min(q0 + e / Cfg::kPiece, a.q.rows - 1);
+                piece[j] = __ldg(a.q.scale + (int64_t)q * a.q.ld_scale + kb0 + min(i + e % Cfg::kPiece, nkb - 1));
+            }
+        };
+        if (QROWS) fetch(0);
+        Ring<Cfg::kBufs> buf;
+        bool alive = true;  // once a wait has run out no other is waited for, and the rest is garbage
         for (int i = 0; i < nkb; ++i) {
-            const int b = i % Cfg::kBufs;
-            const float r = QROWS ? ps_next : ps_next * qs_next;
-            if (i + 1 < nkb) {
-                ps_next = __ldg(ps + i + 1);
-                if (stage || !QROWS) qs_next = __ldg(qs + i + 1);
-            }
-            if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[b], i / Cfg::kBufs));
-            if (alive) {
-                tc_fence_after();
-                const uint32_t t = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(b * BN + c0);
-                constexpr int kStep = Cfg::kRun < 16 ? 8 : 16;
+            if (QROWS && i % Cfg::kPiece == 0) {
+                named_sync(1, 32 * kEpiWarps);  // the last piece is read
 #pragma unroll
-                for (int c = 0; c < Cfg::kRun; c += kStep) {
-                    float v[kStep];
-                    if constexpr (kStep == 8)
-                        tmem_ld8(t + c, v);
-                    else
-                        tmem_ld16(t + c, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < kStep; ++e)
-                        acc[c + e] += v[e] * (QROWS ? r * col_scale[i & 1][c0 + c + e] : r);
+                for (int j = 0; j < kMine; ++j) {
+                    const int e = tid + 32 * kEpiWarps * j;
+                    if (e < BN * Cfg::kPiece) col_scale[e % Cfg::kPiece][e / Cfg::kPiece] = piece[j];
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[b]);
-            }
-            if constexpr (QROWS) {
-                if (stage) col_scale[(i + 1) & 1][tid] = qs_next;
                 named_sync(1, 32 * kEpiWarps);
+                if (i + Cfg::kPiece < nkb) fetch(i + Cfg::kPiece);
             }
+            const float r = QROWS ? ps_next : ps_next * qs_next;
+            ps_next = ps_then;
+            ps_then = __ldg(ps + min(i + 2, nkb - 1));
+            if constexpr (!QROWS) {
+                qs_next = qs_then;
+                qs_then = __ldg(qs + min(i + 2, nkb - 1));
+            }
+            if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[buf.at], buf.parity));
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < Cfg::kRun; c += Cfg::kLoad) {
+                uint32_t v[Cfg::kLoad];
+                tmem_ld(lane_addr + buf.at * BN + c, v);
+                tmem_wait_ld(v);
+                if (c + Cfg::kLoad == Cfg::kRun) {  // all read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[buf.at]);
+                }
+#pragma unroll
+                for (int e = 0; e < Cfg::kLoad; ++e) {
+                    const float s = QROWS ? r * col_scale[i % Cfg::kPiece][c0 + c + e] : r;
+                    acc[c + e] = fmaf(__uint_as_float(v[e]), s, acc[c + e]);
+                }
+            }
+            buf.next();
         }
         if (a.splits == 1) {
 #pragma unroll
@@ -270,10 +309,10 @@ __global__ void __launch_bounds__(kMmThreads, 2) mm8_kernel(const __grid_constan
 // writes.  An epilogue warp has 32 rows and half of the columns; it stages its
 // part in shared memory of its own and stores it by TMA.
 // ---------------------------------------------------------------------------
-// Warps 0 and 1 issue (2 and 3 fill up their warpgroup), 4-11 are the
-// epilogue.  The issuing warpgroup hands registers to the others, whose
-// accumulators take up to 128 each: 128 x 40 + 256 x 232 = 384 x 168, the
-// registers that the block is launched with.
+// Warps 0 and 1 issue, 2 and 3 gather column scales, 4-11 are the epilogue: 32
+// rows and half of the columns each.  The first warpgroup hands registers to
+// the others, whose accumulators take up to 128 each: 128 x 40 + 256 x 232 =
+// 384 x 168, the registers that the block is launched with.
 constexpr int kPairThreads = 32 * (4 + kEpiWarps);
 
 template <int BN>
@@ -282,7 +321,8 @@ struct PairCfg {
     static constexpr int kStages = BN == 256 ? 5 : 6;
     static constexpr int kBufs = 512 / BN;
     static constexpr int kRun = BN / 2;                          // columns of an epilogue warp
-    static constexpr int kOutBytes = BN == 256 ? 32 * 128 : 32 * 256;  // staging of an epilogue warp
+    static constexpr int kScales = 4;                            // blocks of column scales staged
+    static constexpr int kOutBytes = 32 * 128;                   // staging of an epilogue warp
     static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpiWarps * kOutBytes + 1024;
 };
 
@@ -307,8 +347,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = tc::align1024(smem_raw);
     __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain;
+    __shared__ uint64_t sc_full[Cfg::kScales], sc_empty[Cfg::kScales];
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float col_scale[2][QROWS ? BN : 4];
+    __shared__ __align__(16) float col_scale[Cfg::kScales][QROWS ? BN : 4];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x & 1u), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
@@ -322,6 +363,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         for (int i = 0; i < Cfg::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
 #pragma unroll
         for (int i = 0; i < Cfg::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 2 * kEpiWarps);
+#pragma unroll
+        for (int i = 0; i < Cfg::kScales; ++i) mbar_init(&sc_full[i], 1), mbar_init(&sc_empty[i], kEpiWarps);
         mbar_init(&drain, 1);
         fence_mbar_init();
     }
@@ -332,166 +375,202 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    auto wait = [&](uint64_t* bar, int phase) {
-        if (mbar_wait(bar, (uint32_t)(phase & 1), tc::kWaitBudget)) return true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_wait(bar, parity, tc::kWaitBudget)) return true;
         if (a.fault) atomicCAS(a.fault, 0u, (unsigned)kFaultProduct);
         return false;
     };
 
     if (warp < 4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-      if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;  // blocks of k, over all tiles
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0 && lane == 0) {
+            Ring<Cfg::kStages> st;  // runs over the blocks of k of all tiles
+            int issued = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < n_tiles; tile += pairs) {
                 int tp, tq;
                 pair_tile(tile, tiles_p, a.tiles_q, &tp, &tq);
                 const int row_p = (2 * tp + rank) * kRows, row_q = tq * BN + rank * (BN / 2);
-                for (int kb = 0; kb < nkb; ++kb, ++it) {
-                    const int s = it % Cfg::kStages, turn = it / Cfg::kStages;
-                    if (turn > 0 && !(ok = wait(&empty[s], turn - 1))) break;
-                    uint8_t* st = smem + s * Cfg::kStageBytes;
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (issued >= Cfg::kStages && !(ok = wait(&empty[st.at], st.parity ^ 1u))) break;
+                    uint8_t* to = smem + st.at * Cfg::kStageBytes;
                     // the even CTA's barrier counts both CTAs' bytes
-                    if (rank == 0) mbar_expect_tx(&full[s], 2 * Cfg::kStageBytes);
-                    const uint32_t bar = cluster_addr(&full[s], 0);
-                    tma_load_2d_pair(st, &maps.p, bar, kb * kBk, row_p);
-                    tma_load_2d_pair(st + kRows * kBk, &maps.q, bar, kb * kBk, row_q);
+                    if (rank == 0) mbar_expect_tx(&full[st.at], 2 * Cfg::kStageBytes);
+                    const uint32_t bar = cluster_addr(&full[st.at], 0);
+                    tma_load_2d_pair(to, &maps.p, bar, kb * kBk, row_p);
+                    tma_load_2d_pair(to + kRows * kBk, &maps.q, bar, kb * kBk, row_q);
+                    st.next();
+                    ++issued;
                 }
             }
             // the loads issued land before the pair ends
             if (rank == 0)
-                for (int j = it > Cfg::kStages ? it - Cfg::kStages : 0; j < it; ++j)
+                for (int j = issued > Cfg::kStages ? issued - Cfg::kStages : 0; j < issued; ++j)
                     mbar_wait(&full[j % Cfg::kStages], (uint32_t)((j / Cfg::kStages) & 1), tc::kWaitBudget);
-        }
-      } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        } else if (warp == 1 && lane == 0 && rank == 0) {
             constexpr uint32_t idesc = idesc_e4m3(2 * kRows, BN);
             const uint32_t base = smem_u32(smem);
             const int mine = pair < n_tiles ? (n_tiles - pair + pairs - 1) / pairs : 0;
             const int total = mine * nkb;
+            Ring<Cfg::kStages> st;
+            Ring<Cfg::kBufs> buf;
+            // A wait costs its latency even when nothing is left to wait for;
+            // the next block's two are polled between its issue and its commits.
+            bool ready = total > 0 && mbar_try_wait(&full[0], 0), free = true;
             int it = 0;
             for (; it < total; ++it) {
-                const int s = it % Cfg::kStages, b = it % Cfg::kBufs;
-                if (it >= Cfg::kBufs && !wait(&acc_empty[b], it / Cfg::kBufs - 1)) break;
-                if (!wait(&full[s], it / Cfg::kStages)) break;
+                if (!free && !wait(&acc_empty[buf.at], buf.parity ^ 1u)) break;
+                if (!ready && !wait(&full[st.at], st.parity)) break;
                 tc_fence_after();
-                const uint64_t dp = sdesc_sw128(base + s * Cfg::kStageBytes, 16, 1024);
-                const uint64_t dq = sdesc_sw128(base + s * Cfg::kStageBytes + kRows * kBk, 16, 1024);
+                const uint32_t from = base + st.at * Cfg::kStageBytes;
+                const uint64_t dp = sdesc_sw128(from, 16, 1024), dq = sdesc_sw128(from + kRows * kBk, 16, 1024);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
-                    mma_e4m3_pair(tmem + b * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
-                mma_commit_pair(&empty[s]);
-                mma_commit_pair(&acc_full[b]);
+                    mma_e4m3_pair(tmem + buf.at * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
+                uint64_t *done = &acc_full[buf.at], *read = &empty[st.at];
+                st.next();
+                buf.next();
+                ready = it + 1 < total && mbar_try_wait(&full[st.at], st.parity);
+                free = it + 1 < Cfg::kBufs || mbar_try_wait(&acc_empty[buf.at], buf.parity ^ 1u);
+                mma_commit_pair(done);
+                mma_commit_pair(read);
             }
             if (it < total) {
                 mma_commit_pair(&drain);
                 mbar_wait(&drain, 0, tc::kWaitBudget);
             }
+        } else if (QROWS && warp >= 2) {
+            // column scales: warp 2 the even blocks, warp 3 the odd ones, the
+            // next one's loads in flight
+            constexpr int kPer = BN / 32;
+            float next[kPer];
+            auto fetch = [&](int it) {
+                const int tile = pair + it / nkb * pairs;
+                if (tile >= n_tiles) return;
+                int tp, tq;
+                pair_tile(tile, tiles_p, a.tiles_q, &tp, &tq);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    const int qr = min(tq * BN + 32 * j + lane, a.q.rows - 1);
+                    next[j] = __ldg(a.q.scale + (int64_t)qr * a.q.ld_scale + it % nkb);
+                }
+            };
+            const int mine = pair < n_tiles ? (n_tiles - pair + pairs - 1) / pairs : 0;
+            const int total = mine * nkb;
+            if (warp - 2 < total) fetch(warp - 2);
+            for (int it = warp - 2; it < total; it += 2) {
+                const int slot = it % Cfg::kScales;
+                float cur[kPer];
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) cur[j] = next[j];
+                if (it + 2 < total) fetch(it + 2);
+                if (it >= Cfg::kScales && !__all_sync(0xffffffffu, wait(&sc_empty[slot], (uint32_t)(it / Cfg::kScales - 1) & 1u))) break;
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) col_scale[slot][32 * j + lane] = cur[j];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_full[slot]);
+            }
         }
-      }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        const int half = (warp - 4) / 4;
         const int row = 32 * (warp & 3) + lane;      // the TMEM lane
-        const int c0 = half * Cfg::kRun;
-        const int tid = threadIdx.x - 128;
-        uint8_t* mine = smem + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
+        const int c0 = (warp - 4) / 4 * Cfg::kRun;   // the warp's first column
+        const uint32_t staging = smem_u32(smem) + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
         const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)c0;
-        bool alive = true;
-        int it = 0;
+        bool alive = true;  // once a wait has run out no other is waited for, and the rest is garbage
+        Ring<Cfg::kBufs> buf;
+        Ring<Cfg::kScales> sc;
         for (int tile = pair; tile < n_tiles; tile += pairs) {
             int tp, tq;
             pair_tile(tile, tiles_p, a.tiles_q, &tp, &tq);
             const int p0 = (2 * tp + rank) * kRows, q0 = tq * BN;
-            const int pr = min(p0 + row, a.p.rows - 1);
-            const float* ps = a.p.scale + (int64_t)(pr / a.p.per) * a.p.ld_scale;
-            const int qr = min(q0 + (QROWS ? tid : c0), a.q.rows - 1);
-            const float* qs = a.q.scale + (int64_t)(qr / a.q.per) * a.q.ld_scale;
-            const bool stage = QROWS && tid < BN;
-            float ps_next = __ldg(ps), qs_next = stage || !QROWS ? __ldg(qs) : 0.0f;
-            if constexpr (QROWS) {
-                named_sync(1, 32 * kEpiWarps);  // the last tile's scales are read
-                if (stage) col_scale[0][tid] = qs_next;
-                named_sync(1, 32 * kEpiWarps);
-            }
+            // the scales of the row, and of the columns where they share one,
+            // two blocks ahead
+            const float* ps = a.p.scale + (int64_t)(min(p0 + row, a.p.rows - 1) / a.p.per) * a.p.ld_scale;
+            const float* qs = a.q.scale + (int64_t)(min(q0 + c0, a.q.rows - 1) / a.q.per) * a.q.ld_scale;
+            float ps_next = __ldg(ps), ps_then = __ldg(ps + min(1, nkb - 1));
+            float qs_next = QROWS ? 1.0f : __ldg(qs), qs_then = QROWS ? 1.0f : __ldg(qs + min(1, nkb - 1));
             uint64_t acc[Cfg::kRun / 2];
 #pragma unroll
             for (int i = 0; i < Cfg::kRun / 2; ++i) acc[i] = 0;
-            for (int kb = 0; kb < nkb; ++kb, ++it) {
-                const int b = it % Cfg::kBufs;
+            for (int kb = 0; kb < nkb; ++kb) {
                 const float r = QROWS ? ps_next : ps_next * qs_next;
                 const uint64_t r2 = f2_of(r, r);
-                if (kb + 1 < nkb) {
-                    ps_next = __ldg(ps + kb + 1);
-                    if (stage || !QROWS) qs_next = __ldg(qs + kb + 1);
+                ps_next = ps_then;
+                ps_then = __ldg(ps + min(kb + 2, nkb - 1));
+                if constexpr (!QROWS) {
+                    qs_next = qs_then;
+                    qs_then = __ldg(qs + min(kb + 2, nkb - 1));
                 }
-                if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[b], it / Cfg::kBufs));
-                if (alive) {
-                    tc_fence_after();
+                if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[buf.at], buf.parity));
+                if (QROWS && alive) alive = __all_sync(0xffffffffu, wait(&sc_full[sc.at], sc.parity));
+                tc_fence_after();
+                // 32 columns are read while the 32 before are added up
+                const uint32_t from = lane_addr + buf.at * BN;
+                uint32_t v[2][32];
+                tmem_ld(from, v[0]);
 #pragma unroll
-                    for (int c = 0; c < Cfg::kRun; c += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(lane_addr + b * BN + c, v);
-                        tmem_wait_ld();
+                for (int c = 0; c < Cfg::kRun; c += 32) {
+                    uint32_t(&w)[32] = v[c / 32 & 1];
+                    tmem_wait_ld(w);
+                    if (c + 32 < Cfg::kRun) {
+                        tmem_ld(from + c + 32, v[(c / 32 & 1) ^ 1]);
+                    } else {  // all read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[buf.at], 0));
+                    }
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const uint64_t d = f2_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
-                            uint64_t& o = acc[c / 2 + e];
-                            if constexpr (QROWS) {
-                                const float2 cs =
-                                    *reinterpret_cast<const float2*>(&col_scale[kb & 1][c0 + c + 2 * e]);
-                                o = f2_fma(d, f2_mul(r2, f2_of(cs.x, cs.y)), o);
-                            } else {
-                                o = f2_fma(d, r2, o);
-                            }
+                    for (int e = 0; e < 16; ++e) {
+                        const uint64_t d = f2_of(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+                        uint64_t& o = acc[c / 2 + e];
+                        if constexpr (QROWS) {
+                            const float2 cs = *reinterpret_cast<const float2*>(&col_scale[sc.at][c0 + c + 2 * e]);
+                            o = f2_fma(d, f2_mul(r2, f2_of(cs.x, cs.y)), o);
+                        } else {
+                            o = f2_fma(d, r2, o);
                         }
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[b], 0));
                 }
                 if constexpr (QROWS) {
-                    if (stage) col_scale[(kb + 1) & 1][tid] = qs_next;
-                    named_sync(1, 32 * kEpiWarps);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_empty[sc.at]);
                 }
+                buf.next();
+                sc.next();
             }
-            // the warp's 32 rows x kRun columns
-            constexpr int kPer = 128 / (int)sizeof(T);      // columns of a 128-byte row
-            constexpr int kRound = Cfg::kOutBytes / 32 / 128 * kPer < Cfg::kRun ? Cfg::kOutBytes / 32 / 128 * kPer : Cfg::kRun;
+            // the warp's 32 rows: 128 bytes of each row at a time
+            // through its staging, or straight to memory
+            constexpr int kPer = 128 / (int)sizeof(T);
             if (a.vec_out) {
+                const bool in = p0 + 32 * (warp & 3) < a.p.rows;
 #pragma unroll
-                for (int c = 0; c < Cfg::kRun; c += kRound) {
-                    bulk_wait_read0();  // (lane 0) the staging's last store has been read
+                for (int c = 0; c < Cfg::kRun; c += kPer) {
+                    bulk_wait_read0();  // (lane 0) the last store has read the staging
                     __syncwarp();
 #pragma unroll
-                    for (int x = 0; x < kRound; x += kPer) {
-                        uint8_t* box = mine + x / kPer * 32 * 128;
+                    for (int u = 0; u < 8; ++u) {  // 16-byte units of the lane's row
+                        uint32_t w[4];
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {  // 16-byte units of the lane's row
-                            uint32_t w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float lo, up;
-                                if constexpr (sizeof(T) == 2) {
-                                    f2_to(acc[(c + x) / 2 + 4 * u + e], lo, up);
-                                    w[e] = bf16x2(lo, up);
-                                } else {
-                                    f2_to(acc[(c + x) / 2 + 2 * u + e / 2], lo, up);
-                                    w[e] = __float_as_uint(e & 1 ? up : lo);
-                                }
+                        for (int e = 0; e < 4; ++e) {
+                            float lo, up;
+                            if constexpr (sizeof(T) == 2) {
+                                f2_to(acc[c / 2 + 4 * u + e], lo, up);
+                                w[e] = bf16x2(lo, up);
+                            } else {
+                                f2_to(acc[c / 2 + 2 * u + e / 2], lo, up);
+                                w[e] = __float_as_uint(e & 1 ? up : lo);
                             }
-                            *reinterpret_cast<uint4*>(box + sw128_off(lane, u)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + sw128_off(lane, u)),
+                                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                     : "memory");
                     }
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-#pragma unroll
-                        for (int x = 0; x < kRound; x += kPer)
-                            if (p0 + 32 * (warp & 3) < a.p.rows && q0 + c0 + c + x < a.q.rows)
-                                tma_store_2d(&maps.out, smem_u32(mine) + x / kPer * 32 * 128, q0 + c0 + c + x,
-                                             p0 + 32 * (warp & 3));
+                        if (in && q0 + c0 + c < a.q.rows)
+                            tma_store_2d(&maps.out, staging, q0 + c0 + c, p0 + 32 * (warp & 3));
                         bulk_commit();
                     }
                 }
@@ -633,6 +712,13 @@ int configure_mm8() {
     return configure_pair_n<256>();
 }
 
+// Few rows of a become the MMA's columns (swap).  Otherwise, and where whole
+// tiles leave SMs idle, a tile's blocks of k go to several CTAs, one CTA per
+// SM at most (measured at 16 x 8192 x 4096: 12.9 us with 128 CTAs, 18.2 with
+// 64, 17.2 with 256) and at least 8 blocks for each of 8 (a cluster of 8 costs
+// 4 us more than one of 4).  Products with more tiles than that run on pairs of
+// CTAs, whose tile is the one with the shorter estimate: waves of pairs times
+// the measured time of a block of k, plus the start and end of a tile.
 Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
     Mm8Plan pl{};
     pl.swap = d.m <= 64;
@@ -640,8 +726,19 @@ Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
     const int64_t tiles = (int64_t)tiles_of(pl.swap ? d.n : d.m, kRows) * tiles_of(pl.swap ? d.m : d.n, pl.bn);
     const int kb = tiles_of(d.k, kBk);
     pl.splits = 1;
-    if (const char* e = getenv("XP")) { if (!pl.swap) { pl.pair = atoi(e) > 0; if (pl.pair) { pl.bn = atoi(e); return pl; } } }
-    while (pl.splits < 8 && tiles * pl.splits * 2 <= 2 * ctx->n_sm && kb >= 4 * pl.splits) pl.splits *= 2;
+    while (pl.splits < 8 && tiles * pl.splits * 2 <= ctx->n_sm && kb >= (pl.splits == 4 ? 64 : 4 * pl.splits))
+        pl.splits *= 2;
+    if (pl.swap || tiles * 2 <= ctx->n_sm) return pl;
+    const bool rows = d.b_form == HELIX_SCALE_ROWS;
+    auto estimate = [&](int bn, double block, double tile) {
+        const int64_t n = (int64_t)tiles_of(d.m, 2 * kRows) * tiles_of(d.n, bn);
+        const int64_t waves = (n + ctx->n_sm / 2 - 1) / (ctx->n_sm / 2);
+        return (double)waves * (block * kb + tile);  // us
+    };
+    const double wide = rows ? estimate(256, 1.02, 4.0) : estimate(256, 0.58, 3.0);
+    const double narrow = rows ? estimate(128, 0.57, 3.0) : estimate(128, 0.40, 2.5);
+    pl.pair = true;
+    pl.bn = wide <= narrow ? 256 : 128;
     return pl;
 }
 
