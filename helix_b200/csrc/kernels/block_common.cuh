@@ -19,9 +19,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// The scale of a group whose largest magnitude is amax.  The floor keeps 1 /
-// scale finite for a group of zeros; max.NaN lets a NaN through.
-__device__ __forceinline__ float group_scale(float amax) { return max_nan(amax, 0x1p-100f) / 448.0f; }
+// The scale of a group whose largest magnitude is amax, and its reciprocal,
+// both within 2 ulp (an exact division takes as long as the rest of a group).
+// The floor keeps the reciprocal finite for a group of zeros; max.NaN lets a
+// NaN through.
+__device__ __forceinline__ float group_scale(float amax, float* inv) {
+    const float scale = max_nan(amax, 0x1p-100f) * (1.0f / 448.0f);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(*inv) : "f"(scale));
+    return scale;
+}
 
 // Two values as e4m3, the first in the low byte; round to nearest even, NaN
 // stays NaN.  Values are at most 448 in magnitude up to rounding of 1 / scale.
@@ -39,20 +45,36 @@ __device__ __forceinline__ T from_f32(float v) {
         return __float2bfloat16_rn(v);
 }
 
-// Eight consecutive values of a 16-byte aligned address.
-__device__ __forceinline__ void ld8(const float* p, float (&v)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void ld8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight consecutive values of a 16-byte aligned address: as loaded, and as
+// fp32.  Loading apart from unpacking lets a thread have all of its loads in
+// flight before it looks at the first.
+template <typename T>
+struct Raw8 {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // a bf16 is the top half of its fp32
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
     }
-}
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void unpack(float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(T) == 4) {
+                    f[4 * i + k] = __uint_as_float(w[k]);
+                } else {  // a bf16 is the top half of its fp32
+                    f[2 * k] = __uint_as_float(w[k] << 16);
+                    f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+                }
+            }
+        }
+    }
+};
 __device__ __forceinline__ void st8(float* p, const float (&v)[8]) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);

@@ -27,19 +27,40 @@ __device__ __forceinline__ int col_of(int c0, int lane, int e) {
     return VEC ? c0 + 8 * lane + e : c0 + 32 * e + lane;
 }
 
-// The lane's 8 values of the segment at c0; 0 past the row's end.
+// The lane's 8 values of the segment at c0, 0 past the row's end; loaded
+// first and looked at later.
 template <bool VEC, typename T>
-__device__ __forceinline__ void ld_seg(const T* row, int c0, int lane, int n_col, float (&v)[8]) {
-    if (VEC && c0 + 8 * lane + 8 <= n_col) {
-        ld8(row + c0 + 8 * lane, v);
-        return;
-    }
+struct Seg {
+    Raw8<T> raw;
+    T       one[VEC ? 1 : 8];
+    __device__ __forceinline__ void load(const T* row, int c0, int lane, int n_col) {
+        if constexpr (VEC) {
+            raw.zero();
+            if (c0 + 8 * lane + 8 <= n_col) raw.load(row + c0 + 8 * lane);
+        } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int c = col_of<VEC>(c0, lane, e);
-        v[e] = c < n_col ? to_f32(row[c]) : 0.0f;
+            for (int e = 0; e < 8; ++e) {
+                const int c = col_of<VEC>(c0, lane, e);
+                one[e] = c < n_col ? row[c] : from_f32<T>(0.0f);
+            }
+        }
     }
-}
+    __device__ __forceinline__ void get(const T* row, int c0, int lane, int n_col, float (&v)[8]) const {
+        if constexpr (VEC) {
+            raw.unpack(v);
+            // a row's last values where they are no whole eight
+            const int c = c0 + 8 * lane;
+            if (c < n_col && c + 8 > n_col) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < n_col) v[e] = to_f32(row[c + e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = to_f32(one[e]);
+        }
+    }
+};
 template <bool VEC, typename T>
 __device__ __forceinline__ void st_seg(T* row, int c0, int lane, int n_col, const float (&v)[8]) {
     if (VEC && c0 + 8 * lane + 8 <= n_col) {
@@ -51,6 +72,12 @@ __device__ __forceinline__ void st_seg(T* row, int c0, int lane, int n_col, cons
         const int c = col_of<VEC>(c0, lane, e);
         if (c < n_col) row[c] = from_f32<T>(v[e]);
     }
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void ld_seg(const T* row, int c0, int lane, int n_col, float (&v)[8]) {
+    Seg<VEC, T> s;
+    s.load(row, c0, lane, n_col);
+    s.get(row, c0, lane, n_col, v);
 }
 template <bool VEC>
 __device__ __forceinline__ void ld_weight(const NormParams& p, int c0, int lane, float (&v)[8]) {
@@ -87,7 +114,8 @@ __device__ __forceinline__ void st_seg_e4m3(const NormParams& p, int64_t row, in
         for (int e = 1; e < 8; ++e) a = max_nan(a, fabsf(n[e]));
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const float scale = group_scale(a), inv = 1.0f / scale;
+        float inv;
+        const float scale = group_scale(a, &inv);
         const int c = c0 + 8 * lane;
         if ((lane & 15) == 0 && c < p.n_col) sc[c / HELIX_GROUP] = scale;
         if (c + 8 <= p.n_col) {
@@ -107,7 +135,8 @@ __device__ __forceinline__ void st_seg_e4m3(const NormParams& p, int64_t row, in
             for (int e = 4 * g; e < 4 * g + 4; ++e) a = max_nan(a, fabsf(n[e]));
 #pragma unroll
             for (int o = 16; o >= 1; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-            const float scale = group_scale(a), inv = 1.0f / scale;
+            float inv;
+            const float scale = group_scale(a, &inv);
             const int first = c0 + HELIX_GROUP * g;
             if (lane == 0 && first < p.n_col) sc[first / HELIX_GROUP] = scale;
 #pragma unroll
@@ -119,37 +148,47 @@ __device__ __forceinline__ void st_seg_e4m3(const NormParams& p, int64_t row, in
     }
 }
 
+// Threads of a block: a row of more than 8 warps has the block to itself.
+template <int V>
+constexpr int norm_threads() {
+    return 32 * (V == 4 ? kMaxWarps : kMaxWarps / 2);
+}
+
 template <typename TX, typename TR, int V, bool VEC>
-__global__ void __launch_bounds__(32 * kMaxWarps) norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(norm_threads<V>(), V == 4 ? 1 : 4) norm_kernel(const NormParams p) {
     __shared__ float part[kMaxWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * p.rpb + warp / p.wpr;
     const int wr = warp % p.wpr;
     const bool live = row < p.n_row;
+    const int n = live ? p.n_col : 0;
+    const TX* x = static_cast<const TX*>(p.x) + (live ? row : 0) * p.ld_x;
+    const TR* r = static_cast<const TR*>(p.res) + (live ? row : 0) * p.ld_res;
 
     float s[V][8];
     float ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c0 = (j * p.wpr + wr) * kSeg;
-        const int n = live ? p.n_col : 0;
-        ld_seg<VEC>(static_cast<const TX*>(p.x) + (live ? row : 0) * p.ld_x, c0, lane, n, s[j]);
-    }
-    if (p.res) {
+    {
+        Seg<VEC, TX> sx[V];
+        Seg<VEC, TR> sr[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c0 = (j * p.wpr + wr) * kSeg;
-            float r[8];
-            ld_seg<VEC>(static_cast<const TR*>(p.res) + (live ? row : 0) * p.ld_res, c0, lane, live ? p.n_col : 0,
-                        r);
+            sx[j].load(x, c0, lane, n);
+            sr[j].load(r, c0, lane, p.res ? n : 0);
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[j][e] += r[e];
+        for (int j = 0; j < V; ++j) {
+            const int c0 = (j * p.wpr + wr) * kSeg;
+            float v[8];
+            sx[j].get(x, c0, lane, n, s[j]);
+            sr[j].get(r, c0, lane, p.res ? n : 0, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (p.res) s[j][e] += v[e];
+                ss += s[j][e] * s[j][e];
+            }
         }
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += s[j][e] * s[j][e];
     ss = row_sum(ss, p.wpr, warp, lane, part);
     if (!live) return;
     const float rstd = 1.0f / sqrtf(ss / (float)p.n_col + p.eps);
@@ -175,58 +214,86 @@ __global__ void __launch_bounds__(32 * kMaxWarps) norm_kernel(const NormParams p
 // Persistent: a row slot takes every slots-th row and keeps its share of
 // dweight in registers, written to partial[slot] at the end.
 template <typename TX, typename TR, int V, bool VEC>
-__global__ void __launch_bounds__(32 * kMaxWarps) norm_grad_kernel(const NormParams p) {
+__global__ void __launch_bounds__(32 * kMaxWarps, 1) norm_grad_kernel(const NormParams p) {
     __shared__ float part[2][kMaxWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rg = warp / p.wpr, wr = warp % p.wpr;
-    float dw[V][8];
+    // The widest rows (V = 4) leave no registers for dweight, which then stays
+    // in shared memory, nor for loads ahead.
+    constexpr bool kWide = V == 4;
+    extern __shared__ float dw_smem[];
+    float dw[kWide ? 1 : V][8];
+    auto dw_at = [&](int j, int e) -> float& {
+        if constexpr (kWide)
+            return dw_smem[(8 * j + e) * blockDim.x + threadIdx.x];
+        else
+            return dw[j][e];
+    };
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dw[j][e] = 0.0f;
+        for (int e = 0; e < 8; ++e) dw_at(j, e) = 0.0f;
+
+    // a row's loads are in flight while the row before is worked on
+    Seg<VEC, TX> sd[V];
+    Seg<VEC, TR> ss[V], sa[V];
+    float rstd_next = 0.0f;
+    const TX* dout = static_cast<const TX*>(p.dout);
+    const TR* sum = static_cast<const TR*>(p.sum);
+    const TR* dsum = static_cast<const TR*>(p.dsum);
+    auto fetch = [&](int64_t row) {
+        const int n = row < p.n_row ? p.n_col : 0;
+        row = n ? row : 0;
+        rstd_next = n ? p.rstd[row] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c0 = (j * p.wpr + wr) * kSeg;
+            sd[j].load(dout + row * p.ld_dout, c0, lane, n);
+            ss[j].load(sum + row * p.ld_sum, c0, lane, n);
+            if (!kWide) sa[j].load(dsum + row * p.ld_dsum, c0, lane, p.dsum ? n : 0);
+        }
+    };
 
     int turn = 0;
-    for (int64_t base = (int64_t)blockIdx.x * p.rpb; base < p.n_row; base += (int64_t)gridDim.x * p.rpb) {
+    const int64_t step = (int64_t)gridDim.x * p.rpb;
+    if (!kWide) fetch((int64_t)blockIdx.x * p.rpb + rg);
+    for (int64_t base = (int64_t)blockIdx.x * p.rpb; base < p.n_row; base += step) {
         const bool live = base + rg < p.n_row;
         const int64_t row = live ? base + rg : 0;
         const int n = live ? p.n_col : 0;
-        const float rstd = live ? p.rstd[row] : 0.0f;
-        float d[V][8], s[V][8];
+        if (kWide) fetch(base + rg);
+        const float rstd = rstd_next;
+        float d[V][8], s[V][8], o[kWide ? 1 : V][8];
         float along = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c0 = (j * p.wpr + wr) * kSeg;
-            ld_seg<VEC>(static_cast<const TX*>(p.dout) + row * p.ld_dout, c0, lane, n, d[j]);
-            ld_seg<VEC>(static_cast<const TR*>(p.sum) + row * p.ld_sum, c0, lane, n, s[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
             float w[8];
-            ld_weight<VEC>(p, (j * p.wpr + wr) * kSeg, lane, w);
+            sd[j].get(dout + row * p.ld_dout, c0, lane, n, d[j]);
+            ss[j].get(sum + row * p.ld_sum, c0, lane, n, s[j]);
+            if constexpr (!kWide) sa[j].get(dsum + row * p.ld_dsum, c0, lane, p.dsum ? n : 0, o[j]);
+            ld_weight<VEC>(p, c0, lane, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 s[j][e] *= rstd;              // s rstd
-                dw[j][e] += d[j][e] * s[j][e];
+                dw_at(j, e) += d[j][e] * s[j][e];
                 d[j][e] *= w[e];              // dn w
                 along += d[j][e] * s[j][e];
             }
         }
+        if (!kWide) fetch(base + step + rg);
         along = row_sum(along, p.wpr, warp, lane, part[turn]) / (float)p.n_col;
         turn ^= 1;
         if (!live) continue;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c0 = (j * p.wpr + wr) * kSeg;
-            float o[8];
-            if (p.dsum)
-                ld_seg<VEC>(static_cast<const TR*>(p.dsum) + row * p.ld_dsum, c0, lane, n, o);
-            else
+            float(&v)[8] = o[kWide ? 0 : j];
+            if constexpr (kWide) ld_seg<VEC>(dsum + row * p.ld_dsum, c0, lane, p.dsum ? n : 0, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] += rstd * (d[j][e] - s[j][e] * along);
-            st_seg<VEC>(static_cast<TX*>(p.dx) + row * p.ld_dx, c0, lane, n, o);
-            if (p.dres) st_seg<VEC>(static_cast<TR*>(p.dres) + row * p.ld_dres, c0, lane, n, o);
+            for (int e = 0; e < 8; ++e) v[e] += rstd * (d[j][e] - s[j][e] * along);
+            st_seg<VEC>(static_cast<TX*>(p.dx) + row * p.ld_dx, c0, lane, n, v);
+            if (p.dres) st_seg<VEC>(static_cast<TR*>(p.dres) + row * p.ld_dres, c0, lane, n, v);
         }
     }
     float* mine = p.partial + ((int64_t)blockIdx.x * p.rpb + rg) * p.n_col;
@@ -236,7 +303,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) norm_grad_kernel(const NormPar
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int c = col_of<VEC>(c0, lane, e);
-            if (c < p.n_col) mine[c] = dw[j][e];
+            if (c < p.n_col) mine[c] = dw_at(j, e);
         }
     }
 }
@@ -250,6 +317,7 @@ __global__ void __launch_bounds__(32 * kDwRows) norm_dw_kernel(const float* part
     const int c = blockIdx.x * 32 + lane;
     float v = 0.0f;
     if (c < n_col)
+#pragma unroll 8
         for (int s = r; s < slots; s += kDwRows) v += partial[(int64_t)s * n_col + c];
     part[r][lane] = v;
     __syncthreads();
@@ -260,12 +328,14 @@ __global__ void __launch_bounds__(32 * kDwRows) norm_dw_kernel(const float* part
     }
 }
 
+constexpr size_t kWideSmem = sizeof(float) * 32 * 32 * kMaxWarps;  // dweight of a block's rows at V = 4
+
 template <typename TX, typename TR, bool VEC>
 int launch_norm_v(const NormParams& p, int v, dim3 grid, dim3 block, bool grad, void* stream) {
     if (grad)
         return v == 1   ? block_launch(norm_grad_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
                : v == 2 ? block_launch(norm_grad_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p)
-                        : block_launch(norm_grad_kernel<TX, TR, 4, VEC>, grid, block, 0, stream, p);
+                        : block_launch(norm_grad_kernel<TX, TR, 4, VEC>, grid, block, kWideSmem, stream, p);
     return v == 1   ? block_launch(norm_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
            : v == 2 ? block_launch(norm_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p)
                     : block_launch(norm_kernel<TX, TR, 4, VEC>, grid, block, 0, stream, p);
@@ -284,12 +354,31 @@ int launch_norm_any(const helix_rms_norm_desc& d, const NormParams& p, int v, di
                : launch_norm_v<bf, bf, false>(p, v, grid, block, grad, stream);
 }
 
+template <typename TX, typename TR>
+int configure_norm_t() {
+    const int e = cudaFuncSetAttribute(norm_grad_kernel<TX, TR, 4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)kWideSmem);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(norm_grad_kernel<TX, TR, 4, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)kWideSmem);
+}
+
 }  // namespace
 
-NormShape norm_shape(const helix_rms_norm_desc& d) {
+int configure_norm() {
+    int e;
+    if ((e = configure_norm_t<float, float>()) != cudaSuccess) return e;
+    if ((e = configure_norm_t<__nv_bfloat16, float>()) != cudaSuccess) return e;
+    return configure_norm_t<__nv_bfloat16, __nv_bfloat16>();
+}
+
+// Segments per warp: few enough that the row stays in registers (forward: 8
+// warps of 2 segments fit four blocks to an SM; the gradient holds three rows
+// and dweight).
+NormShape norm_shape(const helix_rms_norm_desc& d, bool grad) {
     const int segs = (d.n_col + kSeg - 1) / kSeg;
     NormShape s{};
-    s.v = segs <= 1 ? 1 : segs <= 2 * kMaxWarps ? 2 : 4;
+    s.v = segs <= 1 ? 1 : segs <= (grad ? 2 * kMaxWarps : kMaxWarps) ? 2 : 4;
     s.wpr = (segs + s.v - 1) / s.v;
     s.rpb = s.wpr >= 8 ? 1 : 8 / s.wpr;
     return s;
@@ -297,9 +386,9 @@ NormShape norm_shape(const helix_rms_norm_desc& d) {
 
 NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d) {
     NormGradPlan pl{};
-    pl.shape = norm_shape(d);
+    pl.shape = norm_shape(d, true);
     const int n_sm = ctx && ctx->n_sm > 0 ? ctx->n_sm : 148;
-    const int64_t per_sm = 32 / (pl.shape.wpr * pl.shape.rpb);  // about 1024 threads per SM
+    const int64_t per_sm = 16 / (pl.shape.wpr * pl.shape.rpb);  // 512 threads per SM: what the registers allow
     const int64_t need = (d.n_row + pl.shape.rpb - 1) / pl.shape.rpb;
     const int64_t most = (int64_t)n_sm * (per_sm > 0 ? per_sm : 1);
     pl.blocks = (int)(need < most ? need : most);
@@ -309,7 +398,7 @@ NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d) 
 }
 
 int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream) {
-    const NormShape s = norm_shape(d);
+    const NormShape s = norm_shape(d, false);
     const dim3 grid((unsigned)((d.n_row + s.rpb - 1) / s.rpb)), block(32 * s.wpr * s.rpb);
     return launch_norm_any(d, p, s.v, grid, block, vec, false, stream);
 }

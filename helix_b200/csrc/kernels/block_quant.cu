@@ -29,19 +29,24 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
     const int rows = (int)(p.n_row - r0 < kTile ? p.n_row - r0 : kTile);
     const int cols = (int)(p.n_col - c0 < kTile ? p.n_col - c0 : kTile);
     const int rt = 16 * warp + 8 * hi;  // the lane's first row
+    const bool full = rows == kTile && cols == kTile;
     auto col = [&](int e) { return VEC ? 8 * l + e : l + 16 * e; };
 
     float x[8][8];
     const T* src = static_cast<const T*>(p.x) + r0 * p.ld_x + c0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const T* row = src + (int64_t)(rt + i) * p.ld_x;
-        if (VEC && rt + i < rows && 8 * l + 8 <= cols) {
-            ld8(row + 8 * l, x[i]);
-        } else {
+    for (int i = 0; i < 8; ++i)
+        if (!VEC || !full) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = rt + i < rows && col(e) < cols ? to_f32(row[col(e)]) : 0.0f;
+            for (int e = 0; e < 8; ++e)
+                x[i][e] = rt + i < rows && col(e) < cols ? to_f32(src[(int64_t)(rt + i) * p.ld_x + col(e)]) : 0.0f;
         }
+    if (VEC && full) {
+        Raw8<T> raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i].load(src + (int64_t)(rt + i) * p.ld_x + 8 * l);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i].unpack(x[i]);
     }
 
     // every value becomes value / scale
@@ -58,7 +63,8 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
         a = peak[0][0];
 #pragma unroll
         for (int w = 1; w < 8; ++w) a = max_nan(a, peak[w][0]);
-        const float scale = group_scale(a), inv = 1.0f / scale;
+        float inv;
+        const float scale = group_scale(a, &inv);
         if (threadIdx.x == 0)
             p.scale[(TURN ? c0 / kTile : r0 / kTile) * p.ld_scale + (TURN ? r0 / kTile : c0 / kTile)] = scale;
 #pragma unroll
@@ -73,7 +79,8 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
             for (int e = 0; e < 8; ++e) a = max_nan(a, fabsf(x[i][e]));
 #pragma unroll
             for (int o = 8; o >= 1; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-            const float scale = group_scale(a), inv = 1.0f / scale;
+            float inv;
+            const float scale = group_scale(a, &inv);
             if (l == 0 && rt + i < rows) p.scale[(r0 + rt + i) * p.ld_scale + c0 / kTile] = scale;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[i][e] *= inv;
@@ -93,8 +100,7 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
             float a = peak[0][c];
 #pragma unroll
             for (int w = 1; w < 8; ++w) a = max_nan(a, peak[w][c]);
-            const float scale = group_scale(a);
-            col_scale[c] = 1.0f / scale;
+            const float scale = group_scale(a, &col_scale[c]);
             if (c < cols) p.scale[(c0 + c) * p.ld_scale + r0 / kTile] = scale;
         }
         __syncthreads();

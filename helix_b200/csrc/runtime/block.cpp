@@ -194,7 +194,7 @@ extern "C" helix_status helix_rms_norm_encode(helix_ctx* ctx, void* stream, cons
         hx::NormParams p{};
         p.n_row = n;
         p.n_col = d->n_col;
-        const hx::NormShape s = hx::norm_shape(*d);
+        const hx::NormShape s = hx::norm_shape(*d, false);
         p.wpr = s.wpr;
         p.rpb = s.rpb;
         p.eps = d->eps;

@@ -17,7 +17,8 @@ struct NormShape {
     int wpr;   // warps per row
     int rpb;   // rows per block
 };
-NormShape norm_shape(const helix_rms_norm_desc& d);
+NormShape norm_shape(const helix_rms_norm_desc& d, bool grad);
+int configure_norm();
 // Gradient: slots of rows, each with its own partial sum of dweight.
 struct NormGradPlan {
     NormShape shape;
