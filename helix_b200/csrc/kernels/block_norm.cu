@@ -14,13 +14,15 @@
 //
 // Sums, statistics and the products are fp32; the only roundings are those
 // of the stored sum, the output and (8 bits) 1 / scale.
+#include <algorithm>
+
 #include "block_common.cuh"
 
 namespace hx {
 namespace {
 
 constexpr int kSeg = 256;        // columns of a warp's segment
-constexpr int kMaxWarps = 16;    // 16 warps x 4 segments x 256 = 16384 columns
+constexpr int kMaxWarps = 32;    // 32 warps x 2 segments x 256 = 16384 columns
 
 template <bool VEC>
 __device__ __forceinline__ int col_of(int c0, int lane, int e) {
@@ -148,14 +150,11 @@ __device__ __forceinline__ void st_seg_e4m3(const NormParams& p, int64_t row, in
     }
 }
 
-// Threads of a block: a row of more than 8 warps has the block to itself.
-template <int V>
-constexpr int norm_threads() {
-    return 32 * (V == 4 ? kMaxWarps : kMaxWarps / 2);
-}
-
-template <typename TX, typename TR, int V, bool VEC>
-__global__ void __launch_bounds__(norm_threads<V>(), V == 4 ? 1 : 4) norm_kernel(const NormParams p) {
+// WIDE: rows of more than 8 warps, which have the block to themselves; others
+// keep to 48 registers, so that five blocks fit an SM (8192 x 4096 bf16: 45 us,
+// with four 49).
+template <typename TX, typename TR, int V, bool WIDE, bool VEC>
+__global__ void __launch_bounds__(WIDE ? 1024 : 256, WIDE ? 1 : 5) norm_kernel(const NormParams p) {
     __shared__ float part[kMaxWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * p.rpb + warp / p.wpr;
@@ -214,7 +213,7 @@ __global__ void __launch_bounds__(norm_threads<V>(), V == 4 ? 1 : 4) norm_kernel
 // Persistent: a row slot takes every slots-th row and keeps its share of
 // dweight in registers, written to partial[slot] at the end.
 template <typename TX, typename TR, int V, bool VEC>
-__global__ void __launch_bounds__(32 * kMaxWarps, 1) norm_grad_kernel(const NormParams p) {
+__global__ void __launch_bounds__(V == 1 ? 1024 : 512, 1) norm_grad_kernel(const NormParams p) {
     __shared__ float part[2][kMaxWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rg = warp / p.wpr, wr = warp % p.wpr;
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(32 * kDwRows) norm_dw_kernel(const float* part
     }
 }
 
-constexpr size_t kWideSmem = sizeof(float) * 32 * 32 * kMaxWarps;  // dweight of a block's rows at V = 4
+constexpr size_t kWideSmem = sizeof(float) * 32 * 512;  // dweight of a block's row at V = 4
 
 template <typename TX, typename TR, bool VEC>
 int launch_norm_v(const NormParams& p, int v, dim3 grid, dim3 block, bool grad, void* stream) {
@@ -336,9 +335,9 @@ int launch_norm_v(const NormParams& p, int v, dim3 grid, dim3 block, bool grad, 
         return v == 1   ? block_launch(norm_grad_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
                : v == 2 ? block_launch(norm_grad_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p)
                         : block_launch(norm_grad_kernel<TX, TR, 4, VEC>, grid, block, kWideSmem, stream, p);
-    return v == 1   ? block_launch(norm_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
-           : v == 2 ? block_launch(norm_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p)
-                    : block_launch(norm_kernel<TX, TR, 4, VEC>, grid, block, 0, stream, p);
+    if (block.x > 256) return block_launch(norm_kernel<TX, TR, 2, true, VEC>, grid, block, 0, stream, p);
+    return v == 1 ? block_launch(norm_kernel<TX, TR, 1, false, VEC>, grid, block, 0, stream, p)
+                  : block_launch(norm_kernel<TX, TR, 2, false, VEC>, grid, block, 0, stream, p);
 }
 
 int launch_norm_any(const helix_rms_norm_desc& d, const NormParams& p, int v, dim3 grid, dim3 block, bool vec,
@@ -372,33 +371,40 @@ int configure_norm() {
     return configure_norm_t<__nv_bfloat16, __nv_bfloat16>();
 }
 
-// Segments per warp: few enough that the row stays in registers (forward: 8
-// warps of 2 segments fit four blocks to an SM; the gradient holds three rows
-// and dweight).
-NormShape norm_shape(const helix_rms_norm_desc& d, bool grad) {
-    const int segs = (d.n_col + kSeg - 1) / kSeg;
+namespace {
+
+NormShape shape_of(int n_col, int v) {
     NormShape s{};
-    s.v = segs <= 1 ? 1 : segs <= (grad ? 2 * kMaxWarps : kMaxWarps) ? 2 : 4;
-    s.wpr = (segs + s.v - 1) / s.v;
+    s.v = v;
+    s.wpr = ((n_col + kSeg - 1) / kSeg + v - 1) / v;
     s.rpb = s.wpr >= 8 ? 1 : 8 / s.wpr;
     return s;
 }
 
-NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d) {
+}  // namespace
+
+NormShape norm_shape(const helix_rms_norm_desc& d) { return shape_of(d.n_col, d.n_col <= kSeg ? 1 : 2); }
+
+// The gradient holds two rows, a third on its way, and dweight.  One segment
+// per warp leaves 64 registers enough (16384 x 4096 bf16: 113 us, with two 142);
+// single accesses need twice the registers, and two segments (8192 x 4095: 99
+// us, with one 163); the widest rows have four.
+NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d, bool vec) {
     NormGradPlan pl{};
-    pl.shape = norm_shape(d, true);
+    const int segs = (d.n_col + kSeg - 1) / kSeg;
+    pl.shape = shape_of(d.n_col, segs > 32 ? 4 : vec || segs == 1 ? 1 : 2);
     const int n_sm = ctx && ctx->n_sm > 0 ? ctx->n_sm : 148;
-    const int64_t per_sm = 16 / (pl.shape.wpr * pl.shape.rpb);  // 512 threads per SM: what the registers allow
+    // blocks that the registers of an SM allow
+    const int64_t per_sm = std::max((pl.shape.v == 1 ? 32 : 16) / (pl.shape.wpr * pl.shape.rpb), 1);
     const int64_t need = (d.n_row + pl.shape.rpb - 1) / pl.shape.rpb;
-    const int64_t most = (int64_t)n_sm * (per_sm > 0 ? per_sm : 1);
-    pl.blocks = (int)(need < most ? need : most);
+    pl.blocks = (int)std::min(need, n_sm * per_sm);
     pl.slots = pl.blocks * pl.shape.rpb;
     pl.total = ((size_t)pl.slots * (size_t)d.n_col * sizeof(float) + 255) & ~(size_t)255;
     return pl;
 }
 
 int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream) {
-    const NormShape s = norm_shape(d, false);
+    const NormShape s = norm_shape(d);
     const dim3 grid((unsigned)((d.n_row + s.rpb - 1) / s.rpb)), block(32 * s.wpr * s.rpb);
     return launch_norm_any(d, p, s.v, grid, block, vec, false, stream);
 }

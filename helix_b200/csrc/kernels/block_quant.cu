@@ -17,6 +17,37 @@ constexpr int kQThreads = 256;
 
 __device__ __forceinline__ int unit_of(int col, int unit) { return unit ^ (((col >> 3) ^ col) & 15); }
 
+// Eight consecutive values at any address of the type's alignment, of which
+// those from `end` on do not exist (and read as anything): the aligned
+// 16-byte pieces that hold them, shifted together.  Every piece read holds a
+// value that exists.
+template <typename T>
+__device__ __forceinline__ void ld8_any(const T* p, const T* end, float (&f)[8]) {
+    constexpr int kPieces = (int)sizeof(T) / 2 + 1;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), to = reinterpret_cast<uintptr_t>(end);
+    const uint32_t off = (uint32_t)(at & 15);
+    uint32_t w[4 * kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const uintptr_t q = at - off + 16 * i;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (q < to && (i < kPieces - 1 || off)) v = *reinterpret_cast<const uint4*>(q);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+#pragma unroll
+    for (int i = 0; i + 2 < 4 * kPieces; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i + 3 < 4 * kPieces; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = off & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+    }
+    Raw8<T> raw;
+#pragma unroll
+    for (int i = 0; i < kPieces - 1; ++i) raw.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    raw.unpack(f);
+}
+
 template <typename T, bool BLOCKS, bool TURN, bool VEC>
 __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p) {
     __shared__ __align__(16) uint8_t turned[TURN ? kTile * kTile : 16];
@@ -30,23 +61,25 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
     const int cols = (int)(p.n_col - c0 < kTile ? p.n_col - c0 : kTile);
     const int rt = 16 * warp + 8 * hi;  // the lane's first row
     const bool full = rows == kTile && cols == kTile;
-    auto col = [&](int e) { return VEC ? 8 * l + e : l + 16 * e; };
+    auto col = [&](int e) { return 8 * l + e; };
 
     float x[8][8];
     const T* src = static_cast<const T*>(p.x) + r0 * p.ld_x + c0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (!VEC || !full) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[i][e] = rt + i < rows && col(e) < cols ? to_f32(src[(int64_t)(rt + i) * p.ld_x + col(e)]) : 0.0f;
-        }
     if (VEC && full) {
         Raw8<T> raw[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i].load(src + (int64_t)(rt + i) * p.ld_x + 8 * l);
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i].unpack(x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const T* row = src + (int64_t)(rt + i) * p.ld_x;
+            if (rt + i < rows && 8 * l < cols) ld8_any(row + 8 * l, row + cols, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (rt + i >= rows || col(e) >= cols) x[i][e] = 0.0f;
+        }
     }
 
     // every value becomes value / scale
@@ -117,7 +150,7 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
         for (int i = 0; i < 8; ++i) {
             if (rt + i >= rows) break;
             uint8_t* q = p.q + (r0 + rt + i) * p.ld_q + c0;
-            if (VEC && 8 * l + 8 <= cols) {
+            if (p.q_vec && 8 * l + 8 <= cols) {
                 *reinterpret_cast<uint2*>(q + 8 * l) =
                     make_uint2(e4m3x2(x[i][0], x[i][1]) | e4m3x2(x[i][2], x[i][3]) << 16,
                                e4m3x2(x[i][4], x[i][5]) | e4m3x2(x[i][6], x[i][7]) << 16);
@@ -140,7 +173,7 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
             if (c >= cols) continue;
             const uint2 v = *reinterpret_cast<const uint2*>(turned + c * kTile + 8 * unit_of(c, l));
             uint8_t* q = p.q + (c0 + c) * p.ld_q + r0 + 8 * l;
-            if (VEC && 8 * l + 8 <= rows) {
+            if (p.q_vec && 8 * l + 8 <= rows) {
                 *reinterpret_cast<uint2*>(q) = v;
             } else {
 #pragma unroll

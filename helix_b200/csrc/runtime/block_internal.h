@@ -17,7 +17,7 @@ struct NormShape {
     int wpr;   // warps per row
     int rpb;   // rows per block
 };
-NormShape norm_shape(const helix_rms_norm_desc& d, bool grad);
+NormShape norm_shape(const helix_rms_norm_desc& d);
 int configure_norm();
 // Gradient: slots of rows, each with its own partial sum of dweight.
 struct NormGradPlan {
@@ -26,7 +26,7 @@ struct NormGradPlan {
     int       slots;   // blocks * rpb
     size_t    total;   // scratch bytes: f32 [slots][n_col]
 };
-NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d);
+NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d, bool vec);
 
 struct NormParams {
     int64_t     n_row;
@@ -47,6 +47,7 @@ struct QuantParams {
     int64_t     n_row, n_col;
     int64_t     ld_x, ld_q, ld_scale;
     int32_t     n_tile_col;  // ceil(n_col / 128)
+    int32_t     q_vec;       // rows of q can be written in 8-byte pieces
     const void* x;
     uint8_t*    q;
     float*      scale;
@@ -102,7 +103,8 @@ int launch_gated(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedPara
 int launch_gated_grad(const helix_ctx* ctx, const helix_gated_scan_desc& d, GatedParams p, bool word, void* stream);
 
 // Kernel launchers (kernels/block_*.cu): cudaSuccess or the launch error.
-// `vec`: every tensor allows whole 16-byte accesses at 8-column boundaries.
+// `vec`: every tensor (the quantiser: x) allows whole 16-byte accesses at
+// 8-column boundaries.
 int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream);
 int launch_norm_grad(const helix_rms_norm_desc& d, const NormGradPlan& pl, const NormParams& p, bool vec,
                      float* dweight, void* stream);
