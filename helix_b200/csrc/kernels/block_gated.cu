@@ -352,6 +352,67 @@ struct Walk {
     }
 };
 
+// Plain access to K token tensors: a lane's words of a step, loaded one step
+// before they are looked at.  Rows at odd 2-byte addresses (kHalf) are read by
+// the aligned words that hold them; a lane then shifts its word and the next
+// lane's together, and lanes 0 .. 15 (16 .. 31) hold the word that lane 31
+// lacks of the 16 rows of tensor 0 (1), in extra[1] of tensor 2.  A word is
+// read only if it holds a channel that exists.
+template <typename T, Access A, int K>
+struct Ahead {
+    uint32_t w[K][kTok];
+    uint32_t extra[(K + 1) / 2];
+    uint32_t odd;  // bit k: row 0 of tensor k is at an odd address; bit 8 + k: its pitch is odd
+
+    __device__ __forceinline__ bool shifted(int k, int i) const {
+        return ((odd >> k) ^ ((odd >> (8 + k)) & (uint32_t)i)) & 1u;
+    }
+    // rows[k]: row t0 of tensor k at the lane's first channel; live: rows that exist
+    __device__ __forceinline__ void load(const T* const (&rows)[K], const int64_t (&pitch)[K], const Place<T>& at,
+                                         int n_chan, int live) {
+        if constexpr (A == kHalf) {
+            odd = 0;
+#pragma unroll
+            for (int e = 0; e < (K + 1) / 2; ++e) extra[e] = 0;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if constexpr (A == kHalf) {
+                odd |= (uint32_t)(reinterpret_cast<uintptr_t>(rows[k]) >> 1 & 1) << k | (uint32_t)(pitch[k] & 1) << (8 + k);
+                const int i = at.lane & 15;
+                if ((K == 2 || k < 2 ? (at.lane >> 4) == k : at.lane < 16) && i < live && shifted(k, i)) {
+                    const T* end = rows[k] - Lane<T>::kN * at.lane + 32 * Lane<T>::kN + i * pitch[k];
+                    if (at.slab0() + 32 * Lane<T>::kN - 1 < n_chan)  // lane 31's second channel
+                        extra[k / 2] = __ldcs(reinterpret_cast<const unsigned int*>(end - 1));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kTok; ++i) {
+                w[k][i] = 0u;
+                if constexpr (A == kHalf) {
+                    const bool sh = shifted(k, i);
+                    const T* p = rows[k] + i * pitch[k] - (sh ? 1 : 0);
+                    // a shifted word also holds the lane before's second channel
+                    if (i < live && at.c0 - (sh ? 1 : 0) < n_chan)
+                        w[k][i] = __ldcs(reinterpret_cast<const unsigned int*>(p));
+                } else {
+                    if (i < live && at.n > 0) w[k][i] = ld_raw<T, A>(rows[k] + i * pitch[k], at.n);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t get(int k, int i, int lane) const {
+        if constexpr (A == kHalf) {
+            if (shifted(k, i)) {  // the same for the whole warp
+                const uint32_t next = __shfl_down_sync(0xffffffffu, w[k][i], 1);
+                const uint32_t last = __shfl_sync(0xffffffffu, extra[k / 2], i + (k == 1 ? 16 : 0));
+                return __funnelshift_r(w[k][i], lane == 31 ? last : next, 16);
+            }
+        }
+        return w[k][i];
+    }
+};
+
 template <typename T, Access A, int kStages>
 __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     gated_kernel(const __grid_constant__ GatedMaps maps, const __grid_constant__ GatedParams p) {
@@ -371,18 +432,15 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
         for (int s = 0; s < kStages && s < steps; ++s) walk.load(s, chunk_of(s));
     __syncwarp();
 
-    uint32_t ahead[A == kTma ? 1 : 2][A == kTma ? 1 : kTok];
-    auto fetch = [&](int s) {  // plain access: the lane's words of step s
+    Ahead<T, A, A == kTma ? 1 : 2> ahead;
+    auto fetch = [&](int s) {
         if constexpr (A != kTma) {
-            const T* g = static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0;
-            const T* v = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0;
             const int t0 = chunk_of(s) * kChunk + warp * kTok;
-#pragma unroll
-            for (int i = 0; i < kTok; ++i) {
-                const bool live = n > 0 && t0 + i < at.len;
-                ahead[0][i] = live ? ld_raw<T, A>(g + (int64_t)(t0 + i) * p.s_g, n) : 0u;
-                ahead[1][i] = live ? ld_raw<T, A>(v + (int64_t)(t0 + i) * p.s_v, n) : 0u;
-            }
+            const T* const rows[2] = {
+                static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0 + (int64_t)t0 * p.s_g,
+                static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0 + (int64_t)t0 * p.s_v};
+            const int64_t pitch[2] = {p.s_g, p.s_v};
+            ahead.load(rows, pitch, at, p.n_chan, at.len - t0);
         }
     };
     V h = ld_state<L>(p.h0 ? p.h0 + (int64_t)at.seq * p.seq_h0 + at.c0 : nullptr, n);
@@ -401,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
                 if constexpr (A == kTma) {
                     gw = lds(my + word_of(0, i)), vw = lds(my + word_of(1, i));
                 } else {
-                    gw = ahead[0][i], vw = ahead[1][i];
+                    gw = ahead.get(0, i, lane), vw = ahead.get(1, i, lane);
                     sts(my + word_of(1, i), vw);
                 }
                 if (!decltype(all)::value && t0 + i >= at.len) gw = L::kInf, vw = 0u;
@@ -487,7 +545,20 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         for (int s = 0; s < kStages && s < steps; ++s) walk.load(s, chunk_of(s));
     __syncwarp();
 
+    Ahead<T, A, A == kTma ? 1 : 3> ahead;
+    auto fetch = [&](int s) {
+        if constexpr (A != kTma) {
+            const int t0 = chunk_of(s) * kChunk + warp * kTok;
+            const T* const rows[3] = {
+                static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0 + (int64_t)t0 * p.s_g,
+                static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0 + (int64_t)t0 * p.s_v,
+                static_cast<const T*>(p.dy) + (int64_t)at.seq * p.seq_dy + at.c0 + (int64_t)t0 * p.s_dy};
+            const int64_t pitch[3] = {p.s_g, p.s_v, p.s_dy};
+            ahead.load(rows, pitch, at, p.n_chan, at.len - t0);
+        }
+    };
     V c = ld_state<L>(p.dh1 ? p.dh1 + (int64_t)at.seq * p.seq_dh1 + at.c0 : nullptr, n);
+    if (steps > 0) fetch(0);
     for (int s = 0; s < steps; ++s) {
         const int chunk = chunk_of(s), t0 = chunk * kChunk + warp * kTok, b = s & 1;
         const uint32_t my = walk.mine(s);
@@ -496,17 +567,11 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         V h = ld_state<L>(chunk < p.n_chunk ? p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0 : nullptr,
                           n);
         if constexpr (A != kTma) {  // the lane's words, into its own slots
-            const T* g = static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0;
-            const T* v = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0;
-            const T* dy = static_cast<const T*>(p.dy) + (int64_t)at.seq * p.seq_dy + at.c0;
 #pragma unroll
-            for (int i = 0; i < kTok; ++i) {
-                const bool live = n > 0 && t0 + i < at.len;
-                const uint32_t gw = live ? ld_raw<T, A>(g + (int64_t)(t0 + i) * p.s_g, n) : 0u;
-                const uint32_t vw = live ? ld_raw<T, A>(v + (int64_t)(t0 + i) * p.s_v, n) : 0u;
-                const uint32_t yw = live ? ld_raw<T, A>(dy + (int64_t)(t0 + i) * p.s_dy, n) : 0u;
-                sts(my + word_of(0, i), gw), sts(my + word_of(1, i), vw), sts(my + word_of(2, i), yw);
-            }
+            for (int i = 0; i < kTok; ++i)
+#pragma unroll
+                for (int k = 0; k < 3; ++k) sts(my + word_of(k, i), ahead.get(k, i, lane));
+            if (s + 1 < steps) fetch(s + 1);
         }
         V z[kTok], q[kTok], D = L::splat(0.0f), B = D, E = D;
         walk.wait_tiles(s);
@@ -743,6 +808,7 @@ int launch_gated_a(const helix_ctx* ctx, const GatedMaps& maps, GatedParams p, b
     bool deep = false;
     p.cluster = cluster_of(ctx, groups, p.n_chunk, &deep);
     const int64_t grid = groups * p.cluster;
+    if (grad && A != kTma) deep = true;  // its loads ahead need the registers of one CTA per SM
     if (grad) {
         ClusterLaunch l(grid, p.cluster, tiles_smem(3, deep ? kGradDeep : kGradStages), stream);
         return deep ? cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep>, maps, p)
