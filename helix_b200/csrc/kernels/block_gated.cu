@@ -174,6 +174,11 @@ __device__ __forceinline__ void st_raw(T* p, int n, uint32_t w) {
     if (n == 2) q[1] = (unsigned short)(w >> 16);
 }
 template <typename L>
+__device__ __forceinline__ void ld_state(const float* p, int n, float (&a)[L::kN]) {
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) a[e] = p && e < n ? __ldg(p + e) : 0.0f;
+}
+template <typename L>
 __device__ __forceinline__ typename L::V ld_state(const float* p, int n) {
     float a[L::kN];
 #pragma unroll
@@ -224,11 +229,12 @@ struct Place {
 };
 
 // The warps' (D, B) of a step, and the totals of the cluster's CTAs with the
-// mbarrier they arrive on; two steps' worth each, since a warp may be a step
-// ahead of another.
-template <typename V, int K>
+// mbarrier they arrive on; two steps' worth, since a warp may be a step ahead
+// of another (the gradient's warps are not, and the 6 KB decide whether two of
+// its CTAs fit an SM).
+template <typename V, int K, int kSteps = 2>
 struct Meet {
-    V        warp[2][K][kWarps][32];
+    V        warp[kSteps][K][kWarps][32];
     V        total[2][2][kMaxCluster][32];
     uint64_t arrived[2];
 };
@@ -270,7 +276,7 @@ struct GatedMaps {
 
 // What the threads of a CTA share in the walk over its chunks: the tiles of
 // the K input tensors, kStages steps of them, and the meetings of a step.
-template <typename T, Access A, int K, int kStages>
+template <typename T, Access A, int K, int kStages, typename M>
 struct Walk {
     using L = Lane<T>;
     using V = typename L::V;
@@ -279,7 +285,7 @@ struct Walk {
     const Place<T>&    at;
     uint32_t           base;  // shared-memory address of the tiles
     uint64_t*          full;
-    Meet<V, K>*        meet;
+    M*                 meet;
     int                steps;
     bool               alive = true;
 
@@ -419,12 +425,13 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     using L = Lane<T>;
     using V = typename L::V;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ Meet<V, 2> meet;
+    using M = Meet<V, 2>;
+    __shared__ M meet;
     __shared__ uint64_t full[kStages];
 
     const Place<T> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
-    Walk<T, A, 2, kStages> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
+    Walk<T, A, 2, kStages, M> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
     const int steps = walk.steps;
     auto chunk_of = [&](int s) { return s * R + at.rank; };
     walk.begin();
@@ -532,12 +539,13 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
     using L = Lane<T>;
     using V = typename L::V;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ Meet<V, 3> meet;
+    using M = Meet<V, 3, 1>;
+    __shared__ M meet;
     __shared__ uint64_t full[kStages];
 
     const Place<T> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
-    Walk<T, A, 3, kStages> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
+    Walk<T, A, 3, kStages, M> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
     const int steps = walk.steps;
     auto chunk_of = [&](int s) { return (steps - 1 - s) * R + at.rank; };  // from the end
     walk.begin();
@@ -564,8 +572,9 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         const uint32_t my = walk.mine(s);
         // every token and channel of the warp counts
         const bool whole = t0 + kTok <= at.len && at.slab0() + 32 * L::kN <= p.n_chan;
-        V h = ld_state<L>(chunk < p.n_chunk ? p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0 : nullptr,
-                          n);
+        float entry[L::kN];  // the chunk's state; looked at after the warps have met
+        ld_state<L>(chunk < p.n_chunk ? p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0 : nullptr, n,
+                    entry);
         if constexpr (A != kTma) {  // the lane's words, into its own slots
 #pragma unroll
             for (int i = 0; i < kTok; ++i)
@@ -594,24 +603,25 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
             first(std::true_type{});
         else
             first(std::false_type{});
-        meet.warp[b][0][warp][lane] = D;
-        meet.warp[b][1][warp][lane] = B;
-        meet.warp[b][2][warp][lane] = E;
+        meet.warp[0][0][warp][lane] = D;
+        meet.warp[0][1][warp][lane] = B;
+        meet.warp[0][2][warp][lane] = E;
         __syncthreads();
         // what the CTA's later warps, and all of them, make of a gradient
         V dp = L::splat(0.0f), ep = dp, d = dp, t = dp;
 #pragma unroll
         for (int w = kWarps - 1; w >= 0; --w) {
             if (w == warp) dp = d, ep = t;
-            const V dw = meet.warp[b][0][w][lane];
-            t = fold<L>(t, dw, meet.warp[b][2][w][lane]);
+            const V dw = meet.warp[0][0][w][lane];
+            t = fold<L>(t, dw, meet.warp[0][2][w][lane]);
             d = grow<L>(d, dw);
         }
         if (R > 1) walk.send(s, d, t);
         // h_{t-1} - v_t of the warp's tokens, times the slopes
+        V h = L::of(entry);
 #pragma unroll
         for (int w = 0; w < kWarps - 1; ++w)
-            if (w < warp) h = fold<L>(h, meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
+            if (w < warp) h = fold<L>(h, meet.warp[0][0][w][lane], meet.warp[0][1][w][lane]);
 #pragma unroll
         for (int i = 0; i < kTok; ++i) {
             const V off = L::fma(whole || t0 + i < at.len ? L::unpack(lds(my + word_of(1, i))) : L::splat(0.0f),
@@ -650,11 +660,9 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
             second(std::true_type{});
         else
             second(std::false_type{});
-        if (s + kStages < steps) {
-            __syncthreads();
-            if (walk.issuer()) walk.load(s + kStages, chunk_of(s + kStages));
-            __syncwarp();
-        }
+        __syncthreads();  // every warp is done with the tiles and the meeting
+        if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
+        __syncwarp();
     }
     walk.end();
     if (p.dh0 && at.rank == 0 && warp == 0) st_state<L>(p.dh0 + (int64_t)at.seq * p.seq_dh0 + at.c0, n, c);
