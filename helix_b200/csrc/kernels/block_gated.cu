@@ -207,26 +207,49 @@ __device__ __forceinline__ uint32_t lds(uint32_t a) {
     return v;
 }
 __device__ __forceinline__ void sts(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v)); }
-__host__ __device__ constexpr uint32_t word_of(int k, int i) { return (uint32_t)(k * kTileBytes + i * 128); }
 
-// Where a thread is: its group of channels, and its tokens of a chunk.
-template <typename T>
+// How a CTA cuts its tile: rows of LW lanes' channels (32, or 16 to make twice
+// as many CTAs of few channels), a run of 16 tokens for each LW lanes.
+template <int LW>
+struct Cut {
+    static constexpr int kRuns = 32 / LW;                    // runs of a warp
+    static constexpr int kTokens = kWarps * kRuns * kTok;    // of a CTA and step
+    static constexpr int kRow = 4 * LW;                      // bytes
+    static_assert(kTokens * kRow == kTileBytes, "tile");
+    // Word i of tensor k, from the lane's first word.
+    static __host__ __device__ constexpr uint32_t word(int k, int i) { return (uint32_t)(k * kTileBytes + i * kRow); }
+};
+
+// Where a thread is: its group of channels, and its run of a step's tokens.
+template <typename T, int LW>
 struct Place {
-    int warp, lane, rank, seq, c0, n, len;
+    int warp, lane, l, run, rank, seq, c0, n, len;
     __device__ __forceinline__ Place(const GatedParams& p) {
-        constexpr int N = Lane<T>::kN, CB = 32 * N;
+        constexpr int N = Lane<T>::kN, CB = LW * N;
         warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
         lane = threadIdx.x & 31;
+        l = lane % LW;
+        run = warp * Cut<LW>::kRuns + lane / LW;
         rank = (int)(blockIdx.x % (unsigned)p.cluster);
         const int slabs = (p.n_chan + CB - 1) / CB;
         const unsigned group = blockIdx.x / (unsigned)p.cluster;
         seq = (int)(group / (unsigned)slabs);
-        c0 = (int)(group % (unsigned)slabs) * CB + N * lane;
+        c0 = (int)(group % (unsigned)slabs) * CB + N * l;
         n = max(0, min(N, p.n_chan - c0));
         len = length_of(p, seq);
     }
-    __device__ __forceinline__ int slab0() const { return c0 - Lane<T>::kN * lane; }
+    __device__ __forceinline__ int slab0() const { return c0 - Lane<T>::kN * l; }
+    // Whether every token and channel of the warp counts, in the step at `base`.
+    __device__ __forceinline__ bool whole(const GatedParams& p, int base) const {
+        return base + (warp + 1) * Cut<LW>::kRuns * kTok <= len && slab0() + LW * Lane<T>::kN <= p.n_chan;
+    }
 };
+
+// The values of the warp's first and last run, where it has two.
+__device__ __forceinline__ float of_lane(float v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
+    return __shfl_sync(0xffffffffu, (unsigned long long)v, lane);
+}
 
 // The warps' (D, B) of a step, and the totals of the cluster's CTAs with the
 // mbarrier they arrive on; two steps' worth, since a warp may be a step ahead
@@ -276,22 +299,22 @@ struct GatedMaps {
 
 // What the threads of a CTA share in the walk over its chunks: the tiles of
 // the K input tensors, kStages steps of them, and the meetings of a step.
-template <typename T, Access A, int K, int kStages, typename M>
+template <typename T, Access A, int K, int kStages, int LW, typename M>
 struct Walk {
     using L = Lane<T>;
     using V = typename L::V;
     const GatedMaps&   maps;
     const GatedParams& p;
-    const Place<T>&    at;
+    const Place<T, LW>& at;
     uint32_t           base;  // shared-memory address of the tiles
     uint64_t*          full;
     M*                 meet;
     int                steps;
     bool               alive = true;
 
-    // The lane's words of step s; word i of tensor k is 128 i + kTileBytes k further on.
+    // The lane's words of step s.
     __device__ __forceinline__ uint32_t mine(int s) const {
-        return base + (uint32_t)((s % kStages) * K * kTileBytes + at.warp * kTok * 128 + at.lane * 4);
+        return base + (uint32_t)((s % kStages) * K * kTileBytes + at.run * kTok * Cut<LW>::kRow + at.l * 4);
     }
     __device__ __forceinline__ bool issuer() const { return A == kTma && threadIdx.x == kThreads - 1; }
     // One thread: step s's tiles (chunk `chunk`) start to arrive.
@@ -301,7 +324,7 @@ struct Walk {
 #pragma unroll
         for (int k = 0; k < K; ++k)
             tma_load_3d(base + (uint32_t)(((s % kStages) * K + k) * kTileBytes), &maps.in[k], bar, at.slab0(),
-                        chunk * kChunk, at.seq);
+                        chunk * Cut<LW>::kTokens, at.seq);
     }
     __device__ __forceinline__ void gave_up() {
         alive = false;
@@ -374,7 +397,7 @@ struct Ahead {
         return ((odd >> k) ^ ((odd >> (8 + k)) & (uint32_t)i)) & 1u;
     }
     // rows[k]: row t0 of tensor k at the lane's first channel; live: rows that exist
-    __device__ __forceinline__ void load(const T* const (&rows)[K], const int64_t (&pitch)[K], const Place<T>& at,
+    __device__ __forceinline__ void load(const T* const (&rows)[K], const int64_t (&pitch)[K], const Place<T, 32>& at,
                                          int n_chan, int live) {
         if constexpr (A == kHalf) {
             odd = 0;
@@ -419,7 +442,7 @@ struct Ahead {
     }
 };
 
-template <typename T, Access A, int kStages>
+template <typename T, Access A, int kStages, int LW>
 __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     gated_kernel(const __grid_constant__ GatedMaps maps, const __grid_constant__ GatedParams p) {
     using L = Lane<T>;
@@ -429,9 +452,10 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     __shared__ M meet;
     __shared__ uint64_t full[kStages];
 
-    const Place<T> at(p);
+    const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
-    Walk<T, A, 2, kStages, M> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
+    const int chunks = (p.n_tok + Cut<LW>::kTokens - 1) / Cut<LW>::kTokens;
+    Walk<T, A, 2, kStages, LW, M> walk{maps, p, at, align128(smem_raw), full, &meet, (chunks + R - 1) / R};
     const int steps = walk.steps;
     auto chunk_of = [&](int s) { return s * R + at.rank; };
     walk.begin();
@@ -442,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     Ahead<T, A, A == kTma ? 1 : 2> ahead;
     auto fetch = [&](int s) {
         if constexpr (A != kTma) {
-            const int t0 = chunk_of(s) * kChunk + warp * kTok;
+            const int t0 = chunk_of(s) * Cut<LW>::kTokens + at.run * kTok;
             const T* const rows[2] = {
                 static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0 + (int64_t)t0 * p.s_g,
                 static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0 + (int64_t)t0 * p.s_v};
@@ -453,10 +477,9 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     V h = ld_state<L>(p.h0 ? p.h0 + (int64_t)at.seq * p.seq_h0 + at.c0 : nullptr, n);
     if (steps > 0) fetch(0);
     for (int s = 0; s < steps; ++s) {
-        const int chunk = chunk_of(s), t0 = chunk * kChunk + warp * kTok, b = s & 1;
+        const int base = chunk_of(s) * Cut<LW>::kTokens, t0 = base + at.run * kTok, b = s & 1;
         const uint32_t my = walk.mine(s);
-        // every token and channel of the warp counts
-        const bool whole = t0 + kTok <= at.len && at.slab0() + 32 * L::kN <= p.n_chan;
+        const bool whole = at.whole(p, base);
         V z[kTok], D = L::splat(0.0f), B = D;
         walk.wait_tiles(s);
         auto first = [&](auto all) {
@@ -464,10 +487,10 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
             for (int i = 0; i < kTok; ++i) {
                 uint32_t gw, vw;
                 if constexpr (A == kTma) {
-                    gw = lds(my + word_of(0, i)), vw = lds(my + word_of(1, i));
+                    gw = lds(my + Cut<LW>::word(0, i)), vw = lds(my + Cut<LW>::word(1, i));
                 } else {
                     gw = ahead.get(0, i, lane), vw = ahead.get(1, i, lane);
-                    sts(my + word_of(1, i), vw);
+                    sts(my + Cut<LW>::word(1, i), vw);
                 }
                 if (!decltype(all)::value && t0 + i >= at.len) gw = L::kInf, vw = 0u;
                 z[i] = gate<T>(L::unpack(gw));
@@ -480,6 +503,13 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
         else
             first(std::false_type{});
         if (s + 1 < steps) fetch(s + 1);
+        V d0 = D, b0 = B;  // the warp's first run
+        if (LW == 16) {
+            const V d1 = of_lane(D, at.l + 16), b1 = of_lane(B, at.l + 16);
+            d0 = of_lane(D, at.l), b0 = of_lane(B, at.l);
+            D = grow<L>(d0, d1);
+            B = fold<L>(b0, d1, b1);
+        }
         meet.warp[b][0][warp][lane] = D;
         meet.warp[b][1][warp][lane] = B;
         __syncthreads();
@@ -503,15 +533,16 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
         } else {
             h = fold<L>(h, d, t);
         }
-        if (p.states && warp == 0 && chunk < p.n_chunk)
-            st_state<L>(p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0, n, hw);
         hw = fold<L>(hw, dp, bp);
+        if (LW == 16 && lane >= 16) hw = fold<L>(hw, d0, b0);
+        if (p.states && t0 % kChunk == 0 && t0 < p.n_tok)
+            st_state<L>(p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0, n, hw);
         T* y = static_cast<T*>(p.y) + (int64_t)at.seq * p.seq_y + at.c0 + (int64_t)t0 * p.s_y;
         auto second = [&](auto all) {
 #pragma unroll
             for (int i = 0; i < kTok; ++i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
-                hw = step<L>(hw, z[i], past ? L::splat(0.0f) : L::unpack(lds(my + word_of(1, i))));
+                hw = step<L>(hw, z[i], past ? L::splat(0.0f) : L::unpack(lds(my + Cut<LW>::word(1, i))));
                 if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok))
                     st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(hw));
                 y += p.s_y;
@@ -530,10 +561,10 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     walk.end();
     // Every CTA holds the last state.  In place of h0 is safe: each has read
     // h0 before the cluster's last barrier.
-    if (at.rank == 0 && warp == 0) st_state<L>(p.h1 + (int64_t)at.seq * p.seq_h1 + at.c0, n, h);
+    if (at.rank == 0 && warp == 0 && lane < LW) st_state<L>(p.h1 + (int64_t)at.seq * p.seq_h1 + at.c0, n, h);
 }
 
-template <typename T, Access A, int kStages>
+template <typename T, Access A, int kStages, int LW>
 __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
     gated_grad_kernel(const __grid_constant__ GatedMaps maps, const __grid_constant__ GatedParams p) {
     using L = Lane<T>;
@@ -543,9 +574,10 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
     __shared__ M meet;
     __shared__ uint64_t full[kStages];
 
-    const Place<T> at(p);
+    const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
-    Walk<T, A, 3, kStages, M> walk{maps, p, at, align128(smem_raw), full, &meet, (p.n_chunk + R - 1) / R};
+    const int chunks = (p.n_tok + Cut<LW>::kTokens - 1) / Cut<LW>::kTokens;
+    Walk<T, A, 3, kStages, LW, M> walk{maps, p, at, align128(smem_raw), full, &meet, (chunks + R - 1) / R};
     const int steps = walk.steps;
     auto chunk_of = [&](int s) { return (steps - 1 - s) * R + at.rank; };  // from the end
     walk.begin();
@@ -556,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
     Ahead<T, A, A == kTma ? 1 : 3> ahead;
     auto fetch = [&](int s) {
         if constexpr (A != kTma) {
-            const int t0 = chunk_of(s) * kChunk + warp * kTok;
+            const int t0 = chunk_of(s) * Cut<LW>::kTokens + at.run * kTok;
             const T* const rows[3] = {
                 static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0 + (int64_t)t0 * p.s_g,
                 static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0 + (int64_t)t0 * p.s_v,
@@ -568,18 +600,17 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
     V c = ld_state<L>(p.dh1 ? p.dh1 + (int64_t)at.seq * p.seq_dh1 + at.c0 : nullptr, n);
     if (steps > 0) fetch(0);
     for (int s = 0; s < steps; ++s) {
-        const int chunk = chunk_of(s), t0 = chunk * kChunk + warp * kTok, b = s & 1;
+        const int base = chunk_of(s) * Cut<LW>::kTokens, t0 = base + at.run * kTok, b = s & 1;
         const uint32_t my = walk.mine(s);
-        // every token and channel of the warp counts
-        const bool whole = t0 + kTok <= at.len && at.slab0() + 32 * L::kN <= p.n_chan;
+        const bool whole = at.whole(p, base);
         float entry[L::kN];  // the chunk's state; looked at after the warps have met
-        ld_state<L>(chunk < p.n_chunk ? p.states + ((int64_t)at.seq * p.n_chunk + chunk) * p.n_chan + at.c0 : nullptr, n,
+        ld_state<L>(t0 < p.n_tok ? p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0 : nullptr, n,
                     entry);
         if constexpr (A != kTma) {  // the lane's words, into its own slots
 #pragma unroll
             for (int i = 0; i < kTok; ++i)
 #pragma unroll
-                for (int k = 0; k < 3; ++k) sts(my + word_of(k, i), ahead.get(k, i, lane));
+                for (int k = 0; k < 3; ++k) sts(my + Cut<LW>::word(k, i), ahead.get(k, i, lane));
             if (s + 1 < steps) fetch(s + 1);
         }
         V z[kTok], q[kTok], D = L::splat(0.0f), B = D, E = D;
@@ -588,14 +619,14 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
             auto past = [&](int i) { return !decltype(all)::value && t0 + i >= at.len; };
 #pragma unroll
             for (int i = 0; i < kTok; ++i) {
-                const uint32_t gw = past(i) ? L::kInf : lds(my + word_of(0, i)), vw = past(i) ? 0u : lds(my + word_of(1, i));
+                const uint32_t gw = past(i) ? L::kInf : lds(my + Cut<LW>::word(0, i)), vw = past(i) ? 0u : lds(my + Cut<LW>::word(1, i));
                 gate_slope<T>(L::unpack(gw), z[i], q[i]);
                 D = grow<L>(D, z[i]);
                 B = step<L>(B, z[i], L::unpack(vw));
             }
 #pragma unroll
             for (int i = kTok - 1; i >= 0; --i) {
-                const V lam = L::add(L::unpack(past(i) ? 0u : lds(my + word_of(2, i))), E);
+                const V lam = L::add(L::unpack(past(i) ? 0u : lds(my + Cut<LW>::word(2, i))), E);
                 E = L::fma(z[i], lam, lam);
             }
         };
@@ -603,6 +634,15 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
             first(std::true_type{});
         else
             first(std::false_type{});
+        V d0 = D, b0 = B, d1 = D, e1 = E;  // the warp's first run, and its last
+        if (LW == 16) {
+            const V b1 = of_lane(B, at.l + 16), e0 = of_lane(E, at.l);
+            d0 = of_lane(D, at.l), b0 = of_lane(B, at.l);
+            d1 = of_lane(D, at.l + 16), e1 = of_lane(E, at.l + 16);
+            D = grow<L>(d0, d1);
+            B = fold<L>(b0, d1, b1);
+            E = fold<L>(e1, d0, e0);
+        }
         meet.warp[0][0][warp][lane] = D;
         meet.warp[0][1][warp][lane] = B;
         meet.warp[0][2][warp][lane] = E;
@@ -621,10 +661,12 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         V h = L::of(entry);
 #pragma unroll
         for (int w = 0; w < kWarps - 1; ++w)
-            if (w < warp) h = fold<L>(h, meet.warp[0][0][w][lane], meet.warp[0][1][w][lane]);
+            if (w < warp && w * Cut<LW>::kRuns * kTok >= at.run * kTok / kChunk * kChunk)
+                h = fold<L>(h, meet.warp[0][0][w][lane], meet.warp[0][1][w][lane]);
+        if (LW == 16 && lane >= 16) h = fold<L>(h, d0, b0);
 #pragma unroll
         for (int i = 0; i < kTok; ++i) {
-            const V off = L::fma(whole || t0 + i < at.len ? L::unpack(lds(my + word_of(1, i))) : L::splat(0.0f),
+            const V off = L::fma(whole || t0 + i < at.len ? L::unpack(lds(my + Cut<LW>::word(1, i))) : L::splat(0.0f),
                                  L::splat(-1.0f), h);
             q[i] = L::mul(q[i], off);
             h = L::fma(z[i], off, h);
@@ -640,13 +682,14 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
             c = fold<L>(c, d, t);
         }
         cw = fold<L>(cw, dp, ep);
+        if (LW == 16 && lane < 16) cw = fold<L>(cw, d1, e1);
         T* dg = static_cast<T*>(p.dg) + (int64_t)at.seq * p.seq_dg + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dg;
         T* dv = static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dv;
         auto second = [&](auto all) {
 #pragma unroll
             for (int i = kTok - 1; i >= 0; --i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
-                const V lam = L::add(past ? L::splat(0.0f) : L::unpack(lds(my + word_of(2, i))), cw);
+                const V lam = L::add(past ? L::splat(0.0f) : L::unpack(lds(my + Cut<LW>::word(2, i))), cw);
                 if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok)) {
                     const int k = decltype(all)::value ? L::kN : n;
                     st_raw<T, A>(dg, k, past ? 0u : L::pack(L::mul(lam, q[i])));
@@ -665,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         __syncwarp();
     }
     walk.end();
-    if (p.dh0 && at.rank == 0 && warp == 0) st_state<L>(p.dh0 + (int64_t)at.seq * p.seq_dh0 + at.c0, n, c);
+    if (p.dh0 && at.rank == 0 && warp == 0 && lane < LW) st_state<L>(p.dh0 + (int64_t)at.seq * p.seq_dh0 + at.c0, n, c);
 }
 
 // Up to NT tokens: a warp has the channels of one slab of one sequence.
@@ -740,10 +783,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 constexpr int kFwdStages = 3, kFwdDeep = 6, kGradStages = 2, kGradDeep = 4;
 constexpr size_t tiles_smem(int tensors, int stages) { return (size_t)stages * tensors * kTileBytes + 128; }
 
-// [n_seq][n_tok][n_chan] in boxes of 128 tokens x 128 bytes; false when TMA
+// [n_seq][n_tok][n_chan] in boxes of row_bytes bytes of a tile's tokens; false when TMA
 // cannot describe it.  Rows and channels past the ends read as zero.
 bool make_map_tok(const helix_ctx* ctx, CUtensorMap* m, const GatedParams& p, const void* base, int64_t s_tok,
-                  int64_t s_seq, int size) {
+                  int64_t s_seq, int size, int row_bytes) {
     if (reinterpret_cast<uintptr_t>(base) % 16) return false;
     const int64_t row = ((int64_t)p.n_chan * size + 15) / 16 * 16;
     const int64_t bt = p.n_tok > 1 ? s_tok * size : row, bs = p.n_seq > 1 ? s_seq * size : row;
@@ -751,7 +794,7 @@ bool make_map_tok(const helix_ctx* ctx, CUtensorMap* m, const GatedParams& p, co
     const auto fn = reinterpret_cast<tc::EncodeFn>(ctx->encode_tiled);
     cuuint64_t dims[3] = {(cuuint64_t)p.n_chan, (cuuint64_t)p.n_tok, (cuuint64_t)p.n_seq};
     cuuint64_t strides[2] = {(cuuint64_t)bt, (cuuint64_t)bs};
-    cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)kChunk, 1};
+    cuuint32_t box[3] = {(cuuint32_t)(row_bytes / size), (cuuint32_t)(kTileBytes / row_bytes), 1};
     cuuint32_t es[3] = {1, 1, 1};
     return fn(m, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
               const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -759,25 +802,38 @@ bool make_map_tok(const helix_ctx* ctx, CUtensorMap* m, const GatedParams& p, co
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool make_maps(const helix_ctx* ctx, GatedMaps* m, const GatedParams& p, bool grad, int size) {
+bool make_maps(const helix_ctx* ctx, GatedMaps* m, const GatedParams& p, bool grad, int size, int row_bytes) {
     std::memset(m, 0, sizeof(*m));
     if (!ctx->encode_tiled || p.n_tok <= 0) return false;
-    if (!make_map_tok(ctx, &m->in[0], p, p.g, p.s_g, p.seq_g, size)) return false;
-    if (!make_map_tok(ctx, &m->in[1], p, p.v, p.s_v, p.seq_v, size)) return false;
-    return !grad || make_map_tok(ctx, &m->in[2], p, p.dy, p.s_dy, p.seq_dy, size);
+    if (!make_map_tok(ctx, &m->in[0], p, p.g, p.s_g, p.seq_g, size, row_bytes)) return false;
+    if (!make_map_tok(ctx, &m->in[1], p, p.v, p.s_v, p.seq_v, size, row_bytes)) return false;
+    return !grad || make_map_tok(ctx, &m->in[2], p, p.dy, p.s_dy, p.seq_dy, size, row_bytes);
 }
 
-// CTAs of a cluster: the size with the fewest steps, counting the waves that
-// its clusters take, two CTAs per SM (large clusters leave SMs of a GPC idle),
-// and two steps to fill and drain each.
-int cluster_of(const helix_ctx* ctx, int64_t groups, int chunks, bool* deep) {
-    int best = 1;
+// Lanes of a row, CTAs of a cluster, and whether one CTA per SM is enough: the
+// choice with the fewest steps, counting the waves that its clusters take, two
+// CTAs per SM (large clusters leave SMs of a GPC idle), and two steps to fill
+// and drain each.  Narrow rows (TMA only) serve few channels: 1 x 131072 x 1024
+// bf16 takes 208 us with them, 338 without.
+struct GatedCut {
+    int  lanes = 32, cluster = 1;
+    bool deep = false;
+};
+GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, bool narrow) {
+    GatedCut best;
     int64_t least = INT64_MAX;
-    for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
-        const int64_t at_once = ctx->gated_clusters[i];
-        if (at_once <= 0 || (r > 1 && r >= 2 * chunks)) continue;
-        const int64_t cost = (groups + at_once - 1) / at_once * ((chunks + r - 1) / r + 2);
-        if (cost < least) least = cost, best = r, *deep = groups <= ctx->gated_deep[i];
+    for (int lanes = 32; lanes >= (narrow ? 16 : 32); lanes /= 2) {
+        const int64_t cb = lanes * lane_channels, groups = (int64_t)p.n_seq * ((p.n_chan + cb - 1) / cb);
+        const int64_t tokens = kChunk * (32 / lanes), chunks = (p.n_tok + tokens - 1) / tokens;
+        for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
+            const int64_t at_once = ctx->gated_clusters[i];
+            if (at_once <= 0 || (r > 1 && r >= 2 * chunks)) continue;
+            const int64_t cost = (groups + at_once - 1) / at_once * ((chunks + r - 1) / r + 2);
+            if (cost < least) {
+                least = cost;
+                best.lanes = lanes, best.cluster = r, best.deep = groups <= ctx->gated_deep[i];
+            }
+        }
     }
     return best;
 }
@@ -805,39 +861,61 @@ int launch_few(const GatedParams& p, int64_t groups, bool grad, void* stream) {
                 : block_launch(gated_few_kernel<T, A, false, NT>, grid, block, 0, stream, p);
 }
 
-template <typename T, Access A>
-int launch_gated_a(const helix_ctx* ctx, const GatedMaps& maps, GatedParams p, bool grad, void* stream) {
-    constexpr int CB = 32 * Lane<T>::kN;
-    constexpr Access few = A == kTma ? kWord : A;
+template <typename T, Access A, int LW>
+int launch_gated_a(const GatedMaps& maps, GatedParams p, const GatedCut& cut, bool grad, void* stream) {
+    constexpr int CB = LW * Lane<T>::kN;
     const int64_t groups = (int64_t)p.n_seq * ((p.n_chan + CB - 1) / CB);
-    if (p.n_tok <= 1) return launch_few<T, few, 1>(p, groups, grad, stream);
-    if (p.n_tok <= 4) return launch_few<T, few, 4>(p, groups, grad, stream);
-    if (p.n_tok <= kTok) return launch_few<T, few, kTok>(p, groups, grad, stream);
-    bool deep = false;
-    p.cluster = cluster_of(ctx, groups, p.n_chunk, &deep);
+    p.cluster = cut.cluster;
     const int64_t grid = groups * p.cluster;
-    if (grad && A != kTma) deep = true;  // its loads ahead need the registers of one CTA per SM
     if (grad) {
+        // plain loads ahead need the registers of one CTA per SM
+        const bool deep = cut.deep || A != kTma;
         ClusterLaunch l(grid, p.cluster, tiles_smem(3, deep ? kGradDeep : kGradStages), stream);
-        return deep ? cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep>, maps, p)
-                    : cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradStages>, maps, p);
+        if (deep) return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep, LW>, maps, p);
+        if constexpr (A == kTma) return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradStages, LW>, maps, p);
     }
-    ClusterLaunch l(grid, p.cluster, tiles_smem(2, deep ? kFwdDeep : kFwdStages), stream);
-    return deep ? cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdDeep>, maps, p)
-                : cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdStages>, maps, p);
+    ClusterLaunch l(grid, p.cluster, tiles_smem(2, cut.deep ? kFwdDeep : kFwdStages), stream);
+    return cut.deep ? cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdDeep, LW>, maps, p)
+                    : cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdStages, LW>, maps, p);
+}
+
+template <typename T, Access A>
+int launch_gated_few(const GatedParams& p, bool grad, void* stream) {
+    constexpr int CB = 32 * Lane<T>::kN;
+    const int64_t groups = (int64_t)p.n_seq * ((p.n_chan + CB - 1) / CB);
+    return p.n_tok <= 1   ? launch_few<T, A, 1>(p, groups, grad, stream)
+           : p.n_tok <= 4 ? launch_few<T, A, 4>(p, groups, grad, stream)
+                          : launch_few<T, A, kTok>(p, groups, grad, stream);
+}
+
+template <typename T>
+int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool grad, void* stream) {
+    constexpr int N = Lane<T>::kN;
+    if (p.n_tok <= kTok) {
+        if constexpr (N == 2)
+            if (!word) return launch_gated_few<T, kHalf>(p, grad, stream);
+        return launch_gated_few<T, kWord>(p, grad, stream);
+    }
+    // outputs are stored a word at a time in the TMA form too
+    if (word) {
+        const GatedCut cut = cut_of(ctx, p, N, true);
+        GatedMaps maps;
+        if (make_maps(ctx, &maps, p, grad, sizeof(T), 4 * cut.lanes))
+            return cut.lanes == 16 ? launch_gated_a<T, kTma, 16>(maps, p, cut, grad, stream)
+                                   : launch_gated_a<T, kTma, 32>(maps, p, cut, grad, stream);
+    }
+    GatedMaps none;
+    std::memset(&none, 0, sizeof(none));
+    const GatedCut cut = cut_of(ctx, p, N, false);
+    if constexpr (N == 2)
+        if (!word) return launch_gated_a<T, kHalf, 32>(none, p, cut, grad, stream);
+    return launch_gated_a<T, kWord, 32>(none, p, cut, grad, stream);
 }
 
 int launch_gated_any(const helix_ctx* ctx, const helix_gated_scan_desc& d, const GatedParams& p, bool word, bool grad,
                      void* stream) {
-    GatedMaps maps;
-    const bool tma = p.n_tok > kTok && make_maps(ctx, &maps, p, grad, d.io_dtype == HELIX_F32 ? 4 : 2);
-    if (d.io_dtype == HELIX_F32)
-        return tma ? launch_gated_a<float, kTma>(ctx, maps, p, grad, stream)
-                   : launch_gated_a<float, kWord>(ctx, maps, p, grad, stream);
-    // outputs are stored a word at a time in the TMA form too
-    if (tma && word) return launch_gated_a<__nv_bfloat16, kTma>(ctx, maps, p, grad, stream);
-    return word ? launch_gated_a<__nv_bfloat16, kWord>(ctx, maps, p, grad, stream)
-                : launch_gated_a<__nv_bfloat16, kHalf>(ctx, maps, p, grad, stream);
+    return d.io_dtype == HELIX_F32 ? launch_gated_t<float>(ctx, p, word, grad, stream)
+                                   : launch_gated_t<__nv_bfloat16>(ctx, p, word, grad, stream);
 }
 
 template <typename K>
@@ -845,31 +923,34 @@ int set_smem(K kernel, int tensors, int stages) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles_smem(tensors, stages));
 }
 
-template <typename T, Access A>
+template <typename T, Access A, int LW>
 int configure_gated_a() {
     int e;
-    if ((e = set_smem(gated_kernel<T, A, kFwdStages>, 2, kFwdStages)) != cudaSuccess) return e;
-    if ((e = set_smem(gated_kernel<T, A, kFwdDeep>, 2, kFwdDeep)) != cudaSuccess) return e;
-    if ((e = set_smem(gated_grad_kernel<T, A, kGradStages>, 3, kGradStages)) != cudaSuccess) return e;
-    return set_smem(gated_grad_kernel<T, A, kGradDeep>, 3, kGradDeep);
+    if ((e = set_smem(gated_kernel<T, A, kFwdStages, LW>, 2, kFwdStages)) != cudaSuccess) return e;
+    if ((e = set_smem(gated_kernel<T, A, kFwdDeep, LW>, 2, kFwdDeep)) != cudaSuccess) return e;
+    if constexpr (A == kTma)
+        if ((e = set_smem(gated_grad_kernel<T, A, kGradStages, LW>, 3, kGradStages)) != cudaSuccess) return e;
+    return set_smem(gated_grad_kernel<T, A, kGradDeep, LW>, 3, kGradDeep);
 }
 
 }  // namespace
 
 int configure_gated(helix_ctx* ctx) {
     int e;
-    if ((e = configure_gated_a<float, kTma>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<float, kWord>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<__nv_bfloat16, kTma>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<__nv_bfloat16, kWord>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<__nv_bfloat16, kHalf>()) != cudaSuccess) return e;
+    if ((e = configure_gated_a<float, kTma, 32>()) != cudaSuccess) return e;
+    if ((e = configure_gated_a<float, kTma, 16>()) != cudaSuccess) return e;
+    if ((e = configure_gated_a<float, kWord, 32>()) != cudaSuccess) return e;
+    if ((e = configure_gated_a<__nv_bfloat16, kTma, 32>()) != cudaSuccess) return e;
+    if ((e = configure_gated_a<__nv_bfloat16, kTma, 16>()) != cudaSuccess) return e;
+    if ((e = configure_gated_a<__nv_bfloat16, kWord, 32>()) != cudaSuccess) return e;
+    if ((e = configure_gated_a<__nv_bfloat16, kHalf, 32>()) != cudaSuccess) return e;
     for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
         ClusterLaunch l(r, r, tiles_smem(2, kFwdStages), nullptr);
-        e = cudaOccupancyMaxActiveClusters(&ctx->gated_clusters[i], gated_kernel<__nv_bfloat16, kTma, kFwdStages>,
+        e = cudaOccupancyMaxActiveClusters(&ctx->gated_clusters[i], gated_kernel<__nv_bfloat16, kTma, kFwdStages, 32>,
                                            &l.cfg);
         if (e != cudaSuccess) return e;
         l.cfg.dynamicSmemBytes = tiles_smem(2, kFwdDeep);
-        e = cudaOccupancyMaxActiveClusters(&ctx->gated_deep[i], gated_kernel<__nv_bfloat16, kTma, kFwdDeep>, &l.cfg);
+        e = cudaOccupancyMaxActiveClusters(&ctx->gated_deep[i], gated_kernel<__nv_bfloat16, kTma, kFwdDeep, 32>, &l.cfg);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
