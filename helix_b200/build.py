@@ -1,4 +1,5 @@
-"""Builds libhelix.so (the C-ABI library) in-tree for sm_100a.
+"""Builds libhelix.so (the C-ABI library) in-tree for sm_100a, and the torch
+extension _block_torch.so over it (csrc/torch, host code only).
 
 Every CUDA source is compiled by nvcc with
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo``; host sources go through
@@ -11,10 +12,12 @@ Usage: python -m helix_b200.build [-v] [--force]
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,6 +25,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libhelix.so"
+TORCH_SRC = CSRC / "torch" / "block_torch.cpp"
+TORCH_EXT = PKG / "_block_torch.so"
 
 NVCC = os.environ.get("NVCC", shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -55,6 +60,29 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_torch(force: bool) -> None:
+    """The extension is left out where torch is not installed."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return
+    newest = max(p.stat().st_mtime for p in [TORCH_SRC, *headers()])
+    if not force and TORCH_EXT.exists() and TORCH_EXT.stat().st_mtime >= newest:
+        return
+    torch = Path(list(spec.submodule_search_locations)[0])
+    cuda = Path(NVCC).resolve().parent.parent
+    tmp = BUILD / TORCH_EXT.name
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-I{ROOT / 'include'}", f"-isystem{torch / 'include'}",
+           f"-isystem{torch / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-isystem{cuda / 'include'}",
+           f"-isystem{sysconfig.get_paths()['include']}", str(TORCH_SRC), "-o", str(tmp), f"-L{PKG}", "-l:libhelix.so",
+           f"-L{torch / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {TORCH_SRC}\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    shutil.move(tmp, TORCH_EXT)
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     srcs = sources()
@@ -70,6 +98,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    _build_torch(force)
     return LIB
 
 
