@@ -17,36 +17,41 @@ constexpr int kQThreads = 256;
 
 __device__ __forceinline__ int unit_of(int col, int unit) { return unit ^ (((col >> 3) ^ col) & 15); }
 
-// Eight consecutive values at any address of the type's alignment, of which
-// those from `end` on do not exist (and read as anything): the aligned
-// 16-byte pieces that hold them, shifted together.  Every piece read holds a
-// value that exists.
+// Eight consecutive values at any address of the type's alignment: the
+// aligned 16-byte pieces that hold those before `end` (zeros for the others),
+// and the values shifted out of them.  Every piece read holds a value that
+// exists.
 template <typename T>
-__device__ __forceinline__ void ld8_any(const T* p, const T* end, float (&f)[8]) {
-    constexpr int kPieces = (int)sizeof(T) / 2 + 1;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p), to = reinterpret_cast<uintptr_t>(end);
-    const uint32_t off = (uint32_t)(at & 15);
-    uint32_t w[4 * kPieces];
+struct Any8 {
+    static constexpr int kPieces = (int)sizeof(T) / 2 + 1;
+    uint32_t w[4 * kPieces], off;
+    __device__ __forceinline__ void load(const T* p, const T* end) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p), to = reinterpret_cast<uintptr_t>(end);
+        off = (uint32_t)(at & 15);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-        const uintptr_t q = at - off + 16 * i;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (q < to && (i < kPieces - 1 || off)) v = *reinterpret_cast<const uint4*>(q);
-        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        for (int i = 0; i < kPieces; ++i) {
+            const uintptr_t q = at - off + 16 * i;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (at < to && q < to && (i < kPieces - 1 || off)) v = *reinterpret_cast<const uint4*>(q);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
     }
+    __device__ __forceinline__ void get(float (&f)[8]) {
 #pragma unroll
-    for (int i = 0; i + 2 < 4 * kPieces; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+        for (int i = 0; i + 2 < 4 * kPieces; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
 #pragma unroll
-    for (int i = 0; i + 3 < 4 * kPieces; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
-    if constexpr (sizeof(T) == 2) {
+        for (int i = 0; i + 3 < 4 * kPieces; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = off & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+            for (int i = 0; i < 4; ++i) w[i] = off & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+        }
+        Raw8<T> raw;
+#pragma unroll
+        for (int i = 0; i < kPieces - 1; ++i)
+            raw.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        raw.unpack(f);
     }
-    Raw8<T> raw;
-#pragma unroll
-    for (int i = 0; i < kPieces - 1; ++i) raw.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    raw.unpack(f);
-}
+};
 
 template <typename T, bool BLOCKS, bool TURN, bool VEC>
 __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p) {
@@ -60,25 +65,43 @@ __global__ void __launch_bounds__(kQThreads, 3) quant_kernel(const QuantParams p
     const int rows = (int)(p.n_row - r0 < kTile ? p.n_row - r0 : kTile);
     const int cols = (int)(p.n_col - c0 < kTile ? p.n_col - c0 : kTile);
     const int rt = 16 * warp + 8 * hi;  // the lane's first row
-    const bool full = rows == kTile && cols == kTile;
     auto col = [&](int e) { return 8 * l + e; };
 
     float x[8][8];
     const T* src = static_cast<const T*>(p.x) + r0 * p.ld_x + c0;
-    if (VEC && full) {
+    // every load of a row (misaligned: of half the rows) before the first look
+    if constexpr (VEC) {
         Raw8<T> raw[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw[i].load(src + (int64_t)(rt + i) * p.ld_x + 8 * l);
+        for (int i = 0; i < 8; ++i) {
+            raw[i].zero();
+            if (rt + i < rows && 8 * l + 8 <= cols) raw[i].load(src + (int64_t)(rt + i) * p.ld_x + 8 * l);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i].unpack(x[i]);
+        if (8 * l < cols && 8 * l + 8 > cols) {  // a row's last values where they are no whole eight
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (rt + i < rows && col(e) < cols) x[i][e] = to_f32(src[(int64_t)(rt + i) * p.ld_x + col(e)]);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const T* row = src + (int64_t)(rt + i) * p.ld_x;
-            if (rt + i < rows && 8 * l < cols) ld8_any(row + 8 * l, row + cols, x[i]);
+        for (int h = 0; h < 8; h += 4) {
+            Any8<T> any[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (rt + i >= rows || col(e) >= cols) x[i][e] = 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const T* row = src + (int64_t)(rt + h + i) * p.ld_x;
+                any[i].load(row + 8 * l, row + (rt + h + i < rows ? cols : 0));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                any[i].get(x[h + i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col(e) >= cols) x[h + i][e] = 0.0f;
+            }
         }
     }
 
