@@ -89,6 +89,14 @@ __device__ __forceinline__ void ld_weight(const NormParams& p, int c0, int lane,
         ld_seg<VEC>(static_cast<const float*>(p.w), c0, lane, p.n_col, v);
 }
 
+// Starts the segment at c0 on its way to L2.
+template <typename T>
+__device__ __forceinline__ void prefetch_seg(const T* row, int c0, int lane, int n_col) {
+    constexpr int kLanes = 128 / 8 / (int)sizeof(T);  // lanes whose 8 values make a line
+    const int c = c0 + 8 * lane;
+    if (lane % kLanes == 0 && c < n_col) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
+}
+
 // Sum over the wpr warps of a row (every warp of the block calls it).
 // `part` holds one float per warp; buffers alternate between calls so that
 // one barrier a call is enough.
@@ -150,16 +158,10 @@ __device__ __forceinline__ void st_seg_e4m3(const NormParams& p, int64_t row, in
     }
 }
 
-// WIDE: rows of more than 8 warps, which have the block to themselves; others
-// keep to 48 registers, so that five blocks fit an SM (8192 x 4096 bf16: 45 us,
-// with four 49).
-template <typename TX, typename TR, int V, bool WIDE, bool VEC>
-__global__ void __launch_bounds__(WIDE ? 1024 : 256, WIDE ? 1 : 5) norm_kernel(const NormParams p) {
-    __shared__ float part[kMaxWarps];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * p.rpb + warp / p.wpr;
+// One row.  `part` holds one float per warp.
+template <typename TX, typename TR, int V, bool VEC>
+__device__ __forceinline__ void norm_row(const NormParams& p, int64_t row, bool live, int warp, int lane, float* part) {
     const int wr = warp % p.wpr;
-    const bool live = row < p.n_row;
     const int n = live ? p.n_col : 0;
     const TX* x = static_cast<const TX*>(p.x) + (live ? row : 0) * p.ld_x;
     const TR* r = static_cast<const TR*>(p.res) + (live ? row : 0) * p.ld_res;
@@ -207,6 +209,38 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 256, WIDE ? 1 : 5) norm_kernel(c
             st_seg<VEC>(static_cast<__nv_bfloat16*>(p.out) + row * p.ld_out, c0, lane, p.n_col, w);
         else
             st_seg<VEC>(static_cast<float*>(p.out) + row * p.ld_out, c0, lane, p.n_col, w);
+    }
+}
+
+// 48 registers, so that five blocks fit an SM (8192 x 4096 bf16: 45 us, with
+// four 49).
+template <typename TX, typename TR, int V, bool VEC>
+__global__ void __launch_bounds__(256, 5) norm_kernel(const NormParams p) {
+    __shared__ float part[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * p.rpb + warp / p.wpr;
+    norm_row<TX, TR, V, VEC>(p, row, row < p.n_row, warp, lane, part);
+}
+
+// Rows of more than 8 warps: too few blocks fit an SM for one's loads to
+// cover another's barrier, so blocks stay and send their next row to L2 first.
+template <typename TX, typename TR, bool VEC>
+__global__ void __launch_bounds__(1024, 1) norm_wide_kernel(const NormParams p) {
+    __shared__ float part[2][kMaxWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.n_row; row += gridDim.x) {
+        const int64_t next = row + gridDim.x;
+        if (next < p.n_row) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int c0 = (j * p.wpr + warp) * kSeg;
+                prefetch_seg(static_cast<const TX*>(p.x) + next * p.ld_x, c0, lane, p.n_col);
+                if (p.res) prefetch_seg(static_cast<const TR*>(p.res) + next * p.ld_res, c0, lane, p.n_col);
+            }
+        }
+        norm_row<TX, TR, 2, VEC>(p, row, true, warp, lane, part[turn]);
+        turn ^= 1;
     }
 }
 
@@ -260,7 +294,18 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512, 1) norm_grad_kernel(const
         const bool live = base + rg < p.n_row;
         const int64_t row = live ? base + rg : 0;
         const int n = live ? p.n_col : 0;
-        if (kWide) fetch(base + rg);
+        if (kWide) {
+            fetch(base + rg);
+            if (base + step < p.n_row) {  // the next row goes to L2
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int c0 = (j * p.wpr + wr) * kSeg;
+                    prefetch_seg(dout + (base + step) * p.ld_dout, c0, lane, p.n_col);
+                    prefetch_seg(sum + (base + step) * p.ld_sum, c0, lane, p.n_col);
+                    if (p.dsum) prefetch_seg(dsum + (base + step) * p.ld_dsum, c0, lane, p.n_col);
+                }
+            }
+        }
         const float rstd = rstd_next;
         float d[V][8], s[V][8], o[kWide ? 1 : V][8];
         float along = 0.0f;
@@ -335,9 +380,9 @@ int launch_norm_v(const NormParams& p, int v, dim3 grid, dim3 block, bool grad, 
         return v == 1   ? block_launch(norm_grad_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
                : v == 2 ? block_launch(norm_grad_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p)
                         : block_launch(norm_grad_kernel<TX, TR, 4, VEC>, grid, block, kWideSmem, stream, p);
-    if (block.x > 256) return block_launch(norm_kernel<TX, TR, 2, true, VEC>, grid, block, 0, stream, p);
-    return v == 1 ? block_launch(norm_kernel<TX, TR, 1, false, VEC>, grid, block, 0, stream, p)
-                  : block_launch(norm_kernel<TX, TR, 2, false, VEC>, grid, block, 0, stream, p);
+    if (block.x > 256) return block_launch(norm_wide_kernel<TX, TR, VEC>, grid, block, 0, stream, p);
+    return v == 1 ? block_launch(norm_kernel<TX, TR, 1, VEC>, grid, block, 0, stream, p)
+                  : block_launch(norm_kernel<TX, TR, 2, VEC>, grid, block, 0, stream, p);
 }
 
 int launch_norm_any(const helix_rms_norm_desc& d, const NormParams& p, int v, dim3 grid, dim3 block, bool vec,
@@ -403,9 +448,12 @@ NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d, 
     return pl;
 }
 
-int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream) {
+int launch_norm(const helix_ctx* ctx, const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream) {
     const NormShape s = norm_shape(d);
-    const dim3 grid((unsigned)((d.n_row + s.rpb - 1) / s.rpb)), block(32 * s.wpr * s.rpb);
+    const dim3 block(32 * s.wpr * s.rpb);
+    int64_t blocks = (d.n_row + s.rpb - 1) / s.rpb;
+    if (block.x > 256) blocks = std::min<int64_t>(blocks, (int64_t)ctx->n_sm * (block.x > 512 ? 1 : 2));
+    const dim3 grid((unsigned)blocks);
     return launch_norm_any(d, p, s.v, grid, block, vec, false, stream);
 }
 

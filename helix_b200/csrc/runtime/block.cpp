@@ -212,7 +212,7 @@ extern "C" helix_status helix_rms_norm_encode(helix_ctx* ctx, void* stream, cons
         p.scale = ptr<float>(scale), p.rstd = ptr<float>(rstd);
         const bool vec = whole(m[0], 16) && whole(m[1], 16) && whole(m[2], 16) && whole(m[3], q ? 8 : 16) &&
                          whole(m[4], 16);
-        return hx::launch_norm(*d, p, vec, stream);
+        return hx::launch_norm(ctx, *d, p, vec, stream);
     });
 }
 

@@ -105,7 +105,7 @@ int launch_gated_grad(const helix_ctx* ctx, const helix_gated_scan_desc& d, Gate
 // Kernel launchers (kernels/block_*.cu): cudaSuccess or the launch error.
 // `vec`: every tensor (the quantiser: x) allows whole 16-byte accesses at
 // 8-column boundaries.
-int launch_norm(const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream);
+int launch_norm(const helix_ctx* ctx, const helix_rms_norm_desc& d, const NormParams& p, bool vec, void* stream);
 int launch_norm_grad(const helix_rms_norm_desc& d, const NormGradPlan& pl, const NormParams& p, bool vec,
                      float* dweight, void* stream);
 int launch_quant(const helix_quant8_desc& d, const QuantParams& p, bool vec, void* stream);
