@@ -309,10 +309,13 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
 // writes.  An epilogue warp has 32 rows and half of the columns; it stages its
 // part in shared memory of its own and stores it by TMA.
 // ---------------------------------------------------------------------------
-// Warps 0 and 1 issue, 2 and 3 gather column scales, 4-11 are the epilogue: 32
-// rows and half of the columns each.  The first warpgroup hands registers to
-// the others, whose accumulators take up to 128 each: 128 x 40 + 256 x 232 =
-// 384 x 168, the registers that the block is launched with.
+// Warp 0 issues the loads, 1 and 2 the MMAs of every other block of k (a
+// block's waits, four MMAs and commits take one thread 750 cycles, three times
+// what the MMAs themselves take at BN = 128), 3 stages scales, 4-11 are
+// the epilogue: 32 rows and half of the columns each.  The first warpgroup hands registers to
+// the others, whose accumulators take up to 128 each: 128 x 40 + 256 x 232 (or
+// 72 and 216, when warp 3 has work) = 384 x 168, the registers that the block
+// is launched with.
 constexpr int kPairThreads = 32 * (4 + kEpiWarps);
 
 template <int BN>
@@ -321,7 +324,7 @@ struct PairCfg {
     static constexpr int kStages = BN == 256 ? 5 : 6;
     static constexpr int kBufs = 512 / BN;
     static constexpr int kRun = BN / 2;                          // columns of an epilogue warp
-    static constexpr int kScales = 4;                            // blocks of column scales staged
+    static constexpr int kPiece = 8;                             // blocks of k whose scales are staged at once
     static constexpr int kOutBytes = 32 * 128;                   // staging of an epilogue warp
     static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpiWarps * kOutBytes + 1024;
 };
@@ -346,10 +349,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     using Cfg = PairCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = tc::align1024(smem_raw);
-    __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain;
-    __shared__ uint64_t sc_full[Cfg::kScales], sc_empty[Cfg::kScales];
+    __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain[2];
+    __shared__ uint64_t sc_full[2], sc_empty[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ __align__(16) float col_scale[Cfg::kScales][QROWS ? BN : 4];
+    __shared__ __align__(16) float row_scale[2][QROWS ? Cfg::kPiece : 1][QROWS ? kRows : 4];
+    __shared__ __align__(16) float col_scale[2][QROWS ? Cfg::kPiece : 1][QROWS ? BN : 4];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x & 1u), pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
@@ -364,8 +368,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
         for (int i = 0; i < Cfg::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], 2 * kEpiWarps);
 #pragma unroll
-        for (int i = 0; i < Cfg::kScales; ++i) mbar_init(&sc_full[i], 1), mbar_init(&sc_empty[i], kEpiWarps);
-        mbar_init(&drain, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&sc_full[i], 1), mbar_init(&sc_empty[i], kEpiWarps);
+        mbar_init(&drain[0], 1), mbar_init(&drain[1], 1);
         fence_mbar_init();
     }
     if (warp == 1) tmem_alloc_pair(&tmem_slot, 512);
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(QROWS ? 72 : 40));
         if (warp == 0 && lane == 0) {
             Ring<Cfg::kStages> st;  // runs over the blocks of k of all tiles
             int issued = 0;
@@ -407,18 +411,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             if (rank == 0)
                 for (int j = issued > Cfg::kStages ? issued - Cfg::kStages : 0; j < issued; ++j)
                     mbar_wait(&full[j % Cfg::kStages], (uint32_t)((j / Cfg::kStages) & 1), tc::kWaitBudget);
-        } else if (warp == 1 && lane == 0 && rank == 0) {
+        } else if (warp < 3 && lane == 0 && rank == 0) {
             constexpr uint32_t idesc = idesc_e4m3(2 * kRows, BN);
             const uint32_t base = smem_u32(smem);
             const int mine = pair < n_tiles ? (n_tiles - pair + pairs - 1) / pairs : 0;
-            const int total = mine * nkb;
+            const int total = mine * nkb, first = warp - 1;
             Ring<Cfg::kStages> st;
             Ring<Cfg::kBufs> buf;
+            if (first) st.next(), buf.next();
             // A wait costs its latency even when nothing is left to wait for;
             // the next block's two are polled between its issue and its commits.
-            bool ready = total > 0 && mbar_try_wait(&full[0], 0), free = true;
-            int it = 0;
-            for (; it < total; ++it) {
+            bool ready = false, free = first < Cfg::kBufs;
+            int it = first;
+            for (; it < total; it += 2) {
                 if (!free && !wait(&acc_empty[buf.at], buf.parity ^ 1u)) break;
                 if (!ready && !wait(&full[st.at], st.parity)) break;
                 tc_fence_after();
@@ -428,82 +433,90 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 for (int ks = 0; ks < 4; ++ks)
                     mma_e4m3_pair(tmem + buf.at * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
                 uint64_t *done = &acc_full[buf.at], *read = &empty[st.at];
-                st.next();
-                buf.next();
-                ready = it + 1 < total && mbar_try_wait(&full[st.at], st.parity);
-                free = it + 1 < Cfg::kBufs || mbar_try_wait(&acc_empty[buf.at], buf.parity ^ 1u);
+                st.next(), st.next();
+                buf.next(), buf.next();
+                ready = it + 2 < total && mbar_try_wait(&full[st.at], st.parity);
+                free = it + 2 < Cfg::kBufs || mbar_try_wait(&acc_empty[buf.at], buf.parity ^ 1u);
                 mma_commit_pair(done);
                 mma_commit_pair(read);
             }
             if (it < total) {
-                mma_commit_pair(&drain);
-                mbar_wait(&drain, 0, tc::kWaitBudget);
+                mma_commit_pair(&drain[first]);
+                mbar_wait(&drain[first], 0, tc::kWaitBudget);
             }
-        } else if (QROWS && warp >= 2) {
-            // column scales: warp 2 the even blocks, warp 3 the odd ones, the
-            // next one's loads in flight
-            constexpr int kPer = BN / 32;
-            float next[kPer];
-            auto fetch = [&](int it) {
-                const int tile = pair + it / nkb * pairs;
-                if (tile >= n_tiles) return;
-                int tp, tq;
-                pair_tile(tile, tiles_p, a.tiles_q, &tp, &tq);
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    const int qr = min(tq * BN + 32 * j + lane, a.q.rows - 1);
-                    next[j] = __ldg(a.q.scale + (int64_t)qr * a.q.ld_scale + it % nkb);
-                }
-            };
+        } else if (QROWS && warp == 3) {
+            // Scales: a row's of kPiece blocks lie side by side, and are read
+            // together while their sectors are in L1 (one block at a time for
+            // all rows, each would come from L2 again: L1 has what the stages
+            // leave of it).
             const int mine = pair < n_tiles ? (n_tiles - pair + pairs - 1) / pairs : 0;
-            const int total = mine * nkb;
-            if (warp - 2 < total) fetch(warp - 2);
-            for (int it = warp - 2; it < total; it += 2) {
-                const int slot = it % Cfg::kScales;
-                float cur[kPer];
+            Ring<2> sc;
+            int done = 0;
+            bool ok = true;
+            for (int i = 0; ok && i < mine; ++i) {
+                int tp, tq;
+                pair_tile(pair + i * pairs, tiles_p, a.tiles_q, &tp, &tq);
+                for (int kb = 0; kb < nkb; kb += Cfg::kPiece, ++done) {
+                    if (done >= 2 && !(ok = __all_sync(0xffffffffu, wait(&sc_empty[sc.at], sc.parity ^ 1u)))) break;
+                    auto stage = [&](const Mm8Operand& o, int row, float* to, int pitch) {
+                        const float* from = o.scale + (int64_t)(min(row, o.rows - 1) / o.per) * o.ld_scale;
+                        float v[Cfg::kPiece];
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) cur[j] = next[j];
-                if (it + 2 < total) fetch(it + 2);
-                if (it >= Cfg::kScales && !__all_sync(0xffffffffu, wait(&sc_empty[slot], (uint32_t)(it / Cfg::kScales - 1) & 1u))) break;
+                        for (int g = 0; g < Cfg::kPiece; ++g) v[g] = __ldg(from + min(kb + g, nkb - 1));
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) col_scale[slot][32 * j + lane] = cur[j];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sc_full[slot]);
+                        for (int g = 0; g < Cfg::kPiece; ++g) to[g * pitch] = v[g];
+                    };
+#pragma unroll 2
+                    for (int j = lane; j < kRows; j += 32)
+                        stage(a.p, (2 * tp + rank) * kRows + j, &row_scale[sc.at][0][j], kRows);
+#pragma unroll 2
+                    for (int j = lane; j < BN; j += 32) stage(a.q, tq * BN + j, &col_scale[sc.at][0][j], BN);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_full[sc.at]);
+                    sc.next();
+                }
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(QROWS ? 216 : 232));
         const int row = 32 * (warp & 3) + lane;      // the TMEM lane
         const int c0 = (warp - 4) / 4 * Cfg::kRun;   // the warp's first column
         const uint32_t staging = smem_u32(smem) + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
         const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)c0;
         bool alive = true;  // once a wait has run out no other is waited for, and the rest is garbage
         Ring<Cfg::kBufs> buf;
-        Ring<Cfg::kScales> sc;
+        Ring<2> sc;
         for (int tile = pair; tile < n_tiles; tile += pairs) {
             int tp, tq;
             pair_tile(tile, tiles_p, a.tiles_q, &tp, &tq);
             const int p0 = (2 * tp + rank) * kRows, q0 = tq * BN;
-            // the scales of the row, and of the columns where they share one,
-            // two blocks ahead
+            // the scales of the row and of the columns that share one, two
+            // blocks ahead (otherwise staged)
             const float* ps = a.p.scale + (int64_t)(min(p0 + row, a.p.rows - 1) / a.p.per) * a.p.ld_scale;
             const float* qs = a.q.scale + (int64_t)(min(q0 + c0, a.q.rows - 1) / a.q.per) * a.q.ld_scale;
-            float ps_next = __ldg(ps), ps_then = __ldg(ps + min(1, nkb - 1));
-            float qs_next = QROWS ? 1.0f : __ldg(qs), qs_then = QROWS ? 1.0f : __ldg(qs + min(1, nkb - 1));
+            float ps_next = 0.0f, ps_then = 0.0f, qs_next = 0.0f, qs_then = 0.0f;
+            if constexpr (!QROWS) {
+                ps_next = __ldg(ps), ps_then = __ldg(ps + min(1, nkb - 1));
+                qs_next = __ldg(qs), qs_then = __ldg(qs + min(1, nkb - 1));
+            }
             uint64_t acc[Cfg::kRun / 2];
 #pragma unroll
             for (int i = 0; i < Cfg::kRun / 2; ++i) acc[i] = 0;
             for (int kb = 0; kb < nkb; ++kb) {
-                const float r = QROWS ? ps_next : ps_next * qs_next;
-                const uint64_t r2 = f2_of(r, r);
-                ps_next = ps_then;
-                ps_then = __ldg(ps + min(kb + 2, nkb - 1));
-                if constexpr (!QROWS) {
+                const int at = kb % Cfg::kPiece;
+                float r;
+                if constexpr (QROWS) {
+                    if (at == 0 && alive) alive = __all_sync(0xffffffffu, wait(&sc_full[sc.at], sc.parity));
+                    r = row_scale[sc.at][at][row];
+                } else {
+                    r = ps_next * qs_next;
+                    ps_next = ps_then;
+                    ps_then = __ldg(ps + min(kb + 2, nkb - 1));
                     qs_next = qs_then;
                     qs_then = __ldg(qs + min(kb + 2, nkb - 1));
                 }
+                const uint64_t r2 = f2_of(r, r);
                 if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[buf.at], buf.parity));
-                if (QROWS && alive) alive = __all_sync(0xffffffffu, wait(&sc_full[sc.at], sc.parity));
                 tc_fence_after();
                 // 32 columns are read while the 32 before are added up
                 const uint32_t from = lane_addr + buf.at * BN;
@@ -525,19 +538,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         const uint64_t d = f2_of(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
                         uint64_t& o = acc[c / 2 + e];
                         if constexpr (QROWS) {
-                            const float2 cs = *reinterpret_cast<const float2*>(&col_scale[sc.at][c0 + c + 2 * e]);
+                            const float2 cs = *reinterpret_cast<const float2*>(&col_scale[sc.at][at][c0 + c + 2 * e]);
                             o = f2_fma(d, f2_mul(r2, f2_of(cs.x, cs.y)), o);
                         } else {
                             o = f2_fma(d, r2, o);
                         }
                     }
                 }
-                if constexpr (QROWS) {
+                if (QROWS && (at == Cfg::kPiece - 1 || kb == nkb - 1)) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_empty[sc.at]);
+                    sc.next();
                 }
                 buf.next();
-                sc.next();
             }
             // the warp's 32 rows: 128 bytes of each row at a time
             // through its staging, or straight to memory
@@ -735,8 +748,8 @@ Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
         const int64_t waves = (n + ctx->n_sm / 2 - 1) / (ctx->n_sm / 2);
         return (double)waves * (block * kb + tile);  // us
     };
-    const double wide = rows ? estimate(256, 1.02, 4.0) : estimate(256, 0.58, 3.0);
-    const double narrow = rows ? estimate(128, 0.57, 3.0) : estimate(128, 0.40, 2.5);
+    const double wide = rows ? estimate(256, 0.91, 4.0) : estimate(256, 0.57, 2.5);
+    const double narrow = rows ? estimate(128, 0.55, 3.0) : estimate(128, 0.335, 3.5);
     pl.pair = true;
     pl.bn = wide <= narrow ? 256 : 128;
     return pl;
