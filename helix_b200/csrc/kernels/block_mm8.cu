@@ -9,15 +9,19 @@
 // (sa sb) D_b to fp32 registers while the next blocks' MMAs run.
 //
 // A CTA has a tile of 128 rows of P x BN rows of Q: warp 0 issues the TMA
-// loads (128-byte rows, one block of k per stage), warp 1 the MMAs, warps
-// 2-9 are the epilogue, each with a quarter of the rows (the TMEM lanes it
-// can reach) and half of the columns.  P is a and Q is b, or the other way
-// round where a has few rows: the MMA is always 128 rows tall, so the weight
-// takes those and the tokens become a narrow N.
+// loads (128-byte rows, one block of k per stage), warps 1 and 2 the MMAs of
+// the even and the odd blocks, warps 3-10 are the epilogue, four of them (one
+// for each quarter of the rows, the TMEM lanes that a warp can reach) for the
+// even blocks and four for the odd ones.  A block's hand-offs take a thread
+// longer than its MMAs take the tensor core, so each has two blocks' time.  P
+// is a and Q is b, or the other way round where a has few rows: the MMA is
+// always 128 rows tall, so the weight takes those and the tokens become a
+// narrow N.
 //
-// With few tiles the blocks of k are shared by a cluster of CTAs; their
-// partial sums meet in distributed shared memory and every CTA adds up and
-// writes a share of the columns, in the order of the ranks.
+// With few tiles the blocks of k are shared by a cluster of CTAs.  The partial
+// sums (of even and odd blocks, of all CTAs) meet in (distributed) shared
+// memory, and every CTA adds up and writes a share of the columns, in the
+// order of the ranks.
 //
 // Every wait is bounded: one that runs out records kFaultProduct, the CTA
 // lets its copies and MMAs land, frees its TMEM and returns.
@@ -39,19 +43,19 @@ using namespace umma;
 constexpr int kRows = 128;                 // of P in a tile
 constexpr int kBk = HELIX_GROUP;           // bytes of k in a stage: one scale block
 constexpr int kEpiWarps = 8;
-constexpr int kMmThreads = 32 * (2 + kEpiWarps);
+constexpr int kMmThreads = 32 * (3 + kEpiWarps);
 
 template <int BN>
 struct Mm8Cfg {
     static constexpr int kStageBytes = (kRows + BN) * kBk;
-    static constexpr int kStages = BN == 64 ? 4 : BN == 32 ? 5 : 6;
-    static constexpr int kPerSm = BN == 128 ? 1 : 2;         // CTAs that fit
-    static constexpr int kBufs = BN >= 128 ? 2 : 4;          // TMEM accumulators
-    static constexpr int kCols = kBufs * BN < 32 ? 32 : kBufs * BN;
-    static constexpr int kRun = BN / 2;                      // columns of an epilogue thread
-    static constexpr int kLoad = kRun < 32 ? kRun : 32;      // of them, read at once
+    static constexpr int kStages = BN == 64 ? 8 : BN == 32 ? 5 : 6;
+    static constexpr int kPerSm = BN == 64 ? 1 : 2;          // CTAs that fit
+    static constexpr int kBufs = 4;                          // TMEM accumulators
+    static constexpr int kCols = kBufs * BN;
+    static constexpr int kLoad = BN < 32 ? BN : 32;          // columns read at once
     static constexpr int kPiece = 16;                        // blocks of k whose column scales are staged at once
     static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
+    static_assert(2 * BN * kRows * sizeof(float) <= (size_t)kStages * kStageBytes, "partial sums");
 };
 
 struct Mm8Maps {
@@ -91,11 +95,11 @@ __device__ __forceinline__ void st_out(const Mm8Params& a, int pr, int qc, int n
 
 template <int BN, bool QROWS, typename T>
 __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(const __grid_constant__ Mm8Maps maps,
-                                                            const __grid_constant__ Mm8Params a) {
+                                                                             const __grid_constant__ Mm8Params a) {
     using Cfg = Mm8Cfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = tc::align1024(smem_raw);
-    __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain;
+    __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain[2];
     __shared__ uint32_t tmem_slot;
     __shared__ __align__(16) float col_scale[QROWS ? Cfg::kPiece : 1][QROWS ? BN : 4];
 
@@ -115,8 +119,8 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
 #pragma unroll
         for (int i = 0; i < Cfg::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
 #pragma unroll
-        for (int i = 0; i < Cfg::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps);
-        mbar_init(&drain, 1);
+        for (int i = 0; i < Cfg::kBufs; ++i) mbar_init(&acc_full[i], 1), mbar_init(&acc_empty[i], kEpiWarps / 2);
+        mbar_init(&drain[0], 1), mbar_init(&drain[1], 1);
         fence_mbar_init();
         // the first loads wait for nobody
         for (int i = 0; i < Cfg::kStages && i < nkb; ++i) load(i, i);
@@ -134,9 +138,11 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
         return false;
     };
 
-    float acc[Cfg::kRun];
+    const int group = (warp - 3) / 4;                 // of an epilogue warp: 0 even blocks, 1 odd
+    const int row = 32 * (warp & 3) + lane;           // its TMEM lane
+    float acc[BN];
 #pragma unroll
-    for (int i = 0; i < Cfg::kRun; ++i) acc[i] = 0.0f;
+    for (int i = 0; i < BN; ++i) acc[i] = 0.0f;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -151,17 +157,19 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
             for (int j = i > Cfg::kStages ? i - Cfg::kStages : 0; j < i; ++j)
                 mbar_wait(&full[j % Cfg::kStages], (uint32_t)((j / Cfg::kStages) & 1), tc::kWaitBudget);
         }
-    } else if (warp == 1) {
+    } else if (warp < 3) {
         if (lane == 0) {
             constexpr uint32_t idesc = idesc_e4m3(kRows, BN);
             const uint32_t base = smem_u32(smem);
+            const int first = warp - 1;
             Ring<Cfg::kStages> st;
             Ring<Cfg::kBufs> buf;
+            if (first) st.next(), buf.next();
             // A wait costs its latency even when nothing is left to wait for;
             // the next block's two are polled between its issue and its commits.
             bool ready = false, free = true;
-            int i = 0;
-            for (; i < nkb; ++i) {
+            int i = first;
+            for (; i < nkb; i += 2) {
                 if (!free && !wait(&acc_empty[buf.at], buf.parity ^ 1u)) break;
                 if (!ready && !wait(&full[st.at], st.parity)) break;
                 tc_fence_after();
@@ -171,45 +179,47 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
                 for (int ks = 0; ks < 4; ++ks)
                     mma_e4m3(tmem + buf.at * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
                 uint64_t *done = &acc_full[buf.at], *read = &empty[st.at];
-                st.next();
-                buf.next();
-                ready = i + 1 < nkb && mbar_try_wait(&full[st.at], st.parity);
-                free = i + 1 < Cfg::kBufs || mbar_try_wait(&acc_empty[buf.at], buf.parity ^ 1u);
+                st.next(), st.next();
+                buf.next(), buf.next();
+                ready = i + 2 < nkb && mbar_try_wait(&full[st.at], st.parity);
+                free = i + 2 < Cfg::kBufs || mbar_try_wait(&acc_empty[buf.at], buf.parity ^ 1u);
                 mma_commit(done);
                 mma_commit(read);
             }
             if (i < nkb) {
-                mma_commit(&drain);
-                mbar_wait(&drain, 0, tc::kWaitBudget);
+                mma_commit(&drain[first]);
+                mbar_wait(&drain[first], 0, tc::kWaitBudget);
             }
         }
     } else {
-        const int row = 32 * (warp & 3) + lane;       // the TMEM lane
-        const int c0 = (warp - 2) / 4 * Cfg::kRun;    // the thread's first column
-        const int tid = threadIdx.x - 64;             // 0 .. 255
-        const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)c0;
-        // the row's scale two blocks ahead; the columns', where they share
-        // one, too
+        const int tid = threadIdx.x - 96;             // 0 .. 255
+        const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        // the row's scale one of the group's blocks ahead; the columns', where
+        // they share one, too
         const float* ps = a.p.scale + (int64_t)(min(p0 + row, a.p.rows - 1) / a.p.per) * a.p.ld_scale + kb0;
         const float* qs = a.q.scale + (int64_t)(min(q0, a.q.rows - 1) / a.q.per) * a.q.ld_scale + kb0;
-        float ps_next = __ldg(ps), ps_then = __ldg(ps + min(1, nkb - 1));
-        float qs_next = QROWS ? 1.0f : __ldg(qs), qs_then = QROWS ? 1.0f : __ldg(qs + min(1, nkb - 1));
+        float ps_next = __ldg(ps + min(group, nkb - 1)), ps_then = __ldg(ps + min(group + 2, nkb - 1));
+        float qs_next = 1.0f, qs_then = 1.0f;
+        if (!QROWS) qs_next = __ldg(qs + min(group, nkb - 1)), qs_then = __ldg(qs + min(group + 2, nkb - 1));
         // column scales of kPiece blocks: value j of the piece at i is block
         // i + j % kPiece of column j / kPiece
         constexpr int kMine = (BN * Cfg::kPiece + 32 * kEpiWarps - 1) / (32 * kEpiWarps);
-        float piece[kMine];
+        float piece[QROWS ? kMine : 1];
         auto fetch = [&](int i) {
+            if constexpr (QROWS) {
 #pragma unroll
-            for (int j = 0; j < kMine; ++j) {
-                const int e = tid + 32 * kEpiWarps * j, q = min(q0 + e / Cfg::kPiece, a.q.rows - 1);
-                piece[j] = __ldg(a.q.scale + (int64_t)q * a.q.ld_scale + kb0 + min(i + e % Cfg::kPiece, nkb - 1));
+                for (int j = 0; j < kMine; ++j) {
+                    const int e = tid + 32 * kEpiWarps * j, q = min(q0 + e / Cfg::kPiece, a.q.rows - 1);
+                    piece[j] = __ldg(a.q.scale + (int64_t)q * a.q.ld_scale + kb0 + min(i + e % Cfg::kPiece, nkb - 1));
+                }
             }
         };
-        if (QROWS) fetch(0);
+        fetch(0);
         Ring<Cfg::kBufs> buf;
+        if (group) buf.next();
         bool alive = true;  // once a wait has run out no other is waited for, and the rest is garbage
-        for (int i = 0; i < nkb; ++i) {
-            if (QROWS && i % Cfg::kPiece == 0) {
+        for (int i0 = 0; i0 < nkb; i0 += Cfg::kPiece) {
+            if constexpr (QROWS) {
                 named_sync(1, 32 * kEpiWarps);  // the last piece is read
 #pragma unroll
                 for (int j = 0; j < kMine; ++j) {
@@ -217,77 +227,69 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
                     if (e < BN * Cfg::kPiece) col_scale[e % Cfg::kPiece][e / Cfg::kPiece] = piece[j];
                 }
                 named_sync(1, 32 * kEpiWarps);
-                if (i + Cfg::kPiece < nkb) fetch(i + Cfg::kPiece);
+                if (i0 + Cfg::kPiece < nkb) fetch(i0 + Cfg::kPiece);
             }
-            const float r = QROWS ? ps_next : ps_next * qs_next;
-            ps_next = ps_then;
-            ps_then = __ldg(ps + min(i + 2, nkb - 1));
-            if constexpr (!QROWS) {
-                qs_next = qs_then;
-                qs_then = __ldg(qs + min(i + 2, nkb - 1));
-            }
-            if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[buf.at], buf.parity));
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < Cfg::kRun; c += Cfg::kLoad) {
-                uint32_t v[Cfg::kLoad];
-                tmem_ld(lane_addr + buf.at * BN + c, v);
-                tmem_wait_ld(v);
-                if (c + Cfg::kLoad == Cfg::kRun) {  // all read
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[buf.at]);
+            for (int i = i0 + group; i < nkb && i < i0 + Cfg::kPiece; i += 2) {
+                const float r = QROWS ? ps_next : ps_next * qs_next;
+                ps_next = ps_then;
+                ps_then = __ldg(ps + min(i + 4, nkb - 1));
+                if constexpr (!QROWS) {
+                    qs_next = qs_then;
+                    qs_then = __ldg(qs + min(i + 4, nkb - 1));
                 }
+                if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[buf.at], buf.parity));
+                tc_fence_after();
 #pragma unroll
-                for (int e = 0; e < Cfg::kLoad; ++e) {
-                    const float s = QROWS ? r * col_scale[i % Cfg::kPiece][c0 + c + e] : r;
-                    acc[c + e] = fmaf(__uint_as_float(v[e]), s, acc[c + e]);
+                for (int c = 0; c < BN; c += Cfg::kLoad) {
+                    uint32_t v[Cfg::kLoad];
+                    tmem_ld(lane_addr + buf.at * BN + c, v);
+                    tmem_wait_ld(v);
+                    if (c + Cfg::kLoad == BN) {  // all read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acc_empty[buf.at]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < Cfg::kLoad; ++e) {
+                        const float s = QROWS ? r * col_scale[i % Cfg::kPiece][c + e] : r;
+                        acc[c + e] = fmaf(__uint_as_float(v[e]), s, acc[c + e]);
+                    }
                 }
-            }
-            buf.next();
-        }
-        if (a.splits == 1) {
-#pragma unroll
-            for (int c = 0; c < Cfg::kRun; c += 8) {
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = acc[c + e];
-                st_out<T>(a, p0 + row, q0 + c0 + c, 8, v);
+                buf.next(), buf.next();
             }
         }
     }
 
-    if (a.splits > 1) {
-        cg::cluster_group cluster = cg::this_cluster();
-        // every MMA of this CTA has retired, so the stages are free
-        __syncthreads();
-        float* part = reinterpret_cast<float*>(smem);  // [BN][128]
-        if (warp >= 2) {
-            const int row = 32 * (warp & 3) + lane, c0 = (warp - 2) / 4 * Cfg::kRun;
+    // every load and MMA of this CTA has retired, so the stages are free
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(smem);  // [2][BN][128]
+    if (warp >= 3) {
 #pragma unroll
-            for (int c = 0; c < Cfg::kRun; ++c) part[(c0 + c) * kRows + row] = acc[c];
-        }
-        cluster.sync();
-        if (warp >= 2) {
-            const int row = 32 * (warp & 3) + lane;
-            const int run = Cfg::kRun / a.splits;  // columns of this thread's share
-            const int c0 = rank * (BN / a.splits) + (warp - 2) / 4 * run;
-            for (int c = 0; c < run; c += 8) {
-                const int n = min(8, run - c);
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-                for (int k = 0; k < a.splits; ++k) {
-                    const float* other = cluster.map_shared_rank(part, k);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < n) v[e] += other[(c0 + c + e) * kRows + row];
-                }
-                st_out<T>(a, p0 + row, q0 + c0 + c, n, v);
-            }
-        }
-        cluster.sync();  // a peer may still be reading this CTA's share
+        for (int c = 0; c < BN; ++c) part[(group * BN + c) * kRows + row] = acc[c];
     }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (a.splits > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+    if (warp >= 3) {
+        const int run = BN / 2 / a.splits;  // columns of this thread's share
+        const int c0 = rank * (BN / a.splits) + group * run;
+        for (int c = 0; c < run; c += 8) {
+            const int n = min(8, run - c);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            for (int k = 0; k < a.splits; ++k) {
+                const float* from = a.splits > 1 ? cluster.map_shared_rank(part, k) : part;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < n) v[e] += from[(c0 + c + e) * kRows + row] + from[(BN + c0 + c + e) * kRows + row];
+            }
+            st_out<T>(a, p0 + row, q0 + c0 + c, n, v);
+        }
+    }
+    if (a.splits > 1) cluster.sync();  // a peer may still be reading this CTA's share
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -720,7 +722,6 @@ int configure_mm8() {
     if ((e = configure_mm8_n<16>()) != cudaSuccess) return e;
     if ((e = configure_mm8_n<32>()) != cudaSuccess) return e;
     if ((e = configure_mm8_n<64>()) != cudaSuccess) return e;
-    if ((e = configure_mm8_n<128>()) != cudaSuccess) return e;
     if ((e = configure_pair_n<128>()) != cudaSuccess) return e;
     return configure_pair_n<256>();
 }
@@ -735,13 +736,13 @@ int configure_mm8() {
 Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
     Mm8Plan pl{};
     pl.swap = d.m <= 64;
-    pl.bn = !pl.swap ? 128 : d.m <= 16 ? 16 : d.m <= 32 ? 32 : 64;
+    pl.bn = !pl.swap ? 64 : d.m <= 16 ? 16 : d.m <= 32 ? 32 : 64;
     const int64_t tiles = (int64_t)tiles_of(pl.swap ? d.n : d.m, kRows) * tiles_of(pl.swap ? d.m : d.n, pl.bn);
     const int kb = tiles_of(d.k, kBk);
     pl.splits = 1;
     while (pl.splits < 8 && tiles * pl.splits * 2 <= ctx->n_sm && kb >= (pl.splits == 4 ? 64 : 4 * pl.splits))
         pl.splits *= 2;
-    if (pl.swap || tiles * 2 <= ctx->n_sm) return pl;
+    if (pl.swap || tiles <= ctx->n_sm) return pl;
     const bool rows = d.b_form == HELIX_SCALE_ROWS;
     auto estimate = [&](int bn, double block, double tile) {
         const int64_t n = (int64_t)tiles_of(d.m, 2 * kRows) * tiles_of(d.n, bn);
@@ -786,8 +787,7 @@ int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan&
     switch (pl.bn) {
         case 16: return launch_mm8_n<16>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
         case 32: return launch_mm8_n<32>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
-        case 64: return launch_mm8_n<64>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
-        default: return launch_mm8_n<128>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
+        default: return launch_mm8_n<64>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
     }
 }
 
