@@ -480,7 +480,8 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
         const int base = chunk_of(s) * Cut<LW>::kTokens, t0 = base + at.run * kTok, b = s & 1;
         const uint32_t my = walk.mine(s);
         const bool whole = at.whole(p, base);
-        V z[kTok], D = L::splat(0.0f), B = D;
+        // -D and B of the run up to each token: h_t = h - D h + B
+        V nd[kTok], hb[kTok], D = L::splat(0.0f), B = D;
         walk.wait_tiles(s);
         auto first = [&](auto all) {
 #pragma unroll
@@ -490,12 +491,11 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
                     gw = lds(my + Cut<LW>::word(0, i)), vw = lds(my + Cut<LW>::word(1, i));
                 } else {
                     gw = ahead.get(0, i, lane), vw = ahead.get(1, i, lane);
-                    sts(my + Cut<LW>::word(1, i), vw);
                 }
                 if (!decltype(all)::value && t0 + i >= at.len) gw = L::kInf, vw = 0u;
-                z[i] = gate<T>(L::unpack(gw));
-                D = grow<L>(D, z[i]);
-                B = step<L>(B, z[i], L::unpack(vw));
+                const V z = gate<T>(L::unpack(gw));
+                nd[i] = D = grow<L>(D, z);
+                hb[i] = B = step<L>(B, z, L::unpack(vw));
             }
         };
         if (whole)
@@ -542,9 +542,8 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
 #pragma unroll
             for (int i = 0; i < kTok; ++i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
-                hw = step<L>(hw, z[i], past ? L::splat(0.0f) : L::unpack(lds(my + Cut<LW>::word(1, i))));
                 if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok))
-                    st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(hw));
+                    st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(fold<L>(hw, nd[i], hb[i])));
                 y += p.s_y;
             }
         };
