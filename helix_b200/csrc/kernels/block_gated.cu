@@ -19,9 +19,9 @@
 // on an mbarrier, every CTA folds them onto the running state, and a second
 // walk writes the outputs.  Then the cluster moves on by its chunks.  Tiles
 // arrive by TMA, steps ahead; two CTAs per SM fill each other's waits.  Tensors
-// that TMA cannot describe take the same kernel with plain loads, a lane's
-// words one step ahead.  Folds go in the order of the tokens: results do not
-// depend on timing.
+// that TMA cannot describe arrive row by row, by copies of the 16-byte pieces
+// that hold a row, and a lane reads its channels at the row's offset in them.
+// Folds go in the order of the tokens: results do not depend on timing.
 //
 // The gradient walks the chunks from the end with c_t = f_t lam_t, the
 // gradient that leaves token t for h_{t-1}: lam_t = dy_t + c_{t+1}, c_t =
@@ -48,10 +48,12 @@ constexpr int kWarps = kChunk / kTok;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
 constexpr int kTileBytes = kChunk * 128;  // 128 tokens x 128 bytes of channels
+constexpr int kSlot = 144;                // a copied row: 128 bytes at an offset of up to 15
+constexpr int kRowTile = kChunk * kSlot;  // copied rows of a tensor
 constexpr int kFewWarps = 8;              // of a CTA of the few-token kernels
 
 // How a kernel reaches the token tensors.
-enum Access { kTma, kWord, kHalf };       // tiles; a lane's 4 bytes; its 2-byte halves
+enum Access { kTma, kWord, kHalf };       // tiles; rows at multiples of 4 bytes, or of 2
 
 // A lane's channels: one f32, or two bf16 as a packed fp32 pair.
 template <typename T>
@@ -199,6 +201,11 @@ __device__ __forceinline__ int length_of(const GatedParams& p, int seq) {
 }
 
 __device__ __forceinline__ uint32_t align128(const uint8_t* p) { return (smem_u32(p) + 127u) & ~127u; }
+__device__ __forceinline__ uint32_t lds_half(uint32_t a) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+    return v;
+}
 // Shared memory by its 32-bit address: 64-bit generic addresses cost two more
 // instructions an access.
 __device__ __forceinline__ uint32_t lds(uint32_t a) {
@@ -206,7 +213,6 @@ __device__ __forceinline__ uint32_t lds(uint32_t a) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
     return v;
 }
-__device__ __forceinline__ void sts(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v)); }
 
 // How a CTA cuts its tile: rows of LW lanes' channels (32, or 16 to make twice
 // as many CTAs of few channels), a run of 16 tokens for each LW lanes.
@@ -281,6 +287,12 @@ __device__ __forceinline__ void st_async(uint32_t at, float v, uint32_t bar) {
                  "r"(__float_as_uint(v)), "r"(bar)
                  : "memory");
 }
+// Bytes of global memory, in whole 16s, to shared memory.
+__device__ __forceinline__ void bulk_load(uint32_t to, uintptr_t from, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                 "l"(from), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
 __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -291,6 +303,23 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
     return ok != 0;
+}
+
+template <int N>
+struct Size {
+    __device__ __forceinline__ constexpr operator int() const { return N; }
+};
+// The body with the cluster's size as a constant , so that its loop's shared loads are
+// all issued before the first is looked at.
+template <typename F>
+__device__ __forceinline__ void by_cluster(int size, F body) {
+    static_assert(kMaxCluster == 8, "");
+    if (size == 8)
+        body(Size<8>{});
+    else if (size == 4)
+        body(Size<4>{});
+    else
+        body(Size<2>{});
 }
 
 struct GatedMaps {
@@ -311,34 +340,92 @@ struct Walk {
     M*                 meet;
     int                steps;
     bool               alive = true;
+    static constexpr int kFulls = A == kTma ? 1 : kWarps;  // barriers of a stage: a warp's rows are its own
 
-    // The lane's words of step s.
+    // Tensor k of a token tensor's call: its rows of the sequence at the slab's first channel, and their pitch.
+    const T* rows[A == kTma ? 1 : K];
+    int64_t  pitch[A == kTma ? 1 : K];
+
+    // Tiles.  The lane's words of step s.
     __device__ __forceinline__ uint32_t mine(int s) const {
-        return base + (uint32_t)((s % kStages) * K * kTileBytes + at.run * kTok * Cut<LW>::kRow + at.l * 4);
+        if (A == kTma) return base + (uint32_t)((s % kStages) * K * kTileBytes + at.run * kTok * Cut<LW>::kRow + at.l * 4);
+        return base + (uint32_t)((s % kStages) * K * kRowTile + at.run * kTok * kSlot + at.l * 4);
+    }
+    // Offset in its 16-byte piece of the run's first row of a step's tensor,
+    // and what a row adds to it.
+    struct Shift {
+        uint32_t first, step;
+    };
+    __device__ __forceinline__ Shift shift(int k, int t0) const {
+        if (A == kTma) return {0u, 0u};
+        return {(uint32_t)(reinterpret_cast<uintptr_t>(rows[k] + t0 * pitch[k])) & 15u, (uint32_t)(pitch[k] * (int64_t)sizeof(T)) & 15u};
+    }
+    // The lane's channels of token i of tensor k.
+    __device__ __forceinline__ uint32_t get(uint32_t my, const Shift& sh, int k, int i) const {
+        if (A == kTma) return lds(my + Cut<LW>::word(k, i));
+        const uint32_t a = my + (uint32_t)(k * kRowTile + i * kSlot) + ((sh.first + i * sh.step) & 15u);
+        if (A == kWord) return lds(a);
+        return lds_half(a) | lds_half(a + 2) << 16;
     }
     __device__ __forceinline__ bool issuer() const { return A == kTma && threadIdx.x == kThreads - 1; }
     // One thread: step s's tiles (chunk `chunk`) start to arrive.
     __device__ __forceinline__ void load(int s, int chunk) const {
-        uint64_t* bar = &full[s % kStages];
+        uint64_t* bar = &full[s % kStages * kFulls];
         mbar_expect_tx(bar, K * kTileBytes);
 #pragma unroll
         for (int k = 0; k < K; ++k)
             tma_load_3d(base + (uint32_t)(((s % kStages) * K + k) * kTileBytes), &maps.in[k], bar, at.slab0(),
                         chunk * Cut<LW>::kTokens, at.seq);
     }
+    // Every warp: step s's rows of its run start to arrive.  A copy takes the
+    // 16-byte pieces that hold the row's channels, each of which holds one
+    // that exists.
+    __device__ __forceinline__ void copy_rows(int s, int chunk) const {
+        if constexpr (A != kTma) {
+            const int t0 = chunk * Cut<LW>::kTokens + at.run * kTok;
+            uint64_t* bar = &full[s % kStages * kFulls + at.warp];
+            const uint32_t to = base + (uint32_t)((s % kStages) * K * kRowTile + at.run * kTok * kSlot);
+            const uint32_t width = (uint32_t)min(LW * Lane<T>::kN, p.n_chan - at.slab0()) * (uint32_t)sizeof(T);
+            uint32_t size[(K + 1) / 2], total = 0;
+            uintptr_t from[(K + 1) / 2];
+#pragma unroll
+            for (int j = 0; j < (K + 1) / 2; ++j) {
+                const int k = 2 * j + (at.lane >> 4), i = at.lane & 15;
+                size[j] = 0;
+                from[j] = 0;
+                if (k < K && t0 + i < at.len) {
+                    const uintptr_t a = reinterpret_cast<uintptr_t>(row_of(k) + (t0 + i) * pitch_of(k));
+                    from[j] = a & ~uintptr_t(15);
+                    size[j] = (uint32_t)(((a & 15) + width + 15) & ~uintptr_t(15));
+                }
+                total += size[j];
+            }
+            total = __reduce_add_sync(0xffffffffu, total);
+            if (at.lane == 0) mbar_expect_tx(bar, total);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < (K + 1) / 2; ++j)
+                if (size[j]) {
+                    const int k = 2 * j + (at.lane >> 4), i = at.lane & 15;
+                    bulk_load(to + (uint32_t)(k * kRowTile + i * kSlot), from[j], size[j], bar);
+                }
+        }
+    }
+    __device__ __forceinline__ const T* row_of(int k) const { return K == 3 && k == 2 ? rows[A == kTma ? 0 : K - 1] : k ? rows[A == kTma ? 0 : 1] : rows[0]; }
+    __device__ __forceinline__ int64_t pitch_of(int k) const { return K == 3 && k == 2 ? pitch[A == kTma ? 0 : K - 1] : k ? pitch[A == kTma ? 0 : 1] : pitch[0]; }
     __device__ __forceinline__ void gave_up() {
         alive = false;
         if (p.fault) atomicCAS(p.fault, 0u, (unsigned)kFaultGated);
     }
     __device__ __forceinline__ void wait_tiles(int s) {
-        if (A != kTma) return;
-        if (alive && !mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget)) gave_up();
+        uint64_t* bar = &full[s % kStages * kFulls + (A == kTma ? 0 : at.warp)];
+        if (alive && !mbar_wait(bar, (uint32_t)((s / kStages) & 1), tc::kWaitBudget)) gave_up();
         __syncwarp();
     }
     __device__ __forceinline__ void begin() {
         if (threadIdx.x == kThreads - 1) {
 #pragma unroll
-            for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
+            for (int k = 0; k < kStages * kFulls; ++k) mbar_init(&full[k], 1);
             mbar_init(&meet->arrived[0], 1);
             mbar_init(&meet->arrived[1], 1);
             fence_mbar_init();
@@ -373,72 +460,13 @@ struct Walk {
         __syncwarp();
     }
     __device__ __forceinline__ void end() {
-        if (issuer())  // whatever the other threads made of their waits, the loads land
+        // whatever became of the other waits, the loads land
+        if (A == kTma ? issuer() : at.lane == 0)
             for (int s = max(0, steps - kStages); s < steps; ++s)
-                mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget);
+                mbar_wait(&full[s % kStages * kFulls + (A == kTma ? 0 : at.warp)], (uint32_t)((s / kStages) & 1),
+                          tc::kWaitBudget);
         __syncwarp();
         if (p.cluster > 1) cluster_sync();  // no CTA leaves while another may store to it
-    }
-};
-
-// Plain access to K token tensors: a lane's words of a step, loaded one step
-// before they are looked at.  Rows at odd 2-byte addresses (kHalf) are read by
-// the aligned words that hold them; a lane then shifts its word and the next
-// lane's together, and lanes 0 .. 15 (16 .. 31) hold the word that lane 31
-// lacks of the 16 rows of tensor 0 (1), in extra[1] of tensor 2.  A word is
-// read only if it holds a channel that exists.
-template <typename T, Access A, int K>
-struct Ahead {
-    uint32_t w[K][kTok];
-    uint32_t extra[(K + 1) / 2];
-    uint32_t odd;  // bit k: row 0 of tensor k is at an odd address; bit 8 + k: its pitch is odd
-
-    __device__ __forceinline__ bool shifted(int k, int i) const {
-        return ((odd >> k) ^ ((odd >> (8 + k)) & (uint32_t)i)) & 1u;
-    }
-    // rows[k]: row t0 of tensor k at the lane's first channel; live: rows that exist
-    __device__ __forceinline__ void load(const T* const (&rows)[K], const int64_t (&pitch)[K], const Place<T, 32>& at,
-                                         int n_chan, int live) {
-        if constexpr (A == kHalf) {
-            odd = 0;
-#pragma unroll
-            for (int e = 0; e < (K + 1) / 2; ++e) extra[e] = 0;
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if constexpr (A == kHalf) {
-                odd |= (uint32_t)(reinterpret_cast<uintptr_t>(rows[k]) >> 1 & 1) << k | (uint32_t)(pitch[k] & 1) << (8 + k);
-                const int i = at.lane & 15;
-                if ((K == 2 || k < 2 ? (at.lane >> 4) == k : at.lane < 16) && i < live && shifted(k, i)) {
-                    const T* end = rows[k] - Lane<T>::kN * at.lane + 32 * Lane<T>::kN + i * pitch[k];
-                    if (at.slab0() + 32 * Lane<T>::kN - 1 < n_chan)  // lane 31's second channel
-                        extra[k / 2] = __ldcs(reinterpret_cast<const unsigned int*>(end - 1));
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kTok; ++i) {
-                w[k][i] = 0u;
-                if constexpr (A == kHalf) {
-                    const bool sh = shifted(k, i);
-                    const T* p = rows[k] + i * pitch[k] - (sh ? 1 : 0);
-                    // a shifted word also holds the lane before's second channel
-                    if (i < live && at.c0 - (sh ? 1 : 0) < n_chan)
-                        w[k][i] = __ldcs(reinterpret_cast<const unsigned int*>(p));
-                } else {
-                    if (i < live && at.n > 0) w[k][i] = ld_raw<T, A>(rows[k] + i * pitch[k], at.n);
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ uint32_t get(int k, int i, int lane) const {
-        if constexpr (A == kHalf) {
-            if (shifted(k, i)) {  // the same for the whole warp
-                const uint32_t next = __shfl_down_sync(0xffffffffu, w[k][i], 1);
-                const uint32_t last = __shfl_sync(0xffffffffu, extra[k / 2], i + (k == 1 ? 16 : 0));
-                return __funnelshift_r(w[k][i], lane == 31 ? last : next, 16);
-            }
-        }
-        return w[k][i];
     }
 };
 
@@ -450,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     extern __shared__ uint8_t smem_raw[];
     using M = Meet<V, 2>;
     __shared__ M meet;
-    __shared__ uint64_t full[kStages];
+    __shared__ uint64_t full[kStages * (A == kTma ? 1 : kWarps)];
 
     const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
@@ -459,39 +487,29 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
     const int steps = walk.steps;
     auto chunk_of = [&](int s) { return s * R + at.rank; };
     walk.begin();
-    if (walk.issuer())
-        for (int s = 0; s < kStages && s < steps; ++s) walk.load(s, chunk_of(s));
+    if constexpr (A != kTma) {
+        walk.rows[0] = static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.slab0(), walk.pitch[0] = p.s_g;
+        walk.rows[1] = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.slab0(), walk.pitch[1] = p.s_v;
+    }
+    for (int s = 0; s < kStages && s < steps; ++s) {
+        if (walk.issuer()) walk.load(s, chunk_of(s));
+        walk.copy_rows(s, chunk_of(s));
+    }
     __syncwarp();
 
-    Ahead<T, A, A == kTma ? 1 : 2> ahead;
-    auto fetch = [&](int s) {
-        if constexpr (A != kTma) {
-            const int t0 = chunk_of(s) * Cut<LW>::kTokens + at.run * kTok;
-            const T* const rows[2] = {
-                static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0 + (int64_t)t0 * p.s_g,
-                static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0 + (int64_t)t0 * p.s_v};
-            const int64_t pitch[2] = {p.s_g, p.s_v};
-            ahead.load(rows, pitch, at, p.n_chan, at.len - t0);
-        }
-    };
     V h = ld_state<L>(p.h0 ? p.h0 + (int64_t)at.seq * p.seq_h0 + at.c0 : nullptr, n);
-    if (steps > 0) fetch(0);
     for (int s = 0; s < steps; ++s) {
         const int base = chunk_of(s) * Cut<LW>::kTokens, t0 = base + at.run * kTok, b = s & 1;
         const uint32_t my = walk.mine(s);
         const bool whole = at.whole(p, base);
         // -D and B of the run up to each token: h_t = h - D h + B
         V nd[kTok], hb[kTok], D = L::splat(0.0f), B = D;
+        const auto shift_g = walk.shift(0, t0), shift_v = walk.shift(1, t0);
         walk.wait_tiles(s);
         auto first = [&](auto all) {
 #pragma unroll
             for (int i = 0; i < kTok; ++i) {
-                uint32_t gw, vw;
-                if constexpr (A == kTma) {
-                    gw = lds(my + Cut<LW>::word(0, i)), vw = lds(my + Cut<LW>::word(1, i));
-                } else {
-                    gw = ahead.get(0, i, lane), vw = ahead.get(1, i, lane);
-                }
+                uint32_t gw = walk.get(my, shift_g, 0, i), vw = walk.get(my, shift_v, 1, i);
                 if (!decltype(all)::value && t0 + i >= at.len) gw = L::kInf, vw = 0u;
                 const V z = gate<T>(L::unpack(gw));
                 nd[i] = D = grow<L>(D, z);
@@ -502,7 +520,10 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
             first(std::true_type{});
         else
             first(std::false_type{});
-        if (s + 1 < steps) fetch(s + 1);
+        if (A != kTma && s + kStages < steps) {  // the warp is done with its rows
+            __syncwarp();
+            walk.copy_rows(s + kStages, chunk_of(s + kStages));
+        }
         V d0 = D, b0 = B;  // the warp's first run
         if (LW == 16) {
             const V d1 = of_lane(D, at.l + 16), b1 = of_lane(B, at.l + 16);
@@ -512,7 +533,9 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
         }
         meet.warp[b][0][warp][lane] = D;
         meet.warp[b][1][warp][lane] = B;
-        __syncthreads();
+        __syncthreads();  // and every warp is done with the tiles
+        if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
+        __syncwarp();
         // what the CTA's earlier warps, and all of them, make of a state
         V dp = L::splat(0.0f), bp = dp, d = dp, t = dp;
 #pragma unroll
@@ -526,10 +549,13 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
         if (R > 1) {
             walk.send(s, d, t);
             walk.receive(s);
-            for (int k = 0; k < R; ++k) {
-                if (k == at.rank) hw = h;
-                h = fold<L>(h, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
-            }
+            by_cluster(R, [&](auto size) {
+#pragma unroll
+                for (int k = 0; k < size; ++k) {
+                    if (k == at.rank) hw = h;
+                    h = fold<L>(h, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
+                }
+            });
         } else {
             h = fold<L>(h, d, t);
         }
@@ -551,11 +577,6 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
             second(std::true_type{});
         else
             second(std::false_type{});
-        if (s + kStages < steps) {
-            __syncthreads();  // every warp is done with the tiles
-            if (walk.issuer()) walk.load(s + kStages, chunk_of(s + kStages));
-            __syncwarp();
-        }
     }
     walk.end();
     // Every CTA holds the last state.  In place of h0 is safe: each has read
@@ -571,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
     extern __shared__ uint8_t smem_raw[];
     using M = Meet<V, 3, 1>;
     __shared__ M meet;
-    __shared__ uint64_t full[kStages];
+    __shared__ uint64_t full[kStages * (A == kTma ? 1 : kWarps)];
 
     const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
@@ -580,24 +601,18 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
     const int steps = walk.steps;
     auto chunk_of = [&](int s) { return (steps - 1 - s) * R + at.rank; };  // from the end
     walk.begin();
-    if (walk.issuer())
-        for (int s = 0; s < kStages && s < steps; ++s) walk.load(s, chunk_of(s));
+    if constexpr (A != kTma) {
+        walk.rows[0] = static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.slab0(), walk.pitch[0] = p.s_g;
+        walk.rows[1] = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.slab0(), walk.pitch[1] = p.s_v;
+        walk.rows[2] = static_cast<const T*>(p.dy) + (int64_t)at.seq * p.seq_dy + at.slab0(), walk.pitch[2] = p.s_dy;
+    }
+    for (int s = 0; s < kStages && s < steps; ++s) {
+        if (walk.issuer()) walk.load(s, chunk_of(s));
+        walk.copy_rows(s, chunk_of(s));
+    }
     __syncwarp();
 
-    Ahead<T, A, A == kTma ? 1 : 3> ahead;
-    auto fetch = [&](int s) {
-        if constexpr (A != kTma) {
-            const int t0 = chunk_of(s) * Cut<LW>::kTokens + at.run * kTok;
-            const T* const rows[3] = {
-                static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.c0 + (int64_t)t0 * p.s_g,
-                static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.c0 + (int64_t)t0 * p.s_v,
-                static_cast<const T*>(p.dy) + (int64_t)at.seq * p.seq_dy + at.c0 + (int64_t)t0 * p.s_dy};
-            const int64_t pitch[3] = {p.s_g, p.s_v, p.s_dy};
-            ahead.load(rows, pitch, at, p.n_chan, at.len - t0);
-        }
-    };
     V c = ld_state<L>(p.dh1 ? p.dh1 + (int64_t)at.seq * p.seq_dh1 + at.c0 : nullptr, n);
-    if (steps > 0) fetch(0);
     for (int s = 0; s < steps; ++s) {
         const int base = chunk_of(s) * Cut<LW>::kTokens, t0 = base + at.run * kTok, b = s & 1;
         const uint32_t my = walk.mine(s);
@@ -605,27 +620,21 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         float entry[L::kN];  // the chunk's state; looked at after the warps have met
         ld_state<L>(t0 < p.n_tok ? p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0 : nullptr, n,
                     entry);
-        if constexpr (A != kTma) {  // the lane's words, into its own slots
-#pragma unroll
-            for (int i = 0; i < kTok; ++i)
-#pragma unroll
-                for (int k = 0; k < 3; ++k) sts(my + Cut<LW>::word(k, i), ahead.get(k, i, lane));
-            if (s + 1 < steps) fetch(s + 1);
-        }
+        const auto shift_g = walk.shift(0, t0), shift_v = walk.shift(1, t0), shift_dy = walk.shift(2, t0);
         V z[kTok], q[kTok], D = L::splat(0.0f), B = D, E = D;
         walk.wait_tiles(s);
         auto first = [&](auto all) {
             auto past = [&](int i) { return !decltype(all)::value && t0 + i >= at.len; };
 #pragma unroll
             for (int i = 0; i < kTok; ++i) {
-                const uint32_t gw = past(i) ? L::kInf : lds(my + Cut<LW>::word(0, i)), vw = past(i) ? 0u : lds(my + Cut<LW>::word(1, i));
+                const uint32_t gw = past(i) ? L::kInf : walk.get(my, shift_g, 0, i), vw = past(i) ? 0u : walk.get(my, shift_v, 1, i);
                 gate_slope<T>(L::unpack(gw), z[i], q[i]);
                 D = grow<L>(D, z[i]);
                 B = step<L>(B, z[i], L::unpack(vw));
             }
 #pragma unroll
             for (int i = kTok - 1; i >= 0; --i) {
-                const V lam = L::add(L::unpack(past(i) ? 0u : lds(my + Cut<LW>::word(2, i))), E);
+                const V lam = L::add(L::unpack(past(i) ? 0u : walk.get(my, shift_dy, 2, i)), E);
                 E = L::fma(z[i], lam, lam);
             }
         };
@@ -665,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         if (LW == 16 && lane >= 16) h = fold<L>(h, d0, b0);
 #pragma unroll
         for (int i = 0; i < kTok; ++i) {
-            const V off = L::fma(whole || t0 + i < at.len ? L::unpack(lds(my + Cut<LW>::word(1, i))) : L::splat(0.0f),
+            const V off = L::fma(whole || t0 + i < at.len ? L::unpack(walk.get(my, shift_v, 1, i)) : L::splat(0.0f),
                                  L::splat(-1.0f), h);
             q[i] = L::mul(q[i], off);
             h = L::fma(z[i], off, h);
@@ -688,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
 #pragma unroll
             for (int i = kTok - 1; i >= 0; --i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
-                const V lam = L::add(past ? L::splat(0.0f) : L::unpack(lds(my + Cut<LW>::word(2, i))), cw);
+                const V lam = L::add(past ? L::splat(0.0f) : L::unpack(walk.get(my, shift_dy, 2, i)), cw);
                 if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok)) {
                     const int k = decltype(all)::value ? L::kN : n;
                     st_raw<T, A>(dg, k, past ? 0u : L::pack(L::mul(lam, q[i])));
@@ -703,7 +712,10 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         else
             second(std::false_type{});
         __syncthreads();  // every warp is done with the tiles and the meeting
-        if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
+        if (s + kStages < steps) {
+            if (walk.issuer()) walk.load(s + kStages, chunk_of(s + kStages));
+            walk.copy_rows(s + kStages, chunk_of(s + kStages));
+        }
         __syncwarp();
     }
     walk.end();
@@ -780,7 +792,9 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 // Stages of tiles: with two CTAs per SM, or (deep) with one, when the device
 // holds all clusters at once that way too.
 constexpr int kFwdStages = 3, kFwdDeep = 6, kGradStages = 2, kGradDeep = 4;
+constexpr int kRowStages = 2;  // of copied rows
 constexpr size_t tiles_smem(int tensors, int stages) { return (size_t)stages * tensors * kTileBytes + 128; }
+constexpr size_t rows_smem(int tensors) { return (size_t)kRowStages * tensors * kRowTile + 128; }
 
 // [n_seq][n_tok][n_chan] in boxes of row_bytes bytes of a tile's tokens; false when TMA
 // cannot describe it.  Rows and channels past the ends read as zero.
@@ -812,20 +826,21 @@ bool make_maps(const helix_ctx* ctx, GatedMaps* m, const GatedParams& p, bool gr
 // Lanes of a row, CTAs of a cluster, and whether one CTA per SM is enough: the
 // choice with the fewest steps, counting the waves that its clusters take, two
 // CTAs per SM (large clusters leave SMs of a GPC idle), and two steps to fill
-// and drain each.  Narrow rows (TMA only) serve few channels: 1 x 131072 x 1024
+// and drain each (the gradient of copied rows: one CTA, whose stages fill the
+// SM).  Narrow rows (tiles only) serve few channels: 1 x 131072 x 1024
 // bf16 takes 208 us with them, 338 without.
 struct GatedCut {
     int  lanes = 32, cluster = 1;
     bool deep = false;
 };
-GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, bool narrow) {
+GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, bool tma, bool grad) {
     GatedCut best;
     int64_t least = INT64_MAX;
-    for (int lanes = 32; lanes >= (narrow ? 16 : 32); lanes /= 2) {
+    for (int lanes = 32; lanes >= (tma ? 16 : 32); lanes /= 2) {
         const int64_t cb = lanes * lane_channels, groups = (int64_t)p.n_seq * ((p.n_chan + cb - 1) / cb);
         const int64_t tokens = kChunk * (32 / lanes), chunks = (p.n_tok + tokens - 1) / tokens;
         for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
-            const int64_t at_once = ctx->gated_clusters[i];
+            const int64_t at_once = grad && !tma ? ctx->gated_deep[i] : ctx->gated_clusters[i];
             if (at_once <= 0 || (r > 1 && r >= 2 * chunks)) continue;
             const int64_t cost = (groups + at_once - 1) / at_once * ((chunks + r - 1) / r + 2);
             if (cost < least) {
@@ -867,15 +882,20 @@ int launch_gated_a(const GatedMaps& maps, GatedParams p, const GatedCut& cut, bo
     p.cluster = cut.cluster;
     const int64_t grid = groups * p.cluster;
     if (grad) {
-        // plain loads ahead need the registers of one CTA per SM
-        const bool deep = cut.deep || A != kTma;
-        ClusterLaunch l(grid, p.cluster, tiles_smem(3, deep ? kGradDeep : kGradStages), stream);
-        if (deep) return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep, LW>, maps, p);
-        if constexpr (A == kTma) return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradStages, LW>, maps, p);
+        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, cut.deep ? kGradDeep : kGradStages) : rows_smem(3),
+                        stream);
+        if constexpr (A != kTma)
+            return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kRowStages, LW>, maps, p);
+        else
+            return cut.deep ? cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep, LW>, maps, p)
+                            : cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradStages, LW>, maps, p);
     }
-    ClusterLaunch l(grid, p.cluster, tiles_smem(2, cut.deep ? kFwdDeep : kFwdStages), stream);
-    return cut.deep ? cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdDeep, LW>, maps, p)
-                    : cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdStages, LW>, maps, p);
+    ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, cut.deep ? kFwdDeep : kFwdStages) : rows_smem(2), stream);
+    if constexpr (A != kTma)
+        return cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kRowStages, LW>, maps, p);
+    else
+        return cut.deep ? cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdDeep, LW>, maps, p)
+                        : cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdStages, LW>, maps, p);
 }
 
 template <typename T, Access A>
@@ -897,7 +917,7 @@ int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool g
     }
     // outputs are stored a word at a time in the TMA form too
     if (word) {
-        const GatedCut cut = cut_of(ctx, p, N, true);
+        const GatedCut cut = cut_of(ctx, p, N, true, grad);
         GatedMaps maps;
         if (make_maps(ctx, &maps, p, grad, sizeof(T), 4 * cut.lanes))
             return cut.lanes == 16 ? launch_gated_a<T, kTma, 16>(maps, p, cut, grad, stream)
@@ -905,7 +925,7 @@ int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool g
     }
     GatedMaps none;
     std::memset(&none, 0, sizeof(none));
-    const GatedCut cut = cut_of(ctx, p, N, false);
+    const GatedCut cut = cut_of(ctx, p, N, false, grad);
     if constexpr (N == 2)
         if (!word) return launch_gated_a<T, kHalf, 32>(none, p, cut, grad, stream);
     return launch_gated_a<T, kWord, 32>(none, p, cut, grad, stream);
@@ -918,31 +938,35 @@ int launch_gated_any(const helix_ctx* ctx, const helix_gated_scan_desc& d, const
 }
 
 template <typename K>
-int set_smem(K kernel, int tensors, int stages) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles_smem(tensors, stages));
+int set_smem(K kernel, size_t bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
-template <typename T, Access A, int LW>
-int configure_gated_a() {
+template <typename T, int LW>
+int configure_tiles() {
     int e;
-    if ((e = set_smem(gated_kernel<T, A, kFwdStages, LW>, 2, kFwdStages)) != cudaSuccess) return e;
-    if ((e = set_smem(gated_kernel<T, A, kFwdDeep, LW>, 2, kFwdDeep)) != cudaSuccess) return e;
-    if constexpr (A == kTma)
-        if ((e = set_smem(gated_grad_kernel<T, A, kGradStages, LW>, 3, kGradStages)) != cudaSuccess) return e;
-    return set_smem(gated_grad_kernel<T, A, kGradDeep, LW>, 3, kGradDeep);
+    if ((e = set_smem(gated_kernel<T, kTma, kFwdStages, LW>, tiles_smem(2, kFwdStages))) != cudaSuccess) return e;
+    if ((e = set_smem(gated_kernel<T, kTma, kFwdDeep, LW>, tiles_smem(2, kFwdDeep))) != cudaSuccess) return e;
+    if ((e = set_smem(gated_grad_kernel<T, kTma, kGradStages, LW>, tiles_smem(3, kGradStages))) != cudaSuccess) return e;
+    return set_smem(gated_grad_kernel<T, kTma, kGradDeep, LW>, tiles_smem(3, kGradDeep));
+}
+template <typename T, Access A>
+int configure_rows() {
+    const int e = set_smem(gated_kernel<T, A, kRowStages, 32>, rows_smem(2));
+    return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, A, kRowStages, 32>, rows_smem(3));
 }
 
 }  // namespace
 
 int configure_gated(helix_ctx* ctx) {
     int e;
-    if ((e = configure_gated_a<float, kTma, 32>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<float, kTma, 16>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<float, kWord, 32>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<__nv_bfloat16, kTma, 32>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<__nv_bfloat16, kTma, 16>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<__nv_bfloat16, kWord, 32>()) != cudaSuccess) return e;
-    if ((e = configure_gated_a<__nv_bfloat16, kHalf, 32>()) != cudaSuccess) return e;
+    if ((e = configure_tiles<float, 32>()) != cudaSuccess) return e;
+    if ((e = configure_tiles<float, 16>()) != cudaSuccess) return e;
+    if ((e = configure_tiles<__nv_bfloat16, 32>()) != cudaSuccess) return e;
+    if ((e = configure_tiles<__nv_bfloat16, 16>()) != cudaSuccess) return e;
+    if ((e = configure_rows<float, kWord>()) != cudaSuccess) return e;
+    if ((e = configure_rows<__nv_bfloat16, kWord>()) != cudaSuccess) return e;
+    if ((e = configure_rows<__nv_bfloat16, kHalf>()) != cudaSuccess) return e;
     for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
         ClusterLaunch l(r, r, tiles_smem(2, kFwdStages), nullptr);
         e = cudaOccupancyMaxActiveClusters(&ctx->gated_clusters[i], gated_kernel<__nv_bfloat16, kTma, kFwdStages, 32>,
