@@ -792,9 +792,9 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 // Stages of tiles: with two CTAs per SM, or (deep) with one, when the device
 // holds all clusters at once that way too.
 constexpr int kFwdStages = 3, kFwdDeep = 6, kGradStages = 2, kGradDeep = 4;
-constexpr int kRowStages = 2;  // of copied rows
+constexpr int kRowStages = 2, kGradRowStages = 1;  // of copied rows: two CTAs per SM
 constexpr size_t tiles_smem(int tensors, int stages) { return (size_t)stages * tensors * kTileBytes + 128; }
-constexpr size_t rows_smem(int tensors) { return (size_t)kRowStages * tensors * kRowTile + 128; }
+constexpr size_t rows_smem(int tensors, int stages) { return (size_t)stages * tensors * kRowTile + 128; }
 
 // [n_seq][n_tok][n_chan] in boxes of row_bytes bytes of a tile's tokens; false when TMA
 // cannot describe it.  Rows and channels past the ends read as zero.
@@ -826,21 +826,20 @@ bool make_maps(const helix_ctx* ctx, GatedMaps* m, const GatedParams& p, bool gr
 // Lanes of a row, CTAs of a cluster, and whether one CTA per SM is enough: the
 // choice with the fewest steps, counting the waves that its clusters take, two
 // CTAs per SM (large clusters leave SMs of a GPC idle), and two steps to fill
-// and drain each (the gradient of copied rows: one CTA, whose stages fill the
-// SM).  Narrow rows (tiles only) serve few channels: 1 x 131072 x 1024
+// and drain each.  Narrow rows (tiles only) serve few channels: 1 x 131072 x 1024
 // bf16 takes 208 us with them, 338 without.
 struct GatedCut {
     int  lanes = 32, cluster = 1;
     bool deep = false;
 };
-GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, bool tma, bool grad) {
+GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, bool tma) {
     GatedCut best;
     int64_t least = INT64_MAX;
     for (int lanes = 32; lanes >= (tma ? 16 : 32); lanes /= 2) {
         const int64_t cb = lanes * lane_channels, groups = (int64_t)p.n_seq * ((p.n_chan + cb - 1) / cb);
         const int64_t tokens = kChunk * (32 / lanes), chunks = (p.n_tok + tokens - 1) / tokens;
         for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
-            const int64_t at_once = grad && !tma ? ctx->gated_deep[i] : ctx->gated_clusters[i];
+            const int64_t at_once = ctx->gated_clusters[i];
             if (at_once <= 0 || (r > 1 && r >= 2 * chunks)) continue;
             const int64_t cost = (groups + at_once - 1) / at_once * ((chunks + r - 1) / r + 2);
             if (cost < least) {
@@ -882,15 +881,15 @@ int launch_gated_a(const GatedMaps& maps, GatedParams p, const GatedCut& cut, bo
     p.cluster = cut.cluster;
     const int64_t grid = groups * p.cluster;
     if (grad) {
-        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, cut.deep ? kGradDeep : kGradStages) : rows_smem(3),
+        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, cut.deep ? kGradDeep : kGradStages) : rows_smem(3, kGradRowStages),
                         stream);
         if constexpr (A != kTma)
-            return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kRowStages, LW>, maps, p);
+            return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradRowStages, LW>, maps, p);
         else
             return cut.deep ? cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep, LW>, maps, p)
                             : cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradStages, LW>, maps, p);
     }
-    ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, cut.deep ? kFwdDeep : kFwdStages) : rows_smem(2), stream);
+    ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, cut.deep ? kFwdDeep : kFwdStages) : rows_smem(2, kRowStages), stream);
     if constexpr (A != kTma)
         return cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kRowStages, LW>, maps, p);
     else
@@ -917,7 +916,7 @@ int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool g
     }
     // outputs are stored a word at a time in the TMA form too
     if (word) {
-        const GatedCut cut = cut_of(ctx, p, N, true, grad);
+        const GatedCut cut = cut_of(ctx, p, N, true);
         GatedMaps maps;
         if (make_maps(ctx, &maps, p, grad, sizeof(T), 4 * cut.lanes))
             return cut.lanes == 16 ? launch_gated_a<T, kTma, 16>(maps, p, cut, grad, stream)
@@ -925,7 +924,7 @@ int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool g
     }
     GatedMaps none;
     std::memset(&none, 0, sizeof(none));
-    const GatedCut cut = cut_of(ctx, p, N, false, grad);
+    const GatedCut cut = cut_of(ctx, p, N, false);
     if constexpr (N == 2)
         if (!word) return launch_gated_a<T, kHalf, 32>(none, p, cut, grad, stream);
     return launch_gated_a<T, kWord, 32>(none, p, cut, grad, stream);
@@ -952,8 +951,8 @@ int configure_tiles() {
 }
 template <typename T, Access A>
 int configure_rows() {
-    const int e = set_smem(gated_kernel<T, A, kRowStages, 32>, rows_smem(2));
-    return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, A, kRowStages, 32>, rows_smem(3));
+    const int e = set_smem(gated_kernel<T, A, kRowStages, 32>, rows_smem(2, kRowStages));
+    return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, A, kGradRowStages, 32>, rows_smem(3, kGradRowStages));
 }
 
 }  // namespace
