@@ -554,48 +554,50 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 }
                 buf.next();
             }
-            // the warp's 32 rows: 128 bytes of each row at a time
-            // through its staging, or straight to memory
+            // the warp's 32 rows: 128 bytes of each at a time through its
+            // staging, then by TMA, or (out at any alignment) by the lanes
             constexpr int kPer = 128 / (int)sizeof(T);
-            if (a.vec_out) {
-                const bool in = p0 + 32 * (warp & 3) < a.p.rows;
+            const int row0 = p0 + 32 * (warp & 3);
 #pragma unroll
-                for (int c = 0; c < Cfg::kRun; c += kPer) {
-                    bulk_wait_read0();  // (lane 0) the last store has read the staging
-                    __syncwarp();
+            for (int c = 0; c < Cfg::kRun; c += kPer) {
+                bulk_wait_read0();  // (lane 0) the last store has read the staging
+                __syncwarp();
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {  // 16-byte units of the lane's row
-                        uint32_t w[4];
+                for (int u = 0; u < 8; ++u) {  // 16-byte units of the lane's row
+                    uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float lo, up;
-                            if constexpr (sizeof(T) == 2) {
-                                f2_to(acc[c / 2 + 4 * u + e], lo, up);
-                                w[e] = bf16x2(lo, up);
-                            } else {
-                                f2_to(acc[c / 2 + 2 * u + e / 2], lo, up);
-                                w[e] = __float_as_uint(e & 1 ? up : lo);
-                            }
+                    for (int e = 0; e < 4; ++e) {
+                        float lo, up;
+                        if constexpr (sizeof(T) == 2) {
+                            f2_to(acc[c / 2 + 4 * u + e], lo, up);
+                            w[e] = bf16x2(lo, up);
+                        } else {
+                            f2_to(acc[c / 2 + 2 * u + e / 2], lo, up);
+                            w[e] = __float_as_uint(e & 1 ? up : lo);
                         }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + sw128_off(lane, u)),
-                                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                                     : "memory");
                     }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + sw128_off(lane, u)),
+                                 "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                 : "memory");
+                }
+                const int col0 = q0 + c0 + c;
+                if (a.vec_out) {
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        if (in && q0 + c0 + c < a.q.rows)
-                            tma_store_2d(&maps.out, staging, q0 + c0 + c, p0 + 32 * (warp & 3));
+                        if (row0 < a.p.rows && col0 < a.q.rows) tma_store_2d(&maps.out, staging, col0, row0);
                         bulk_commit();
                     }
-                }
-            } else {
+                } else {
+                    __syncwarp();
+                    const uint8_t* from = smem + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
+                    for (int r = 0; r < 32 && row0 + r < a.p.rows; ++r) {
+                        T* o = static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.ld_out + col0;
 #pragma unroll
-                for (int c = 0; c < Cfg::kRun; c += 8) {
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) f2_to(acc[c / 2 + e], v[2 * e], v[2 * e + 1]);
-                    st_out<T>(a, p0 + row, q0 + c0 + c, 8, v);
+                        for (int e = lane; e < kPer; e += 32)
+                            if (col0 + e < a.q.rows)
+                                o[e] = *reinterpret_cast<const T*>(from + sw128_off(r, e * sizeof(T) / 16) + e * sizeof(T) % 16);
+                    }
                 }
             }
         }
