@@ -309,8 +309,8 @@ template <int N>
 struct Size {
     __device__ __forceinline__ constexpr operator int() const { return N; }
 };
-// The body with the cluster's size as a constant , so that its loop's shared loads are
-// all issued before the first is looked at.
+// The body with the cluster's size as a constant, so that its loop's shared
+// loads are all issued before the first is looked at.
 template <typename F>
 __device__ __forceinline__ void by_cluster(int size, F body) {
     static_assert(kMaxCluster == 8, "");
@@ -342,14 +342,14 @@ struct Walk {
     bool               alive = true;
     static constexpr int kFulls = A == kTma ? 1 : kWarps;  // barriers of a stage: a warp's rows are its own
 
-    // Tensor k of a token tensor's call: its rows of the sequence at the slab's first channel, and their pitch.
+    // Copied rows: tensor k's of the sequence, at the slab's first channel, and their pitch.
     const T* rows[A == kTma ? 1 : K];
     int64_t  pitch[A == kTma ? 1 : K];
 
     // Tiles.  The lane's words of step s.
     __device__ __forceinline__ uint32_t mine(int s) const {
-        if (A == kTma) return base + (uint32_t)((s % kStages) * K * kTileBytes + at.run * kTok * Cut<LW>::kRow + at.l * 4);
-        return base + (uint32_t)((s % kStages) * K * kRowTile + at.run * kTok * kSlot + at.l * 4);
+        constexpr int kTile = A == kTma ? kTileBytes : kRowTile, kRow = A == kTma ? Cut<LW>::kRow : kSlot;
+        return base + (uint32_t)((s % kStages) * K * kTile + at.run * kTok * kRow + at.l * 4);
     }
     // Offset in its 16-byte piece of the run's first row of a step's tensor,
     // and what a row adds to it.
@@ -358,7 +358,8 @@ struct Walk {
     };
     __device__ __forceinline__ Shift shift(int k, int t0) const {
         if (A == kTma) return {0u, 0u};
-        return {(uint32_t)(reinterpret_cast<uintptr_t>(rows[k] + t0 * pitch[k])) & 15u, (uint32_t)(pitch[k] * (int64_t)sizeof(T)) & 15u};
+        return {(uint32_t)(reinterpret_cast<uintptr_t>(rows[k] + t0 * pitch[k])) & 15u,
+                (uint32_t)(pitch[k] * (int64_t)sizeof(T)) & 15u};
     }
     // The lane's channels of token i of tensor k.
     __device__ __forceinline__ uint32_t get(uint32_t my, const Shift& sh, int k, int i) const {
@@ -394,7 +395,7 @@ struct Walk {
                 size[j] = 0;
                 from[j] = 0;
                 if (k < K && t0 + i < at.len) {
-                    const uintptr_t a = reinterpret_cast<uintptr_t>(row_of(k) + (t0 + i) * pitch_of(k));
+                    const uintptr_t a = reinterpret_cast<uintptr_t>(pick(rows, k) + (t0 + i) * pick(pitch, k));
                     from[j] = a & ~uintptr_t(15);
                     size[j] = (uint32_t)(((a & 15) + width + 15) & ~uintptr_t(15));
                 }
@@ -411,8 +412,12 @@ struct Walk {
                 }
         }
     }
-    __device__ __forceinline__ const T* row_of(int k) const { return K == 3 && k == 2 ? rows[A == kTma ? 0 : K - 1] : k ? rows[A == kTma ? 0 : 1] : rows[0]; }
-    __device__ __forceinline__ int64_t pitch_of(int k) const { return K == 3 && k == 2 ? pitch[A == kTma ? 0 : K - 1] : k ? pitch[A == kTma ? 0 : 1] : pitch[0]; }
+    // An array's element k by selection (an index that is no constant would put
+    // the array into memory).
+    template <typename E>
+    static __device__ __forceinline__ E pick(const E* a, int k) {
+        return K == 3 && k == 2 ? a[K - 1] : k ? a[1] : a[0];
+    }
     __device__ __forceinline__ void gave_up() {
         alive = false;
         if (p.fault) atomicCAS(p.fault, 0u, (unsigned)kFaultGated);
@@ -471,7 +476,7 @@ struct Walk {
 };
 
 template <typename T, Access A, int kStages, int LW>
-__global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, 2)
     gated_kernel(const __grid_constant__ GatedMaps maps, const __grid_constant__ GatedParams p) {
     using L = Lane<T>;
     using V = typename L::V;
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, kStages <= 3 ? 2 : 1)
 }
 
 template <typename T, Access A, int kStages, int LW>
-__global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, 2)
     gated_grad_kernel(const __grid_constant__ GatedMaps maps, const __grid_constant__ GatedParams p) {
     using L = Lane<T>;
     using V = typename L::V;
@@ -618,8 +623,8 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
         const uint32_t my = walk.mine(s);
         const bool whole = at.whole(p, base);
         float entry[L::kN];  // the chunk's state; looked at after the warps have met
-        ld_state<L>(t0 < p.n_tok ? p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0 : nullptr, n,
-                    entry);
+        const int64_t chunk = (int64_t)at.seq * p.n_chunk + t0 / kChunk;
+        ld_state<L>(t0 < p.n_tok ? p.states + chunk * p.n_chan + at.c0 : nullptr, n, entry);
         const auto shift_g = walk.shift(0, t0), shift_v = walk.shift(1, t0), shift_dy = walk.shift(2, t0);
         V z[kTok], q[kTok], D = L::splat(0.0f), B = D, E = D;
         walk.wait_tiles(s);
@@ -627,7 +632,8 @@ __global__ void __launch_bounds__(kThreads, kStages <= 2 ? 2 : 1)
             auto past = [&](int i) { return !decltype(all)::value && t0 + i >= at.len; };
 #pragma unroll
             for (int i = 0; i < kTok; ++i) {
-                const uint32_t gw = past(i) ? L::kInf : walk.get(my, shift_g, 0, i), vw = past(i) ? 0u : walk.get(my, shift_v, 1, i);
+                const uint32_t gw = past(i) ? L::kInf : walk.get(my, shift_g, 0, i);
+                const uint32_t vw = past(i) ? 0u : walk.get(my, shift_v, 1, i);
                 gate_slope<T>(L::unpack(gw), z[i], q[i]);
                 D = grow<L>(D, z[i]);
                 B = step<L>(B, z[i], L::unpack(vw));
@@ -789,10 +795,9 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Stages of tiles: with two CTAs per SM, or (deep) with one, when the device
-// holds all clusters at once that way too.
-constexpr int kFwdStages = 3, kFwdDeep = 6, kGradStages = 2, kGradDeep = 4;
-constexpr int kRowStages = 2, kGradRowStages = 1;  // of copied rows: two CTAs per SM
+// Steps of tiles, and of copied rows, that fit beside two CTAs per SM.
+constexpr int kFwdStages = 3, kGradStages = 2;
+constexpr int kRowStages = 2, kGradRowStages = 1;
 constexpr size_t tiles_smem(int tensors, int stages) { return (size_t)stages * tensors * kTileBytes + 128; }
 constexpr size_t rows_smem(int tensors, int stages) { return (size_t)stages * tensors * kRowTile + 128; }
 
@@ -823,14 +828,14 @@ bool make_maps(const helix_ctx* ctx, GatedMaps* m, const GatedParams& p, bool gr
     return !grad || make_map_tok(ctx, &m->in[2], p, p.dy, p.s_dy, p.seq_dy, size, row_bytes);
 }
 
-// Lanes of a row, CTAs of a cluster, and whether one CTA per SM is enough: the
-// choice with the fewest steps, counting the waves that its clusters take, two
-// CTAs per SM (large clusters leave SMs of a GPC idle), and two steps to fill
-// and drain each.  Narrow rows (tiles only) serve few channels: 1 x 131072 x 1024
-// bf16 takes 208 us with them, 338 without.
+// Lanes of a row and CTAs of a cluster: the choice with the fewest steps,
+// counting the waves that its clusters take, two CTAs per SM (large clusters
+// leave SMs of a GPC idle), and two steps to fill and drain each.  Narrow rows
+// (tiles only) serve few channels: 1 x 131072 x 1024 bf16 takes 193 us with
+// them, 310 without.  Clusters of 8 take those 193 us, of 4 215, of 2 404, one
+// CTA 672; at 4 x 8192 x 2048 one takes 78 us, two 79, four 85, eight 99.
 struct GatedCut {
-    int  lanes = 32, cluster = 1;
-    bool deep = false;
+    int lanes = 32, cluster = 1;
 };
 GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, bool tma) {
     GatedCut best;
@@ -844,7 +849,7 @@ GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, b
             const int64_t cost = (groups + at_once - 1) / at_once * ((chunks + r - 1) / r + 2);
             if (cost < least) {
                 least = cost;
-                best.lanes = lanes, best.cluster = r, best.deep = groups <= ctx->gated_deep[i];
+                best.lanes = lanes, best.cluster = r;
             }
         }
     }
@@ -881,20 +886,11 @@ int launch_gated_a(const GatedMaps& maps, GatedParams p, const GatedCut& cut, bo
     p.cluster = cut.cluster;
     const int64_t grid = groups * p.cluster;
     if (grad) {
-        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, cut.deep ? kGradDeep : kGradStages) : rows_smem(3, kGradRowStages),
-                        stream);
-        if constexpr (A != kTma)
-            return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradRowStages, LW>, maps, p);
-        else
-            return cut.deep ? cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradDeep, LW>, maps, p)
-                            : cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, kGradStages, LW>, maps, p);
+        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, kGradStages) : rows_smem(3, kGradRowStages), stream);
+        return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, A == kTma ? kGradStages : kGradRowStages, LW>, maps, p);
     }
-    ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, cut.deep ? kFwdDeep : kFwdStages) : rows_smem(2, kRowStages), stream);
-    if constexpr (A != kTma)
-        return cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kRowStages, LW>, maps, p);
-    else
-        return cut.deep ? cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdDeep, LW>, maps, p)
-                        : cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, kFwdStages, LW>, maps, p);
+    ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, kFwdStages) : rows_smem(2, kRowStages), stream);
+    return cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, A == kTma ? kFwdStages : kRowStages, LW>, maps, p);
 }
 
 template <typename T, Access A>
@@ -943,11 +939,8 @@ int set_smem(K kernel, size_t bytes) {
 
 template <typename T, int LW>
 int configure_tiles() {
-    int e;
-    if ((e = set_smem(gated_kernel<T, kTma, kFwdStages, LW>, tiles_smem(2, kFwdStages))) != cudaSuccess) return e;
-    if ((e = set_smem(gated_kernel<T, kTma, kFwdDeep, LW>, tiles_smem(2, kFwdDeep))) != cudaSuccess) return e;
-    if ((e = set_smem(gated_grad_kernel<T, kTma, kGradStages, LW>, tiles_smem(3, kGradStages))) != cudaSuccess) return e;
-    return set_smem(gated_grad_kernel<T, kTma, kGradDeep, LW>, tiles_smem(3, kGradDeep));
+    const int e = set_smem(gated_kernel<T, kTma, kFwdStages, LW>, tiles_smem(2, kFwdStages));
+    return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, kTma, kGradStages, LW>, tiles_smem(3, kGradStages));
 }
 template <typename T, Access A>
 int configure_rows() {
@@ -970,9 +963,6 @@ int configure_gated(helix_ctx* ctx) {
         ClusterLaunch l(r, r, tiles_smem(2, kFwdStages), nullptr);
         e = cudaOccupancyMaxActiveClusters(&ctx->gated_clusters[i], gated_kernel<__nv_bfloat16, kTma, kFwdStages, 32>,
                                            &l.cfg);
-        if (e != cudaSuccess) return e;
-        l.cfg.dynamicSmemBytes = tiles_smem(2, kFwdDeep);
-        e = cudaOccupancyMaxActiveClusters(&ctx->gated_deep[i], gated_kernel<__nv_bfloat16, kTma, kFwdDeep, 32>, &l.cfg);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

@@ -433,7 +433,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 const uint64_t dp = sdesc_sw128(from, 16, 1024), dq = sdesc_sw128(from + kRows * kBk, 16, 1024);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
-                    mma_e4m3_pair(tmem + buf.at * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc, ks > 0);
+                    mma_e4m3_pair(tmem + buf.at * BN, tc::desc_add(dp, 32 * ks), tc::desc_add(dq, 32 * ks), idesc,
+                                  ks > 0);
                 uint64_t *done = &acc_full[buf.at], *read = &empty[st.at];
                 st.next(), st.next();
                 buf.next(), buf.next();
@@ -590,13 +591,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     }
                 } else {
                     __syncwarp();
-                    const uint8_t* from = smem + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
+                    const uint8_t* mine = smem + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
                     for (int r = 0; r < 32 && row0 + r < a.p.rows; ++r) {
                         T* o = static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.ld_out + col0;
 #pragma unroll
-                        for (int e = lane; e < kPer; e += 32)
+                        for (int e = lane; e < kPer; e += 32) {
+                            const int at = e * (int)sizeof(T);
                             if (col0 + e < a.q.rows)
-                                o[e] = *reinterpret_cast<const T*>(from + sw128_off(r, e * sizeof(T) / 16) + e * sizeof(T) % 16);
+                                o[e] = *reinterpret_cast<const T*>(mine + sw128_off(r, at / 16) + at % 16);
+                        }
                     }
                 }
             }
@@ -612,20 +615,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
 }
 
+struct Mm8Launch {
+    cudaLaunchConfig_t  cfg{};
+    cudaLaunchAttribute at{};
+    Mm8Launch(int grid, int cluster, size_t smem, int threads, void* stream) {
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3((unsigned)threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = static_cast<cudaStream_t>(stream);
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = (unsigned)cluster;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+    }
+};
+
 template <int BN, bool QROWS, typename T>
 int launch_pair_t(const PairMaps& maps, const Mm8Params& p, int ctas, void* stream) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = PairCfg<BN>::kSmem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = 2;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, mm8_pair_kernel<BN, QROWS, T>, maps, p);
+    Mm8Launch l(ctas, 2, PairCfg<BN>::kSmem, kPairThreads, stream);
+    return cudaLaunchKernelEx(&l.cfg, mm8_pair_kernel<BN, QROWS, T>, maps, p);
 }
 
 template <int BN>
@@ -651,34 +660,19 @@ int configure_pair_n() {
 
 template <int BN, bool QROWS, typename T>
 int launch_mm8_t(const Mm8Maps& maps, const Mm8Params& p, int tiles, void* stream) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * p.splits));
-    cfg.blockDim = dim3(kMmThreads);
-    cfg.dynamicSmemBytes = Mm8Cfg<BN>::kSmem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)p.splits;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, mm8_kernel<BN, QROWS, T>, maps, p);
+    Mm8Launch l(tiles * p.splits, p.splits, Mm8Cfg<BN>::kSmem, kMmThreads, stream);
+    return cudaLaunchKernelEx(&l.cfg, mm8_kernel<BN, QROWS, T>, maps, p);
 }
 
-template <int BN>
-int launch_mm8_n(bool qrows, helix_dtype out, const Mm8Maps& maps, const Mm8Params& p, int tiles, void* stream) {
-    if (out == HELIX_F32)
-        return qrows ? launch_mm8_t<BN, true, float>(maps, p, tiles, stream)
-                     : launch_mm8_t<BN, false, float>(maps, p, tiles, stream);
-    return qrows ? launch_mm8_t<BN, true, __nv_bfloat16>(maps, p, tiles, stream)
-                 : launch_mm8_t<BN, false, __nv_bfloat16>(maps, p, tiles, stream);
+template <int BN, bool QROWS>
+int launch_mm8_n(helix_dtype out, const Mm8Maps& maps, const Mm8Params& p, int tiles, void* stream) {
+    return out == HELIX_F32 ? launch_mm8_t<BN, QROWS, float>(maps, p, tiles, stream)
+                            : launch_mm8_t<BN, QROWS, __nv_bfloat16>(maps, p, tiles, stream);
 }
 
-template <int BN>
+template <int BN, bool QROWS>
 int configure_mm8_n() {
-    const void* k[] = {(const void*)mm8_kernel<BN, true, float>, (const void*)mm8_kernel<BN, false, float>,
-                       (const void*)mm8_kernel<BN, true, __nv_bfloat16>,
-                       (const void*)mm8_kernel<BN, false, __nv_bfloat16>};
+    const void* k[] = {(const void*)mm8_kernel<BN, QROWS, float>, (const void*)mm8_kernel<BN, QROWS, __nv_bfloat16>};
     for (const void* f : k) {
         const int e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Mm8Cfg<BN>::kSmem);
         if (e != cudaSuccess) return e;
@@ -719,22 +713,35 @@ int tiles_of(int64_t rows, int64_t per) { return (int)((rows + per - 1) / per); 
 
 }  // namespace
 
-int configure_mm8() {
+int configure_mm8(helix_ctx* ctx) {
     int e;
-    if ((e = configure_mm8_n<16>()) != cudaSuccess) return e;
-    if ((e = configure_mm8_n<32>()) != cudaSuccess) return e;
-    if ((e = configure_mm8_n<64>()) != cudaSuccess) return e;
+    if ((e = configure_mm8_n<16, true>()) != cudaSuccess) return e;
+    if ((e = configure_mm8_n<32, true>()) != cudaSuccess) return e;
+    if ((e = configure_mm8_n<64, true>()) != cudaSuccess) return e;
+    if ((e = configure_mm8_n<64, false>()) != cudaSuccess) return e;
     if ((e = configure_pair_n<128>()) != cudaSuccess) return e;
-    return configure_pair_n<256>();
+    if ((e = configure_pair_n<256>()) != cudaSuccess) return e;
+    // clusters of 2, 4 and 8 that run at once with an SM for each CTA
+    static_assert(Mm8Cfg<64>::kPerSm == 1, "");
+    for (int i = 0; i < 3; ++i) {
+        Mm8Launch l(2 << i, 2 << i, Mm8Cfg<64>::kSmem, kMmThreads, nullptr);
+        e = cudaOccupancyMaxActiveClusters(&ctx->mm8_clusters[i], mm8_kernel<64, true, float>, &l.cfg);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
-// Few rows of a become the MMA's columns (swap).  Otherwise, and where whole
-// tiles leave SMs idle, a tile's blocks of k go to several CTAs, one CTA per
-// SM at most (measured at 16 x 8192 x 4096: 12.9 us with 128 CTAs, 18.2 with
-// 64, 17.2 with 256) and at least 8 blocks for each of 8 (a cluster of 8 costs
-// 4 us more than one of 4).  Products with more tiles than that run on pairs of
-// CTAs, whose tile is the one with the shorter estimate: waves of pairs times
-// the measured time of a block of k, plus the start and end of a tile.
+// Few rows of a become the MMA's columns (swap).  Where whole tiles leave SMs
+// idle, a tile's blocks of k go to a cluster of CTAs, at least 4 blocks each
+// (64 x 4096 x 1024: 8.0 us with 8 blocks each, 7.5 with 4, 8.2 with 2; 16 x
+// 1024 x 4096: 8.2 with 16, 6.9 with 8, 6.7 with 4), while each CTA still has an
+// SM of its own (16 x 8192 x 4096: 11.0 us with 64 CTAs, 8.3 with 128, 13.2 with
+// 256; 16 x 2048 x 8192: 8.9 in clusters of 4, 14.0 in 16 clusters of 8, which
+// the GPCs do not hold at once).  Products with more tiles than SMs run on pairs
+// of CTAs, on the tile with the shorter estimate: waves of pairs times the
+// measured time of a block of k, plus the start and end of a tile (128 wide
+// where 256 leaves pairs idle, 512 x 4096 x 4096: 15.5 us against 21.1; else 256,
+// 8192 x 8192 x 4096: 260 against 304).
 Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
     Mm8Plan pl{};
     pl.swap = d.m <= 64;
@@ -742,8 +749,7 @@ Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
     const int64_t tiles = (int64_t)tiles_of(pl.swap ? d.n : d.m, kRows) * tiles_of(pl.swap ? d.m : d.n, pl.bn);
     const int kb = tiles_of(d.k, kBk);
     pl.splits = 1;
-    while (pl.splits < 8 && tiles * pl.splits * 2 <= ctx->n_sm && kb >= (pl.splits == 4 ? 64 : 4 * pl.splits))
-        pl.splits *= 2;
+    for (int i = 0; i < 3 && tiles <= ctx->mm8_clusters[i] && kb >= 4 << (i + 1); ++i) pl.splits = 2 << i;
     if (pl.swap || tiles <= ctx->n_sm) return pl;
     const bool rows = d.b_form == HELIX_SCALE_ROWS;
     auto estimate = [&](int bn, double block, double tile) {
@@ -751,8 +757,8 @@ Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
         const int64_t waves = (n + ctx->n_sm / 2 - 1) / (ctx->n_sm / 2);
         return (double)waves * (block * kb + tile);  // us
     };
-    const double wide = rows ? estimate(256, 0.91, 4.0) : estimate(256, 0.57, 2.5);
-    const double narrow = rows ? estimate(128, 0.55, 3.0) : estimate(128, 0.335, 3.5);
+    const double wide = rows ? estimate(256, 0.82, 3.9) : estimate(256, 0.49, 2.9);
+    const double narrow = rows ? estimate(128, 0.52, 1.8) : estimate(128, 0.29, 1.6);
     pl.pair = true;
     pl.bn = wide <= narrow ? 256 : 128;
     return pl;
@@ -770,7 +776,8 @@ int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan&
         p.tiles_q = tiles_of(d.n, pl.bn);
         const int64_t tiles = (int64_t)tiles_of(d.m, 2 * kRows) * p.tiles_q;
         // a pair counts its blocks of k in 32 bits
-        if (tiles > INT32_MAX / 2 || (tiles / (ctx->n_sm / 2) + 1) * p.k_blocks > INT32_MAX) return cudaErrorInvalidValue;
+        if (tiles > INT32_MAX / 2 || (tiles / (ctx->n_sm / 2) + 1) * p.k_blocks > INT32_MAX)
+            return cudaErrorInvalidValue;
         const int ctas = 2 * (int)std::min<int64_t>(tiles, ctx->n_sm / 2);
         return pl.bn == 256 ? launch_pair_n<256>(p.q.per == 1, d.out_dtype, maps, p, ctas, stream)
                             : launch_pair_n<128>(p.q.per == 1, d.out_dtype, maps, p, ctas, stream);
@@ -785,12 +792,11 @@ int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan&
     p.tiles_q = tiles_of(p.q.rows, pl.bn);
     const int64_t tiles = (int64_t)tiles_of(p.p.rows, kRows) * p.tiles_q;
     if (tiles * p.splits > INT32_MAX) return cudaErrorInvalidValue;
-    const bool qrows = p.q.per == 1;
-    switch (pl.bn) {
-        case 16: return launch_mm8_n<16>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
-        case 32: return launch_mm8_n<32>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
-        default: return launch_mm8_n<64>(qrows, d.out_dtype, maps, p, (int)tiles, stream);
-    }
+    // narrow tiles have rows of a for columns, each with its own scales
+    if (pl.bn == 16) return launch_mm8_n<16, true>(d.out_dtype, maps, p, (int)tiles, stream);
+    if (pl.bn == 32) return launch_mm8_n<32, true>(d.out_dtype, maps, p, (int)tiles, stream);
+    return p.q.per == 1 ? launch_mm8_n<64, true>(d.out_dtype, maps, p, (int)tiles, stream)
+                        : launch_mm8_n<64, false>(d.out_dtype, maps, p, (int)tiles, stream);
 }
 
 }  // namespace hx

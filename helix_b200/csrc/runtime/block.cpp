@@ -254,7 +254,8 @@ extern "C" helix_status helix_rms_norm_grad_encode(helix_ctx* ctx, void* stream,
         p.n_row = n;
         p.n_col = d->n_col;
         p.w_bf16 = d->w_dtype == HELIX_BF16;
-        p.ld_dout = d->ld_dout, p.ld_sum = d->ld_sum, p.ld_dsum = d->ld_dsum, p.ld_dx = d->ld_dx, p.ld_dres = d->ld_dres;
+        p.ld_dout = d->ld_dout, p.ld_sum = d->ld_sum, p.ld_dsum = d->ld_dsum;
+        p.ld_dx = d->ld_dx, p.ld_dres = d->ld_dres;
         p.dout = ptr(dout), p.sum = ptr(sum), p.dsum = ptr(dsum), p.w = ptr(weight);
         p.dx = ptr(dx), p.dres = ptr(dres), p.rstd = ptr<float>(rstd);
         p.partial = ptr<float>(scratch);

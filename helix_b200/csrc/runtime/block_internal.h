@@ -78,7 +78,7 @@ struct Mm8Params {
     unsigned*  fault;
 };
 Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d);
-int configure_mm8();
+int configure_mm8(helix_ctx* ctx);    // fills ctx->mm8_clusters
 // a, b: operands as the caller laid them out.
 int launch_mm8(const helix_ctx* ctx, const helix_matmul8_desc& d, const Mm8Plan& pl, Mm8Params p, const void* a,
                const void* b, void* stream);

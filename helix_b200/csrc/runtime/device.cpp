@@ -100,7 +100,8 @@ extern "C" helix_status helix_ctx_create(helix_ctx** out, void* device, const ch
     {
         DeviceGuard g(dev);
         if (hx::configure_simt(ctx) != cudaSuccess || hx::configure_diag(ctx) != cudaSuccess ||
-            hx::configure_norm() != cudaSuccess || hx::configure_mm8() != cudaSuccess || hx::configure_gated(ctx) != cudaSuccess) {
+            hx::configure_norm() != cudaSuccess || hx::configure_mm8(ctx) != cudaSuccess ||
+            hx::configure_gated(ctx) != cudaSuccess) {
             hx::set_error(nullptr, std::string("configuring kernels failed: ") +
                                        cudaGetErrorString(cudaGetLastError()));
             delete ctx;

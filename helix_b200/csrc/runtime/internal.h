@@ -160,9 +160,9 @@ struct helix_ctx {
     bool   tc_ready    = false;   // tensor-core kernels configured
     unsigned* fault_word = nullptr; // device address of the fault word
     void*  encode_tiled = nullptr; // cuTensorMapEncodeTiled entry point
-    // Gated recurrence: clusters of 1, 2, 4, 8 CTAs the device holds at once,
-    // two CTAs per SM and (deep) one.
-    int    gated_clusters[4] = {}, gated_deep[4] = {};
+    // Clusters the device holds at once: of 1, 2, 4, 8 CTAs of the gated
+    // recurrence, two per SM; of 2, 4, 8 CTAs of the 8-bit product, one per SM.
+    int    gated_clusters[4] = {}, mm8_clusters[3] = {};
 };
 
 namespace hx {
