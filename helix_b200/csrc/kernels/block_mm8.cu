@@ -72,6 +72,19 @@ struct Ring {
     }
 };
 
+// Whether the phase is over, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // The first n of v: consecutive columns qc.. of row pr of P.
 template <typename T>
 __device__ __forceinline__ void st_out(const Mm8Params& a, int pr, int qc, int n, const float (&v)[8]) {
@@ -310,6 +323,21 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
 // stages and TMEM buffers, and the next tile's MMAs run while the epilogue
 // writes.  An epilogue warp has 32 rows and half of the columns; it stages its
 // part in shared memory of its own and stores it by TMA.
+//
+// Where b's scales go by blocks of 128, an accumulator of one row per lane needs
+// one scale per block of k.  Where they go by rows every column has its own:
+// with a row per lane, a lane would read all of them from shared memory (64
+// 8-byte reads per block of k); with the fragments of 16 lanes x 8 columns it has
+// 4 rows, and a quarter of the columns.  There the epilogue is also what the
+// MMAs wait for (two multiply-adds a value and block, not one), so a block's
+// first TMEM read is issued before the last block's sums are done, if its MMAs
+// are (8192 x 8192 x 4096 to f32: 414 -> 376 us; by blocks, where the epilogue
+// waits for the MMAs, 264 -> 278, so not there).
+//
+// Measured: 8192 x 8192 x 4096 bf16 258 us, 2.1 PFLOP/s, 64 % of twice the
+// measured bf16 rate; by rows to f32 352 us.  Bound by the tensor core and the
+// hand-offs between it and the epilogue (a block's sum has to leave TMEM before
+// its buffer is free, and there are two), by rows by the epilogue's arithmetic.
 // ---------------------------------------------------------------------------
 // Warp 0 issues the loads, 1 and 2 the MMAs of every other block of k (a
 // block's waits, four MMAs and commits take one thread 750 cycles, three times
@@ -320,15 +348,17 @@ __global__ void __launch_bounds__(kMmThreads, Mm8Cfg<BN>::kPerSm) mm8_kernel(con
 // is launched with.
 constexpr int kPairThreads = 32 * (4 + kEpiWarps);
 
-template <int BN>
+template <int BN, bool QROWS>
 struct PairCfg {
     static constexpr int kStageBytes = (kRows + BN / 2) * kBk;   // per CTA
     static constexpr int kStages = BN == 256 ? 5 : 6;
+    static constexpr int kOuts = QROWS ? 1 : 2;                  // stagings of an epilogue warp
     static constexpr int kBufs = 512 / BN;
     static constexpr int kRun = BN / 2;                          // columns of an epilogue warp
     static constexpr int kPiece = 8;                             // blocks of k whose scales are staged at once
-    static constexpr int kOutBytes = 32 * 128;                   // staging of an epilogue warp
-    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpiWarps * kOutBytes + 1024;
+    static_assert(kPiece == 8, "two quads");
+    static constexpr int kOutBytes = 32 * 128;                   // of one
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kEpiWarps * kOuts * kOutBytes + 1024;
 };
 
 struct PairMaps {
@@ -348,7 +378,7 @@ __device__ __forceinline__ void pair_tile(int tile, int tiles_p, int tiles_q, in
 template <int BN, bool QROWS, typename T>
 __global__ void __launch_bounds__(kPairThreads, 1)
     mm8_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Mm8Params a) {
-    using Cfg = PairCfg<BN>;
+    using Cfg = PairCfg<BN, QROWS>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = tc::align1024(smem_raw);
     __shared__ uint64_t full[Cfg::kStages], empty[Cfg::kStages], acc_full[Cfg::kBufs], acc_empty[Cfg::kBufs], drain[2];
@@ -462,18 +492,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 for (int kb = 0; kb < nkb; kb += Cfg::kPiece, ++done) {
                     if (done >= 2 && !(ok = __all_sync(0xffffffffu, wait(&sc_empty[sc.at], sc.parity ^ 1u)))) break;
                     auto stage = [&](const Mm8Operand& o, int row, float* to, int pitch) {
-                        const float* from = o.scale + (int64_t)(min(row, o.rows - 1) / o.per) * o.ld_scale;
+                        const float* from = o.scale + (int64_t)(min(row, o.rows - 1) / o.per) * o.ld_scale + kb;
                         float v[Cfg::kPiece];
+                        if (o.quads) {  // a piece of 4 is read if it holds a block that exists
+                            const float4 lo = __ldg(reinterpret_cast<const float4*>(from));
+                            const float4 up = __ldg(reinterpret_cast<const float4*>(from) + (kb + 4 < nkb));
+                            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+                            v[4] = up.x, v[5] = up.y, v[6] = up.z, v[7] = up.w;
+                        } else {
 #pragma unroll
-                        for (int g = 0; g < Cfg::kPiece; ++g) v[g] = __ldg(from + min(kb + g, nkb - 1));
+                            for (int g = 0; g < Cfg::kPiece; ++g) v[g] = __ldg(from + min(g, nkb - 1 - kb));
+                        }
 #pragma unroll
                         for (int g = 0; g < Cfg::kPiece; ++g) to[g * pitch] = v[g];
                     };
-#pragma unroll 2
-                    for (int j = lane; j < kRows; j += 32)
-                        stage(a.p, (2 * tp + rank) * kRows + j, &row_scale[sc.at][0][j], kRows);
-#pragma unroll 2
-                    for (int j = lane; j < BN; j += 32) stage(a.q, tq * BN + j, &col_scale[sc.at][0][j], BN);
+#pragma unroll
+                    for (int j = 0; j < kRows; j += 32)
+                        stage(a.p, (2 * tp + rank) * kRows + j + lane, &row_scale[sc.at][0][j + lane], kRows);
+#pragma unroll 4
+                    for (int j = 0; j < BN; j += 32)
+                        stage(a.q, tq * BN + j + lane, &col_scale[sc.at][0][j + lane], BN);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[sc.at]);
                     sc.next();
@@ -482,9 +520,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(QROWS ? 216 : 232));
-        const int row = 32 * (warp & 3) + lane;      // the TMEM lane
+        const int row = 32 * (warp & 3) + lane;      // of the tile
         const int c0 = (warp - 4) / 4 * Cfg::kRun;   // the warp's first column
-        const uint32_t staging = smem_u32(smem) + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
+        uint8_t* const staged = smem + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOuts * Cfg::kOutBytes;
+        int turn = 0;                                // of the stagings
         const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)c0;
         bool alive = true;  // once a wait has run out no other is waited for, and the rest is garbage
         Ring<Cfg::kBufs> buf;
@@ -505,47 +544,72 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             uint64_t acc[Cfg::kRun / 2];
 #pragma unroll
             for (int i = 0; i < Cfg::kRun / 2; ++i) acc[i] = 0;
+            // 32 columns are read while the 32 before are added up
+            uint32_t v[2][32];
+            auto ld = [&](int c, uint32_t(&to)[32]) {
+                if constexpr (QROWS)
+                    tmem_ld_frag(lane_addr + buf.at * BN + c, to);
+                else
+                    tmem_ld(lane_addr + buf.at * BN + c, to);
+            };
+            bool loading = false;  // the block's first columns are on their way
             for (int kb = 0; kb < nkb; ++kb) {
                 const int at = kb % Cfg::kPiece;
-                float r;
+                uint64_t r2[QROWS ? 4 : 1];
                 if constexpr (QROWS) {
                     if (at == 0 && alive) alive = __all_sync(0xffffffffu, wait(&sc_full[sc.at], sc.parity));
-                    r = row_scale[sc.at][at][row];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float r = row_scale[sc.at][at][32 * (warp & 3) + 8 * j + lane / 4];
+                        r2[j] = f2_of(r, r);
+                    }
                 } else {
-                    r = ps_next * qs_next;
+                    const float r = ps_next * qs_next;
+                    r2[0] = f2_of(r, r);
                     ps_next = ps_then;
                     ps_then = __ldg(ps + min(kb + 2, nkb - 1));
                     qs_next = qs_then;
                     qs_then = __ldg(qs + min(kb + 2, nkb - 1));
                 }
-                const uint64_t r2 = f2_of(r, r);
-                if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[buf.at], buf.parity));
-                tc_fence_after();
-                // 32 columns are read while the 32 before are added up
-                const uint32_t from = lane_addr + buf.at * BN;
-                uint32_t v[2][32];
-                tmem_ld(from, v[0]);
+                if (!loading) {
+                    if (alive) alive = __all_sync(0xffffffffu, wait(&acc_full[buf.at], buf.parity));
+                    tc_fence_after();
+                    ld(0, v[0]);
+                }
 #pragma unroll
                 for (int c = 0; c < Cfg::kRun; c += 32) {
                     uint32_t(&w)[32] = v[c / 32 & 1];
                     tmem_wait_ld(w);
                     if (c + 32 < Cfg::kRun) {
-                        tmem_ld(from + c + 32, v[(c / 32 & 1) ^ 1]);
+                        ld(c + 32, v[(c / 32 & 1) ^ 1]);
                     } else {  // all read
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[buf.at], 0));
+                        buf.next();
+                        loading = QROWS && kb + 1 < nkb && __all_sync(0xffffffffu, mbar_test(&acc_full[buf.at], buf.parity));
+                        if (loading) {
+                            tc_fence_after();
+                            ld(0, v[0]);
+                        }
+                    }
+                    uint64_t cs[QROWS ? 4 : 1];
+                    if constexpr (QROWS) {
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const float* at2 = &col_scale[sc.at][at][c0 + c + 8 * m + 2 * (lane & 3)];
+                            const float2 f = *reinterpret_cast<const float2*>(at2);
+                            cs[m] = f2_of(f.x, f.y);
+                        }
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const uint64_t d = f2_of(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
                         uint64_t& o = acc[c / 2 + e];
-                        if constexpr (QROWS) {
-                            const float2 cs = *reinterpret_cast<const float2*>(&col_scale[sc.at][at][c0 + c + 2 * e]);
-                            o = f2_fma(d, f2_mul(r2, f2_of(cs.x, cs.y)), o);
-                        } else {
-                            o = f2_fma(d, r2, o);
-                        }
+                        if constexpr (QROWS)
+                            o = f2_fma(d, f2_mul(r2[2 * (e / 8) + e % 2], cs[e / 2 % 4]), o);
+                        else
+                            o = f2_fma(d, r2[0], o);
                     }
                 }
                 if (QROWS && (at == Cfg::kPiece - 1 || kb == nkb - 1)) {
@@ -553,7 +617,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     if (lane == 0) mbar_arrive(&sc_empty[sc.at]);
                     sc.next();
                 }
-                buf.next();
             }
             // the warp's 32 rows: 128 bytes of each at a time through its
             // staging, then by TMA, or (out at any alignment) by the lanes
@@ -561,25 +624,47 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const int row0 = p0 + 32 * (warp & 3);
 #pragma unroll
             for (int c = 0; c < Cfg::kRun; c += kPer) {
-                bulk_wait_read0();  // (lane 0) the last store has read the staging
+                // (lane 0) the last store from this staging has read it
+                if constexpr (Cfg::kOuts == 2)
+                    bulk_wait_read1();
+                else
+                    bulk_wait_read0();
                 __syncwarp();
+                const uint8_t* mine = staged + turn * Cfg::kOutBytes;
+                const uint32_t staging = smem_u32(mine);
+                turn = (turn + 1) % Cfg::kOuts;
+                if constexpr (QROWS) {  // fragments
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {  // 16-byte units of the lane's row
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int e = 0; e < kPer / 2; ++e) {
+                        const int r = 16 * (e / 8 % 2) + 8 * (e % 2) + lane / 4;
+                        const int byte = (32 * (e / 16) + 8 * (e / 2 % 4) + 2 * (lane & 3)) * (int)sizeof(T);
+                        const uint32_t to = staging + sw128_off(r, byte / 16) + byte % 16;
                         float lo, up;
-                        if constexpr (sizeof(T) == 2) {
-                            f2_to(acc[c / 2 + 4 * u + e], lo, up);
-                            w[e] = bf16x2(lo, up);
-                        } else {
-                            f2_to(acc[c / 2 + 2 * u + e / 2], lo, up);
-                            w[e] = __float_as_uint(e & 1 ? up : lo);
-                        }
+                        f2_to(acc[c / 2 + e], lo, up);
+                        if constexpr (sizeof(T) == 2)
+                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(bf16x2(lo, up)) : "memory");
+                        else
+                            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(lo), "f"(up) : "memory");
                     }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + sw128_off(lane, u)),
-                                 "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                                 : "memory");
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {  // 16-byte units of the lane's row
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float lo, up;
+                            if constexpr (sizeof(T) == 2) {
+                                f2_to(acc[c / 2 + 4 * u + e], lo, up);
+                                w[e] = bf16x2(lo, up);
+                            } else {
+                                f2_to(acc[c / 2 + 2 * u + e / 2], lo, up);
+                                w[e] = __float_as_uint(e & 1 ? up : lo);
+                            }
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + sw128_off(lane, u)),
+                                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                     : "memory");
+                    }
                 }
                 const int col0 = q0 + c0 + c;
                 if (a.vec_out) {
@@ -591,7 +676,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     }
                 } else {
                     __syncwarp();
-                    const uint8_t* mine = smem + Cfg::kStages * Cfg::kStageBytes + (warp - 4) * Cfg::kOutBytes;
                     for (int r = 0; r < 32 && row0 + r < a.p.rows; ++r) {
                         T* o = static_cast<T*>(a.out) + (int64_t)(row0 + r) * a.ld_out + col0;
 #pragma unroll
@@ -633,7 +717,7 @@ struct Mm8Launch {
 
 template <int BN, bool QROWS, typename T>
 int launch_pair_t(const PairMaps& maps, const Mm8Params& p, int ctas, void* stream) {
-    Mm8Launch l(ctas, 2, PairCfg<BN>::kSmem, kPairThreads, stream);
+    Mm8Launch l(ctas, 2, PairCfg<BN, QROWS>::kSmem, kPairThreads, stream);
     return cudaLaunchKernelEx(&l.cfg, mm8_pair_kernel<BN, QROWS, T>, maps, p);
 }
 
@@ -646,13 +730,13 @@ int launch_pair_n(bool qrows, helix_dtype out, const PairMaps& maps, const Mm8Pa
                  : launch_pair_t<BN, false, __nv_bfloat16>(maps, p, ctas, stream);
 }
 
-template <int BN>
+template <int BN, bool QROWS>
 int configure_pair_n() {
-    const void* k[] = {(const void*)mm8_pair_kernel<BN, true, float>, (const void*)mm8_pair_kernel<BN, false, float>,
-                       (const void*)mm8_pair_kernel<BN, true, __nv_bfloat16>,
-                       (const void*)mm8_pair_kernel<BN, false, __nv_bfloat16>};
+    const void* k[] = {(const void*)mm8_pair_kernel<BN, QROWS, float>,
+                       (const void*)mm8_pair_kernel<BN, QROWS, __nv_bfloat16>};
     for (const void* f : k) {
-        const int e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairCfg<BN>::kSmem);
+        const int e =
+            cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairCfg<BN, QROWS>::kSmem);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -719,8 +803,10 @@ int configure_mm8(helix_ctx* ctx) {
     if ((e = configure_mm8_n<32, true>()) != cudaSuccess) return e;
     if ((e = configure_mm8_n<64, true>()) != cudaSuccess) return e;
     if ((e = configure_mm8_n<64, false>()) != cudaSuccess) return e;
-    if ((e = configure_pair_n<128>()) != cudaSuccess) return e;
-    if ((e = configure_pair_n<256>()) != cudaSuccess) return e;
+    if ((e = configure_pair_n<128, true>()) != cudaSuccess) return e;
+    if ((e = configure_pair_n<128, false>()) != cudaSuccess) return e;
+    if ((e = configure_pair_n<256, true>()) != cudaSuccess) return e;
+    if ((e = configure_pair_n<256, false>()) != cudaSuccess) return e;
     // clusters of 2, 4 and 8 that run at once with an SM for each CTA
     static_assert(Mm8Cfg<64>::kPerSm == 1, "");
     for (int i = 0; i < 3; ++i) {
@@ -741,7 +827,7 @@ int configure_mm8(helix_ctx* ctx) {
 // of CTAs, on the tile with the shorter estimate: waves of pairs times the
 // measured time of a block of k, plus the start and end of a tile (128 wide
 // where 256 leaves pairs idle, 512 x 4096 x 4096: 15.5 us against 21.1; else 256,
-// 8192 x 8192 x 4096: 260 against 304).
+// 8192 x 8192 x 4096: 258 against 304).
 Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
     Mm8Plan pl{};
     pl.swap = d.m <= 64;
@@ -757,8 +843,8 @@ Mm8Plan mm8_plan(const helix_ctx* ctx, const helix_matmul8_desc& d) {
         const int64_t waves = (n + ctx->n_sm / 2 - 1) / (ctx->n_sm / 2);
         return (double)waves * (block * kb + tile);  // us
     };
-    const double wide = rows ? estimate(256, 0.82, 3.9) : estimate(256, 0.49, 2.9);
-    const double narrow = rows ? estimate(128, 0.52, 1.8) : estimate(128, 0.29, 1.6);
+    const double wide = rows ? estimate(256, 0.65, 4.3) : estimate(256, 0.49, 2.6);
+    const double narrow = rows ? estimate(128, 0.45, 2.0) : estimate(128, 0.29, 1.7);
     pl.pair = true;
     pl.bn = wide <= narrow ? 256 : 128;
     return pl;

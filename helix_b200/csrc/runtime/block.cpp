@@ -361,8 +361,8 @@ extern "C" helix_status helix_matmul8_encode(helix_ctx* ctx, void* stream, const
         if (d->n > 1 && d->ld_b < d->k) invalid("b: row stride too small");
         const hx::Mm8Plan pl = hx::mm8_plan(ctx, *d);
         hx::Mm8Params p{};
-        const hx::Mm8Operand oa{ptr<float>(a_scale), d->ld_a_scale, d->m, 1};
-        const hx::Mm8Operand ob{ptr<float>(b_scale), d->ld_b_scale, d->n, blocks ? HELIX_GROUP : 1};
+        const hx::Mm8Operand oa{ptr<float>(a_scale), d->ld_a_scale, d->m, 1, whole(m[1], 16)};
+        const hx::Mm8Operand ob{ptr<float>(b_scale), d->ld_b_scale, d->n, blocks ? HELIX_GROUP : 1, whole(m[3], 16)};
         p.p = pl.swap ? ob : oa;
         p.q = pl.swap ? oa : ob;
         p.k_blocks = (int32_t)kb;

@@ -60,6 +60,7 @@ struct Mm8Operand {
     int64_t      ld_scale;
     int32_t      rows;
     int32_t      per;      // rows under one scale: 1 or 128
+    bool         quads;    // rows of scale can be read in 16-byte pieces
 };
 // How one product runs.
 struct Mm8Plan {
