@@ -21,7 +21,8 @@
 // arrive by TMA, steps ahead; two CTAs per SM fill each other's waits.  Tensors
 // that TMA cannot describe arrive row by row, by copies of the 16-byte pieces
 // that hold a row, and a lane reads its channels at the row's offset in them.
-// Folds go in the order of the tokens: results do not depend on timing.
+// Folds go in the order of the tokens: results do not depend on timing.  Chunks
+// wholly past a sequence's end are neither read nor walked, only blanked.
 //
 // The gradient walks the chunks from the end with c_t = f_t lam_t, the
 // gradient that leaves token t for h_{t-1}: lam_t = dy_t + c_{t+1}, c_t =
@@ -30,6 +31,15 @@
 //
 // Sequences of up to 16 tokens (a decoder's step) need none of this: a warp
 // walks its lanes' channels from global memory.
+//
+// Measured (bf16; bytes that have to move at the measured copy rate take 62,
+// 103, 123 and 205 us): 4 x 8192 x 2048 tokens x channels 76 us, its gradient
+// 135; 1 x 131072 x 1024 188 and 326, where the cluster's exchange in every step
+// shows; rows that TMA cannot describe (4 x 8192 x 2047) 143 and 286, bound by
+// the shared-memory reads at odd offsets and the halved stores; one token of 64
+// sequences x 4096 channels 2.0.  What is left in the first two is the gates'
+// exponential and reciprocal and the walks' dependent steps, two CTAs' worth
+// of them per SM.
 #include <cstring>
 #include <type_traits>
 
@@ -251,6 +261,14 @@ struct Place {
     }
 };
 
+// Zeros for the lane's channels of a run's tokens from t0 on.
+template <typename T, Access A>
+__device__ __forceinline__ void blank(T* row, int64_t s_tok, int t0, int n_tok, int n) {
+#pragma unroll
+    for (int i = 0; i < kTok; ++i)
+        if (n > 0 && t0 + i < n_tok) st_raw<T, A>(row + (t0 + i) * s_tok, n, 0u);
+}
+
 // The values of the warp's first and last run, where it has two.
 __device__ __forceinline__ float of_lane(float v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
 __device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
@@ -338,7 +356,7 @@ struct Walk {
     uint32_t           base;  // shared-memory address of the tiles
     uint64_t*          full;
     M*                 meet;
-    int                steps;
+    int                steps;  // that hold tokens before the sequence's end
     bool               alive = true;
     static constexpr int kFulls = A == kTma ? 1 : kWarps;  // barriers of a stage: a warp's rows are its own
 
@@ -487,9 +505,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
-    const int chunks = (p.n_tok + Cut<LW>::kTokens - 1) / Cut<LW>::kTokens;
-    Walk<T, A, 2, kStages, LW, M> walk{maps, p, at, align128(smem_raw), full, &meet, (chunks + R - 1) / R};
-    const int steps = walk.steps;
+    const int steps = ((at.len + Cut<LW>::kTokens - 1) / Cut<LW>::kTokens + R - 1) / R;
+    Walk<T, A, 2, kStages, LW, M> walk{maps, p, at, align128(smem_raw), full, &meet, steps};
     auto chunk_of = [&](int s) { return s * R + at.rank; };
     walk.begin();
     if constexpr (A != kTma) {
@@ -584,6 +601,12 @@ __global__ void __launch_bounds__(kThreads, 2)
             second(std::false_type{});
     }
     walk.end();
+    for (int k = chunk_of(steps); k * Cut<LW>::kTokens < p.n_tok; k += R) {  // past the sequence's end
+        const int t0 = k * Cut<LW>::kTokens + at.run * kTok;
+        blank<T, A>(static_cast<T*>(p.y) + (int64_t)at.seq * p.seq_y + at.c0, p.s_y, t0, p.n_tok, n);
+        if (p.states && t0 % kChunk == 0 && t0 < p.n_tok)
+            st_state<L>(p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0, n, h);
+    }
     // Every CTA holds the last state.  In place of h0 is safe: each has read
     // h0 before the cluster's last barrier.
     if (at.rank == 0 && warp == 0 && lane < LW) st_state<L>(p.h1 + (int64_t)at.seq * p.seq_h1 + at.c0, n, h);
@@ -601,9 +624,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
-    const int chunks = (p.n_tok + Cut<LW>::kTokens - 1) / Cut<LW>::kTokens;
-    Walk<T, A, 3, kStages, LW, M> walk{maps, p, at, align128(smem_raw), full, &meet, (chunks + R - 1) / R};
-    const int steps = walk.steps;
+    const int steps = ((at.len + Cut<LW>::kTokens - 1) / Cut<LW>::kTokens + R - 1) / R;
+    Walk<T, A, 3, kStages, LW, M> walk{maps, p, at, align128(smem_raw), full, &meet, steps};
     auto chunk_of = [&](int s) { return (steps - 1 - s) * R + at.rank; };  // from the end
     walk.begin();
     if constexpr (A != kTma) {
@@ -725,6 +747,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         __syncwarp();
     }
     walk.end();
+    for (int k = steps * R + at.rank; k * Cut<LW>::kTokens < p.n_tok; k += R) {  // past the sequence's end
+        const int t0 = k * Cut<LW>::kTokens + at.run * kTok;
+        blank<T, A>(static_cast<T*>(p.dg) + (int64_t)at.seq * p.seq_dg + at.c0, p.s_dg, t0, p.n_tok, n);
+        blank<T, A>(static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0, p.s_dv, t0, p.n_tok, n);
+    }
     if (p.dh0 && at.rank == 0 && warp == 0 && lane < LW) st_state<L>(p.dh0 + (int64_t)at.seq * p.seq_dh0 + at.c0, n, c);
 }
 
@@ -887,7 +914,8 @@ int launch_gated_a(const GatedMaps& maps, GatedParams p, const GatedCut& cut, bo
     const int64_t grid = groups * p.cluster;
     if (grad) {
         ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, kGradStages) : rows_smem(3, kGradRowStages), stream);
-        return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, A == kTma ? kGradStages : kGradRowStages, LW>, maps, p);
+        return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, A == kTma ? kGradStages : kGradRowStages, LW>, maps,
+                                  p);
     }
     ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, kFwdStages) : rows_smem(2, kRowStages), stream);
     return cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, A == kTma ? kFwdStages : kRowStages, LW>, maps, p);

@@ -481,7 +481,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             // Scales: a row's of kPiece blocks lie side by side, and are read
             // together while their sectors are in L1 (one block at a time for
             // all rows, each would come from L2 again: L1 has what the stages
-            // leave of it).
+            // leave of it), in two pieces of 16 bytes where rows are aligned
+            // to them (4096 x 4096 x 4096 by rows: 111 us, one by one 116).
             const int mine = pair < n_tiles ? (n_tiles - pair + pairs - 1) / pairs : 0;
             Ring<2> sc;
             int done = 0;
