@@ -97,6 +97,14 @@ def test_scan_lengths(cuda, t):
         _check(cuda, 7, T, 67, t, lengths=n)
 
 
+@pytest.mark.parametrize("form,Cn", [("dense", 64), ("odd", 67)])
+def test_scan_ends_early(cuda, form, Cn):
+    """Whole chunks, and whole turns of a cluster, past the ends."""
+    n = torch.tensor([4000, 0, 130, 2049, 3999, 1024], dtype=torch.int32)
+    _check(cuda, 6, 4000, Cn, BF, form, lengths=n)
+    _check(cuda, 2, 4000, Cn, F32, form, lengths=torch.tensor([5, 0], dtype=torch.int32))
+
+
 @pytest.mark.parametrize("mean,std", [(12.0, 1.0), (-12.0, 1.0), (0.0, 30.0), (60.0, 60.0)])
 def test_scan_gates(cuda, mean, std):
     """Gates that keep for tens of thousands of tokens, that forget at once,

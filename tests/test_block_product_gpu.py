@@ -92,6 +92,34 @@ def test_strides_and_leading_dimensions(cuda, m):
     ref.within(got.view(6, 90), want, mag * 21 * ref.U32 + want.abs() * ref.U32, "leading")
 
 
+@pytest.mark.parametrize("k,pitch", [(512, 4), (1536, 12), (700, 8), (700, 6), (700, 7), (1100, 12), (128, 4)])
+@pytest.mark.parametrize("m,n,out", [(2048, 1280, F32), (1100, 1281, BF)])
+def test_scale_strides(cuda, ctx, m, n, k, pitch, out):
+    """Scales by rows whose rows are whole pieces of 16 bytes, or not, NaN
+    between them: a piece's part past the last block counts for nothing."""
+    g = ref.generator(k + pitch)
+    a, sa = _operand(g, m, k, False)
+    b, sb = _operand(g, n, k, False)
+    want, mag = _want(a, sa, b, sb, False)
+    groups = -(-k // 128)
+    wide = []
+    for s in (sa, sb):
+        w = torch.full((s.shape[0], pitch), float("nan"), device=cuda)
+        w[:, :groups] = s.to(cuda)
+        wide.append(w)
+    d = abi.Matmul8Desc()
+    ctx.lib.helix_matmul8_desc_init(C.byref(d), m, n, k, abi.HELIX_SCALE_ROWS)
+    d.out_dtype = abi.HELIX_F32 if out == F32 else abi.HELIX_BF16
+    d.ld_a_scale = d.ld_b_scale = pitch
+    T = helix_b200._t
+    ag, bg = _padded(a.to(cuda)), _padded(b.to(cuda))
+    got = torch.empty(m, n, dtype=out, device=cuda)
+    st = ctx.lib.helix_matmul8_encode(ctx.handle, torch.cuda.current_stream().cuda_stream, C.byref(d), T(ag),
+                                      T(wide[0]), T(bg), T(wide[1]), T(got))
+    assert st == abi.HELIX_OK, ctx.last_error()
+    ref.within(got, want, mag * (19 + groups) * ref.U32 + want.abs() * ref.HALF[out], f"{m}x{n}x{k}")
+
+
 @pytest.mark.parametrize("m,swap_out", [(20, False), (300, False), (20, True), (300, True)])
 def test_output_strides(cuda, ctx, m, swap_out):
     """out as rows of a wider buffer at an odd offset: nothing beside it is touched."""
