@@ -23,6 +23,11 @@
 // memory, and every CTA adds up and writes a share of the columns, in the
 // order of the ranks.
 //
+// Measured (this kernel; that of large products below): 16 x 8192 x 4096 8.2 us,
+// 128 x 8192 x 4096 13.4; the weight's bytes take 5.2 at the measured copy rate.
+// The rest is the chain of one CTA's work: launch, first loads, the last block's
+// hand-offs and the meeting of the cluster, with 16 blocks of k in between.
+//
 // Every wait is bounded: one that runs out records kFaultProduct, the CTA
 // lets its copies and MMAs land, frees its TMEM and returns.
 #include <cooperative_groups.h>

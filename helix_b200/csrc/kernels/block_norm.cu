@@ -14,6 +14,12 @@
 //
 // Sums, statistics and the products are fp32; the only roundings are those
 // of the stored sum, the output and (8 bits) 1 / scale.
+//
+// Measured: 8192 x 4096 bf16 to 8 bits 45 us, 5.2 TB/s; 1537 x 2501 f32 10.9,
+// 5.6; 4096 x 16384 bf16 111; gradient of 16384 x 4096 bf16 113, 4.8 TB/s.  A
+// copy reaches 6.6 at sizes where a launch's start and end do not count.  What
+// the norm lacks is the wait of a row for its statistic, which the SM's other
+// rows cover in part; the gradient also reads the weights from L1 for each row.
 #include <algorithm>
 
 #include "block_common.cuh"

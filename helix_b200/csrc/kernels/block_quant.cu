@@ -7,6 +7,10 @@
 // turn into 8 bytes of each of 8 rows of the transposed output.  Transposed
 // tiles pass through shared memory (16 KB, 8-byte units swizzled so that
 // neither side has bank conflicts) to leave as whole 128-byte rows.
+//
+// Measured: 8192 x 4096 bf16 (15.4 us at the measured copy rate) by blocks 17.6
+// us, by rows 20, transposed by rows 22.6, where every tile waits at two barriers
+// for its columns' largest values; 8192 x 4095, rows at odd addresses, 28.
 #include "block_common.cuh"
 
 namespace hx {

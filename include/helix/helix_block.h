@@ -12,7 +12,9 @@
  * 8-bit tensors are e4m3 floats (HELIX_E4M3) with one fp32 scale for each
  * group of HELIX_GROUP: a value is (float)q * scale, and
  *     scale = max(largest magnitude of the group, 2^-100) / 448,
- *     q     = value / scale rounded to nearest even.
+ *     q     = value / scale rounded to nearest even,
+ * where scale is within 2 units in its last place of that, and the quotient,
+ * before it is rounded to 8 bits, within 4.
  * A group that holds a NaN or an infinity has that as its scale, and NaN (or
  * zero, for the finite values beside an infinity) as its q.
  */
