@@ -19,6 +19,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+// Largest of a >= 0 and two magnitudes, NaN as above.
+__device__ __forceinline__ float max_abs_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // The scale of a group whose largest magnitude is amax, and its reciprocal,
 // both within 2 ulp (an exact division takes as long as the rest of a group).
 // The floor keeps the reciprocal finite for a group of zeros; max.NaN lets a

@@ -156,11 +156,6 @@ void check_norm_desc(const helix_rms_norm_desc& d) {
     if (!(d.eps >= 0.0f)) invalid("eps must be >= 0");
 }
 
-// Whichever way the tensors are accessed.
-size_t norm_grad_scratch(helix_ctx* ctx, const helix_rms_norm_desc& d) {
-    return std::max(hx::norm_grad_plan(ctx, d, true).total, hx::norm_grad_plan(ctx, d, false).total);
-}
-
 }  // namespace
 
 extern "C" void helix_rms_norm_desc_init(helix_rms_norm_desc* d, int64_t n_row, int32_t n_col) {
@@ -200,6 +195,7 @@ extern "C" helix_status helix_rms_norm_encode(helix_ctx* ctx, void* stream, cons
         hx::NormParams p{};
         p.n_row = n;
         p.n_col = d->n_col;
+        p.inv_col = 1.0f / (float)d->n_col;
         const hx::NormShape s = hx::norm_shape(*d);
         p.wpr = s.wpr;
         p.rpb = s.rpb;
@@ -218,7 +214,7 @@ extern "C" helix_status helix_rms_norm_encode(helix_ctx* ctx, void* stream, cons
 
 extern "C" size_t helix_rms_norm_grad_scratch_size(helix_ctx* ctx, const helix_rms_norm_desc* d) {
     if (!d || d->n_row < 0 || d->n_col < 1 || d->n_col > 16384) return 0;
-    return norm_grad_scratch(ctx, *d);
+    return hx::norm_grad_plan(ctx, *d).total;
 }
 
 extern "C" helix_status helix_rms_norm_grad_encode(helix_ctx* ctx, void* stream, const helix_rms_norm_desc* d,
@@ -236,8 +232,8 @@ extern "C" helix_status helix_rms_norm_grad_encode(helix_ctx* ctx, void* stream,
             need(rstd, "rstd");
             need(dx, "dx");
         }
-        const size_t bytes = norm_grad_scratch(ctx, *d);
-        check_scratch(scratch, bytes, "helix_rms_norm_grad_scratch_size");
+        const hx::NormGradPlan pl = hx::norm_grad_plan(ctx, *d);
+        check_scratch(scratch, pl.total, "helix_rms_norm_grad_scratch_size");
         const int64_t n = d->n_row, c = d->n_col, ts = elem(d->sum_dtype), tx = elem(d->x_dtype);
         const Mat m[] = {{"dout", dout, n, c, d->ld_dout, tx, false},
                          {"sum", sum, n, c, d->ld_sum, ts, false},
@@ -247,12 +243,13 @@ extern "C" helix_status helix_rms_norm_grad_encode(helix_ctx* ctx, void* stream,
                          {"dx", dx, n, c, d->ld_dx, tx, true},
                          {"dres", dres, n, c, d->ld_dres, ts, true},
                          {"dweight", dweight, 1, c, c, 4, true},
-                         {"scratch", scratch, 1, (int64_t)bytes, (int64_t)bytes, 1, true}};
+                         {"scratch", scratch, 1, (int64_t)pl.total, (int64_t)pl.total, 1, true}};
         const int in_place[][2] = {{5, 0}, {6, 4}};
         check_mats(m, in_place);
         hx::NormParams p{};
         p.n_row = n;
         p.n_col = d->n_col;
+        p.inv_col = 1.0f / (float)d->n_col;
         p.w_bf16 = d->w_dtype == HELIX_BF16;
         p.ld_dout = d->ld_dout, p.ld_sum = d->ld_sum, p.ld_dsum = d->ld_dsum;
         p.ld_dx = d->ld_dx, p.ld_dres = d->ld_dres;
@@ -261,7 +258,6 @@ extern "C" helix_status helix_rms_norm_grad_encode(helix_ctx* ctx, void* stream,
         p.partial = ptr<float>(scratch);
         const bool vec = whole(m[0], 16) && whole(m[1], 16) && whole(m[3], 16) && whole(m[4], 16) &&
                          whole(m[5], 16) && whole(m[6], 16);
-        const hx::NormGradPlan pl = hx::norm_grad_plan(ctx, *d, vec);
         p.wpr = pl.shape.wpr;
         p.rpb = pl.shape.rpb;
         return hx::launch_norm_grad(*d, pl, p, vec, ptr<float>(dweight), stream);

@@ -26,12 +26,12 @@ struct NormGradPlan {
     int       slots;   // blocks * rpb
     size_t    total;   // scratch bytes: f32 [slots][n_col]
 };
-NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d, bool vec);
+NormGradPlan norm_grad_plan(const helix_ctx* ctx, const helix_rms_norm_desc& d);
 
 struct NormParams {
     int64_t     n_row;
     int32_t     n_col, wpr, rpb;
-    float       eps;
+    float       eps, inv_col;  // inv_col: 1 / n_col
     int32_t     out_dtype, w_bf16;
     int64_t     ld_x, ld_res, ld_sum, ld_out, ld_scale;
     int64_t     ld_dout, ld_dsum, ld_dx, ld_dres;

@@ -74,7 +74,7 @@ helix_status helix_rms_norm_encode(helix_ctx* ctx, void* stream, const helix_rms
  *     dweight = sum over rows of dout s rstd         (f32, [n_col])
  * dx (x_dtype) and, when not null, dres (sum_dtype) both receive ds.  dx may
  * be in place of dout, dres in place of dsum.  The sum over rows is taken in
- * an order that depends on the sizes, the alignment and the device alone.  Needs
+ * an order that depends on the sizes and the device alone.  Needs
  * helix_rms_norm_grad_scratch_size() bytes of 256-byte-aligned scratch. */
 size_t       helix_rms_norm_grad_scratch_size(helix_ctx* ctx, const helix_rms_norm_desc* d);
 helix_status helix_rms_norm_grad_encode(helix_ctx* ctx, void* stream, const helix_rms_norm_desc* d,
