@@ -301,7 +301,7 @@ __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Rows on their way to a gradient's warps, kStages of them: a tensor's segment
+// Rows on their way to a gradient's warps, kGradStages of them: a tensor's segment
 // of 256 columns in shared memory of the warp's own, which nobody else reads,
 // so no barrier.  Lanes copy consecutive 16-byte pieces: of the segment's whole
 // pieces with vector accesses (with 2-byte types those that a lane reads back
