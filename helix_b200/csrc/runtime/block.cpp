@@ -6,9 +6,7 @@
 
 #include <cuda_runtime.h>
 
-#include <algorithm>
 #include <climits>
-#include <cstdlib>
 #include <string>
 
 namespace {
