@@ -497,6 +497,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512, 1) norm_grad_kernel(const
             if (p.dres) st_seg<VEC>(static_cast<TR*>(p.dres) + row * p.ld_dres, c0, lane, n, o);
         }
     }
+    umma::grid_dep_launch();
     float* mine = p.partial + ((int64_t)blockIdx.x * p.rpb + rg) * p.n_col;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -512,16 +513,19 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512, 1) norm_grad_kernel(const
     }
 }
 
-// dweight[c] = the partials' sum in the order of the slots.
-constexpr int kDwRows = 16;
+// dweight[c] = the partials' sum in the order of the slots.  Its blocks may
+// start as the gradient's end (a programmatic dependent launch), and wait for
+// all of them.
+constexpr int kDwRows = 32;
 __global__ void __launch_bounds__(32 * kDwRows) norm_dw_kernel(const float* partial, int slots, int n_col,
                                                               float* dweight) {
     __shared__ float part[kDwRows][33];
     const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
+    umma::grid_dep_wait();
     float v = 0.0f;
     if (c < n_col)
-#pragma unroll 8
+#pragma unroll 10
         for (int s = r; s < slots; s += kDwRows) v += partial[(int64_t)s * n_col + c];
     part[r][lane] = v;
     __syncthreads();
@@ -626,8 +630,16 @@ int launch_norm_grad(const helix_rms_norm_desc& d, const NormGradPlan& pl, const
         const int e = launch_norm_any(d, p, pl.shape.v, grid, block, vec, true, stream);
         if (e != cudaSuccess) return e;
     }
-    return block_launch(norm_dw_kernel, dim3((unsigned)((d.n_col + 31) / 32)), dim3(32 * kDwRows), 0, stream,
-                        (const float*)p.partial, pl.slots, d.n_col, dweight);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute early{};
+    cfg.gridDim = dim3((unsigned)((d.n_col + 31) / 32));
+    cfg.blockDim = dim3(32 * kDwRows);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = pl.blocks > 0 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, norm_dw_kernel, (const float*)p.partial, pl.slots, d.n_col, dweight);
 }
 
 }  // namespace hx
