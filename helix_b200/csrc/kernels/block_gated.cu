@@ -58,8 +58,6 @@ constexpr int kWarps = kChunk / kTok;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
 constexpr int kTileBytes = kChunk * 128;  // 128 tokens x 128 bytes of channels
-constexpr int kSlot = 144;                // a copied row: 128 bytes at an offset of up to 15
-constexpr int kRowTile = kChunk * kSlot;  // copied rows of a tensor
 constexpr int kFewWarps = 8;              // of a CTA of the few-token kernels
 
 // How a kernel reaches the token tensors.
@@ -232,6 +230,11 @@ struct Cut {
     static constexpr int kTokens = kWarps * kRuns * kTok;    // of a CTA and step
     static constexpr int kRow = 4 * LW;                      // bytes
     static_assert(kTokens * kRow == kTileBytes, "tile");
+    // Copied rows: at an offset of up to 15 in a slot; the runs of a warp half
+    // the banks apart.
+    static constexpr int kSlot = kRow + 16;
+    static constexpr int kRun = kTok * kSlot + (LW == 16 ? 64 : 0);
+    static constexpr int kRowTile = kWarps * kRuns * kRun;
     // Word i of tensor k, from the lane's first word.
     static __host__ __device__ constexpr uint32_t word(int k, int i) { return (uint32_t)(k * kTileBytes + i * kRow); }
 };
@@ -305,11 +308,9 @@ __device__ __forceinline__ void st_async(uint32_t at, float v, uint32_t bar) {
                  "r"(__float_as_uint(v)), "r"(bar)
                  : "memory");
 }
-// Bytes of global memory, in whole 16s, to shared memory.
-__device__ __forceinline__ void bulk_load(uint32_t to, uintptr_t from, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
-                 "l"(from), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
+// Asynchronous copy of 16 bytes to shared memory.
+__device__ __forceinline__ void copy16(uint32_t to, uintptr_t from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
@@ -358,7 +359,6 @@ struct Walk {
     M*                 meet;
     int                steps;  // that hold tokens before the sequence's end
     bool               alive = true;
-    static constexpr int kFulls = A == kTma ? 1 : kWarps;  // barriers of a stage: a warp's rows are its own
 
     // Copied rows: tensor k's of the sequence, at the slab's first channel, and their pitch.
     const T* rows[A == kTma ? 1 : K];
@@ -366,8 +366,9 @@ struct Walk {
 
     // Tiles.  The lane's words of step s.
     __device__ __forceinline__ uint32_t mine(int s) const {
-        constexpr int kTile = A == kTma ? kTileBytes : kRowTile, kRow = A == kTma ? Cut<LW>::kRow : kSlot;
-        return base + (uint32_t)((s % kStages) * K * kTile + at.run * kTok * kRow + at.l * 4);
+        constexpr int kTile = A == kTma ? kTileBytes : Cut<LW>::kRowTile;
+        constexpr int kRun = A == kTma ? kTok * Cut<LW>::kRow : Cut<LW>::kRun;
+        return base + (uint32_t)((s % kStages) * K * kTile + at.run * kRun + at.l * 4);
     }
     // Offset in its 16-byte piece of the run's first row of a step's tensor,
     // and what a row adds to it.
@@ -382,73 +383,65 @@ struct Walk {
     // The lane's channels of token i of tensor k.
     __device__ __forceinline__ uint32_t get(uint32_t my, const Shift& sh, int k, int i) const {
         if (A == kTma) return lds(my + Cut<LW>::word(k, i));
-        const uint32_t a = my + (uint32_t)(k * kRowTile + i * kSlot) + ((sh.first + i * sh.step) & 15u);
+        const uint32_t a = my + (uint32_t)(k * Cut<LW>::kRowTile + i * Cut<LW>::kSlot) + ((sh.first + i * sh.step) & 15u);
         if (A == kWord) return lds(a);
         return lds_half(a) | lds_half(a + 2) << 16;
     }
     __device__ __forceinline__ bool issuer() const { return A == kTma && threadIdx.x == kThreads - 1; }
     // One thread: step s's tiles (chunk `chunk`) start to arrive.
     __device__ __forceinline__ void load(int s, int chunk) const {
-        uint64_t* bar = &full[s % kStages * kFulls];
+        uint64_t* bar = &full[s % kStages];
         mbar_expect_tx(bar, K * kTileBytes);
 #pragma unroll
         for (int k = 0; k < K; ++k)
             tma_load_3d(base + (uint32_t)(((s % kStages) * K + k) * kTileBytes), &maps.in[k], bar, at.slab0(),
                         chunk * Cut<LW>::kTokens, at.seq);
     }
-    // Every warp: step s's rows of its run start to arrive.  A copy takes the
-    // 16-byte pieces that hold the row's channels, each of which holds one
-    // that exists.
+    // Every warp: step s's rows of its runs (none past the last step) start to
+    // arrive, one group of copies: the 16-byte pieces that hold a row's
+    // channels, each of which holds one that exists.  A row's whole pieces go
+    // to as many lanes, the one that an offset adds to one lane per row.
     __device__ __forceinline__ void copy_rows(int s, int chunk) const {
         if constexpr (A != kTma) {
-            const int t0 = chunk * Cut<LW>::kTokens + at.run * kTok;
-            uint64_t* bar = &full[s % kStages * kFulls + at.warp];
-            const uint32_t to = base + (uint32_t)((s % kStages) * K * kRowTile + at.run * kTok * kSlot);
-            const uint32_t width = (uint32_t)min(LW * Lane<T>::kN, p.n_chan - at.slab0()) * (uint32_t)sizeof(T);
-            uint32_t size[(K + 1) / 2], total = 0;
-            uintptr_t from[(K + 1) / 2];
+            constexpr int kPieces = Cut<LW>::kRow / 16, kAtOnce = 32 / kPieces, kRows = Cut<LW>::kRuns * kTok;
+            if (s < steps) {
+                const int t0 = chunk * Cut<LW>::kTokens + at.warp * kRows;
+                const uint32_t to = base + (uint32_t)((s % kStages) * K * Cut<LW>::kRowTile + at.warp * Cut<LW>::kRuns * Cut<LW>::kRun);
+                const int width = min(LW * Lane<T>::kN, p.n_chan - at.slab0()) * (int)sizeof(T);
+                auto piece = [&](int k, const T* row, int r, int b) {  // the one at byte b of row r
+                    const uintptr_t a = reinterpret_cast<uintptr_t>(row);
+                    if (t0 + r < at.len && b < (int)(a & 15) + width)
+                        copy16(to + (uint32_t)(k * Cut<LW>::kRowTile + r / kTok * Cut<LW>::kRun + r % kTok * Cut<LW>::kSlot + b),
+                               (a & ~uintptr_t(15)) + b);
+                };
 #pragma unroll
-            for (int j = 0; j < (K + 1) / 2; ++j) {
-                const int k = 2 * j + (at.lane >> 4), i = at.lane & 15;
-                size[j] = 0;
-                from[j] = 0;
-                if (k < K && t0 + i < at.len) {
-                    const uintptr_t a = reinterpret_cast<uintptr_t>(pick(rows, k) + (t0 + i) * pick(pitch, k));
-                    from[j] = a & ~uintptr_t(15);
-                    size[j] = (uint32_t)(((a & 15) + width + 15) & ~uintptr_t(15));
+                for (int k = 0; k < K; ++k) {
+                    const T* row = rows[k] + (t0 + at.lane / kPieces) * pitch[k];
+#pragma unroll
+                    for (int r = 0; r < kRows; r += kAtOnce, row += kAtOnce * pitch[k])
+                        piece(k, row, r + at.lane / kPieces, at.lane % kPieces * 16);
+                    if (at.lane < kRows) piece(k, rows[k] + (t0 + at.lane) * pitch[k], at.lane, Cut<LW>::kRow);
                 }
-                total += size[j];
             }
-            total = __reduce_add_sync(0xffffffffu, total);
-            if (at.lane == 0) mbar_expect_tx(bar, total);
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < (K + 1) / 2; ++j)
-                if (size[j]) {
-                    const int k = 2 * j + (at.lane >> 4), i = at.lane & 15;
-                    bulk_load(to + (uint32_t)(k * kRowTile + i * kSlot), from[j], size[j], bar);
-                }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-    }
-    // An array's element k by selection (an index that is no constant would put
-    // the array into memory).
-    template <typename E>
-    static __device__ __forceinline__ E pick(const E* a, int k) {
-        return K == 3 && k == 2 ? a[K - 1] : k ? a[1] : a[0];
     }
     __device__ __forceinline__ void gave_up() {
         alive = false;
         if (p.fault) atomicCAS(p.fault, 0u, (unsigned)kFaultGated);
     }
     __device__ __forceinline__ void wait_tiles(int s) {
-        uint64_t* bar = &full[s % kStages * kFulls + (A == kTma ? 0 : at.warp)];
-        if (alive && !mbar_wait(bar, (uint32_t)((s / kStages) & 1), tc::kWaitBudget)) gave_up();
+        if (A == kTma) {
+            if (alive && !mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget)) gave_up();
+        } else {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        }
         __syncwarp();
     }
     __device__ __forceinline__ void begin() {
         if (threadIdx.x == kThreads - 1) {
 #pragma unroll
-            for (int k = 0; k < kStages * kFulls; ++k) mbar_init(&full[k], 1);
+            for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
             mbar_init(&meet->arrived[0], 1);
             mbar_init(&meet->arrived[1], 1);
             fence_mbar_init();
@@ -484,10 +477,10 @@ struct Walk {
     }
     __device__ __forceinline__ void end() {
         // whatever became of the other waits, the loads land
-        if (A == kTma ? issuer() : at.lane == 0)
+        if (issuer())
             for (int s = max(0, steps - kStages); s < steps; ++s)
-                mbar_wait(&full[s % kStages * kFulls + (A == kTma ? 0 : at.warp)], (uint32_t)((s / kStages) & 1),
-                          tc::kWaitBudget);
+                mbar_wait(&full[s % kStages], (uint32_t)((s / kStages) & 1), tc::kWaitBudget);
+        if (A != kTma) asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncwarp();
         if (p.cluster > 1) cluster_sync();  // no CTA leaves while another may store to it
     }
@@ -501,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     extern __shared__ uint8_t smem_raw[];
     using M = Meet<V, 2>;
     __shared__ M meet;
-    __shared__ uint64_t full[kStages * (A == kTma ? 1 : kWarps)];
+    __shared__ uint64_t full[kStages];
 
     const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
@@ -513,8 +506,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         walk.rows[0] = static_cast<const T*>(p.g) + (int64_t)at.seq * p.seq_g + at.slab0(), walk.pitch[0] = p.s_g;
         walk.rows[1] = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.slab0(), walk.pitch[1] = p.s_v;
     }
-    for (int s = 0; s < kStages && s < steps; ++s) {
-        if (walk.issuer()) walk.load(s, chunk_of(s));
+    for (int s = 0; s < kStages; ++s) {
+        if (walk.issuer() && s < steps) walk.load(s, chunk_of(s));
         walk.copy_rows(s, chunk_of(s));
     }
     __syncwarp();
@@ -542,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             first(std::true_type{});
         else
             first(std::false_type{});
-        if (A != kTma && s + kStages < steps) {  // the warp is done with its rows
+        if (A != kTma) {  // the warp is done with its rows
             __syncwarp();
             walk.copy_rows(s + kStages, chunk_of(s + kStages));
         }
@@ -620,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     extern __shared__ uint8_t smem_raw[];
     using M = Meet<V, 3, 1>;
     __shared__ M meet;
-    __shared__ uint64_t full[kStages * (A == kTma ? 1 : kWarps)];
+    __shared__ uint64_t full[kStages];
 
     const Place<T, LW> at(p);
     const int R = p.cluster, warp = at.warp, lane = at.lane, n = at.n;
@@ -633,8 +626,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         walk.rows[1] = static_cast<const T*>(p.v) + (int64_t)at.seq * p.seq_v + at.slab0(), walk.pitch[1] = p.s_v;
         walk.rows[2] = static_cast<const T*>(p.dy) + (int64_t)at.seq * p.seq_dy + at.slab0(), walk.pitch[2] = p.s_dy;
     }
-    for (int s = 0; s < kStages && s < steps; ++s) {
-        if (walk.issuer()) walk.load(s, chunk_of(s));
+    for (int s = 0; s < kStages; ++s) {
+        if (walk.issuer() && s < steps) walk.load(s, chunk_of(s));
         walk.copy_rows(s, chunk_of(s));
     }
     __syncwarp();
@@ -740,10 +733,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         else
             second(std::false_type{});
         __syncthreads();  // every warp is done with the tiles and the meeting
-        if (s + kStages < steps) {
-            if (walk.issuer()) walk.load(s + kStages, chunk_of(s + kStages));
-            walk.copy_rows(s + kStages, chunk_of(s + kStages));
-        }
+        if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
+        walk.copy_rows(s + kStages, chunk_of(s + kStages));
         __syncwarp();
     }
     walk.end();
@@ -826,7 +817,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 constexpr int kFwdStages = 3, kGradStages = 2;
 constexpr int kRowStages = 2, kGradRowStages = 1;
 constexpr size_t tiles_smem(int tensors, int stages) { return (size_t)stages * tensors * kTileBytes + 128; }
-constexpr size_t rows_smem(int tensors, int stages) { return (size_t)stages * tensors * kRowTile + 128; }
+template <int LW>
+constexpr size_t rows_smem(int tensors, int stages) { return (size_t)stages * tensors * Cut<LW>::kRowTile + 128; }
 
 // [n_seq][n_tok][n_chan] in boxes of row_bytes bytes of a tile's tokens; false when TMA
 // cannot describe it.  Rows and channels past the ends read as zero.
@@ -858,16 +850,16 @@ bool make_maps(const helix_ctx* ctx, GatedMaps* m, const GatedParams& p, bool gr
 // Lanes of a row and CTAs of a cluster: the choice with the fewest steps,
 // counting the waves that its clusters take, two CTAs per SM (large clusters
 // leave SMs of a GPC idle), and two steps to fill and drain each.  Narrow rows
-// (tiles only) serve few channels: 1 x 131072 x 1024 bf16 takes 193 us with
+// serve few channels: 1 x 131072 x 1024 bf16 takes 193 us with
 // them, 310 without.  Clusters of 8 take those 193 us, of 4 215, of 2 404, one
 // CTA 672; at 4 x 8192 x 2048 one takes 78 us, two 79, four 85, eight 99.
 struct GatedCut {
     int lanes = 32, cluster = 1;
 };
-GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels, bool tma) {
+GatedCut cut_of(const helix_ctx* ctx, const GatedParams& p, int lane_channels) {
     GatedCut best;
     int64_t least = INT64_MAX;
-    for (int lanes = 32; lanes >= (tma ? 16 : 32); lanes /= 2) {
+    for (int lanes = 32; lanes >= 16; lanes /= 2) {
         const int64_t cb = lanes * lane_channels, groups = (int64_t)p.n_seq * ((p.n_chan + cb - 1) / cb);
         const int64_t tokens = kChunk * (32 / lanes), chunks = (p.n_tok + tokens - 1) / tokens;
         for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
@@ -913,11 +905,11 @@ int launch_gated_a(const GatedMaps& maps, GatedParams p, const GatedCut& cut, bo
     p.cluster = cut.cluster;
     const int64_t grid = groups * p.cluster;
     if (grad) {
-        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, kGradStages) : rows_smem(3, kGradRowStages), stream);
+        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, kGradStages) : rows_smem<LW>(3, kGradRowStages), stream);
         return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, A == kTma ? kGradStages : kGradRowStages, LW>, maps,
                                   p);
     }
-    ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, kFwdStages) : rows_smem(2, kRowStages), stream);
+    ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(2, kFwdStages) : rows_smem<LW>(2, kRowStages), stream);
     return cudaLaunchKernelEx(&l.cfg, gated_kernel<T, A, A == kTma ? kFwdStages : kRowStages, LW>, maps, p);
 }
 
@@ -938,9 +930,9 @@ int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool g
             if (!word) return launch_gated_few<T, kHalf>(p, grad, stream);
         return launch_gated_few<T, kWord>(p, grad, stream);
     }
+    const GatedCut cut = cut_of(ctx, p, N);
     // outputs are stored a word at a time in the TMA form too
     if (word) {
-        const GatedCut cut = cut_of(ctx, p, N, true);
         GatedMaps maps;
         if (make_maps(ctx, &maps, p, grad, sizeof(T), 4 * cut.lanes))
             return cut.lanes == 16 ? launch_gated_a<T, kTma, 16>(maps, p, cut, grad, stream)
@@ -948,10 +940,12 @@ int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool g
     }
     GatedMaps none;
     std::memset(&none, 0, sizeof(none));
-    const GatedCut cut = cut_of(ctx, p, N, false);
     if constexpr (N == 2)
-        if (!word) return launch_gated_a<T, kHalf, 32>(none, p, cut, grad, stream);
-    return launch_gated_a<T, kWord, 32>(none, p, cut, grad, stream);
+        if (!word)
+            return cut.lanes == 16 ? launch_gated_a<T, kHalf, 16>(none, p, cut, grad, stream)
+                                   : launch_gated_a<T, kHalf, 32>(none, p, cut, grad, stream);
+    return cut.lanes == 16 ? launch_gated_a<T, kWord, 16>(none, p, cut, grad, stream)
+                           : launch_gated_a<T, kWord, 32>(none, p, cut, grad, stream);
 }
 
 int launch_gated_any(const helix_ctx* ctx, const helix_gated_scan_desc& d, const GatedParams& p, bool word, bool grad,
@@ -970,10 +964,10 @@ int configure_tiles() {
     const int e = set_smem(gated_kernel<T, kTma, kFwdStages, LW>, tiles_smem(2, kFwdStages));
     return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, kTma, kGradStages, LW>, tiles_smem(3, kGradStages));
 }
-template <typename T, Access A>
+template <typename T, Access A, int LW>
 int configure_rows() {
-    const int e = set_smem(gated_kernel<T, A, kRowStages, 32>, rows_smem(2, kRowStages));
-    return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, A, kGradRowStages, 32>, rows_smem(3, kGradRowStages));
+    const int e = set_smem(gated_kernel<T, A, kRowStages, LW>, rows_smem<LW>(2, kRowStages));
+    return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, A, kGradRowStages, LW>, rows_smem<LW>(3, kGradRowStages));
 }
 
 }  // namespace
@@ -984,9 +978,12 @@ int configure_gated(helix_ctx* ctx) {
     if ((e = configure_tiles<float, 16>()) != cudaSuccess) return e;
     if ((e = configure_tiles<__nv_bfloat16, 32>()) != cudaSuccess) return e;
     if ((e = configure_tiles<__nv_bfloat16, 16>()) != cudaSuccess) return e;
-    if ((e = configure_rows<float, kWord>()) != cudaSuccess) return e;
-    if ((e = configure_rows<__nv_bfloat16, kWord>()) != cudaSuccess) return e;
-    if ((e = configure_rows<__nv_bfloat16, kHalf>()) != cudaSuccess) return e;
+    if ((e = configure_rows<float, kWord, 32>()) != cudaSuccess) return e;
+    if ((e = configure_rows<float, kWord, 16>()) != cudaSuccess) return e;
+    if ((e = configure_rows<__nv_bfloat16, kWord, 32>()) != cudaSuccess) return e;
+    if ((e = configure_rows<__nv_bfloat16, kWord, 16>()) != cudaSuccess) return e;
+    if ((e = configure_rows<__nv_bfloat16, kHalf, 32>()) != cudaSuccess) return e;
+    if ((e = configure_rows<__nv_bfloat16, kHalf, 16>()) != cudaSuccess) return e;
     for (int i = 0, r = 1; r <= kMaxCluster; ++i, r *= 2) {
         ClusterLaunch l(r, r, tiles_smem(2, kFwdStages), nullptr);
         e = cudaOccupancyMaxActiveClusters(&ctx->gated_clusters[i], gated_kernel<__nv_bfloat16, kTma, kFwdStages, 32>,
