@@ -35,8 +35,9 @@
 // Measured (bf16; bytes that have to move at the measured copy rate take 62,
 // 103, 123 and 205 us): 4 x 8192 x 2048 tokens x channels 76 us, its gradient
 // 135; 1 x 131072 x 1024 188 and 326, where the cluster's exchange in every step
-// shows; rows that TMA cannot describe (4 x 8192 x 2047) 143 and 286, bound by
-// the shared-memory reads at odd offsets and the halved stores; one token of 64
+// shows; rows that TMA cannot describe (4 x 8192 x 2047) 136 and 275, bound by
+// the shared-memory reads at odd offsets and the halved stores (f32 there 166 and
+// 349); one token of 64
 // sequences x 4096 channels 2.0.  What is left in the first two is the gates'
 // exponential and reciprocal and the walks' dependent steps, two CTAs' worth
 // of them per SM.
@@ -383,7 +384,8 @@ struct Walk {
     // The lane's channels of token i of tensor k.
     __device__ __forceinline__ uint32_t get(uint32_t my, const Shift& sh, int k, int i) const {
         if (A == kTma) return lds(my + Cut<LW>::word(k, i));
-        const uint32_t a = my + (uint32_t)(k * Cut<LW>::kRowTile + i * Cut<LW>::kSlot) + ((sh.first + i * sh.step) & 15u);
+        const uint32_t off = (sh.first + i * sh.step) & 15u;
+        const uint32_t a = my + (uint32_t)(k * Cut<LW>::kRowTile + i * Cut<LW>::kSlot) + off;
         if (A == kWord) return lds(a);
         return lds_half(a) | lds_half(a + 2) << 16;
     }
@@ -406,12 +408,13 @@ struct Walk {
             constexpr int kPieces = Cut<LW>::kRow / 16, kAtOnce = 32 / kPieces, kRows = Cut<LW>::kRuns * kTok;
             if (s < steps) {
                 const int t0 = chunk * Cut<LW>::kTokens + at.warp * kRows;
-                const uint32_t to = base + (uint32_t)((s % kStages) * K * Cut<LW>::kRowTile + at.warp * Cut<LW>::kRuns * Cut<LW>::kRun);
+                const uint32_t to = mine(s) - (uint32_t)((at.run % Cut<LW>::kRuns) * Cut<LW>::kRun + at.l * 4);
                 const int width = min(LW * Lane<T>::kN, p.n_chan - at.slab0()) * (int)sizeof(T);
                 auto piece = [&](int k, const T* row, int r, int b) {  // the one at byte b of row r
                     const uintptr_t a = reinterpret_cast<uintptr_t>(row);
                     if (t0 + r < at.len && b < (int)(a & 15) + width)
-                        copy16(to + (uint32_t)(k * Cut<LW>::kRowTile + r / kTok * Cut<LW>::kRun + r % kTok * Cut<LW>::kSlot + b),
+                        copy16(to + (uint32_t)(k * Cut<LW>::kRowTile + r / kTok * Cut<LW>::kRun +
+                                               r % kTok * Cut<LW>::kSlot + b),
                                (a & ~uintptr_t(15)) + b);
                 };
 #pragma unroll
@@ -905,7 +908,8 @@ int launch_gated_a(const GatedMaps& maps, GatedParams p, const GatedCut& cut, bo
     p.cluster = cut.cluster;
     const int64_t grid = groups * p.cluster;
     if (grad) {
-        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, kGradStages) : rows_smem<LW>(3, kGradRowStages), stream);
+        ClusterLaunch l(grid, p.cluster, A == kTma ? tiles_smem(3, kGradStages) : rows_smem<LW>(3, kGradRowStages),
+                        stream);
         return cudaLaunchKernelEx(&l.cfg, gated_grad_kernel<T, A, A == kTma ? kGradStages : kGradRowStages, LW>, maps,
                                   p);
     }
@@ -922,6 +926,14 @@ int launch_gated_few(const GatedParams& p, bool grad, void* stream) {
                           : launch_few<T, A, kTok>(p, groups, grad, stream);
 }
 
+bool whole_lines(const GatedParams& p, bool grad, int64_t size) {
+    auto lines = [&](const void* at, int64_t s_tok, int64_t s_seq) {
+        return reinterpret_cast<uintptr_t>(at) % 128 == 0 && s_tok * size % 128 == 0 &&
+               (p.n_seq <= 1 || s_seq * size % 128 == 0);
+    };
+    return lines(p.v, p.s_v, p.seq_v) && lines(p.g, p.s_g, p.seq_g) && (!grad || lines(p.dy, p.s_dy, p.seq_dy));
+}
+
 template <typename T>
 int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool grad, void* stream) {
     constexpr int N = Lane<T>::kN;
@@ -931,8 +943,11 @@ int launch_gated_t(const helix_ctx* ctx, const GatedParams& p, bool word, bool g
         return launch_gated_few<T, kWord>(p, grad, stream);
     }
     const GatedCut cut = cut_of(ctx, p, N);
-    // outputs are stored a word at a time in the TMA form too
-    if (word) {
+    // Outputs are stored a word at a time in the TMA form too.  Rows of f32
+    // that do not start at lines of 128 bytes are read faster as rows (4 x 8192
+    // x 2040: 143 us against 203, gradient 306 against 358; bf16 118 against 93),
+    // unless the cut is narrow.
+    if (word && (N == 2 || cut.lanes == 16 || whole_lines(p, grad, sizeof(T)))) {
         GatedMaps maps;
         if (make_maps(ctx, &maps, p, grad, sizeof(T), 4 * cut.lanes))
             return cut.lanes == 16 ? launch_gated_a<T, kTma, 16>(maps, p, cut, grad, stream)
@@ -967,7 +982,8 @@ int configure_tiles() {
 template <typename T, Access A, int LW>
 int configure_rows() {
     const int e = set_smem(gated_kernel<T, A, kRowStages, LW>, rows_smem<LW>(2, kRowStages));
-    return e != cudaSuccess ? e : set_smem(gated_grad_kernel<T, A, kGradRowStages, LW>, rows_smem<LW>(3, kGradRowStages));
+    if (e != cudaSuccess) return e;
+    return set_smem(gated_grad_kernel<T, A, kGradRowStages, LW>, rows_smem<LW>(3, kGradRowStages));
 }
 
 }  // namespace
