@@ -19,7 +19,9 @@
 // issue slots before the arithmetic went in pairs (fp32 x 2) and the
 // gradient's rows came by asynchronous copies, its weights in registers.
 //
-// Measured: 8192 x 4096 bf16 to 8 bits 44.5 us, 5.3 TB/s; 1537 x 2501 f32 10.9,
+// Measured: 8192 x 4096 bf16 to bf16 43.5 us, 6.2 TB/s, to 8 bits, where a
+// group's maximum and scale come between the row's statistic and its output,
+// 44.4, 5.3; f32 82, 6.5; 1537 x 2501 f32 10.9,
 // 5.6; 8192 x 8192 bf16 88, 4096 x 16384 96; gradient of 16384 x 4096 bf16 88.5
 // us, 6.1 TB/s (a copy's rate is 6.55), of 8192 x 4096 f32 96, 5.6; of 8192 x
 // 4095, whose rows start anywhere, bf16 78, f32 98.
@@ -259,8 +261,8 @@ __device__ __forceinline__ void norm_row(const NormParams& p, int64_t row, bool 
     }
 }
 
-// 48 registers, so that five blocks fit an SM (8192 x 4096 bf16: 45 us, with
-// four 49).
+// 48 registers, so that five blocks fit an SM (8192 x 4096 bf16 to 8 bits: 44.4
+// us, with four 48.4; six spill, 8192 x 4096 f32: 82 -> 102).
 template <typename TX, typename TR, int V, bool VEC>
 __global__ void __launch_bounds__(256, 5) norm_kernel(const NormParams p) {
     __shared__ float part[8];
