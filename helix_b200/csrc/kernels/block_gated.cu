@@ -149,6 +149,39 @@ __device__ __forceinline__ void gate_slope(typename Lane<T>::V g, typename Lane<
     s = L::mul(tr, L::of(r));
 }
 
+// The smaller of f and z = 1 - f, which fixes both with full precision: -z
+// where g >= 0, f where it is negative.  In the sign, not in a comparison with
+// zero: a gate that is open for good has -0.
+template <typename T>
+__device__ __forceinline__ typename Lane<T>::V gate_small(typename Lane<T>::V g) {
+    using L = Lane<T>;
+    float x[L::kN], t[L::kN], r[L::kN];
+    L::to(g, x);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) {
+        t[e] = fmaf(-fabsf(x[e]), 1.4426950408889634f, 8.0f);
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t[e]));
+    }
+    const typename L::V tv = L::mul(L::of(t), L::splat(0x1p-8f));
+    L::to(L::add(tv, L::splat(1.0f)), r);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r[e]));
+    L::to(L::mul(tv, L::of(r)), t);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) t[e] = copysignf(t[e], -x[e]);
+    return L::of(t);
+}
+__device__ __forceinline__ bool opens(float w) { return __float_as_int(w) < 0; }
+// f x and z x; f h + z v; z f, with w from gate_small.  Each is as accurate as
+// w: where f is near 1 it is not rounded (over 1 / z steps that would add up),
+// and where it is small its digits are not lost in 1 - z.
+__device__ __forceinline__ float kept(float w, float x) { return fmaf(w, x, opens(w) ? x : 0.0f); }
+__device__ __forceinline__ float taken(float w, float x) { return opens(w) ? -w * x : fmaf(-w, x, x); }
+__device__ __forceinline__ float moved(float w, float h, float v) {
+    return fmaf(w, h - v, opens(w) ? h : v);
+}
+__device__ __forceinline__ float slope(float w) { return fmaf(-w, w, fabsf(w)); }
+
 // Packed arithmetic has no negation, so z and D are carried as -z and -D.
 // h - D h + B
 template <typename L>
@@ -766,50 +799,70 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
     const T* v = static_cast<const T*>(p.v) + (int64_t)seq * p.seq_v + c0;
     const T* dy = static_cast<const T*>(p.dy) + (int64_t)seq * p.seq_dy + c0;
 
-    V z[NT], q[GRAD ? NT : 1];
-    uint32_t vw[NT], yw[GRAD ? NT : 1];
+    V w[NT];
+    uint32_t gw[NT], vw[NT], yw[GRAD ? NT : 1];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         const bool live = i < len;
-        const uint32_t gw = live ? ld_raw<T, A>(g + i * p.s_g, n) : L::kInf;
+        gw[i] = live ? ld_raw<T, A>(g + i * p.s_g, n) : L::kInf;
         vw[i] = live ? ld_raw<T, A>(v + i * p.s_v, n) : 0u;
         if constexpr (GRAD) yw[i] = live ? ld_raw<T, A>(dy + i * p.s_dy, n) : 0u;
-        if constexpr (GRAD)
-            gate_slope<T>(L::unpack(gw), z[i], q[i]);
-        else
-            z[i] = gate<T>(L::unpack(gw));
     }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) w[i] = gate_small<T>(L::unpack(gw[i]));
+    // the lane's channels one by one
+    auto move = [](V w_, float (&h)[N], V v_) {
+        float x[N], y[N];
+        L::to(w_, x), L::to(v_, y);
+#pragma unroll
+        for (int e = 0; e < N; ++e) h[e] = moved(x[e], h[e], y[e]);
+    };
     if constexpr (!GRAD) {
         T* y = static_cast<T*>(p.y) + (int64_t)seq * p.seq_y + c0;
-        V h = ld_state<L>(p.h0 ? p.h0 + (int64_t)seq * p.seq_h0 + c0 : nullptr, n);
-        if (p.states && p.n_tok > 0) st_state<L>(p.states + (int64_t)seq * p.n_chan + c0, n, h);
+        float h[N];
+        L::to(ld_state<L>(p.h0 ? p.h0 + (int64_t)seq * p.seq_h0 + c0 : nullptr, n), h);
+        if (p.states && p.n_tok > 0) st_state<L>(p.states + (int64_t)seq * p.n_chan + c0, n, L::of(h));
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            if (i < len) h = step<L>(h, z[i], L::unpack(vw[i]));
-            if (i < p.n_tok) st_raw<T, A>(y + i * p.s_y, n, i < len ? L::pack(h) : 0u);
+        for (int i = 0; i < NT; ++i) {  // past the end z is 0
+            move(w[i], h, L::unpack(vw[i]));
+            vw[i] = i < len ? L::pack(L::of(h)) : 0u;
         }
-        st_state<L>(p.h1 + (int64_t)seq * p.seq_h1 + c0, n, h);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            if (i < p.n_tok) st_raw<T, A>(y + i * p.s_y, n, vw[i]);
+        st_state<L>(p.h1 + (int64_t)seq * p.seq_h1 + c0, n, L::of(h));
     } else {
         T* dg = static_cast<T*>(p.dg) + (int64_t)seq * p.seq_dg + c0;
         T* dv = static_cast<T*>(p.dv) + (int64_t)seq * p.seq_dv + c0;
-        V h = ld_state<L>(p.n_tok > 0 ? p.states + (int64_t)seq * p.n_chan + c0 : nullptr, n);
+        float h[N], c[N];
+        L::to(ld_state<L>(p.n_tok > 0 ? p.states + (int64_t)seq * p.n_chan + c0 : nullptr, n), h);
+        L::to(ld_state<L>(p.dh1 ? p.dh1 + (int64_t)seq * p.seq_dh1 + c0 : nullptr, n), c);
+        V q[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const V off = L::fma(L::unpack(vw[i]), L::splat(-1.0f), h);
-            q[i] = L::mul(q[i], off);
-            h = L::fma(z[i], off, h);
+            float x[N], v_[N];
+            L::to(w[i], x), L::to(L::unpack(vw[i]), v_);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = slope(x[e]) * (h[e] - v_[e]);
+            q[i] = L::of(x);
+            move(w[i], h, L::unpack(vw[i]));
         }
-        V c = ld_state<L>(p.dh1 ? p.dh1 + (int64_t)seq * p.seq_dh1 + c0 : nullptr, n);
 #pragma unroll
         for (int i = NT - 1; i >= 0; --i) {
             if (i >= p.n_tok) continue;
             const bool live = i < len;
-            const V lam = L::add(L::unpack(yw[i]), c);
-            st_raw<T, A>(dg + i * p.s_dg, n, live ? L::pack(L::mul(lam, q[i])) : 0u);
-            st_raw<T, A>(dv + i * p.s_dv, n, live ? L::pack_neg(L::mul(z[i], lam)) : 0u);
-            if (live) c = L::fma(z[i], lam, lam);
+            float x[N], y_[N], lam[N], take[N];
+            L::to(w[i], x), L::to(L::unpack(yw[i]), y_);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                lam[e] = y_[e] + c[e];
+                take[e] = taken(x[e], lam[e]);
+                c[e] = kept(x[e], lam[e]);
+            }
+            st_raw<T, A>(dg + i * p.s_dg, n, live ? L::pack(L::mul(L::of(lam), q[i])) : 0u);
+            st_raw<T, A>(dv + i * p.s_dv, n, live ? L::pack(L::of(take)) : 0u);
         }
-        if (p.dh0) st_state<L>(p.dh0 + (int64_t)seq * p.seq_dh0 + c0, n, c);
+        if (p.dh0) st_state<L>(p.dh0 + (int64_t)seq * p.seq_dh0 + c0, n, L::of(c));
     }
 }
 
