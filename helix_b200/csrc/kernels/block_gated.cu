@@ -3,21 +3,26 @@
 //
 //     h_t = f_t h_{t-1} + (1 - f_t) v_t,  f = 1 / (1 + e^-g)
 //
-// in terms of z = 1 - f alone: h += z (v - h).  f rounded to fp32 near 1
-// would be off by a fixed 2^-25 in every step, which a memory of 1 / z steps
-// multiplies; z is accurate to a few ulp however small it is.  Over a run of
-// tokens the state goes from h to h - D h + B, where B is the run's answer
-// from a zero state and D = 1 - prod(1 - z) its answer to v = 1 (the same
-// recurrence), so D is as accurate as z.
+// with both f and z = 1 - f to a few ulp of themselves (and of the exponent,
+// 2 |g| ulp).  Neither can stand for the other: z = 1 - f has lost its digits
+// where f is near 1, and f rounded there would be off by a fixed 2^-25 in every
+// step, which a memory of 1 / z steps multiplies; f = 1 - z has lost them where
+// f is small, and what should have vanished of a large state stays.
+//
+// Over a run of tokens the state goes from h to P h + B, where P = prod f and B
+// is the run's answer from a zero state; D = 1 - P is its answer to v = 1, so
+// accurate where it is small.  Runs are handed on as B and the smaller of P and
+// D, and folded as P h + B or h - D h + B: decays stay accurate relative to
+// themselves, and the rounding of P near 1 stays within 16 tokens.
 //
 // Bound by memory: every token is read once.  A CTA has 128 bytes of channels
 // (4 per lane: 2 bf16 channels, worked on as a pair, or 1 f32) of one chunk of
 // 128 tokens, a warp 16 consecutive tokens of it: one walk over them forms the
-// gates, which stay in registers, and (D, B); the warps' (D, B) meet in shared
-// memory, a CTA's totals go to the other CTAs of its cluster (as many
-// consecutive chunks of the same channels) by asynchronous stores that arrive
-// on an mbarrier, every CTA folds them onto the running state, and a second
-// walk writes the outputs.  Then the cluster moves on by its chunks.  Tiles
+// gates, and P and B up to every token, which stay in registers; the warps'
+// meet in shared memory, a CTA's totals go to the other CTAs of its cluster (as
+// many consecutive chunks of the same channels) by asynchronous stores that
+// arrive on an mbarrier, every CTA folds them onto the running state, and a
+// second walk writes the outputs.  Then the cluster moves on by its chunks.  Tiles
 // arrive by TMA, steps ahead; two CTAs per SM fill each other's waits.  Tensors
 // that TMA cannot describe arrive row by row, by copies of the 16-byte pieces
 // that hold a row, and a lane reads its channels at the row's offset in them.
@@ -25,20 +30,20 @@
 // wholly past a sequence's end are neither read nor walked, only blanked.
 //
 // The gradient walks the chunks from the end with c_t = f_t lam_t, the
-// gradient that leaves token t for h_{t-1}: lam_t = dy_t + c_{t+1}, c_t =
-// lam_t - z_t lam_t, so a run takes c to c - D c + E with the same D; h_{t-1}
-// is walked forward again from the chunk's stored state.
+// gradient that leaves token t for h_{t-1}: lam_t = dy_t + c_{t+1}, so a run
+// takes c to P c + E with the same P; h_{t-1} is walked forward again from the
+// chunk's stored state.
 //
 // Sequences of up to 16 tokens (a decoder's step) need none of this: a warp
 // walks its lanes' channels from global memory.
 //
 // Measured (bf16; bytes that have to move at the measured copy rate take 62,
-// 103, 123 and 205 us): 4 x 8192 x 2048 tokens x channels 76 us, its gradient
-// 135; 1 x 131072 x 1024 188 and 326, where the cluster's exchange in every step
-// shows; rows that TMA cannot describe (4 x 8192 x 2047) 136 and 275, bound by
-// the shared-memory reads at odd offsets and the halved stores (f32 there 166 and
-// 349); one token of 64
-// sequences x 4096 channels 2.0.  What is left in the first two is the gates'
+// 103, 123 and 205 us): 4 x 8192 x 2048 tokens x channels 78 us, its gradient
+// 137; 1 x 131072 x 1024 186 and 347, where the cluster's exchange in every step
+// shows; rows that TMA cannot describe (4 x 8192 x 2047) 131 and 241, bound by
+// the shared-memory reads at odd offsets and the halved stores (f32 there 165 and
+// 335); one token of 64
+// sequences x 4096 channels 2.2.  What is left in the first two is the gates'
 // exponential and reciprocal and the walks' dependent steps, two CTAs' worth
 // of them per SM.
 #include <cstring>
@@ -58,6 +63,10 @@ constexpr int kTok = 16;                  // tokens of a warp
 constexpr int kWarps = kChunk / kTok;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
+constexpr int kAhead = 4;                 // tokens of v that the gradient reads at once (an even number)
+// Warps that form a CTA's total and hand it to its cluster (1 x 131072 x 1024
+// bf16, gradient: 348 us with two, 352 with four, 379 with eight).
+constexpr int kSenders = 2;
 constexpr int kTileBytes = kChunk * 128;  // 128 tokens x 128 bytes of channels
 constexpr int kFewWarps = 8;              // of a CTA of the few-token kernels
 
@@ -79,7 +88,6 @@ struct Lane<float> {
     static __device__ __forceinline__ V mul(V a, V b) { return a * b; }
     static __device__ __forceinline__ V unpack(uint32_t w) { return __uint_as_float(w); }
     static __device__ __forceinline__ uint32_t pack(V v) { return __float_as_uint(v); }
-    static __device__ __forceinline__ uint32_t pack_neg(V v) { return __float_as_uint(-v); }
     static constexpr uint32_t kInf = 0x7f800000u;
 };
 template <>
@@ -98,106 +106,121 @@ struct Lane<__nv_bfloat16> {
         to(v, a);
         return bf16x2(a[0], a[1]);
     }
-    static __device__ __forceinline__ uint32_t pack_neg(V v) {
-        float a[2];
-        to(v, a);
-        return bf16x2(-a[0], -a[1]);
-    }
     static constexpr uint32_t kInf = 0x7f807f80u;
 };
 
-// z = 1 - sigmoid(g), accurate relative to z for every g down to subnormal z,
-// and +infinity gives exactly 0 (what tokens past the end are given).
-//
-// gate gives -z: with t = 2^-8 e^g, z = 2^-8 / (2^-8 + t).  The 2^-8 keeps the
-// reciprocal's result normal until z is below 2^-134, so that small z come
-// out as subnormals and not as zero.
+// f = sigmoid(g) and z = 1 - f, each to (12 + 2 |g|) 2^-24 of itself (the
+// exponent's rounding, the exponential, the reciprocal): with t = e^g, z = 1 /
+// (1 + t) and f = t z.  f is zero below 2^-126.  t stops at 2^126, where the
+// reciprocal is still normal: larger g have z = 2^-126 and f = 1 exactly, so
+// that +infinity with v = 0, which tokens past the end are given, leaves every
+// state as it is.
 template <typename T>
-__device__ __forceinline__ typename Lane<T>::V gate(typename Lane<T>::V g) {
+__device__ __forceinline__ void gate(typename Lane<T>::V g, typename Lane<T>::V& f, typename Lane<T>::V& z) {
     using L = Lane<T>;
-    float a[L::kN], r[L::kN];
-    L::to(L::fma(g, L::splat(1.4426950408889634f), L::splat(-8.0f)), a);
+    float t[L::kN], r[L::kN];
+    L::to(L::mul(g, L::splat(1.4426950408889634f)), t);
 #pragma unroll
-    for (int e = 0; e < L::kN; ++e) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a[e]));
-    L::to(L::add(L::of(a), L::splat(0x1p-8f)), r);
+    for (int e = 0; e < L::kN; ++e)
+        asm("ex2.approx.ftz.f32 %0, %0;\n\tmin.NaN.f32 %0, %0, 0f7e800000;" : "+f"(t[e]));
+    const typename L::V tv = L::of(t);
+    L::to(L::add(tv, L::splat(1.0f)), r);
 #pragma unroll
     for (int e = 0; e < L::kN; ++e) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r[e]));
-    return L::mul(L::of(r), L::splat(-0x1p-8f));
+    z = L::of(r);
+    f = L::mul(tv, z);
 }
-// -z with s = z (1 - z), which needs 1 - z just as accurate: t = e^-|g| (formed
-// as 2^8 t, for the same reason), r = 1 / (1 + t), sigmoid(|g|) = r,
-// sigmoid(-|g|) = t r.
+// The smaller one, m = t / (1 + t) with t = e^-|g| (formed as 2^8 t, for the
+// same reason), down to subnormal values on both sides.
 template <typename T>
-__device__ __forceinline__ void gate_slope(typename Lane<T>::V g, typename Lane<T>::V& z, typename Lane<T>::V& s) {
+__device__ __forceinline__ typename Lane<T>::V gate_min(const float (&g)[Lane<T>::kN]) {
     using L = Lane<T>;
-    float x[L::kN], t[L::kN], r[L::kN], zz[L::kN];
-    L::to(g, x);
+    float t[L::kN], r[L::kN];
 #pragma unroll
     for (int e = 0; e < L::kN; ++e) {
-        t[e] = fmaf(-fabsf(x[e]), 1.4426950408889634f, 8.0f);
+        t[e] = fmaf(-fabsf(g[e]), 1.4426950408889634f, 8.0f);
         asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t[e]));
     }
     const typename L::V tv = L::mul(L::of(t), L::splat(0x1p-8f));
     L::to(L::add(tv, L::splat(1.0f)), r);
 #pragma unroll
     for (int e = 0; e < L::kN; ++e) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r[e]));
-    const typename L::V tr = L::mul(tv, L::of(r));
-    L::to(tr, t);
-#pragma unroll
-    for (int e = 0; e < L::kN; ++e) zz[e] = x[e] >= 0.0f ? -t[e] : -r[e];
-    z = L::of(zz);
-    s = L::mul(tr, L::of(r));
+    return L::mul(tv, L::of(r));
 }
-
-// The smaller of f and z = 1 - f, which fixes both with full precision: -z
-// where g >= 0, f where it is negative.  In the sign, not in a comparison with
-// zero: a gate that is open for good has -0.
+// Both from it: the gradient's dg needs f z on that range.
 template <typename T>
-__device__ __forceinline__ typename Lane<T>::V gate_small(typename Lane<T>::V g) {
+__device__ __forceinline__ void gate_both(typename Lane<T>::V g, typename Lane<T>::V& f, typename Lane<T>::V& z) {
     using L = Lane<T>;
-    float x[L::kN], t[L::kN], r[L::kN];
+    float x[L::kN], m[L::kN], o[L::kN], a[L::kN], b[L::kN];
     L::to(g, x);
+    const typename L::V mv = gate_min<T>(x);
+    L::to(mv, m), L::to(L::fma(mv, L::splat(-1.0f), L::splat(1.0f)), o);
 #pragma unroll
     for (int e = 0; e < L::kN; ++e) {
-        t[e] = fmaf(-fabsf(x[e]), 1.4426950408889634f, 8.0f);
-        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t[e]));
+        a[e] = x[e] >= 0.0f ? o[e] : m[e];
+        b[e] = x[e] >= 0.0f ? m[e] : o[e];
     }
-    const typename L::V tv = L::mul(L::of(t), L::splat(0x1p-8f));
-    L::to(L::add(tv, L::splat(1.0f)), r);
-#pragma unroll
-    for (int e = 0; e < L::kN; ++e) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r[e]));
-    L::to(L::mul(tv, L::of(r)), t);
-#pragma unroll
-    for (int e = 0; e < L::kN; ++e) t[e] = copysignf(t[e], -x[e]);
-    return L::of(t);
+    f = L::of(a), z = L::of(b);
 }
-__device__ __forceinline__ bool opens(float w) { return __float_as_int(w) < 0; }
-// f x and z x; f h + z v; z f, with w from gate_small.  Each is as accurate as
-// w: where f is near 1 it is not rounded (over 1 / z steps that would add up),
-// and where it is small its digits are not lost in 1 - z.
-__device__ __forceinline__ float kept(float w, float x) { return fmaf(w, x, opens(w) ? x : 0.0f); }
-__device__ __forceinline__ float taken(float w, float x) { return opens(w) ? -w * x : fmaf(-w, x, x); }
-__device__ __forceinline__ float moved(float w, float h, float v) {
-    return fmaf(w, h - v, opens(w) ? h : v);
-}
-__device__ __forceinline__ float slope(float w) { return fmaf(-w, w, fabsf(w)); }
+// What is left of a state after a step, or a run of them, as one number: the
+// smaller of the decay P = prod f and D = 1 - P, which fixes both with full
+// precision: P itself, or -D.  In the sign, not in a comparison with zero: what
+// keeps all of a state is -0.
+__device__ __forceinline__ bool keeps(float c) { return __float_as_int(c) < 0; }
 
-// Packed arithmetic has no negation, so z and D are carried as -z and -D.
-// h - D h + B
-template <typename L>
-__device__ __forceinline__ typename L::V fold(typename L::V h, typename L::V nd, typename L::V b) {
-    return L::add(L::fma(nd, h, h), b);
+// Of a step.
+template <typename T>
+__device__ __forceinline__ typename Lane<T>::V gate_decay(typename Lane<T>::V g) {
+    using L = Lane<T>;
+    float x[L::kN], c[L::kN];
+    L::to(g, x);
+    L::to(gate_min<T>(x), c);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) c[e] = copysignf(c[e], -x[e]);
+    return L::of(c);
 }
-// a + z (v - a): a step of the recurrence
+// f x and z x; f h + z v; z f.  Where f is near 1 it is not rounded: over the
+// 1 / z steps of its memory that would add up.
+__device__ __forceinline__ float kept(float c, float x) { return fmaf(c, x, keeps(c) ? x : 0.0f); }
+__device__ __forceinline__ float taken(float c, float x) { return keeps(c) ? -c * x : fmaf(-c, x, x); }
+__device__ __forceinline__ float moved(float c, float h, float v) { return fmaf(c, h - v, keeps(c) ? h : v); }
+__device__ __forceinline__ float slope(float c) { return fmaf(-c, c, fabsf(c)); }
+
+// Of a run with P and D.  (Packed arithmetic has no negation and no absolute
+// value; single selects have both for nothing.)
 template <typename L>
-__device__ __forceinline__ typename L::V step(typename L::V a, typename L::V nz, typename L::V v) {
-    return L::fma(nz, L::fma(v, L::splat(-1.0f), a), a);
+__device__ __forceinline__ typename L::V decay_of(typename L::V p, typename L::V d) {
+    float a[L::kN], b[L::kN];
+    L::to(p, a), L::to(d, b);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) a[e] = a[e] > 0.5f ? -fabsf(b[e]) : a[e];
+    return L::of(a);
 }
-// -D after a step (or run) with -z: the step towards v = 1, negated
+// P h + b.
 template <typename L>
-__device__ __forceinline__ typename L::V grow(typename L::V nd, typename L::V nz) {
-    return L::fma(nz, L::add(nd, L::splat(1.0f)), nd);
+__device__ __forceinline__ typename L::V fold(typename L::V h, typename L::V c, typename L::V b) {
+    float x[L::kN], d[L::kN];
+    L::to(h, x), L::to(c, d);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) x[e] = keeps(d[e]) ? x[e] : 0.0f;
+    return L::add(L::fma(c, h, L::of(x)), b);
 }
+// P and -D of several runs, one after the other (D counts only where every
+// run keeps more than half, and there each has -D).
+template <typename L>
+struct Runs {
+    typename L::V p = L::splat(1.0f), nd = L::splat(0.0f), b = nd;
+    __device__ __forceinline__ void add(typename L::V c, typename L::V bc) {
+        float k[L::kN], d[L::kN];
+        L::to(L::add(c, L::splat(1.0f)), k), L::to(c, d);
+#pragma unroll
+        for (int e = 0; e < L::kN; ++e) k[e] = keeps(d[e]) ? k[e] : d[e];
+        p = L::mul(p, L::of(k));
+        nd = L::add(L::fma(nd, c, nd), c);
+        b = fold<L>(b, c, bc);
+    }
+    __device__ __forceinline__ typename L::V decay() const { return decay_of<L>(p, nd); }
+};
 
 // A lane's 4 bytes of a row; n: its channels that exist.
 template <typename T, Access A>
@@ -254,6 +277,10 @@ __device__ __forceinline__ uint32_t lds(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
     return v;
+}
+
+__device__ __forceinline__ void sts(uint32_t a, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 
 // How a CTA cuts its tile: rows of LW lanes' channels (32, or 16 to make twice
@@ -415,12 +442,74 @@ struct Walk {
                 (uint32_t)(pitch[k] * (int64_t)sizeof(T)) & 15u};
     }
     // The lane's channels of token i of tensor k.
-    __device__ __forceinline__ uint32_t get(uint32_t my, const Shift& sh, int k, int i) const {
-        if (A == kTma) return lds(my + Cut<LW>::word(k, i));
+    __device__ __forceinline__ uint32_t word_at(uint32_t my, const Shift& sh, int k, int i) const {
+        if (A == kTma) return my + Cut<LW>::word(k, i);
         const uint32_t off = (sh.first + i * sh.step) & 15u;
-        const uint32_t a = my + (uint32_t)(k * Cut<LW>::kRowTile + i * Cut<LW>::kSlot) + off;
-        if (A == kWord) return lds(a);
-        return lds_half(a) | lds_half(a + 2) << 16;
+        return my + (uint32_t)(k * Cut<LW>::kRowTile + i * Cut<LW>::kSlot) + off;
+    }
+    __device__ __forceinline__ uint32_t get(uint32_t my, const Shift& sh, int k, int i) const {
+        const uint32_t a = word_at(my, sh, k, i);
+        return A != kHalf ? lds(a) : lds_half(a) | lds_half(a + 2) << 16;
+    }
+    // The lane's tokens past the sequence's end become ones that leave every
+    // state as it is: g = +infinity, v = dy = 0.  (In the tiles, so that the
+    // walks have one form, whose registers need no merging.)
+    __device__ __forceinline__ void close(uint32_t my, int t0, const Shift& sg, const Shift& sv, const Shift& sdy) const {
+#pragma unroll 1
+        for (int i = max(0, at.len - t0); i < kTok; ++i) {
+            put(my, sg, 0, i, L::kInf);
+            put(my, sv, 1, i, 0u);
+            if (K > 2) put(my, sdy, 2, i, 0u);
+        }
+        if (A == kTma) fence_async_smem();
+    }
+    __device__ __forceinline__ void put(uint32_t my, const Shift& sh, int k, int i, uint32_t w) const {
+        const uint32_t a = word_at(my, sh, k, i);
+        if (A != kHalf) {
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(w) : "memory");
+        } else {
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((unsigned short)w) : "memory");
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(a + 2), "h"((unsigned short)(w >> 16)) : "memory");
+        }
+    }
+    // The gates of the lane's token i of step s, put aside where registers are
+    // short: into the words of the first two tensors' tiles that the lane has
+    // read, or beside copied rows, whose words may be at odd addresses.  Runs
+    // of narrow tiles lie on the same banks, so one of a warp's two takes tokens
+    // i ^ 1 (1 x 131072 x 1024 bf16: 366 -> 352 us).
+    __device__ __forceinline__ uint32_t gate_at(int s, int i) const {
+        if (A == kTma) {
+            const int turn = LW == 16 ? at.run & 1 : 0;
+            return mine(s) + Cut<LW>::word(0, i) + (i & 1 ? -turn : turn) * Cut<LW>::kRow;
+        }
+        return base + (uint32_t)(kStages * K * Cut<LW>::kRowTile +
+                                 ((at.run * kTok + i) * LW + at.l) * (int)sizeof(float) * L::kN);
+    }
+    __device__ __forceinline__ void put_gate(int s, int i, V f) const {
+        const uint32_t to = gate_at(s, i);
+        float a[L::kN];
+        L::to(f, a);
+        if constexpr (L::kN == 1) {
+            sts(to, a[0]);
+        } else if constexpr (A == kTma) {
+            sts(to, a[0]);
+            sts(to + kTileBytes, a[1]);
+        } else {
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(a[0]), "f"(a[1]) : "memory");
+        }
+    }
+    __device__ __forceinline__ V take_gate(int s, int i) const {
+        const uint32_t from = gate_at(s, i);
+        float a[L::kN];
+        if constexpr (L::kN == 1) {
+            a[0] = __uint_as_float(lds(from));
+        } else if constexpr (A == kTma) {
+            a[0] = __uint_as_float(lds(from));
+            a[1] = __uint_as_float(lds(from + kTileBytes));
+        } else {
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(a[0]), "=f"(a[1]) : "r"(from));
+        }
+        return L::of(a);
     }
     __device__ __forceinline__ bool issuer() const { return A == kTma && threadIdx.x == kThreads - 1; }
     // One thread: step s's tiles (chunk `chunk`) start to arrive.
@@ -485,15 +574,25 @@ struct Walk {
         __syncthreads();
         if (p.cluster > 1) cluster_sync();  // no CTA writes to another before that one's barriers stand
     }
-    // Hands the totals of step s to every CTA of the cluster.
-    __device__ __forceinline__ void send(int s, V d, V t) {
-        const int b = s & 1;
+    // The totals of step s, of warps whose values add() adds in the order of the
+    // walk, to every CTA of the cluster.  Formed and sent by the first warps
+    // of that order (nth: this one's place), which have the least to fold
+    // once the others' totals are there.
+    template <typename F>
+    __device__ __forceinline__ void send(int s, int nth, F add) {
+        const int b = s & 1, senders = min(p.cluster, kSenders);
         if (at.warp == 0 && at.lane == 0)
             mbar_expect_tx(&meet->arrived[b], (uint32_t)(p.cluster * 2 * 32 * sizeof(V)));
-        if (at.warp < p.cluster) {
-            const uint32_t bar = in_rank(&meet->arrived[b], at.warp);
-            st_async(in_rank(&meet->total[b][0][at.rank][at.lane], at.warp), d, bar);
-            st_async(in_rank(&meet->total[b][1][at.rank][at.lane], at.warp), t, bar);
+        if (nth < senders) {
+            Runs<L> all;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) add(all, w);
+            const V d = all.decay();
+            for (int r = nth; r < p.cluster; r += senders) {
+                const uint32_t bar = in_rank(&meet->arrived[b], r);
+                st_async(in_rank(&meet->total[b][0][at.rank][at.lane], r), d, bar);
+                st_async(in_rank(&meet->total[b][1][at.rank][at.lane], r), all.b, bar);
+            }
         }
     }
     __device__ __forceinline__ void receive(int s) {
@@ -553,52 +652,42 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int base = chunk_of(s) * Cut<LW>::kTokens, t0 = base + at.run * kTok, b = s & 1;
         const uint32_t my = walk.mine(s);
         const bool whole = at.whole(p, base);
-        // -D and B of the run up to each token: h_t = h - D h + B
-        V nd[kTok], hb[kTok], D = L::splat(0.0f), B = D;
+        // P and B of the run up to each token: h_t = P h + B
+        V ph[kTok], hb[kTok], P = L::splat(1.0f), D = L::splat(0.0f), B = D;
         const auto shift_g = walk.shift(0, t0), shift_v = walk.shift(1, t0);
         walk.wait_tiles(s);
-        auto first = [&](auto all) {
+        if (!whole) walk.close(my, t0, shift_g, shift_v, shift_g);
 #pragma unroll
-            for (int i = 0; i < kTok; ++i) {
-                uint32_t gw = walk.get(my, shift_g, 0, i), vw = walk.get(my, shift_v, 1, i);
-                if (!decltype(all)::value && t0 + i >= at.len) gw = L::kInf, vw = 0u;
-                const V z = gate<T>(L::unpack(gw));
-                nd[i] = D = grow<L>(D, z);
-                hb[i] = B = step<L>(B, z, L::unpack(vw));
-            }
-        };
-        if (whole)
-            first(std::true_type{});
-        else
-            first(std::false_type{});
+        for (int i = 0; i < kTok; ++i) {
+            V f, z;
+            gate<T>(L::unpack(walk.get(my, shift_g, 0, i)), f, z);
+            ph[i] = P = L::mul(P, f);
+            D = L::fma(f, D, z);
+            hb[i] = B = L::fma(f, B, L::mul(z, L::unpack(walk.get(my, shift_v, 1, i))));
+        }
         if (A != kTma) {  // the warp is done with its rows
             __syncwarp();
             walk.copy_rows(s + kStages, chunk_of(s + kStages));
         }
-        V d0 = D, b0 = B;  // the warp's first run
+        V c0 = decay_of<L>(P, D), b0 = B;  // the warp's first run
         if (LW == 16) {
-            const V d1 = of_lane(D, at.l + 16), b1 = of_lane(B, at.l + 16);
-            d0 = of_lane(D, at.l), b0 = of_lane(B, at.l);
-            D = grow<L>(d0, d1);
-            B = fold<L>(b0, d1, b1);
+            const V p0 = of_lane(P, at.l), p1 = of_lane(P, at.l + 16), d0 = of_lane(D, at.l),
+                    d1 = of_lane(D, at.l + 16), b1 = of_lane(B, at.l + 16);
+            c0 = decay_of<L>(p0, d0), b0 = of_lane(B, at.l);
+            P = L::mul(p0, p1);
+            D = L::fma(p0, d1, d0);
+            B = fold<L>(b0, decay_of<L>(p1, d1), b1);
         }
-        meet.warp[b][0][warp][lane] = D;
+        meet.warp[b][0][warp][lane] = LW == 16 ? decay_of<L>(P, D) : c0;
         meet.warp[b][1][warp][lane] = B;
         __syncthreads();  // and every warp is done with the tiles
         if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
         __syncwarp();
-        // what the CTA's earlier warps, and all of them, make of a state
-        V dp = L::splat(0.0f), bp = dp, d = dp, t = dp;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w == warp) dp = d, bp = t;
-            const V dw = meet.warp[b][0][w][lane];
-            t = fold<L>(t, dw, meet.warp[b][1][w][lane]);
-            d = grow<L>(d, dw);
-        }
         V hw = h;
         if (R > 1) {
-            walk.send(s, d, t);
+            walk.send(s, warp, [&](Runs<L>& all, int w) {
+                all.add(meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
+            });
             walk.receive(s);
             by_cluster(R, [&](auto size) {
 #pragma unroll
@@ -607,11 +696,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                     h = fold<L>(h, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
                 }
             });
+#pragma unroll
+            for (int w = 0; w < kWarps - 1; ++w)
+                if (w < warp) hw = fold<L>(hw, meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
         } else {
-            h = fold<L>(h, d, t);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (w == warp) hw = h;
+                h = fold<L>(h, meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
+            }
         }
-        hw = fold<L>(hw, dp, bp);
-        if (LW == 16 && lane >= 16) hw = fold<L>(hw, d0, b0);
+        if (LW == 16 && lane >= 16) hw = fold<L>(hw, c0, b0);
         if (p.states && t0 % kChunk == 0 && t0 < p.n_tok)
             st_state<L>(p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0, n, hw);
         T* y = static_cast<T*>(p.y) + (int64_t)at.seq * p.seq_y + at.c0 + (int64_t)t0 * p.s_y;
@@ -620,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int i = 0; i < kTok; ++i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
                 if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok))
-                    st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(fold<L>(hw, nd[i], hb[i])));
+                    st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(L::fma(ph[i], hw, hb[i])));
                 y += p.s_y;
             }
         };
@@ -677,97 +772,100 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int64_t chunk = (int64_t)at.seq * p.n_chunk + t0 / kChunk;
         ld_state<L>(t0 < p.n_tok ? p.states + chunk * p.n_chan + at.c0 : nullptr, n, entry);
         const auto shift_g = walk.shift(0, t0), shift_v = walk.shift(1, t0), shift_dy = walk.shift(2, t0);
-        V z[kTok], q[kTok], D = L::splat(0.0f), B = D, E = D;
+        V z[kTok], q[kTok], P = L::splat(1.0f), D = L::splat(0.0f), B = D, E = D;  // q: f, at first
         walk.wait_tiles(s);
-        auto first = [&](auto all) {
-            auto past = [&](int i) { return !decltype(all)::value && t0 + i >= at.len; };
+        if (!whole) walk.close(my, t0, shift_g, shift_v, shift_dy);
 #pragma unroll
-            for (int i = 0; i < kTok; ++i) {
-                const uint32_t gw = past(i) ? L::kInf : walk.get(my, shift_g, 0, i);
-                const uint32_t vw = past(i) ? 0u : walk.get(my, shift_v, 1, i);
-                gate_slope<T>(L::unpack(gw), z[i], q[i]);
-                D = grow<L>(D, z[i]);
-                B = step<L>(B, z[i], L::unpack(vw));
-            }
-#pragma unroll
-            for (int i = kTok - 1; i >= 0; --i) {
-                const V lam = L::add(L::unpack(past(i) ? 0u : walk.get(my, shift_dy, 2, i)), E);
-                E = L::fma(z[i], lam, lam);
-            }
-        };
-        if (whole)
-            first(std::true_type{});
-        else
-            first(std::false_type{});
-        V d0 = D, b0 = B, d1 = D, e1 = E;  // the warp's first run, and its last
-        if (LW == 16) {
-            const V b1 = of_lane(B, at.l + 16), e0 = of_lane(E, at.l);
-            d0 = of_lane(D, at.l), b0 = of_lane(B, at.l);
-            d1 = of_lane(D, at.l + 16), e1 = of_lane(E, at.l + 16);
-            D = grow<L>(d0, d1);
-            B = fold<L>(b0, d1, b1);
-            E = fold<L>(e1, d0, e0);
+        for (int i = 0; i < kTok; ++i) {
+            gate_both<T>(L::unpack(walk.get(my, shift_g, 0, i)), q[i], z[i]);
+            P = L::mul(P, q[i]);
+            D = L::fma(q[i], D, z[i]);
+            B = L::fma(q[i], B, L::mul(z[i], L::unpack(walk.get(my, shift_v, 1, i))));
         }
-        meet.warp[0][0][warp][lane] = D;
+#pragma unroll
+        for (int i = kTok - 1; i >= 0; --i) E = L::mul(q[i], L::add(L::unpack(walk.get(my, shift_dy, 2, i)), E));
+        V c0 = decay_of<L>(P, D), b0 = B, c1 = c0, e1 = E;  // the warp's first run, and its last
+        if (LW == 16) {
+            const V p0 = of_lane(P, at.l), p1 = of_lane(P, at.l + 16), d0 = of_lane(D, at.l),
+                    d1 = of_lane(D, at.l + 16), b1 = of_lane(B, at.l + 16), e0 = of_lane(E, at.l);
+            c0 = decay_of<L>(p0, d0), c1 = decay_of<L>(p1, d1);
+            b0 = of_lane(B, at.l), e1 = of_lane(E, at.l + 16);
+            P = L::mul(p0, p1);
+            D = L::fma(p0, d1, d0);
+            B = fold<L>(b0, c1, b1);
+            E = fold<L>(e1, c0, e0);
+        }
+        meet.warp[0][0][warp][lane] = LW == 16 ? decay_of<L>(P, D) : c0;
         meet.warp[0][1][warp][lane] = B;
         meet.warp[0][2][warp][lane] = E;
         __syncthreads();
-        // what the CTA's later warps, and all of them, make of a gradient
-        V dp = L::splat(0.0f), ep = dp, d = dp, t = dp;
-#pragma unroll
-        for (int w = kWarps - 1; w >= 0; --w) {
-            if (w == warp) dp = d, ep = t;
-            const V dw = meet.warp[0][0][w][lane];
-            t = fold<L>(t, dw, meet.warp[0][2][w][lane]);
-            d = grow<L>(d, dw);
-        }
-        if (R > 1) walk.send(s, d, t);
-        // h_{t-1} - v_t of the warp's tokens, times the slopes
+        if (R > 1)
+            walk.send(s, kWarps - 1 - warp, [&](Runs<L>& all, int w) {
+                all.add(meet.warp[0][0][kWarps - 1 - w][lane], meet.warp[0][2][kWarps - 1 - w][lane]);
+            });
+        // h_{t-1} - v_t of the warp's tokens, times the slopes; f into the
+        // place of g and v
         V h = L::of(entry);
 #pragma unroll
         for (int w = 0; w < kWarps - 1; ++w)
             if (w < warp && w * Cut<LW>::kRuns * kTok >= at.run * kTok / kChunk * kChunk)
                 h = fold<L>(h, meet.warp[0][0][w][lane], meet.warp[0][1][w][lane]);
-        if (LW == 16 && lane >= 16) h = fold<L>(h, d0, b0);
+        if (LW == 16 && lane >= 16) h = fold<L>(h, c0, b0);
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-            const V off = L::fma(whole || t0 + i < at.len ? L::unpack(walk.get(my, shift_v, 1, i)) : L::splat(0.0f),
-                                 L::splat(-1.0f), h);
-            q[i] = L::mul(q[i], off);
-            h = L::fma(z[i], off, h);
+        for (int i0 = 0; i0 < kTok; i0 += kAhead) {
+            uint32_t vw[kAhead];  // read before the first gate is written, which reads do not pass
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) vw[i] = walk.get(my, shift_v, 1, i0 + i);
+#pragma unroll
+            for (int i = i0; i < i0 + kAhead; ++i) {
+                const V v = L::unpack(vw[i - i0]), f = q[i], off = L::fma(v, L::splat(-1.0f), h);
+                walk.put_gate(s, i, f);
+                q[i] = L::mul(L::mul(z[i], f), off);
+                h = L::fma(f, h, L::mul(z[i], v));
+            }
         }
         V cw = c;
         if (R > 1) {
             walk.receive(s);
-            for (int k = R - 1; k >= 0; --k) {
-                if (k == at.rank) cw = c;
-                c = fold<L>(c, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
-            }
+            by_cluster(R, [&](auto size) {
+#pragma unroll
+                for (int k = size - 1; k >= 0; --k) {
+                    if (k == at.rank) cw = c;
+                    c = fold<L>(c, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
+                }
+            });
+#pragma unroll
+            for (int w = kWarps - 1; w > 0; --w)
+                if (w > warp) cw = fold<L>(cw, meet.warp[0][0][w][lane], meet.warp[0][2][w][lane]);
         } else {
-            c = fold<L>(c, d, t);
+#pragma unroll
+            for (int w = kWarps - 1; w >= 0; --w) {
+                if (w == warp) cw = c;
+                c = fold<L>(c, meet.warp[0][0][w][lane], meet.warp[0][2][w][lane]);
+            }
         }
-        cw = fold<L>(cw, dp, ep);
-        if (LW == 16 && lane < 16) cw = fold<L>(cw, d1, e1);
+        if (LW == 16 && lane < 16) cw = fold<L>(cw, c1, e1);
         T* dg = static_cast<T*>(p.dg) + (int64_t)at.seq * p.seq_dg + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dg;
         T* dv = static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dv;
         auto second = [&](auto all) {
 #pragma unroll
             for (int i = kTok - 1; i >= 0; --i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
-                const V lam = L::add(past ? L::splat(0.0f) : L::unpack(walk.get(my, shift_dy, 2, i)), cw);
+                const V lam = L::add(L::unpack(walk.get(my, shift_dy, 2, i)), cw);
                 if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok)) {
                     const int k = decltype(all)::value ? L::kN : n;
                     st_raw<T, A>(dg, k, past ? 0u : L::pack(L::mul(lam, q[i])));
-                    st_raw<T, A>(dv, k, past ? 0u : L::pack_neg(L::mul(z[i], lam)));
+                    st_raw<T, A>(dv, k, past ? 0u : L::pack(L::mul(z[i], lam)));
                 }
                 dg -= p.s_dg, dv -= p.s_dv;
-                cw = L::fma(z[i], lam, lam);
+                cw = L::mul(walk.take_gate(s, i), lam);
             }
         };
         if (whole)
             second(std::true_type{});
         else
             second(std::false_type{});
+        if (A == kTma) fence_async_smem();  // the gates put there come before the next tiles
         __syncthreads();  // every warp is done with the tiles and the meeting
         if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
         walk.copy_rows(s + kStages, chunk_of(s + kStages));
@@ -809,7 +907,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
         if constexpr (GRAD) yw[i] = live ? ld_raw<T, A>(dy + i * p.s_dy, n) : 0u;
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i) w[i] = gate_small<T>(L::unpack(gw[i]));
+    for (int i = 0; i < NT; ++i) w[i] = gate_decay<T>(L::unpack(gw[i]));
     // the lane's channels one by one
     auto move = [](V w_, float (&h)[N], V v_) {
         float x[N], y[N];
@@ -873,8 +971,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 constexpr int kFwdStages = 3, kGradStages = 2;
 constexpr int kRowStages = 2, kGradRowStages = 1;
 constexpr size_t tiles_smem(int tensors, int stages) { return (size_t)stages * tensors * kTileBytes + 128; }
+// The gradient's rows have their gates beside them, 8 bytes for 4 of a tile.
 template <int LW>
-constexpr size_t rows_smem(int tensors, int stages) { return (size_t)stages * tensors * Cut<LW>::kRowTile + 128; }
+constexpr size_t rows_smem(int tensors, int stages) {
+    return (size_t)stages * tensors * Cut<LW>::kRowTile + (tensors == 3 ? 2 * kTileBytes : 0) + 128;
+}
 
 // [n_seq][n_tok][n_chan] in boxes of row_bytes bytes of a tile's tokens; false when TMA
 // cannot describe it.  Rows and channels past the ends read as zero.

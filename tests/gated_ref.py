@@ -16,7 +16,7 @@ import torch
 
 from block_ref import U32
 
-TINY = 1e-35  # f below 2^-118 counts as 0, z below 2^-134; times magnitudes of order 1
+TINY = 1e-35  # f or z below 2^-118 may count as 0 or as that; times magnitudes of order 1
 
 
 def _gates(g, live):

@@ -77,3 +77,28 @@ KINDS = ["closed8", "closed12", "closed18", "closed40", "closed75", "large_start
 def test_few_tokens(cuda, kind, T, t):
     _check(cuda, kind, 3, T, 70, t)
     _check(cuda, kind, 2, T, 33, t, odd=True)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [17, 130, 1500])
+@pytest.mark.parametrize("t", [BF, F32])
+def test_long(cuda, kind, T, t):
+    """Folds of runs, of a CTA's warps and of a cluster's CTAs."""
+    _check(cuda, kind, 2, T, 70, t)
+    _check(cuda, kind, 1, T, 33, t, odd=True)
+
+
+@pytest.mark.parametrize("kind", ["closed8", "large_start", "ends_alone", "mixed"])
+@pytest.mark.parametrize("S,T,Cn", [(70, 300, 512), (2, 700, 3001), (1, 1000, 2048), (1, 2500, 700)])
+@pytest.mark.parametrize("t", [BF, F32])
+def test_cuts(cuda, kind, S, T, Cn, t):
+    """Wide and narrow rows, single CTAs and clusters of two to eight."""
+    _check(cuda, kind, S, T, Cn, t)
+
+
+@pytest.mark.parametrize("t", [BF, F32])
+def test_long_with_lengths(cuda, t):
+    n = torch.tensor([1100, 0, 1, 550, 130, 1099], dtype=torch.int32)
+    for kind in ("large_start", "closed12"):
+        _check(cuda, kind, 6, 1100, 67, t, lengths=n)
+        _check(cuda, kind, 6, 1100, 67, t, odd=True, lengths=n)
