@@ -14,6 +14,8 @@
 // accurate where it is small.  Runs are handed on as B and the smaller of P and
 // D, and folded as P h + B or h - D h + B: decays stay accurate relative to
 // themselves, and the rounding of P near 1 stays within 16 tokens.
+// An infinite state stays what it is: the folds of a step in which one occurs are
+// made again, since h - D h is no number then.
 //
 // Bound by memory: every token is read once.  A CTA has 128 bytes of channels
 // (4 per lane: 2 bf16 channels, worked on as a pair, or 1 f32) of one chunk of
@@ -39,8 +41,8 @@
 //
 // Measured (bf16; bytes that have to move at the measured copy rate take 62,
 // 103, 123 and 205 us): 4 x 8192 x 2048 tokens x channels 78 us, its gradient
-// 137; 1 x 131072 x 1024 186 and 347, where the cluster's exchange in every step
-// shows; rows that TMA cannot describe (4 x 8192 x 2047) 131 and 241, bound by
+// 141; 1 x 131072 x 1024 190 and 350, where the cluster's exchange in every step
+// shows; rows that TMA cannot describe (4 x 8192 x 2047) 132 and 240, bound by
 // the shared-memory reads at odd offsets and the halved stores (f32 there 165 and
 // 335); one token of 64
 // sequences x 4096 channels 2.2.  What is left in the first two is the gates'
@@ -181,9 +183,22 @@ __device__ __forceinline__ typename Lane<T>::V gate_decay(typename Lane<T>::V g)
 }
 // f x and z x; f h + z v; z f.  Where f is near 1 it is not rounded: over the
 // 1 / z steps of its memory that would add up.
-__device__ __forceinline__ float kept(float c, float x) { return fmaf(c, x, keeps(c) ? x : 0.0f); }
-__device__ __forceinline__ float taken(float c, float x) { return keeps(c) ? -c * x : fmaf(-c, x, x); }
+// (x - z x and h - v are no numbers where x, h or v is infinite, and h - v may
+// not be where it is only large: then the products that the formula has.)
+constexpr float kInfinity = __builtin_huge_valf();
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < kInfinity; }
+__device__ __forceinline__ float f_of(float c) { return keeps(c) ? 1.0f + c : c; }
+__device__ __forceinline__ float z_of(float c) { return keeps(c) ? -c : 1.0f - c; }
+__device__ __forceinline__ float kept(float c, float x) {
+    return finite(x) ? fmaf(c, x, keeps(c) ? x : 0.0f) : f_of(c) * x;
+}
+__device__ __forceinline__ float taken(float c, float x) {
+    return finite(x) ? (keeps(c) ? -c * x : fmaf(-c, x, x)) : z_of(c) * x;
+}
 __device__ __forceinline__ float moved(float c, float h, float v) { return fmaf(c, h - v, keeps(c) ? h : v); }
+__device__ __forceinline__ float moved_any(float c, float h, float v) {
+    return finite(h - v) ? moved(c, h, v) : fmaf(f_of(c), h, z_of(c) * v);
+}
 __device__ __forceinline__ float slope(float c) { return fmaf(-c, c, fabsf(c)); }
 
 // Of a run with P and D.  (Packed arithmetic has no negation and no absolute
@@ -205,11 +220,44 @@ __device__ __forceinline__ typename L::V fold(typename L::V h, typename L::V c, 
     for (int e = 0; e < L::kN; ++e) x[e] = keeps(d[e]) ? x[e] : 0.0f;
     return L::add(L::fma(c, h, L::of(x)), b);
 }
+// The same for infinite h too, which stay what they are (P > 0, even where it
+// is zero in fp32).
+template <typename L>
+__device__ __forceinline__ typename L::V fold_any(typename L::V h, typename L::V c, typename L::V b) {
+    float x[L::kN], d[L::kN], y[L::kN];
+    L::to(h, x), L::to(c, d), L::to(b, y);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e)
+        x[e] = fabsf(x[e]) == kInfinity ? x[e] + y[e] : fmaf(d[e], x[e], keeps(d[e]) ? x[e] : 0.0f) + y[e];
+    return L::of(x);
+}
+// P of a state h, 1 where that is infinite.
+template <typename L>
+__device__ __forceinline__ typename L::V unless_infinite(typename L::V p, typename L::V h) {
+    float a[L::kN], x[L::kN];
+    L::to(p, a), L::to(h, x);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) a[e] = fabsf(x[e]) == kInfinity ? 1.0f : a[e];
+    return L::of(a);
+}
+// Whether one of the lane's n channels is infinite or NaN.  No fold makes
+// either finite again, so it is enough to look at the last of a row of them.
+template <typename L>
+__device__ __forceinline__ bool lost(typename L::V h, int n) {
+    float x[L::kN];
+    L::to(h, x);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) any = any || (e < n && !finite(x[e]));
+    return any;
+}
 // P and -D of several runs, one after the other (D counts only where every
 // run keeps more than half, and there each has -D).
 template <typename L>
 struct Runs {
     typename L::V p = L::splat(1.0f), nd = L::splat(0.0f), b = nd;
+    // kAny: with infinite b's too.
+    template <bool kAny>
     __device__ __forceinline__ void add(typename L::V c, typename L::V bc) {
         float k[L::kN], d[L::kN];
         L::to(L::add(c, L::splat(1.0f)), k), L::to(c, d);
@@ -217,7 +265,7 @@ struct Runs {
         for (int e = 0; e < L::kN; ++e) k[e] = keeps(d[e]) ? k[e] : d[e];
         p = L::mul(p, L::of(k));
         nd = L::add(L::fma(nd, c, nd), c);
-        b = fold<L>(b, c, bc);
+        b = kAny ? fold_any<L>(b, c, bc) : fold<L>(b, c, bc);
     }
     __device__ __forceinline__ typename L::V decay() const { return decay_of<L>(p, nd); }
 };
@@ -348,6 +396,7 @@ struct Meet {
     V        warp[kSteps][K][kWarps][32];
     V        total[2][2][kMaxCluster][32];
     uint64_t arrived[2];
+    uint32_t lost;  // a warp's answer has been infinite or NaN in this or an earlier step
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -551,6 +600,12 @@ struct Walk {
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
     }
+    // Before the warps meet: whether the lane's is infinite or NaN; and after,
+    // whether one was.
+    __device__ __forceinline__ void note(V t) const {
+        if (lost<L>(t, at.n)) *const_cast<volatile uint32_t*>(&meet->lost) = 1;
+    }
+    __device__ __forceinline__ bool noted() const { return *const_cast<const volatile uint32_t*>(&meet->lost) != 0; }
     __device__ __forceinline__ void gave_up() {
         alive = false;
         if (p.fault) atomicCAS(p.fault, 0u, (unsigned)kFaultGated);
@@ -569,24 +624,32 @@ struct Walk {
             for (int k = 0; k < kStages; ++k) mbar_init(&full[k], 1);
             mbar_init(&meet->arrived[0], 1);
             mbar_init(&meet->arrived[1], 1);
+            meet->lost = 0;
             fence_mbar_init();
         }
         __syncthreads();
         if (p.cluster > 1) cluster_sync();  // no CTA writes to another before that one's barriers stand
     }
-    // The totals of step s, of warps whose values add() adds in the order of the
-    // walk, to every CTA of the cluster.  Formed and sent by the first warps
-    // of that order (nth: this one's place), which have the least to fold
-    // once the others' totals are there.
-    template <typename F>
-    __device__ __forceinline__ void send(int s, int nth, F add) {
+    // The totals of step s to every CTA of the cluster, of the warps' decays c
+    // and answers t, taken from warp `from` on in steps of `turn`.  Formed and
+    // sent by the first warps of that order (nth: this one's place), which have
+    // the least to fold once the others' totals are there.
+    __device__ __forceinline__ void send(int s, int nth, const V (&c)[kWarps][32], const V (&t)[kWarps][32], int from,
+                                         int turn) {
         const int b = s & 1, senders = min(p.cluster, kSenders);
         if (at.warp == 0 && at.lane == 0)
             mbar_expect_tx(&meet->arrived[b], (uint32_t)(p.cluster * 2 * 32 * sizeof(V)));
         if (nth < senders) {
             Runs<L> all;
+            if (noted()) {
+#pragma unroll 1
+                for (int w = 0; w < kWarps; ++w)
+                    all.template add<true>(c[from + turn * w][at.lane], t[from + turn * w][at.lane]);
+            } else {
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) add(all, w);
+                for (int w = 0; w < kWarps; ++w)
+                    all.template add<false>(c[from + turn * w][at.lane], t[from + turn * w][at.lane]);
+            }
             const V d = all.decay();
             for (int r = nth; r < p.cluster; r += senders) {
                 const uint32_t bar = in_rank(&meet->arrived[b], r);
@@ -676,18 +739,18 @@ __global__ void __launch_bounds__(kThreads, 2)
             c0 = decay_of<L>(p0, d0), b0 = of_lane(B, at.l);
             P = L::mul(p0, p1);
             D = L::fma(p0, d1, d0);
-            B = fold<L>(b0, decay_of<L>(p1, d1), b1);
+            B = fold_any<L>(b0, decay_of<L>(p1, d1), b1);
         }
         meet.warp[b][0][warp][lane] = LW == 16 ? decay_of<L>(P, D) : c0;
         meet.warp[b][1][warp][lane] = B;
+        walk.note(B);
         __syncthreads();  // and every warp is done with the tiles
         if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
         __syncwarp();
+        const V entry = h;
         V hw = h;
         if (R > 1) {
-            walk.send(s, warp, [&](Runs<L>& all, int w) {
-                all.add(meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
-            });
+            walk.send(s, warp, meet.warp[b][0], meet.warp[b][1], 0, 1);
             walk.receive(s);
             by_cluster(R, [&](auto size) {
 #pragma unroll
@@ -707,22 +770,45 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
         }
         if (LW == 16 && lane >= 16) hw = fold<L>(hw, c0, b0);
-        if (p.states && t0 % kChunk == 0 && t0 < p.n_tok)
-            st_state<L>(p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0, n, hw);
-        T* y = static_cast<T*>(p.y) + (int64_t)at.seq * p.seq_y + at.c0 + (int64_t)t0 * p.s_y;
-        auto second = [&](auto all) {
+        auto second = [&](auto all, auto infinite) {
+            if (p.states && t0 % kChunk == 0 && t0 < p.n_tok)
+                st_state<L>(p.states + ((int64_t)at.seq * p.n_chunk + t0 / kChunk) * p.n_chan + at.c0, n, hw);
+            T* y = static_cast<T*>(p.y) + (int64_t)at.seq * p.seq_y + at.c0 + (int64_t)t0 * p.s_y;
 #pragma unroll
             for (int i = 0; i < kTok; ++i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
+                const V pi = decltype(infinite)::value ? unless_infinite<L>(ph[i], hw) : ph[i];
                 if (decltype(all)::value || (n > 0 && t0 + i < p.n_tok))
-                    st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(L::fma(ph[i], hw, hb[i])));
+                    st_raw<T, A>(y, decltype(all)::value ? L::kN : n, past ? 0u : L::pack(L::fma(pi, hw, hb[i])));
                 y += p.s_y;
             }
         };
         if (whole)
-            second(std::true_type{});
+            second(std::true_type{}, std::false_type{});
         else
-            second(std::false_type{});
+            second(std::false_type{}, std::false_type{});
+        // An infinity or a NaN: once more, with folds that keep infinities.  Here,
+        // where nothing waits for the answer (before the outputs: 1 x 131072 x 1024
+        // bf16 202 us, here 190).
+        if (__any_sync(0xffffffffu, lost<L>(h, n))) {
+            h = hw = entry;
+            if (R > 1) {
+#pragma unroll 1
+                for (int k = 0; k < R; ++k) {
+                    if (k == at.rank) hw = h;
+                    h = fold_any<L>(h, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
+                }
+            }
+            V x = hw;
+#pragma unroll 1
+            for (int w = 0; w < kWarps; ++w) {
+                if (w == warp) hw = x;
+                x = fold_any<L>(x, meet.warp[b][0][w][lane], meet.warp[b][1][w][lane]);
+            }
+            if (R == 1) h = x;
+            if (LW == 16 && lane >= 16) hw = fold_any<L>(hw, c0, b0);
+            second(std::false_type{}, std::true_type{});
+        }
     }
     walk.end();
     for (int k = chunk_of(steps); k * Cut<LW>::kTokens < p.n_tok; k += R) {  // past the sequence's end
@@ -792,25 +878,34 @@ __global__ void __launch_bounds__(kThreads, 2)
             b0 = of_lane(B, at.l), e1 = of_lane(E, at.l + 16);
             P = L::mul(p0, p1);
             D = L::fma(p0, d1, d0);
-            B = fold<L>(b0, c1, b1);
-            E = fold<L>(e1, c0, e0);
+            B = fold_any<L>(b0, c1, b1);
+            E = fold_any<L>(e1, c0, e0);
         }
         meet.warp[0][0][warp][lane] = LW == 16 ? decay_of<L>(P, D) : c0;
         meet.warp[0][1][warp][lane] = B;
         meet.warp[0][2][warp][lane] = E;
+        {  // 0 B + 0 E + 0 entry is NaN where one of them is no finite number
+            const V none = L::splat(0.0f);
+            walk.note(L::fma(B, none, L::fma(E, none, L::mul(L::of(entry), none))));
+        }
         __syncthreads();
         if (R > 1)
-            walk.send(s, kWarps - 1 - warp, [&](Runs<L>& all, int w) {
-                all.add(meet.warp[0][0][kWarps - 1 - w][lane], meet.warp[0][2][kWarps - 1 - w][lane]);
-            });
+            walk.send(s, kWarps - 1 - warp, meet.warp[0][0], meet.warp[0][2], kWarps - 1, -1);
         // h_{t-1} - v_t of the warp's tokens, times the slopes; f into the
         // place of g and v
         V h = L::of(entry);
+        auto of_chunk = [&](int w) { return w < warp && w * Cut<LW>::kRuns * kTok >= at.run * kTok / kChunk * kChunk; };
+        if (walk.noted()) {
+#pragma unroll 1
+            for (int w = 0; w < kWarps - 1; ++w)
+                if (of_chunk(w)) h = fold_any<L>(h, meet.warp[0][0][w][lane], meet.warp[0][1][w][lane]);
+            if (LW == 16 && lane >= 16) h = fold_any<L>(h, c0, b0);
+        } else {
 #pragma unroll
-        for (int w = 0; w < kWarps - 1; ++w)
-            if (w < warp && w * Cut<LW>::kRuns * kTok >= at.run * kTok / kChunk * kChunk)
-                h = fold<L>(h, meet.warp[0][0][w][lane], meet.warp[0][1][w][lane]);
-        if (LW == 16 && lane >= 16) h = fold<L>(h, c0, b0);
+            for (int w = 0; w < kWarps - 1; ++w)
+                if (of_chunk(w)) h = fold<L>(h, meet.warp[0][0][w][lane], meet.warp[0][1][w][lane]);
+            if (LW == 16 && lane >= 16) h = fold<L>(h, c0, b0);
+        }
 #pragma unroll
         for (int i0 = 0; i0 < kTok; i0 += kAhead) {
             uint32_t vw[kAhead];  // read before the first gate is written, which reads do not pass
@@ -824,6 +919,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 h = L::fma(f, h, L::mul(z[i], v));
             }
         }
+        const V c_in = c;
         V cw = c;
         if (R > 1) {
             walk.receive(s);
@@ -845,9 +941,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
         }
         if (LW == 16 && lane < 16) cw = fold<L>(cw, c1, e1);
-        T* dg = static_cast<T*>(p.dg) + (int64_t)at.seq * p.seq_dg + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dg;
-        T* dv = static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dv;
         auto second = [&](auto all) {
+            T* dg = static_cast<T*>(p.dg) + (int64_t)at.seq * p.seq_dg + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dg;
+            T* dv = static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0 + (int64_t)(t0 + kTok - 1) * p.s_dv;
 #pragma unroll
             for (int i = kTok - 1; i >= 0; --i) {
                 const bool past = !decltype(all)::value && t0 + i >= at.len;
@@ -865,6 +961,26 @@ __global__ void __launch_bounds__(kThreads, 2)
             second(std::true_type{});
         else
             second(std::false_type{});
+        // as in the forward walk
+        if (__any_sync(0xffffffffu, lost<L>(c, n))) {
+            c = cw = c_in;
+            if (R > 1) {
+#pragma unroll 1
+                for (int k = R - 1; k >= 0; --k) {
+                    if (k == at.rank) cw = c;
+                    c = fold_any<L>(c, meet.total[b][0][k][lane], meet.total[b][1][k][lane]);
+                }
+            }
+            V x = cw;
+#pragma unroll 1
+            for (int w = kWarps - 1; w >= 0; --w) {
+                if (w == warp) cw = x;
+                x = fold_any<L>(x, meet.warp[0][0][w][lane], meet.warp[0][2][w][lane]);
+            }
+            if (R == 1) c = x;
+            if (LW == 16 && lane < 16) cw = fold_any<L>(cw, c1, e1);
+            second(std::false_type{});
+        }
         if (A == kTma) fence_async_smem();  // the gates put there come before the next tiles
         __syncthreads();  // every warp is done with the tiles and the meeting
         if (walk.issuer() && s + kStages < steps) walk.load(s + kStages, chunk_of(s + kStages));
@@ -878,6 +994,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         blank<T, A>(static_cast<T*>(p.dv) + (int64_t)at.seq * p.seq_dv + at.c0, p.s_dv, t0, p.n_tok, n);
     }
     if (p.dh0 && at.rank == 0 && warp == 0 && lane < LW) st_state<L>(p.dh0 + (int64_t)at.seq * p.seq_dh0 + at.c0, n, c);
+}
+
+// A step of a lane's channels, one by one.
+template <typename L, bool kAny>
+__device__ __forceinline__ void move(typename L::V c, float (&h)[L::kN], typename L::V v) {
+    float x[L::kN], y[L::kN];
+    L::to(c, x), L::to(v, y);
+#pragma unroll
+    for (int e = 0; e < L::kN; ++e) h[e] = kAny ? moved_any(x[e], h[e], y[e]) : moved(x[e], h[e], y[e]);
 }
 
 // Up to NT tokens: a warp has the channels of one slab of one sequence.
@@ -908,26 +1033,30 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) w[i] = gate_decay<T>(L::unpack(gw[i]));
-    // the lane's channels one by one
-    auto move = [](V w_, float (&h)[N], V v_) {
-        float x[N], y[N];
-        L::to(w_, x), L::to(v_, y);
-#pragma unroll
-        for (int e = 0; e < N; ++e) h[e] = moved(x[e], h[e], y[e]);
-    };
     if constexpr (!GRAD) {
         T* y = static_cast<T*>(p.y) + (int64_t)seq * p.seq_y + c0;
+        const V h0 = ld_state<L>(p.h0 ? p.h0 + (int64_t)seq * p.seq_h0 + c0 : nullptr, n);
         float h[N];
-        L::to(ld_state<L>(p.h0 ? p.h0 + (int64_t)seq * p.seq_h0 + c0 : nullptr, n), h);
-        if (p.states && p.n_tok > 0) st_state<L>(p.states + (int64_t)seq * p.n_chan + c0, n, L::of(h));
+        L::to(h0, h);
+        if (p.states && p.n_tok > 0) st_state<L>(p.states + (int64_t)seq * p.n_chan + c0, n, h0);
+        uint32_t out[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {  // past the end z is 0
-            move(w[i], h, L::unpack(vw[i]));
-            vw[i] = i < len ? L::pack(L::of(h)) : 0u;
+            move<L, false>(w[i], h, L::unpack(vw[i]));
+            out[i] = i < len ? L::pack(L::of(h)) : 0u;
+        }
+        // no step makes an infinity or a NaN finite again
+        if (!finite(h[0]) || !finite(h[N - 1])) {
+            L::to(h0, h);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                move<L, true>(w[i], h, L::unpack(vw[i]));
+                out[i] = i < len ? L::pack(L::of(h)) : 0u;
+            }
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            if (i < p.n_tok) st_raw<T, A>(y + i * p.s_y, n, vw[i]);
+            if (i < p.n_tok) st_raw<T, A>(y + i * p.s_y, n, out[i]);
         st_state<L>(p.h1 + (int64_t)seq * p.seq_h1 + c0, n, L::of(h));
     } else {
         T* dg = static_cast<T*>(p.dg) + (int64_t)seq * p.seq_dg + c0;
@@ -943,7 +1072,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) gated_few_kernel(const GatedPa
 #pragma unroll
             for (int e = 0; e < N; ++e) x[e] = slope(x[e]) * (h[e] - v_[e]);
             q[i] = L::of(x);
-            move(w[i], h, L::unpack(vw[i]));
+            move<L, true>(w[i], h, L::unpack(vw[i]));
         }
 #pragma unroll
         for (int i = NT - 1; i >= 0; --i) {
