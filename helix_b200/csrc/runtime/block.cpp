@@ -419,8 +419,9 @@ bool same_tok(const helix_gated_scan_desc& d, const Tok& a, const Tok& b) {
 void check_gated_desc(const helix_gated_scan_desc& d) {
     if (d.n_tok < 0 || d.n_seq < 0 || d.n_chan < 0) unsupported("n_tok, n_seq and n_chan must be >= 0");
     if (!io(d.io_dtype)) unsupported("io_dtype must be F32 or BF16");
-    // chunk indexes and the grid are 32-bit
+    // chunk indexes, the grid and the channels of a slab (64) are 32-bit
     if (d.n_tok > INT_MAX - 4096) unsupported("n_tok must be at most 2^31 - 4097");
+    if (d.n_chan > INT_MAX - 64) unsupported("n_chan must be at most 2^31 - 65");
     const int64_t slabs = ((int64_t)d.n_chan + 31) / 32;
     if ((int64_t)d.n_seq * slabs > INT_MAX / 16) unsupported("problem too large for one launch");
 }

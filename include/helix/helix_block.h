@@ -165,7 +165,7 @@ helix_status helix_matmul8_encode(helix_ctx* ctx, void* stream, const helix_matm
  *
  * n_tok = 1 is the step of a decoder, h1 in place of h0. */
 typedef struct {
-    int32_t     n_tok, n_seq, n_chan;
+    int32_t     n_tok, n_seq, n_chan;        /* at most 2^31 - 4097 tokens, 2^31 - 65 channels */
     helix_dtype io_dtype;                    /* F32 or BF16                     */
     int64_t     s_v, s_g, s_y;               /* token strides                   */
     int64_t     s_dy, s_dv, s_dg;
