@@ -6,8 +6,10 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <string>
+#include <utility>
 
 namespace {
 
@@ -63,12 +65,18 @@ T* ptr(helix_tensor t) {
 int64_t elem(helix_dtype t) { return t == HELIX_F32 ? 4 : t == HELIX_E4M3 ? 1 : 2; }
 bool io(helix_dtype t) { return t == HELIX_F32 || t == HELIX_BF16; }
 
-// A matrix argument of a call: `rows` rows of `cols` elements, `ld` apart.
+// A matrix argument of a call: `rows` rows of `cols` elements, `ld` apart; or
+// `stack` such matrices, `step` elements apart.
 struct Mat {
     const char*  name;
     helix_tensor t;
     int64_t      rows, cols, ld, size;
     bool         written;
+    int64_t      stack = 1, step = 0;
+
+    uintptr_t end() const {
+        return addr(t) + (uintptr_t)(((stack - 1) * step + (rows - 1) * ld + cols) * size);
+    }
 };
 
 void check_mat(const Mat& m) {
@@ -80,14 +88,37 @@ void check_mat(const Mat& m) {
     if (m.rows > 1 && m.ld > 0 && (m.rows - 1) > most / m.ld) invalid(n + ": rows reach past 64-bit offsets");
 }
 
+// Whether a row of one of two stacks with the same strides shares bytes with a
+// row of the other: whether, for some difference i of their places in the
+// stacks and j of their rows, the distance of the rows is less than their width.
+// Exact, unless both differences have more than 2^16 values (then: they may).
+bool stacks_overlap(const Mat& a, const Mat& b) {
+    int64_t n = a.stack, m = a.rows, p = a.step * a.size, q = a.ld * a.size;
+    if (n > m) std::swap(n, m), std::swap(p, q);
+    const int64_t wa = a.cols * a.size, wb = b.cols * b.size;
+    if (n > 1 << 16 || q <= 0) return true;
+    const int64_t apart = (int64_t)(addr(b.t) - addr(a.t));
+    for (int64_t i = 1 - n; i < n; ++i) {
+        const int64_t d = apart + i * p;  // -wb < d + j q < wa
+        int64_t j = (wa - 1 - d) / q;     // the largest such j, and what is below
+        if ((wa - 1 - d) % q < 0) --j;
+        j = std::min(j, m - 1);
+        if (j > -m && d + j * q > -wb) return true;
+    }
+    return false;
+}
+
 // Whether two matrices share bytes.  Matrices with one row pitch may lie
 // side by side in it (slices of one wider matrix).
 bool overlap(const Mat& a, const Mat& b) {
     if (!a.t.buf || !b.t.buf || !a.rows || !b.rows || !a.cols || !b.cols) return false;
     const uintptr_t a0 = addr(a.t), b0 = addr(b.t);
-    const uintptr_t a1 = a0 + (uintptr_t)(((a.rows - 1) * a.ld + a.cols) * a.size);
-    const uintptr_t b1 = b0 + (uintptr_t)(((b.rows - 1) * b.ld + b.cols) * b.size);
-    if (a1 <= b0 || b1 <= a0) return false;
+    if (a.end() <= b0 || b.end() <= a0) return false;
+    if (a.stack > 1 || b.stack > 1) {
+        const bool alike = a.stack == b.stack && a.rows == b.rows && a.step * a.size == b.step * b.size &&
+                           a.ld * a.size == b.ld * b.size;
+        return !alike || stacks_overlap(a, b);
+    }
     const uintptr_t pitch = (uintptr_t)(a.ld * a.size);
     if (a.rows > 1 && b.rows > 1 && pitch && pitch == (uintptr_t)(b.ld * b.size)) {
         const uintptr_t wa = (uintptr_t)(a.cols * a.size), wb = (uintptr_t)(b.cols * b.size);
@@ -401,16 +432,15 @@ void check_tok(const helix_gated_scan_desc& d, const Tok& x) {
         invalid(n + ": reaches past 64-bit offsets");
 }
 
-// One address range per token tensor; where tokens follow one another at one
-// pitch through all sequences, a matrix with that pitch (slices of one wider
-// tensor may then lie side by side).
+// A matrix where tokens follow one another at one pitch through all sequences,
+// else a stack of the sequences' (slices of one wider tensor may lie side by
+// side in both).
 Mat mat_of(const helix_gated_scan_desc& d, const Tok& x) {
     const int64_t size = elem(d.io_dtype);
     if (d.n_seq <= 1 || x.s_seq == (int64_t)d.n_tok * x.s_tok)
         return {x.name, x.t, (int64_t)d.n_tok * d.n_seq, d.n_chan, x.s_tok, size, x.written};
     if (d.n_tok <= 1) return {x.name, x.t, d.n_seq, d.n_chan, x.s_seq, size, x.written};
-    const int64_t last = (int64_t)(d.n_tok - 1) * x.s_tok + (int64_t)(d.n_seq - 1) * x.s_seq + d.n_chan;
-    return {x.name, x.t, 1, last, last, size, x.written};
+    return {x.name, x.t, d.n_tok, d.n_chan, x.s_tok, size, x.written, d.n_seq, x.s_seq};
 }
 bool same_tok(const helix_gated_scan_desc& d, const Tok& a, const Tok& b) {
     return addr(a.t) == addr(b.t) && (d.n_tok <= 1 || a.s_tok == b.s_tok) && (d.n_seq <= 1 || a.s_seq == b.s_seq);
