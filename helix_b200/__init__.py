@@ -10,6 +10,7 @@ path: every call goes through the library, and a missing library raises.
 from __future__ import annotations
 
 import ctypes as C
+import sys
 from typing import Optional
 
 from . import abi
@@ -33,10 +34,15 @@ def _t(x) -> abi.Tensor:
 
 
 class Context:
-    """Owns one helix_ctx bound to a CUDA device."""
+    """Owns one helix_ctx bound to a CUDA device: the given one, or the one that
+    is current (`device` is None where only the CUDA runtime knows which)."""
 
     def __init__(self, device: Optional[int] = None):
         self.lib = abi.load()
+        torch = sys.modules.get("torch")
+        if device is None and torch is not None and torch.cuda.is_initialized():
+            device = torch.cuda.current_device()
+        self.device = device
         h = C.c_void_p()
         dev = C.c_int(device) if device is not None else None
         st = self.lib.helix_ctx_create(C.byref(h), C.byref(dev) if dev is not None else None, None)

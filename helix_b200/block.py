@@ -25,13 +25,15 @@ from . import _block_torch as _native  # noqa: E402
 
 def _ctx(ctx: Optional[Context], t: torch.Tensor) -> int:
     """The helix_ctx of a call, as an integer; one per device without `ctx`."""
+    index = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if index < 0:
+        raise ValueError("tensors must be on a CUDA device")
     if ctx is None:
-        index = t.get_device() if isinstance(t, torch.Tensor) else -1
-        if index < 0:
-            raise ValueError("tensors must be on a CUDA device")
         ctx = _default_ctx.get(index)
         if ctx is None:
             ctx = _default_ctx.setdefault(index, Context(index))
+    elif ctx.device is not None and ctx.device != index:
+        raise ValueError(f"the context is of device {ctx.device}, the tensors are on device {index}")
     return ctx.handle.value
 
 
