@@ -12,6 +12,7 @@ Usage: python -m helix_b200.build [-v] [--force]
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -65,9 +66,6 @@ def _build_torch(force: bool) -> None:
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.submodule_search_locations:
         return
-    newest = max(p.stat().st_mtime for p in [TORCH_SRC, *headers()])
-    if not force and TORCH_EXT.exists() and TORCH_EXT.stat().st_mtime >= newest:
-        return
     torch = Path(list(spec.submodule_search_locations)[0])
     cuda = Path(NVCC).resolve().parent.parent
     tmp = BUILD / TORCH_EXT.name
@@ -77,10 +75,22 @@ def _build_torch(force: bool) -> None:
            f"-isystem{sysconfig.get_paths()['include']}", str(TORCH_SRC), "-o", str(tmp), f"-L{PKG}", "-l:libhelix.so",
            f"-L{torch / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            "-Wl,-rpath,$ORIGIN"]
+    # what it was built with: another torch has another ABI
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        version = (torch / "version.py").read_text()
+    made = BUILD / "block_torch.made"
+    made_with = f"torch {version}\n{' '.join(cmd)}\n".replace(str(ROOT), ".")  # wherever the tree is
+    newest = max(p.stat().st_mtime for p in [TORCH_SRC, *headers()])
+    if (not force and TORCH_EXT.exists() and TORCH_EXT.stat().st_mtime >= newest and made.exists()
+            and made.read_text() == made_with):
+        return
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {TORCH_SRC}\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     shutil.move(tmp, TORCH_EXT)
+    made.write_text(made_with)
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
