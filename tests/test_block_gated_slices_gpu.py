@@ -87,3 +87,27 @@ def test_outputs_beside_inputs(cuda, ctx):
     for off in (4 * Cn - 4, 4 * Cn + 4, 0, 12 * Cn, 12 * Cn * (T + 3)):
         assert call(abi.Tensor(held.data_ptr(), off)) == abi.HELIX_ERR_INVALID_ARG, off
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("S,T,Cn", [(2, 9, 33), (2, 300, 67), (1, 3000, 131), (40, 200, 321)])
+@pytest.mark.parametrize("shift", [1, 2, 3])
+@pytest.mark.parametrize("t", [BF, F32])
+def test_in_place_of_copied_rows(cuda, S, T, Cn, shift, t):
+    """dv in place of dy in rows that are copied in 16-byte pieces, which hold
+    bytes of the rows and channels beside them; what lies between stays."""
+    v, g, dy, dh1, states = _case(cuda, S, T, Cn, t)
+    want = helix_b200.gated_scan_grad(dy, v, g, states, dh1)
+    pitch = Cn + shift
+    held = torch.full((S * T * pitch + shift,), 7.0, dtype=t, device=cuda)
+    rows = held[shift:].view(S, T, pitch)[..., :Cn]
+    rows.copy_(dy)
+    got = helix_b200.gated_scan_grad(rows, v, g, states, dh1, dv=rows)
+    assert got[0] is rows
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    rows.fill_(7.0)
+    assert (held == 7.0).all()
+    # h1 in place of h0, too
+    state = dh1.clone()
+    y, h1 = helix_b200.gated_scan(v, g, dh1)
+    y2, same = helix_b200.gated_scan(v, g, state, h1=state)
+    assert same is state and torch.equal(y, y2) and torch.equal(h1, state)
