@@ -6,6 +6,8 @@ stream); the checks of its tensors and the allocation of its outputs and
 scratch are in the extension module _block_torch (csrc/torch).  There is no
 compute here and no fallback: what the library refuses raises HelixError, a
 tensor of the wrong shape or device ValueError, one of the wrong type TypeError.
+No autograd graph is recorded, whatever the tensors require: outputs are without
+one, and the gradients are calls of their own.
 
 8-bit tensors are torch.float8_e4m3fn with an fp32 scale per 128 columns of a
 row (or per 128 x 128 block); their rows are padded to whole 16 bytes, which is
@@ -83,7 +85,8 @@ def rms_norm_grad(dout: torch.Tensor, sum: torch.Tensor, rstd: torch.Tensor, wei
     dout is the gradient of the norm's output in x's type (rounding to 8 bits
     is passed through), dsum the one that reaches sum by another way; sum and
     rstd are what the forward pass gave.  dx has dout's type and dres, the
-    same gradient for the residual, sum's; dweight is f32."""
+    same gradient for the residual, sum's (where that is dout's, it is dx
+    itself); dweight is f32."""
     return _call(stream, _native.rms_norm_grad, _ctx(ctx, dout), dout, sum, rstd, weight, dsum, keep_dres)
 
 

@@ -458,6 +458,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             if (first) st.next(), buf.next();
             // A wait costs its latency even when nothing is left to wait for;
             // the next block's two are polled between its issue and its commits.
+            // (With the two buffers of BN = 256 the next block's is this block's
+            // own, which the commit below hands on: there that poll fails, and
+            // the wait follows.)
             bool ready = false, free = first < Cfg::kBufs;
             int it = first;
             for (; it < total; it += 2) {

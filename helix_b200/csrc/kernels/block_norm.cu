@@ -12,8 +12,9 @@
 // of the segment, so every access is still a run of 32 values, and the whole
 // warp holds each of the segment's two groups.
 //
-// Sums, statistics and the products are fp32; the only roundings are those
-// of the stored sum, the output and (8 bits) 1 / scale.
+// Sums, statistics and the products are fp32 (the row's mean by a rounded
+// 1 / n_col, rstd by rsqrtf); to fewer bits go the stored sum and the output
+// alone.  In 8 bits a value is multiplied by an approximate 1 / scale.
 //
 // What bounds them beside memory is the instructions: three quarters of the
 // issue slots before the arithmetic went in pairs (fp32 x 2) and the
@@ -22,7 +23,7 @@
 // Measured: 8192 x 4096 bf16 to bf16 43.5 us, 6.2 TB/s, to 8 bits, where a
 // group's maximum and scale come between the row's statistic and its output,
 // 44.4, 5.3; f32 82, 6.5; 1537 x 2501 f32 10.9,
-// 5.6; 8192 x 8192 bf16 88, 4096 x 16384 96; gradient of 16384 x 4096 bf16 88.5
+// 5.6; 8192 x 8192 bf16 87, 4096 x 16384 87; gradient of 16384 x 4096 bf16 88.5
 // us, 6.1 TB/s (a copy's rate is 6.55), of 8192 x 4096 f32 96, 5.6; of 8192 x
 // 4095, whose rows start anywhere, bf16 78, f32 98.
 #include <algorithm>

@@ -119,10 +119,10 @@ helix_status helix_quant8_encode(helix_ctx* ctx, void* stream, const helix_quant
 /* out[i][j] = sum over blocks of 128 columns b of
  *     a_scale[i][b] b_scale[j or j / 128][b] sum_{k in b} a[i][k] b[j][k]
  * a [m][k] has its scales by rows (what the norm and the quantiser write),
- * b [n][k] by blocks (a weight) or by rows.  Products and their sum over a
- * block are exact to fp32 on the tensor cores, blocks are scaled and summed
- * in fp32 in an order that depends on the sizes and the device alone, and
- * out is rounded once.
+ * b [n][k] by blocks (a weight) or by rows.  Products are exact; the tensor
+ * cores sum a block's in fp32 and may truncate (within 16 x 2^-24 of the sum of
+ * their magnitudes), blocks are scaled and summed in fp32 in an order that
+ * depends on the sizes and the device alone, and out is rounded once.
  *
  * The gradients are two more such products: of a, the gradient of out (by
  * rows) with b transposed (blocks); of b, the gradient of out and a, both
@@ -157,7 +157,15 @@ helix_status helix_matmul8_encode(helix_ctx* ctx, void* stream, const helix_matm
  * from h0 (zeros when null) to h1, the state after the last token.  The
  * states are f32, the arithmetic fp32; v, g, y, dy, dv and dg are io_dtype.
  * Token tensors are [n_seq][n_tok][n_chan] with strides of their own for the
- * token and the sequence; states are [n_seq][n_chan].
+ * token and the sequence; those with the same strides may be slices of one
+ * wider tensor.  States are [n_seq][n_chan].
+ *
+ * f and 1 - f are both known to (2 |g| + 14) 2^-24 of themselves (below 2^-126
+ * they may count as 0 or as that), and what is left of a state or a gradient
+ * after many tokens is as accurate relative to itself.  An infinite h0 or v
+ * makes the states from there on infinite, an infinite dh1 or dy the gradients
+ * before it, as the formula does: NaN where two of different sign meet, or
+ * infinity and a difference h_{t-1} - v_t of zero.  NaN stays in its channel.
  *
  * lengths (int32, [n_seq], may be null) ends sequences early: tokens at or
  * past lengths[seq] (taken as 0 .. n_tok) leave the state as it is, whatever
