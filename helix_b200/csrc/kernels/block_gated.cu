@@ -132,8 +132,9 @@ __device__ __forceinline__ void gate(typename Lane<T>::V g, typename Lane<T>::V&
     z = L::of(r);
     f = L::mul(tv, z);
 }
-// The smaller one, m = t / (1 + t) with t = e^-|g| (formed as 2^8 t, for the
-// same reason), down to subnormal values on both sides.
+// The smaller one, m = t / (1 + t) with t = e^-|g|, down to 2^-134 on both
+// sides: the exponential gives 2^8 t, whose normal values reach that far, and the
+// product with 2^-8 keeps subnormal ones.
 template <typename T>
 __device__ __forceinline__ typename Lane<T>::V gate_min(const float (&g)[Lane<T>::kN]) {
     using L = Lane<T>;
@@ -149,7 +150,7 @@ __device__ __forceinline__ typename Lane<T>::V gate_min(const float (&g)[Lane<T>
     for (int e = 0; e < L::kN; ++e) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r[e]));
     return L::mul(tv, L::of(r));
 }
-// Both from it: the gradient's dg needs f z on that range.
+// Both from it, for the gradient, whose dg has f z as a factor.
 template <typename T>
 __device__ __forceinline__ void gate_both(typename Lane<T>::V g, typename Lane<T>::V& f, typename Lane<T>::V& z) {
     using L = Lane<T>;
@@ -182,9 +183,9 @@ __device__ __forceinline__ typename Lane<T>::V gate_decay(typename Lane<T>::V g)
     return L::of(c);
 }
 // f x and z x; f h + z v; z f.  Where f is near 1 it is not rounded: over the
-// 1 / z steps of its memory that would add up.
-// (x - z x and h - v are no numbers where x, h or v is infinite, and h - v may
-// not be where it is only large: then the products that the formula has.)
+// 1 / z steps of its memory that would add up.  (x - z x and h - v are no numbers
+// where x, h or v is infinite, and h - v need not be one where it is only large:
+// then the products that the formula has.)
 constexpr float kInfinity = __builtin_huge_valf();
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < kInfinity; }
 __device__ __forceinline__ float f_of(float c) { return keeps(c) ? 1.0f + c : c; }
